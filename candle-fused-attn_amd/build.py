@@ -12,6 +12,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -19,7 +21,8 @@ REPO = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "lib"
 LIB = LIB_DIR / "libfattn.so"
-SOURCES = [CSRC / "fattn_kernels.hip", CSRC / "fattn_pair.hip", CSRC / "fattn_api.cpp"]
+SOURCES = [CSRC / "fattn_pair.hip", CSRC / "fattn_paged.hip", CSRC / "fattn_rotary.hip",
+           CSRC / "fattn_kernels.hip", CSRC / "fattn_api.cpp", CSRC / "fattn_operators.cpp"]
 HEADERS = [REPO / "include" / "fattn.h", CSRC / "fattn_internal.h", CSRC / "fattn_device.h"]
 # The C++ op layer over the C ABI (the reference's src/lib.rs ops for C++ callers), linked
 # against libfattn.so, and its test program (links the CPU oracle; test infrastructure).
@@ -50,9 +53,15 @@ def hipcc() -> str:
     return path
 
 
-def command(out: Path = LIB) -> list[str]:
-    return [hipcc(), *HIPCC_FLAGS, f"-I{REPO / 'include'}", f"-I{CSRC}",
-            *[str(s) for s in SOURCES], "-o", str(out)]
+def compile_command(src: Path, out: Path) -> list[str]:
+    flags = [f for f in HIPCC_FLAGS if f != "-shared"]
+    return [hipcc(), *flags, f"-I{REPO / 'include'}", f"-I{CSRC}", "-x", "hip", "-c", str(src),
+            "-o", str(out)]
+
+
+def link_command(objects: list[Path], out: Path = LIB) -> list[str]:
+    return [hipcc(), "--offload-arch=gfx950", "-fPIC", "-shared", *[str(o) for o in objects], "-o",
+            str(out)]
 
 
 def _run(cmd: list[str], tmp: Path, out: Path, verbose: bool) -> Path:
@@ -61,7 +70,8 @@ def _run(cmd: list[str], tmp: Path, out: Path, verbose: bool) -> Path:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"hipcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
-    os.replace(tmp, out)
+    if tmp != out:
+        os.replace(tmp, out)
     return out
 
 
@@ -69,7 +79,12 @@ def build(verbose: bool = False) -> Path:
     """Compile libfattn.so in-tree (always; the caller decides when to rebuild)."""
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     tmp = LIB.with_suffix(".so.tmp")
-    return _run(command(tmp), tmp, LIB, verbose)
+    with tempfile.TemporaryDirectory() as d, ThreadPoolExecutor(len(SOURCES)) as pool:
+        objects = [Path(d) / (s.name + ".o") for s in SOURCES]
+        # (list() waits for every source and raises what a compilation raised.)
+        list(pool.map(lambda so: _run(compile_command(*so), so[1], so[1], verbose),
+                      zip(SOURCES, objects)))
+        return _run(link_command(objects, tmp), tmp, LIB, verbose)
 
 
 def host_command(out: Path = HOST_LIB) -> list[str]:

@@ -6,6 +6,7 @@ The public surface mirrors the reference crate's (src/lib.rs:90-161): `fused_att
 `fused_attention_qkv`, `CUDA_HEAD_DIM`.
 """
 from ._lib import FusedAttentionError, LIB_PATH, version
+from .cross import fused_cross_attention
 from .ops import (
     CUDA_HEAD_DIM,
     HIP_HEAD_DIM,
@@ -18,6 +19,8 @@ from .ops import (
     set_dq_sum,
     set_projection_route,
 )
+from .paged import paged_append, paged_attention
+from .rotary import fused_rotary, fused_rotary_qkv, rotary_frequencies
 
 __all__ = [
     "CUDA_HEAD_DIM",
@@ -28,8 +31,14 @@ __all__ = [
     "float4_aligned",
     "fused_attention",
     "fused_attention_qkv",
+    "fused_cross_attention",
+    "fused_rotary",
+    "fused_rotary_qkv",
+    "paged_append",
+    "paged_attention",
     "qkv_projection_of",
     "reads_in_place",
+    "rotary_frequencies",
     "set_dq_sum",
     "set_projection_route",
     "version",

@@ -19,6 +19,9 @@ FATTN_EALIGN = -3
 FATTN_ERANGE = -4
 FATTN_EWORKSPACE = -5
 
+# Element types.
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
 # Every entry point include/fattn.h declares.
 EXPORTS = (
     "fattn_fwd_f32",
@@ -39,6 +42,12 @@ EXPORTS = (
     "fattn_qkv_backward",
     "fattn_forward",
     "fattn_backward",
+    "fattn_rotary",
+    "fattn_paged_append",
+    "fattn_paged_attention_workspace_bytes",
+    "fattn_paged_attention",
+    "fattn_cross_workspace_bytes",
+    "fattn_cross_forward",
     "fattn_last_error",
     "fattn_version",
     "fattn_bwd_status",
@@ -61,6 +70,8 @@ P = ctypes.c_void_p
 A3 = ctypes.POINTER(ctypes.c_int64)
 C_INT = ctypes.c_int
 C_FLOAT = ctypes.c_float
+C_DOUBLE = ctypes.c_double
+PP = ctypes.POINTER(ctypes.c_void_p)
 SIZE = ctypes.c_size_t
 
 
@@ -94,6 +105,19 @@ def _declare(L: ctypes.CDLL) -> None:
                                 P, P, P]
     L.fattn_backward.argtypes = [P, I64, A3, A3, P, I64, A3, A3, P, I64, A3, A3, C_FLOAT, C_INT,
                                  P, P, P, I64, A3, A3, P, P, SIZE, P]
+    L.fattn_rotary.argtypes = [C_INT, I64, I64, I64, A3, PP, PP, A3, A3, C_INT, P, C_INT, A3, P, I64,
+                               C_INT, C_DOUBLE, C_INT, P]
+    L.fattn_paged_append.argtypes = [C_INT, C_INT, I64, I64, I64, I64, I64, P, A3, P, A3, P, A3, P,
+                                     A3, P, A3, P, A3, I64, I64, P, I64, I64, P, P, P, I64, C_INT,
+                                     C_DOUBLE, P]
+    L.fattn_paged_attention_workspace_bytes.argtypes = [I64, I64, I64, I64, I64]
+    L.fattn_paged_attention_workspace_bytes.restype = SIZE
+    L.fattn_paged_attention.argtypes = [C_INT, C_INT, I64, I64, I64, I64, P, A3, P, P, A3, P, A3,
+                                        I64, I64, P, I64, I64, P, C_FLOAT, P, SIZE, P]
+    L.fattn_cross_workspace_bytes.argtypes = [I64, I64, I64, I64, I64, I64]
+    L.fattn_cross_workspace_bytes.restype = SIZE
+    L.fattn_cross_forward.argtypes = [P, A3, P, A3, P, A3, I64, I64, I64, I64, I64, I64, P, C_FLOAT,
+                                      P, P, P, SIZE, P]
     L.fattn_bwd_status.argtypes = [P, SIZE, I64, I64, I64, P, ctypes.POINTER(C_INT)]
     for name in EXPORTS:
         if name not in ("fattn_last_error", "fattn_version") and "workspace" not in name:

@@ -1,0 +1,59 @@
+"""Cross attention: a decoder's queries to an encoder's states of another length, fp32.
+
+As fused_attention, with keys and values of their own length and number of heads, and per-sample key
+lengths in place of a mask.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._call import aligned_rows, launch, require, strides3
+from ._lib import FusedAttentionError
+
+_F32 = (torch.float32,)
+_I32 = (torch.int32,)
+
+
+def _forward(q, k, v, scale, key_lengths):
+    b, h, sq, d = q.shape
+    hk, sk = k.shape[1], k.shape[2]
+    L = _lib.lib()
+    out = torch.empty((b, sq, h, d), dtype=torch.float32, device=q.device)
+    lse = torch.empty((b, h, sq), dtype=torch.float32, device=q.device)
+    size = L.fattn_cross_workspace_bytes(b, h, hk, sq, sk, d)
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    launch(q, L.fattn_cross_forward, q.data_ptr(), strides3(q), k.data_ptr(), strides3(k),
+           v.data_ptr(), strides3(v), b, h, hk, sq, sk, d,
+           key_lengths.data_ptr() if key_lengths is not None else None, scale, out.data_ptr(),
+           lse.data_ptr(), ws.data_ptr() if size else None, size)
+    return out, lse
+
+
+def fused_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
+                          key_lengths: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(q k^T scale) v, each sample seeing its first key_lengths[b] keys (None: all).
+
+    q: [b, h, sq, d], k, v: [b, kv_heads, sk, d] f32 on one HIP device, any strides (copied first when
+    the kernels cannot read them in place), d 32, 64 or 128, h a multiple of kv_heads (query head i
+    reads key head i // (h // kv_heads)); key_lengths: [b] int32 (one outside [0, sk] counts as the
+    nearest). Returns [b, h, sq, d], a transposed view of a contiguous [b, sq, h, d] buffer; a sample
+    that sees no key gives 0.
+    """
+    who = "fused_cross_attention"
+    require(who, "q", q, 4, None, _F32)
+    require(who, "k", k, 4, q.device, _F32)
+    require(who, "v", v, 4, q.device, _F32)
+    b, h, _, d = q.shape
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+        raise FusedAttentionError(f"{who}: q [b, h, sq, d] and k, v [b, kv_heads, sk, d] expected, got "
+                                  f"{list(q.shape)} {list(k.shape)} {list(v.shape)}")
+    if key_lengths is not None:
+        require(who, "key_lengths", key_lengths, 1, q.device, _I32)
+        if key_lengths.shape[0] != b or not key_lengths.is_contiguous():
+            raise FusedAttentionError(f"{who}: contiguous key_lengths [{b}] expected, got "
+                                      f"{list(key_lengths.shape)}")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        raise FusedAttentionError(f"{who}: not differentiable yet")
+    return _forward(aligned_rows(q), aligned_rows(k), aligned_rows(v), float(scale),
+                    key_lengths)[0].transpose(1, 2)

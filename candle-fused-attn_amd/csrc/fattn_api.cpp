@@ -11,6 +11,7 @@
 #include <cstdint>
 #include <climits>
 #include <random>
+#include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -111,6 +112,36 @@ namespace {
 using fattn::View;
 
 thread_local std::string g_error;
+
+}  // namespace
+
+namespace fattn {
+
+int set_error(int code, const char* format, ...) {
+  char text[512];
+  va_list args;
+  va_start(args, format);
+  std::vsnprintf(text, sizeof text, format, args);
+  va_end(args);
+  try {
+    g_error = text;
+  } catch (...) {  // (no memory for the message: no exception leaves a C entry)
+  }
+  return code;
+}
+
+int hip_error(int err, const char* who, const char* what) {
+  return set_error(err, "%s: %s: %s", who, what, hipGetErrorString(static_cast<hipError_t>(err)));
+}
+
+int done() {
+  g_error.clear();
+  return 0;
+}
+
+}  // namespace fattn
+
+namespace {
 
 // A 64-bit value unique to each step 2 launch of this process, the sequence starting at a random
 // point: step 2 tags its flags in the workspace with it.

@@ -168,6 +168,66 @@ int launch_bwd_dq(const float* part, unsigned long long* done, const unsigned lo
 // of fattn_bwd_f32_noalloc) on the device that runs `stream`; a hipError_t value as int.
 int static_scratch(void* stream, void** out);
 
+// --- Rotary positions and the paged cache (fattn_rotary.hip, fattn_paged.hip) --------------------
+// Element types of the C ABI (FATTN_F32, ..).
+constexpr int kF32 = 0, kF16 = 1, kBF16 = 2;
+// One operand of a rotation: heads (0: absent) of a [b, heads, s, d] view x and of its result y,
+// (batch, head, seq) strides in elements, turned or copied.
+struct RotaryPart {
+  const void* x;
+  void* y;
+  int64_t xs[3], ys[3];
+  int heads, rotate;
+};
+// Positions are given ([b, s] through strides, 32 or 64 bits), or, with a page table, lengths[b] + i.
+// With a page table part 0 is q (may be absent) and parts 1 and 2, k and v, go to the pages:
+// page_strides are (page, head, slot) of k's, then of v's.
+struct RotaryArgs {
+  RotaryPart part[3];
+  const void* positions;
+  int64_t pos_strides[2];
+  int pos64;
+  const double* frequencies;  // radians per position, of each pair
+  double magnitude;
+  int B, S, D, pairs, interleaved, inverse;
+  const int32_t *table, *lengths, *counts;
+  int64_t table_stride, table_width, pages, page_size, page_strides[6];
+  int tokens;  // (the launcher's)
+};
+// vec: values per access, 8, 4 or 1 (2 interleaved): every pointer, stride and part of a head is a
+// multiple of it, where it is 4 or more.
+int launch_rotary(RotaryArgs a, int dtype, int cache_dtype, int vec, void* stream);
+
+// Attention of few queries per key head, split over the keys (fattn_paged.hip). Rows of one key head:
+// the G query heads of its group times SQ queries, in blocks of 16.
+constexpr int kSplitTile = 32;  // keys
+struct SplitArgs {
+  const void *q, *k, *v;
+  void* o;     // [b, sq, h, d] contiguous, of q's type
+  float* lse;  // [b, h, sq], or null
+  // q: (batch, head, query); k, v: (page, head, slot) with a page table, else (batch, head, key).
+  int64_t qs[3], ks[3], vs[3];
+  const int32_t *table, *lengths;  // lengths null: SK keys each
+  int64_t table_stride;
+  int page_size, pages;
+  unsigned div_magic, div_shift;  // x / (page_size / 16) = (hi32(x magic) + x) >> shift
+  int B, H, HK, G, SQ, SK, RB;    // SK: the most keys a sequence can have; RB: blocks of rows
+  float scale;
+  float* part;  // the workspace
+  int part_rows, wgs, min_run;  // wgs 0: one workgroup per key head and block of rows, no workspace
+};
+struct SplitPlan {
+  int row_blocks, part_rows, wgs, min_run;
+  size_t bytes;
+};
+SplitPlan split_plan(int64_t b, int64_t hk, int64_t rows, int64_t d, int64_t capacity);
+int launch_split(const SplitArgs& a, int dtype, int cache_dtype, int d, void* stream);
+
+// Sets this thread's message (fattn_last_error) and returns `code`; done() clears it and returns 0.
+int set_error(int code, const char* format, ...) __attribute__((format(printf, 2, 3)));
+int hip_error(int err, const char* who, const char* what);
+int done();
+
 // Grid sizes the launchers will use (for range checks before launching).
 int64_t bwd_main_blocks(int64_t b, int64_t h, int64_t s);
 int64_t bwd_prep_blocks(int64_t b, int64_t h, int64_t s, int d);

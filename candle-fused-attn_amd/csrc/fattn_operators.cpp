@@ -1,0 +1,347 @@
+// The C ABI of the operators around self-attention (include/fattn.h): argument validation and the
+// launches. Validation runs before any HIP call, as in fattn_api.cpp.
+#include <hip/hip_runtime.h>
+
+#include <climits>
+#include <cstdint>
+
+#include "fattn.h"
+#include "fattn_internal.h"
+
+namespace {
+
+using fattn::set_error;
+
+// Workgroups of 256 threads in a grid of fewer than 2^32 threads.
+constexpr int64_t kMaxGrid = (int64_t{1} << 24) - 1;
+constexpr int64_t kMaxHeads = 65535;
+
+bool known(int dtype) { return dtype == FATTN_F32 || dtype == FATTN_F16 || dtype == FATTN_BF16; }
+int64_t size_of(int dtype) { return dtype == FATTN_F32 ? 4 : 2; }
+bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+void copy3(int64_t to[3], const int64_t from[3]) {
+  for (int i = 0; i < 3; ++i) to[i] = from[i];
+}
+// Strides {.., .., ..} of dimensions of n0, n1, n2: those of one entry (or none) are never used.
+void used3(int64_t to[3], const int64_t from[3], int64_t n0, int64_t n1, int64_t n2) {
+  to[0] = n0 > 1 ? from[0] : 0, to[1] = n1 > 1 ? from[1] : 0, to[2] = n2 > 1 ? from[2] : 0;
+}
+bool multiples(const int64_t st[3], int64_t of) {
+  return st[0] % of == 0 && st[1] % of == 0 && st[2] % of == 0;
+}
+bool negative(const int64_t* x, int n) {
+  for (int i = 0; i < n; ++i) {
+    if (x[i] < 0) return true;
+  }
+  return false;
+}
+
+int check_dim(const char* who, int64_t d) {
+  if (fattn::head_dim_supported(d)) return 0;
+  return set_error(FATTN_EHEADDIM, "%s: the HIP kernels take head_dim 32, 64 or 128, got %lld", who,
+                   static_cast<long long>(d));
+}
+int check_types(const char* who, int dtype, int cache_dtype) {
+  if (!known(dtype) || !known(cache_dtype)) {
+    return set_error(FATTN_EINVAL, "%s: f32, f16 or bf16 only", who);
+  }
+  if (dtype != FATTN_F32 && cache_dtype != dtype) {
+    return set_error(FATTN_EINVAL, "%s: a cache of another type than 16-bit activations", who);
+  }
+  return 0;
+}
+int check_heads(const char* who, int64_t heads, int64_t kv_heads) {
+  if (heads < 0 || kv_heads < 0 || heads > kMaxHeads || kv_heads > kMaxHeads) {
+    return set_error(FATTN_ERANGE, "%s: at most %lld heads", who, static_cast<long long>(kMaxHeads));
+  }
+  if (kv_heads == 0 || heads % kv_heads != 0) {
+    return set_error(FATTN_EINVAL, "%s: %lld query heads are no multiple of %lld key heads", who,
+                     static_cast<long long>(heads), static_cast<long long>(kv_heads));
+  }
+  return 0;
+}
+
+// The pages, their table and the lengths of a cache; ks, vs: the strides that its indices use.
+int check_cache(const char* who, int cache_dtype, const void* k, const int64_t k_strides[3],
+                const void* v, const int64_t v_strides[3], int64_t pages, int64_t kv_heads,
+                int64_t page_size, const int32_t* table, int64_t table_stride, int64_t table_width,
+                const int32_t* lengths, int64_t ks[3], int64_t vs[3]) {
+  if (!k || !v || !k_strides || !v_strides || !table || !lengths) {
+    return set_error(FATTN_EINVAL, "%s: null operand", who);
+  }
+  if (pages <= 0 || page_size <= 0 || page_size % 16 != 0 || table_width <= 0 || table_stride < 0) {
+    return set_error(FATTN_EINVAL, "%s: pages of a multiple of 16 slots and a table of them expected, "
+                     "got %lld pages of %lld slots, a table %lld wide", who,
+                     static_cast<long long>(pages), static_cast<long long>(page_size),
+                     static_cast<long long>(table_width));
+  }
+  if (pages > INT32_MAX || page_size > INT32_MAX / 2 || table_width > INT32_MAX) {
+    return set_error(FATTN_ERANGE, "%s: the cache exceeds 32-bit indexing", who);
+  }
+  const int64_t size = size_of(cache_dtype), per = 16 / size;
+  used3(ks, k_strides, pages, kv_heads, page_size);
+  used3(vs, v_strides, pages, kv_heads, page_size);
+  if (negative(ks, 3) || negative(vs, 3)) return set_error(FATTN_EINVAL, "%s: negative strides", who);
+  if (!aligned(k, 16) || !aligned(v, 16) || !multiples(ks, per) || !multiples(vs, per)) {
+    return set_error(FATTN_EALIGN, "%s: the cache's rows must be 16-byte aligned", who);
+  }
+  if (16 * ks[2] * size > INT32_MAX || 16 * vs[2] * size > INT32_MAX) {
+    return set_error(FATTN_ERANGE, "%s: 16 slots of the cache span more than 2 GiB", who);
+  }
+  return 0;
+}
+
+// Whether an operand's rows can be moved `vec` values at a time.
+bool fits(int64_t vec, const void* p, int64_t size, const int64_t st[3], int64_t b, int64_t h, int64_t s) {
+  return aligned(p, vec * size) && (b <= 1 || st[0] % vec == 0) && (h <= 1 || st[1] % vec == 0) &&
+         (s <= 1 || st[2] % vec == 0);
+}
+
+// x / n for x below 2^31, n >= 1: (hi32(x magic) + x) >> shift.
+void divider(int64_t n, unsigned* magic, unsigned* shift) {
+  unsigned s = 0;
+  while ((int64_t{1} << s) < n) ++s;
+  *shift = s;
+  *magic = static_cast<unsigned>(((static_cast<uint64_t>(1) << 32) * ((uint64_t{1} << s) - n)) / n + 1);
+}
+
+int run_rotary(const char* who, fattn::RotaryArgs& a, int dtype, int cache_dtype, int64_t b, int64_t s,
+               int64_t d, int64_t dim, void* stream) {
+  const int64_t size = size_of(dtype);
+  // (The most pairs: what the kernel's LDS holds for one token.)
+  if (d <= 0 || d > 1024 || d % 2 != 0 || dim < 0 || dim % 2 != 0 || dim > d) {
+    return set_error(FATTN_EINVAL, "%s: an even head_dim of at most 1024 and an even part of it to turn "
+                     "expected, got %lld of %lld", who, static_cast<long long>(dim),
+                     static_cast<long long>(d));
+  }
+  if (b > kMaxGrid || s > kMaxGrid || b * s > kMaxGrid) {
+    return set_error(FATTN_ERANGE, "%s: more than %lld tokens", who, static_cast<long long>(kMaxGrid));
+  }
+  if (dim > 0 && !a.frequencies) return set_error(FATTN_EINVAL, "%s: null frequencies", who);
+  a.B = static_cast<int>(b), a.S = static_cast<int>(s), a.D = static_cast<int>(d);
+  a.pairs = static_cast<int>(dim / 2);
+  int64_t vec = 16 / size;
+  auto allowed = [&](int64_t v) {
+    if (d % v != 0 || (a.interleaved ? dim : dim / 2) % v != 0) return false;
+    for (int i = 0; i < 3; ++i) {
+      const fattn::RotaryPart& p = a.part[i];
+      if (p.heads == 0) continue;
+      if (!fits(v, p.x, size, p.xs, b, p.heads, s)) return false;
+      if (a.table == nullptr || i == 0) {
+        if (!fits(v, p.y, size, p.ys, b, p.heads, s)) return false;
+      }  // (the pages' rows are 16-byte aligned)
+    }
+    return true;
+  };
+  while (vec >= 4 && !allowed(vec)) vec /= 2;
+  if (vec < 4) vec = a.interleaved ? 2 : 1;
+  const int err = fattn::launch_rotary(a, dtype, cache_dtype, static_cast<int>(vec), stream);
+  if (err) return fattn::hip_error(err, who, "launch");
+  return fattn::done();
+}
+
+// Shared by the paged and the cross attention: the plan, the workspace, the launch.
+int run_split(const char* who, fattn::SplitArgs& a, int dtype, int cache_dtype, int64_t d,
+              int64_t capacity, void* workspace, size_t workspace_bytes, void* stream) {
+  const int64_t rows = static_cast<int64_t>(a.G) * a.SQ;
+  const fattn::SplitPlan plan = fattn::split_plan(a.B, a.HK, rows, d, capacity);
+  if (static_cast<int64_t>(a.B) * a.HK * plan.row_blocks > kMaxGrid ||
+      static_cast<int64_t>(a.B) * a.H * a.SQ > kMaxGrid) {
+    return set_error(FATTN_ERANGE, "%s: the grid exceeds the launch limit", who);
+  }
+  if (plan.bytes > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < plan.bytes)) {
+    return set_error(FATTN_EWORKSPACE, "%s: a 16-byte aligned workspace of at least %zu bytes expected",
+                     who, plan.bytes);
+  }
+  a.RB = plan.row_blocks, a.part_rows = plan.part_rows, a.wgs = plan.wgs, a.min_run = plan.min_run;
+  a.part = static_cast<float*>(workspace);
+  const int err = fattn::launch_split(a, dtype, cache_dtype, static_cast<int>(d), stream);
+  if (err) return fattn::hip_error(err, who, "launch");
+  return fattn::done();
+}
+
+bool split_shape(int64_t b, int64_t heads, int64_t kv_heads, int64_t d) {
+  return b >= 0 && heads >= 0 && kv_heads > 0 && heads % kv_heads == 0 && fattn::head_dim_supported(d);
+}
+
+}  // namespace
+
+extern "C" {
+
+int fattn_rotary(int dtype, int64_t b, int64_t s, int64_t d, const int64_t heads[3],
+                 const void* const x[3], void* const y[3], const int64_t x_strides[9],
+                 const int64_t y_strides[9], int rotated, const void* positions, int position_bits,
+                 const int64_t position_strides[2], const double* frequencies, int64_t dim,
+                 int interleaved, double magnitude, int inverse, void* stream) {
+  const char* who = "fused_rotary";
+  if (!known(dtype)) return set_error(FATTN_EINVAL, "%s: f32, f16 or bf16 only", who);
+  if (b < 0 || s < 0 || !heads || !x || !y || !x_strides || !y_strides || !position_strides ||
+      (position_bits != 32 && position_bits != 64)) {
+    return set_error(FATTN_EINVAL, "%s: [b, heads, s, d] operands and positions of 32 or 64 bits expected",
+                     who);
+  }
+  fattn::RotaryArgs a{};
+  int64_t all = 0;
+  for (int i = 0; i < 3; ++i) {
+    if (heads[i] < 0 || heads[i] > kMaxHeads) {
+      return set_error(FATTN_ERANGE, "%s: at most %lld heads", who, static_cast<long long>(kMaxHeads));
+    }
+    all += heads[i];
+    fattn::RotaryPart& p = a.part[i];
+    p.heads = static_cast<int>(heads[i]);
+    p.rotate = (rotated >> i) & 1;
+    if (heads[i] == 0) continue;
+    p.x = x[i], p.y = y[i];
+    copy3(p.xs, x_strides + 3 * i);
+    copy3(p.ys, y_strides + 3 * i);
+    if (negative(p.xs, 3) || negative(p.ys, 3)) return set_error(FATTN_EINVAL, "%s: negative strides", who);
+  }
+  if (b == 0 || s == 0 || all == 0) return fattn::done();
+  for (int i = 0; i < 3; ++i) {
+    if (heads[i] > 0 && (!x[i] || !y[i])) return set_error(FATTN_EINVAL, "%s: null operand", who);
+  }
+  if (!positions) return set_error(FATTN_EINVAL, "%s: null positions", who);
+  a.positions = positions, a.pos64 = position_bits == 64;
+  a.pos_strides[0] = position_strides[0], a.pos_strides[1] = position_strides[1];
+  a.frequencies = frequencies, a.magnitude = magnitude;
+  a.interleaved = interleaved ? 1 : 0, a.inverse = inverse ? 1 : 0;
+  return run_rotary(who, a, dtype, dtype, b, s, d, dim, stream);
+}
+
+int fattn_paged_append(int dtype, int cache_dtype, int64_t b, int64_t heads, int64_t kv_heads,
+                       int64_t s, int64_t d, const void* q, const int64_t q_strides[3], void* q_out,
+                       const int64_t q_out_strides[3], const void* k, const int64_t k_strides[3],
+                       const void* v, const int64_t v_strides[3], void* k_pages,
+                       const int64_t k_page_strides[3], void* v_pages,
+                       const int64_t v_page_strides[3], int64_t pages, int64_t page_size,
+                       const int32_t* table, int64_t table_stride, int64_t table_width,
+                       const int32_t* lengths, const int32_t* counts, const double* frequencies,
+                       int64_t dim, int interleaved, double magnitude, void* stream) {
+  const char* who = "paged_append";
+  if (int rc = check_types(who, dtype, cache_dtype)) return rc;
+  if (b < 0 || s < 0) return set_error(FATTN_EINVAL, "%s: negative size", who);
+  if (int rc = check_heads(who, heads, kv_heads)) return rc;
+  if (int rc = check_dim(who, d)) return rc;
+  if (b == 0 || s == 0) return fattn::done();
+  fattn::RotaryArgs a{};
+  if (int rc = check_cache(who, cache_dtype, k_pages, k_page_strides, v_pages, v_page_strides, pages,
+                           kv_heads, page_size, table, table_stride, table_width, lengths,
+                           a.page_strides, a.page_strides + 3)) {
+    return rc;
+  }
+  if (!k || !v || !k_strides || !v_strides || (heads > 0 && (!q || !q_out || !q_strides || !q_out_strides))) {
+    return set_error(FATTN_EINVAL, "%s: null operand", who);
+  }
+  const int turned = frequencies != nullptr ? 1 : 0;
+  a.part[0].heads = static_cast<int>(heads), a.part[0].rotate = turned;
+  if (heads > 0) {
+    a.part[0].x = q, a.part[0].y = q_out;
+    copy3(a.part[0].xs, q_strides);
+    copy3(a.part[0].ys, q_out_strides);
+  }
+  a.part[1] = fattn::RotaryPart{k, k_pages, {}, {}, static_cast<int>(kv_heads), turned};
+  copy3(a.part[1].xs, k_strides);
+  a.part[2] = fattn::RotaryPart{v, v_pages, {}, {}, static_cast<int>(kv_heads), 0};
+  copy3(a.part[2].xs, v_strides);
+  for (const fattn::RotaryPart& p : a.part) {
+    if (negative(p.xs, 3) || negative(p.ys, 3)) return set_error(FATTN_EINVAL, "%s: negative strides", who);
+  }
+  a.frequencies = frequencies, a.magnitude = magnitude, a.interleaved = interleaved ? 1 : 0;
+  a.table = table, a.lengths = lengths, a.counts = counts;
+  a.table_stride = table_stride, a.table_width = table_width, a.pages = pages, a.page_size = page_size;
+  return run_rotary(who, a, dtype, cache_dtype, b, s, d, turned ? dim : 0, stream);
+}
+
+size_t fattn_paged_attention_workspace_bytes(int64_t b, int64_t heads, int64_t kv_heads, int64_t d,
+                                             int64_t capacity) {
+  if (!split_shape(b, heads, kv_heads, d) || capacity < 0) return 0;
+  return fattn::split_plan(b, kv_heads, heads / kv_heads, d, capacity).bytes;
+}
+
+int fattn_paged_attention(int dtype, int cache_dtype, int64_t b, int64_t heads, int64_t kv_heads,
+                          int64_t d, const void* q, const int64_t q_strides[2], void* out,
+                          const void* k_pages, const int64_t k_page_strides[3], const void* v_pages,
+                          const int64_t v_page_strides[3], int64_t pages, int64_t page_size,
+                          const int32_t* table, int64_t table_stride, int64_t table_width,
+                          const int32_t* lengths, float scale, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  const char* who = "paged_attention";
+  if (int rc = check_types(who, dtype, cache_dtype)) return rc;
+  if (b < 0) return set_error(FATTN_EINVAL, "%s: negative size", who);
+  if (int rc = check_heads(who, heads, kv_heads)) return rc;
+  if (int rc = check_dim(who, d)) return rc;
+  if (b == 0 || heads == 0) return fattn::done();
+  fattn::SplitArgs a{};
+  if (int rc = check_cache(who, cache_dtype, k_pages, k_page_strides, v_pages, v_page_strides, pages,
+                           kv_heads, page_size, table, table_stride, table_width, lengths, a.ks, a.vs)) {
+    return rc;
+  }
+  if (!q || !out || !q_strides) return set_error(FATTN_EINVAL, "%s: null operand", who);
+  const int64_t q3[3] = {q_strides[0], q_strides[1], 0};
+  used3(a.qs, q3, b, heads, 1);
+  if (negative(a.qs, 2)) return set_error(FATTN_EINVAL, "%s: negative strides", who);
+  if (!aligned(q, 16) || !aligned(out, 16) || !multiples(a.qs, 16 / size_of(dtype))) {
+    return set_error(FATTN_EALIGN, "%s: rows must be 16-byte aligned", who);
+  }
+  const int64_t capacity = table_width * page_size;
+  if (b > INT32_MAX || capacity > INT32_MAX - 64) {
+    return set_error(FATTN_ERANGE, "%s: the cache exceeds 32-bit indexing", who);
+  }
+  a.q = q, a.o = out;
+  a.k = k_pages, a.v = v_pages;
+  a.table = table, a.table_stride = table_stride, a.lengths = lengths;
+  a.page_size = static_cast<int>(page_size), a.pages = static_cast<int>(pages);
+  divider(page_size / 16, &a.div_magic, &a.div_shift);
+  a.B = static_cast<int>(b), a.H = static_cast<int>(heads), a.HK = static_cast<int>(kv_heads);
+  a.G = static_cast<int>(heads / kv_heads), a.SQ = 1, a.SK = static_cast<int>(capacity);
+  a.scale = scale;
+  return run_split(who, a, dtype, cache_dtype, d, capacity, workspace, workspace_bytes, stream);
+}
+
+size_t fattn_cross_workspace_bytes(int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk,
+                                   int64_t d) {
+  if (!split_shape(b, heads, kv_heads, d) || sq < 0 || sk < 0) return 0;
+  return fattn::split_plan(b, kv_heads, heads / kv_heads * sq, d, sk).bytes;
+}
+
+int fattn_cross_forward(const float* q, const int64_t q_strides[3], const float* k,
+                        const int64_t k_strides[3], const float* v, const int64_t v_strides[3],
+                        int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d,
+                        const int32_t* key_lengths, float scale, float* out, float* lse,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "fused_cross_attention";
+  if (b < 0 || sq < 0 || sk < 0) return set_error(FATTN_EINVAL, "%s: negative size", who);
+  if (int rc = check_heads(who, heads, kv_heads)) return rc;
+  if (int rc = check_dim(who, d)) return rc;
+  if (b == 0 || heads == 0 || sq == 0) return fattn::done();
+  if (!q || !out || !lse || !q_strides || (sk > 0 && (!k || !v || !k_strides || !v_strides))) {
+    return set_error(FATTN_EINVAL, "%s: null operand", who);
+  }
+  fattn::SplitArgs a{};
+  used3(a.qs, q_strides, b, heads, sq);
+  if (sk > 0) {
+    used3(a.ks, k_strides, b, kv_heads, sk);
+    used3(a.vs, v_strides, b, kv_heads, sk);
+  }
+  if (negative(a.qs, 3) || negative(a.ks, 3) || negative(a.vs, 3)) {
+    return set_error(FATTN_EINVAL, "%s: negative strides", who);
+  }
+  if (!aligned(q, 16) || !aligned(out, 16) || (sk > 0 && (!aligned(k, 16) || !aligned(v, 16))) ||
+      !multiples(a.qs, 4) || !multiples(a.ks, 4) || !multiples(a.vs, 4)) {
+    return set_error(FATTN_EALIGN, "%s: rows must be 16-byte aligned", who);
+  }
+  if (b > INT32_MAX || sq > INT32_MAX / kMaxHeads || sk > INT32_MAX - 64) {
+    return set_error(FATTN_ERANGE, "%s: the sizes exceed 32-bit indexing", who);
+  }
+  if (16 * 4 * a.ks[2] > INT32_MAX || 16 * 4 * a.vs[2] > INT32_MAX) {
+    return set_error(FATTN_ERANGE, "%s: 16 keys span more than 2 GiB", who);
+  }
+  a.q = q, a.k = k, a.v = v, a.o = out, a.lse = lse;
+  a.lengths = key_lengths;
+  a.B = static_cast<int>(b), a.H = static_cast<int>(heads), a.HK = static_cast<int>(kv_heads);
+  a.G = static_cast<int>(heads / kv_heads), a.SQ = static_cast<int>(sq), a.SK = static_cast<int>(sk);
+  a.scale = scale;
+  return run_split(who, a, FATTN_F32, FATTN_F32, d, sk, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

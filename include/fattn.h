@@ -211,6 +211,75 @@ int fattn_backward(const float* q, int64_t q_offset, const int64_t q_shape[4],
                    size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Operators around self-attention: rotary positions, a paged key-value cache, cross attention.
+ * None has a counterpart in the reference. Element types are FATTN_F32, FATTN_F16, FATTN_BF16;
+ * strides are in elements, head_dim contiguous. Messages are prefixed with the operator's name
+ * (`fused_rotary:`, `paged_append:`, `paged_attention:`, `fused_cross_attention:`).
+ * ------------------------------------------------------------------------------------------ */
+#define FATTN_F32 0
+#define FATTN_F16 1
+#define FATTN_BF16 2
+
+/* Rotary positions on up to three [b, heads, s, d] operands of one type (d even, at most 1024;
+ * heads[i] 0: absent; strides {batch, head, seq}, three of each operand): y = x, but with bit i of
+ * `rotated` the first `dim` (even) values of operand i's heads in pairs (i, i + dim / 2), or
+ * (2 i, 2 i + 1) with `interleaved`, times `magnitude` and turned by the angle position x
+ * frequencies[i] (radians, formed in 64 bits), or back by it with `inverse` (the gradient).
+ * positions: [b, s] through their strides, position_bits 32 or 64. y may be x itself. */
+int fattn_rotary(int dtype, int64_t b, int64_t s, int64_t d, const int64_t heads[3],
+                 const void* const x[3], void* const y[3], const int64_t x_strides[9],
+                 const int64_t y_strides[9], int rotated, const void* positions, int position_bits,
+                 const int64_t position_strides[2], const double* frequencies, int64_t dim,
+                 int interleaved, double magnitude, int inverse, void* stream);
+
+/* Appends up to s new tokens per sequence to a paged cache: token i < counts[b] (counts NULL: all s)
+ * is token lengths[b] + i of sequence b, and goes to slot t % page_size of page
+ * table[b][t / page_size] of k_pages and v_pages ([pages, kv_heads, page_size, d], page_strides
+ * {page, head, slot}), rounded to cache_dtype (the activations' type, or any for fp32 ones). Keys are
+ * turned as by fattn_rotary at position t (frequencies NULL: not), and so is q ([b, heads, s, d],
+ * heads 0: absent) into q_out, in all s rows. A token whose page the table ([b, table_width], row
+ * stride table_stride) or the cache does not have is not written; nor is anything else. page_size is
+ * a multiple of 16, d 32, 64 or 128. */
+int fattn_paged_append(int dtype, int cache_dtype, int64_t b, int64_t heads, int64_t kv_heads,
+                       int64_t s, int64_t d, const void* q, const int64_t q_strides[3], void* q_out,
+                       const int64_t q_out_strides[3], const void* k, const int64_t k_strides[3],
+                       const void* v, const int64_t v_strides[3], void* k_pages,
+                       const int64_t k_page_strides[3], void* v_pages,
+                       const int64_t v_page_strides[3], int64_t pages, int64_t page_size,
+                       const int32_t* table, int64_t table_stride, int64_t table_width,
+                       const int32_t* lengths, const int32_t* counts, const double* frequencies,
+                       int64_t dim, int interleaved, double magnitude, void* stream);
+
+/* Attention of one token per sequence over its first lengths[b] cached tokens: q [b, heads, d]
+ * (strides {batch, head}), out [b, heads, d] contiguous, query head i reading key head
+ * i / (heads / kv_heads). A sequence of length 0 gives 0; one whose length is negative or more than
+ * table_width x page_size, or that names a page the cache does not have, gives NaN. The workspace
+ * (16-byte aligned, nothing kept in it between calls; its size may be 0, then NULL) takes the partial
+ * sums of keys that several workgroups share; capacity is table_width x page_size. Pages' strides and
+ * base are multiples of 16 bytes. Reruns are bit-identical. */
+size_t fattn_paged_attention_workspace_bytes(int64_t b, int64_t heads, int64_t kv_heads, int64_t d,
+                                             int64_t capacity);
+int fattn_paged_attention(int dtype, int cache_dtype, int64_t b, int64_t heads, int64_t kv_heads,
+                          int64_t d, const void* q, const int64_t q_strides[2], void* out,
+                          const void* k_pages, const int64_t k_page_strides[3], const void* v_pages,
+                          const int64_t v_page_strides[3], int64_t pages, int64_t page_size,
+                          const int32_t* table, int64_t table_stride, int64_t table_width,
+                          const int32_t* lengths, float scale, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* Cross attention, fp32: q [b, heads, sq, d] to k, v [b, kv_heads, sk, d] (strides {batch, head, seq},
+ * rows 16-byte aligned), of which sample b sees the first key_lengths[b] (NULL: all; a length outside
+ * [0, sk] counts as the nearest). out [b, sq, heads, d] contiguous, lse [b, heads, sq]; a sample that
+ * sees no key has out 0 and lse -infinity. Query head i reads key head i / (heads / kv_heads). */
+size_t fattn_cross_workspace_bytes(int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk,
+                                   int64_t d);
+int fattn_cross_forward(const float* q, const int64_t q_strides[3], const float* k,
+                        const int64_t k_strides[3], const float* v, const int64_t v_strides[3],
+                        int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d,
+                        const int32_t* key_lengths, float scale, float* out, float* lse,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Diagnostics (no counterpart in the reference).
  * ------------------------------------------------------------------------------------------ */
 

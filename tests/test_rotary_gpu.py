@@ -1,0 +1,222 @@
+"""Rotary positions on the GPU against the formula in 64 bits: layouts, partial heads, types, far
+positions, strides, gradients (against the formula's, and against differences), graphs.
+
+Tolerance: y = x0 c - x1 s takes four roundings of 2^-24 (c, s, a product, the sum), each of at most
+(|x0| + |x1|) magnitude, and half a step of a 16-bit result."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import candle_fused_attn as cfa
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def formula(x, positions, f, interleaved, magnitude=1.0, sign=1.0):
+    """x [b, h, s, d] turned, 64 bits on the CPU."""
+    x, f = x.double().cpu(), f.cpu()
+    pos = positions.cpu().double()
+    a = (pos if pos.dim() == 2 else pos[None])[:, None, :, None] * f
+    n = f.numel()
+    i, j = (slice(0, 2 * n, 2), slice(1, 2 * n, 2)) if interleaved else (slice(0, n), slice(n, 2 * n))
+    c, s, y = magnitude * a.cos(), sign * magnitude * a.sin(), x.clone()
+    y[..., i], y[..., j] = x[..., i] * c - x[..., j] * s, x[..., j] * c + x[..., i] * s
+    return y
+
+
+def near(got, ref, x, magnitude=1.0):
+    eps = 0.0 if got.dtype == torch.float32 else torch.finfo(got.dtype).eps / 2
+    size = 2 * max(1.0, magnitude) * x.double().cpu().abs().amax(-1, keepdim=True)
+    err = (got.double().cpu() - ref).abs()
+    tiny = 2.0 ** -25 if got.dtype == torch.float16 else 0.0  # half a step of subnormal f16
+    assert bool((err <= 4 * 2.0 ** -24 * size + eps * 1.0001 * ref.abs() + tiny).all()), float(err.max())
+
+
+def operands(dev, dtype, b, h, hk, s, d, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    return [torch.randn(b, s, n, d, generator=gen).to(dtype).to(dev).transpose(1, 2) for n in (h, hk)]
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("d,dim", [(64, 64), (128, 64), (32, 8), (80, 20), (96, 2), (64, 0), (10, 6)])
+def test_forward(cuda, dtype, d, dim, interleaved):
+    b, h, hk, s = 2, 5, 2, 37
+    q, k = operands(cuda, dtype, b, h, hk, s, d)
+    f = cfa.rotary_frequencies(dim, device=cuda) if dim else torch.empty(0, dtype=torch.float64,
+                                                                         device=cuda)
+    pos = torch.randint(0, 5000, (b, s), device=cuda)
+    for magnitude in (1.0, 1.3):
+        got = cfa.fused_rotary(q, k, pos, f, interleaved, magnitude)
+        for x, y in zip((q, k), got):
+            assert y.dtype == dtype and y.shape == x.shape
+            near(y, formula(x, pos, f, interleaved, magnitude), x, magnitude)
+
+
+@pytest.mark.parametrize("b,h,hk,s", [(1, 1, 1, 1), (1, 32, 8, 1), (64, 6, 6, 1), (3, 1, 1, 1000),
+                                      (1, 70, 3, 129), (40, 2, 2, 100)])
+def test_sizes(cuda, b, h, hk, s):
+    q, k = operands(cuda, torch.float32, b, h, hk, s, 64, seed=1)
+    f, pos = cfa.rotary_frequencies(64, device=cuda), torch.arange(s, device=cuda, dtype=torch.int32)
+    for x, y in zip((q, k), cfa.fused_rotary(q, k, pos, f)):
+        near(y, formula(x, pos, f, False), x)
+
+
+def test_far_positions(cuda):
+    """Angles to 1e9 radians, either sign: the 64-bit product's half step, 2^-53 of the angle, is 1e-7."""
+    q, k = operands(cuda, torch.float32, 1, 2, 1, 6, 64, seed=2)
+    f = cfa.rotary_frequencies(64, device=cuda)
+    pos = torch.tensor([[0, 131071, -131071, 2 ** 24 + 1, 10 ** 7, -(10 ** 9)]], device=cuda)
+    for x, y in zip((q, k), cfa.fused_rotary(q, k, pos, f)):
+        err = (y.double().cpu() - formula(x, pos, f, False)).abs()
+        assert float(err.max()) <= 5 * (4 * 2.0 ** -24 * 2 + 3 * 1.2e-7 * 2)
+
+
+def test_layouts(cuda):
+    """Contiguous heads, padded rows, broadcast operands, odd offsets, a head_dim that is not contiguous:
+    the same values bit for bit."""
+    b, h, s, d = 2, 3, 20, 64
+    q, k = operands(cuda, torch.float32, b, h, h, s, d, seed=3)
+    f, pos = cfa.rotary_frequencies(32, device=cuda), torch.arange(s, device=cuda)
+    want = cfa.fused_rotary(q, k, pos, f)
+    padded = torch.zeros(b, h, s, d + 5, device=cuda)
+    padded[..., 1:d + 1] = q
+    for x in (q.contiguous(), padded[..., 1:d + 1], q.permute(3, 2, 1, 0).contiguous().permute(3, 2, 1, 0)):
+        got = cfa.fused_rotary(x, k, pos, f)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    got = cfa.fused_rotary(q, k[:, :1].expand(b, h, s, d), pos[None].expand(b, s), f)
+    assert torch.equal(got[1], want[1][:, :1].expand(b, h, s, d))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_gradients(cuda, dtype, interleaved):
+    """Each operand's gradient is its output's, turned back; an operand that needs none has none, an
+    output without a gradient gives none."""
+    q, k = operands(cuda, dtype, 2, 4, 2, 33, 64, seed=4)
+    gq, gk = operands(cuda, dtype, 2, 4, 2, 33, 64, seed=5)
+    f, pos = cfa.rotary_frequencies(64, device=cuda), torch.arange(100, 133, device=cuda)
+    q.requires_grad_(), k.requires_grad_()
+    yq, yk = cfa.fused_rotary(q, k, pos, f, interleaved, 1.1)
+    dq, dk = torch.autograd.grad((yq, yk), (q, k), (gq, gk))
+    near(dq, formula(gq, pos, f, interleaved, 1.1, -1.0), gq, 1.1)
+    near(dk, formula(gk, pos, f, interleaved, 1.1, -1.0), gk, 1.1)
+    yq, yk = cfa.fused_rotary(q, k.detach(), pos, f, interleaved, 1.1)
+    assert not torch.equal(yk, k) and torch.equal(torch.autograd.grad(yq, q, gq)[0], dq)
+    yq, yk = cfa.fused_rotary(q, k, pos, f, interleaved, 1.1)
+    assert torch.equal(torch.autograd.grad(yk, k, gk)[0], dk)
+    yq, yk = cfa.fused_rotary(q, k, pos, f, interleaved, 1.1)
+    assert torch.equal(torch.autograd.grad(yq, q, gq[:, :1].expand_as(gq))[0][:, 0], dq[:, 0])
+
+
+def test_gradient_against_differences(cuda):
+    """The loss is linear in q: its change under a step is the gradient's product with the step."""
+    q, k = operands(cuda, torch.float32, 1, 2, 2, 9, 32, seed=6)
+    g, step = operands(cuda, torch.float32, 1, 2, 2, 9, 32, seed=7)
+    f, pos = cfa.rotary_frequencies(32, device=cuda), torch.arange(9, device=cuda)
+    q.requires_grad_()
+    out = cfa.fused_rotary(q, k, pos, f)[0]
+    (dq,) = torch.autograd.grad(out, q, g, create_graph=True)
+    more = cfa.fused_rotary(q.detach() + step, k, pos, f)[0]
+    change = float(((more - out).double() * g).sum())
+    # 1152 values of about 1, each off by 8 x 2^-24 or less.
+    assert abs(change - float((dq.double() * step).sum())) <= 1152 * 8 * 2.0 ** -24
+    assert dq.requires_grad is False or dq.grad_fn is not None
+
+
+def test_gradient_of_the_gradient(cuda):
+    """The gradient is linear in the output's gradient, and differentiable in it."""
+    q, k = operands(cuda, torch.float32, 1, 2, 2, 5, 32, seed=8)
+    g, u = operands(cuda, torch.float32, 1, 2, 2, 5, 32, seed=9)
+    f, pos = cfa.rotary_frequencies(32, device=cuda), torch.arange(5, device=cuda)
+    q.requires_grad_(), g.requires_grad_()
+    out = cfa.fused_rotary(q, k, pos, f)[0]
+    (dq,) = torch.autograd.grad(out, q, g, create_graph=True)
+    (dg,) = torch.autograd.grad(dq, g, u)
+    assert torch.equal(dg, cfa.fused_rotary(u, k, pos, f)[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_projection(cuda, dtype):
+    """fused_rotary_qkv: q and k of the projection as fused_rotary turns them, v as it is, one gradient;
+    a projection whose last dimension is not contiguous is copied."""
+    b, s, h, d = 3, 50, 4, 64
+    x = torch.randn(b, s, 3 * h * d, device=cuda).to(dtype)
+    f, pos = cfa.rotary_frequencies(d, device=cuda), torch.randint(0, 999, (b, s), device=cuda)
+    q, k, v = (t.transpose(1, 2) for t in x.view(b, s, 3, h, d).unbind(2))
+    want = torch.stack([t.transpose(1, 2) for t in (*cfa.fused_rotary(q, k, pos, f), v)], 2).view(b, s, -1)
+    x.requires_grad_()
+    out = cfa.fused_rotary_qkv(x, h, pos, f)
+    assert torch.equal(out, want)
+    g = torch.randn_like(x)
+    (dx,) = torch.autograd.grad(out, x, g)
+    dq, dk, dv = (t.transpose(1, 2) for t in dx.view(b, s, 3, h, d).unbind(2))
+    gq, gk, gv = (t.transpose(1, 2) for t in g.view(b, s, 3, h, d).unbind(2))
+    near(dq, formula(gq, pos, f, False, 1.0, -1.0), gq)
+    near(dk, formula(gk, pos, f, False, 1.0, -1.0), gk)
+    assert torch.equal(dv, gv)
+    y = x.detach().transpose(0, 2).contiguous().transpose(0, 2)
+    assert torch.equal(cfa.fused_rotary_qkv(y, h, pos, f), want)
+    wide = torch.zeros(b, s, 3 * h * d + 7, device=cuda, dtype=dtype)
+    wide[..., 3:-4] = x.detach()
+    assert torch.equal(cfa.fused_rotary_qkv(wide[..., 3:-4], h, pos, f), want)
+
+
+def test_projection_into_attention(cuda):
+    """fused_rotary_qkv into fused_attention_qkv, against the two plain formulas with torch's autograd."""
+    b, s, h, d = 2, 65, 2, 64
+    x = torch.randn(b, s, 3 * h * d, device=cuda, requires_grad=True)
+    f, pos = cfa.rotary_frequencies(d, device=cuda), torch.arange(s, device=cuda)
+    g = torch.randn(b, s, h * d, device=cuda)
+    out = cfa.fused_attention_qkv(cfa.fused_rotary_qkv(x, h, pos, f), h, 0.125, True)
+    (dx,) = torch.autograd.grad(out, x, g)
+    y = x.detach().double().cpu().requires_grad_()
+    q, k, v = (t.transpose(1, 2) for t in y.view(b, s, 3, h, d).unbind(2))
+    a = pos.cpu().double()[:, None] * f.cpu()
+
+    def turn(t):
+        i, j = t[..., :32], t[..., 32:]
+        return torch.cat((i * a.cos() - j * a.sin(), j * a.cos() + i * a.sin()), -1)
+
+    w = torch.matmul(turn(q), turn(k).transpose(2, 3)) * 0.125
+    w = torch.softmax(w.masked_fill(torch.ones(s, s, dtype=torch.bool).triu(1), -math.inf), -1)
+    ref = torch.matmul(w, v).transpose(1, 2).reshape(b, s, h * d)
+    (dref,) = torch.autograd.grad(ref, y, g.double().cpu())
+    for got, want in ((out, ref), (dx, dref)):
+        assert float((got.double().cpu() - want).norm() / want.norm()) <= 2e-6
+
+
+def test_captured(cuda):
+    q, k = operands(cuda, torch.float32, 2, 4, 2, 17, 64, seed=10)
+    f, pos = cfa.rotary_frequencies(64, device=cuda), torch.zeros(2, 17, dtype=torch.int64, device=cuda)
+    cfa.fused_rotary(q, k, pos, f)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = cfa.fused_rotary(q, k, pos, f)
+    for i in range(3):
+        pos.random_(0, 10000), q.normal_()
+        graph.replay()
+        want = cfa.fused_rotary(q, k, pos, f)
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_empty(cuda):
+    f, pos = cfa.rotary_frequencies(64, device=cuda), torch.zeros(0, dtype=torch.int64, device=cuda)
+    q, k = operands(cuda, torch.float32, 2, 4, 2, 0, 64)
+    assert [list(y.shape) for y in cfa.fused_rotary(q, k, pos, f)] == [[2, 4, 0, 64], [2, 2, 0, 64]]
+
+
+@pytest.mark.parametrize("scaling", [None, "linear", "base", "ramp"])
+def test_scaled_frequencies(cuda, scaling):
+    f = cfa.rotary_frequencies(64, scaling=scaling, factor=4.0, device=cuda)
+    q, k = operands(cuda, torch.bfloat16, 1, 2, 2, 9, 64, seed=11)
+    pos = torch.arange(70000, 70009, device=cuda)
+    for x, y in zip((q, k), cfa.fused_rotary(q, k, pos, f, True)):
+        near(y, formula(x, pos, f, True), x)

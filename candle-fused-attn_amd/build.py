@@ -21,9 +21,10 @@ REPO = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "lib"
 LIB = LIB_DIR / "libfattn.so"
-SOURCES = [CSRC / "fattn_pair.hip", CSRC / "fattn_paged.hip", CSRC / "fattn_rotary.hip",
+SOURCES = [CSRC / "fattn_pair.hip", CSRC / "fattn_cross.hip", CSRC / "fattn_paged.hip", CSRC / "fattn_rotary.hip",
            CSRC / "fattn_kernels.hip", CSRC / "fattn_api.cpp", CSRC / "fattn_operators.cpp"]
-HEADERS = [REPO / "include" / "fattn.h", CSRC / "fattn_internal.h", CSRC / "fattn_device.h"]
+HEADERS = [REPO / "include" / "fattn.h", CSRC / "fattn_internal.h", CSRC / "fattn_device.h",
+           CSRC / "fattn_pair_kernels.h"]
 # The C++ op layer over the C ABI (the reference's src/lib.rs ops for C++ callers), linked
 # against libfattn.so, and its test program (links the CPU oracle; test infrastructure).
 HOST = PKG_DIR / "host"

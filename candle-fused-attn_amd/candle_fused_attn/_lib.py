@@ -48,6 +48,7 @@ EXPORTS = (
     "fattn_paged_attention",
     "fattn_cross_workspace_bytes",
     "fattn_cross_forward",
+    "fattn_cross_backward",
     "fattn_last_error",
     "fattn_version",
     "fattn_bwd_status",
@@ -118,6 +119,8 @@ def _declare(L: ctypes.CDLL) -> None:
     L.fattn_cross_workspace_bytes.restype = SIZE
     L.fattn_cross_forward.argtypes = [P, A3, P, A3, P, A3, I64, I64, I64, I64, I64, I64, P, C_FLOAT,
                                       P, P, P, SIZE, P]
+    L.fattn_cross_backward.argtypes = [P, A3, P, A3, P, A3, I64, I64, I64, I64, I64, I64, P, C_FLOAT,
+                                       P, P, P, A3, P, P, P]
     L.fattn_bwd_status.argtypes = [P, SIZE, I64, I64, I64, P, ctypes.POINTER(C_INT)]
     for name in EXPORTS:
         if name not in ("fattn_last_error", "fattn_version") and "workspace" not in name:

@@ -6,9 +6,10 @@ lengths in place of a mask.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._call import aligned_rows, launch, require, strides3
+from ._call import A3, aligned_rows, launch, require, strides3
 from ._lib import FusedAttentionError
 
 _F32 = (torch.float32,)
@@ -28,6 +29,34 @@ def _forward(q, k, v, scale, key_lengths):
            key_lengths.data_ptr() if key_lengths is not None else None, scale, out.data_ptr(),
            lse.data_ptr(), ws.data_ptr() if size else None, size)
     return out, lse
+
+
+class _FusedCrossAttention(torch.autograd.Function):
+    """[b, h, sq, d] and [b, kv_heads, sk, d] in, the raw [b, sq, h, d] output out."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, scale, key_lengths):
+        out, lse = _forward(q, k, v, scale, key_lengths)
+        ctx.save_for_backward(q, k, v, key_lengths, out, lse)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        q, k, v, key_lengths, out, lse = ctx.saved_tensors
+        grad = aligned_rows(grad)
+        b, h, sq, d = q.shape
+        hk, sk = k.shape[1], k.shape[2]
+        dq = torch.empty((b, sq, h, d), dtype=torch.float32, device=q.device)
+        dkv = torch.empty((b, sk, 2, hk, d), dtype=torch.float32, device=q.device)
+        gb, gs, gh, _ = grad.stride()
+        launch(q, _lib.lib().fattn_cross_backward, q.data_ptr(), strides3(q), k.data_ptr(), strides3(k),
+               v.data_ptr(), strides3(v), b, h, hk, sq, sk, d,
+               key_lengths.data_ptr() if key_lengths is not None else None, ctx.scale, out.data_ptr(),
+               lse.data_ptr(), grad.data_ptr(), A3(gb, gh, gs), dq.data_ptr(), dkv.data_ptr())
+        return (dq.transpose(1, 2), dkv[:, :, 0].transpose(1, 2), dkv[:, :, 1].transpose(1, 2), None,
+                None)
 
 
 def fused_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
@@ -53,7 +82,7 @@ def fused_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sca
         if key_lengths.shape[0] != b or not key_lengths.is_contiguous():
             raise FusedAttentionError(f"{who}: contiguous key_lengths [{b}] expected, got "
                                       f"{list(key_lengths.shape)}")
+    q, k, v = aligned_rows(q), aligned_rows(k), aligned_rows(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        raise FusedAttentionError(f"{who}: not differentiable yet")
-    return _forward(aligned_rows(q), aligned_rows(k), aligned_rows(v), float(scale),
-                    key_lengths)[0].transpose(1, 2)
+        return _FusedCrossAttention.apply(q, k, v, float(scale), key_lengths).transpose(1, 2)
+    return _forward(q, k, v, float(scale), key_lengths)[0].transpose(1, 2)

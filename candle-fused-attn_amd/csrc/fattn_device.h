@@ -68,6 +68,9 @@ struct FwdArgs {
   int B, H, S, nqb;
   float scale;
   int causal;
+  // Cross attention: the keys' length, query heads per key head, each sample's keys (null: SK).
+  int SK, G;
+  const int32_t* key_lengths;
 };
 
 }  // namespace

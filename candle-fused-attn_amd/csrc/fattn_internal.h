@@ -223,6 +223,17 @@ struct SplitPlan {
 SplitPlan split_plan(int64_t b, int64_t hk, int64_t rows, int64_t d, int64_t capacity);
 int launch_split(const SplitArgs& a, int dtype, int cache_dtype, int d, void* stream);
 
+// Cross attention by blocks of 128 queries and 128 keys (fattn_cross.hip). dq [b, sq, h, d], dkv
+// [b, sk, 2, hk, d].
+int launch_cross_forward(View q, View k, View v, float* o, float* lse, int b, int h, int hk, int sq,
+                         int sk, int d, const int32_t* key_lengths, float scale, void* stream);
+int launch_cross_backward(View q, View k, View v, View d_o, const float* o, const float* lse, float* dq,
+                          float* dkv, int b, int h, int hk, int sq, int sk, int d,
+                          const int32_t* key_lengths, float scale, void* stream);
+// Whether the forward takes the split kernel (few queries) and not blocks.
+bool cross_splits(int64_t b, int64_t h, int64_t hk, int64_t sq, int64_t sk, int64_t d);
+int64_t cross_blocks(int64_t pairs, int64_t s);  // workgroups over `pairs` (b, head) of s rows
+
 // Sets this thread's message (fattn_last_error) and returns `code`; done() clears it and returns 0.
 int set_error(int code, const char* format, ...) __attribute__((format(printf, 2, 3)));
 int hip_error(int err, const char* who, const char* what);

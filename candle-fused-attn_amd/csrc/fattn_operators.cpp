@@ -50,11 +50,13 @@ int check_types(const char* who, int dtype, int cache_dtype) {
   }
   return 0;
 }
-int check_heads(const char* who, int64_t heads, int64_t kv_heads) {
+// (No query heads at all: an append without queries, or an empty call.)
+int check_heads(const char* who, int64_t heads, int64_t kv_heads, bool none) {
   if (heads < 0 || kv_heads < 0 || heads > kMaxHeads || kv_heads > kMaxHeads) {
     return set_error(FATTN_ERANGE, "%s: at most %lld heads", who, static_cast<long long>(kMaxHeads));
   }
-  if (kv_heads == 0 || heads % kv_heads != 0) {
+  if (heads == 0 && none) return 0;
+  if (kv_heads == 0 || heads == 0 || heads % kv_heads != 0) {
     return set_error(FATTN_EINVAL, "%s: %lld query heads are no multiple of %lld key heads", who,
                      static_cast<long long>(heads), static_cast<long long>(kv_heads));
   }
@@ -160,8 +162,55 @@ int run_split(const char* who, fattn::SplitArgs& a, int dtype, int cache_dtype, 
   return fattn::done();
 }
 
+// --- Cross attention's operands --------------------------------------------------------------------
+constexpr const char* kCross = "fused_cross_attention";
+struct Cross {
+  fattn::View q, k, v;
+};
+// A [b, h, s, d] operand; false: strides that are negative or leave rows unaligned, or a base that is.
+bool view(fattn::View& to, const float* p, const int64_t strides[3], int64_t b, int64_t h, int64_t s) {
+  int64_t st[3];
+  used3(st, strides, b, h, s);
+  to = fattn::View{p, st[0], st[1], st[2]};
+  return aligned(p, 16) && !negative(st, 3) && multiples(st, 4);
+}
+int bad_view(const char* who, const int64_t strides[3]) {
+  if (negative(strides, 3)) return set_error(FATTN_EINVAL, "%s: negative strides", who);
+  return set_error(FATTN_EALIGN, "%s: rows must be 16-byte aligned", who);
+}
+// The kernels address the rows of one (batch, head) with 32-bit byte offsets.
+bool slice_fits(const fattn::View& v, int64_t s, int64_t d) {
+  return s <= 1 || (s - 1) * v.ss * 4 + 4 * d <= int64_t{UINT32_MAX};
+}
+int cross_operands(Cross& c, const float* q, const int64_t q_strides[3], const float* k,
+                   const int64_t k_strides[3], const float* v, const int64_t v_strides[3], int64_t b,
+                   int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d, bool* none) {
+  if (b < 0 || sq < 0 || sk < 0) return set_error(FATTN_EINVAL, "%s: negative size", kCross);
+  if (heads == 0 && kv_heads == 0) b = 0;
+  if (int rc = check_heads(kCross, heads, kv_heads, b == 0)) return rc;
+  if (int rc = check_dim(kCross, d)) return rc;
+  *none = b == 0;
+  if (*none) return 0;
+  const int64_t lim = INT32_MAX - 256;
+  if (b > lim || sq > lim || sk > lim || b * heads > lim || b * heads * sq > lim ||
+      b * kv_heads * sk > lim ||
+      fattn::cross_blocks(b * heads, sq) + fattn::cross_blocks(b * kv_heads, sk) > kMaxGrid) {
+    return set_error(FATTN_ERANGE, "%s: the sizes exceed 32-bit indexing or the launch limit", kCross);
+  }
+  if ((sq > 0 && (!q || !q_strides)) || (sk > 0 && (!k || !v || !k_strides || !v_strides))) {
+    return set_error(FATTN_EINVAL, "%s: null operand", kCross);
+  }
+  if (sq > 0 && !view(c.q, q, q_strides, b, heads, sq)) return bad_view(kCross, q_strides);
+  if (sk > 0 && !view(c.k, k, k_strides, b, kv_heads, sk)) return bad_view(kCross, k_strides);
+  if (sk > 0 && !view(c.v, v, v_strides, b, kv_heads, sk)) return bad_view(kCross, v_strides);
+  if (!slice_fits(c.k, sk, d) || !slice_fits(c.v, sk, d)) {
+    return set_error(FATTN_ERANGE, "%s: the keys of one (batch, head) span more than 4 GiB", kCross);
+  }
+  return 0;
+}
+
 bool split_shape(int64_t b, int64_t heads, int64_t kv_heads, int64_t d) {
-  return b >= 0 && heads >= 0 && kv_heads > 0 && heads % kv_heads == 0 && fattn::head_dim_supported(d);
+  return b >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && fattn::head_dim_supported(d);
 }
 
 }  // namespace
@@ -220,7 +269,7 @@ int fattn_paged_append(int dtype, int cache_dtype, int64_t b, int64_t heads, int
   const char* who = "paged_append";
   if (int rc = check_types(who, dtype, cache_dtype)) return rc;
   if (b < 0 || s < 0) return set_error(FATTN_EINVAL, "%s: negative size", who);
-  if (int rc = check_heads(who, heads, kv_heads)) return rc;
+  if (int rc = check_heads(who, heads, kv_heads, kv_heads > 0)) return rc;
   if (int rc = check_dim(who, d)) return rc;
   if (b == 0 || s == 0) return fattn::done();
   fattn::RotaryArgs a{};
@@ -268,9 +317,9 @@ int fattn_paged_attention(int dtype, int cache_dtype, int64_t b, int64_t heads, 
   const char* who = "paged_attention";
   if (int rc = check_types(who, dtype, cache_dtype)) return rc;
   if (b < 0) return set_error(FATTN_EINVAL, "%s: negative size", who);
-  if (int rc = check_heads(who, heads, kv_heads)) return rc;
+  if (int rc = check_heads(who, heads, kv_heads, b == 0)) return rc;
   if (int rc = check_dim(who, d)) return rc;
-  if (b == 0 || heads == 0) return fattn::done();
+  if (b == 0) return fattn::done();
   fattn::SplitArgs a{};
   if (int rc = check_cache(who, cache_dtype, k_pages, k_page_strides, v_pages, v_page_strides, pages,
                            kv_heads, page_size, table, table_stride, table_width, lengths, a.ks, a.vs)) {
@@ -301,6 +350,7 @@ int fattn_paged_attention(int dtype, int cache_dtype, int64_t b, int64_t heads, 
 size_t fattn_cross_workspace_bytes(int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk,
                                    int64_t d) {
   if (!split_shape(b, heads, kv_heads, d) || sq < 0 || sk < 0) return 0;
+  if (!fattn::cross_splits(b, heads, kv_heads, sq, sk, d)) return 0;
   return fattn::split_plan(b, kv_heads, heads / kv_heads * sq, d, sk).bytes;
 }
 
@@ -309,39 +359,63 @@ int fattn_cross_forward(const float* q, const int64_t q_strides[3], const float*
                         int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d,
                         const int32_t* key_lengths, float scale, float* out, float* lse,
                         void* workspace, size_t workspace_bytes, void* stream) {
-  const char* who = "fused_cross_attention";
-  if (b < 0 || sq < 0 || sk < 0) return set_error(FATTN_EINVAL, "%s: negative size", who);
-  if (int rc = check_heads(who, heads, kv_heads)) return rc;
-  if (int rc = check_dim(who, d)) return rc;
-  if (b == 0 || heads == 0 || sq == 0) return fattn::done();
-  if (!q || !out || !lse || !q_strides || (sk > 0 && (!k || !v || !k_strides || !v_strides))) {
-    return set_error(FATTN_EINVAL, "%s: null operand", who);
+  Cross c{};
+  bool none = false;
+  if (int rc = cross_operands(c, q, q_strides, k, k_strides, v, v_strides, b, heads, kv_heads, sq, sk, d,
+                              &none)) {
+    return rc;
   }
-  fattn::SplitArgs a{};
-  used3(a.qs, q_strides, b, heads, sq);
-  if (sk > 0) {
-    used3(a.ks, k_strides, b, kv_heads, sk);
-    used3(a.vs, v_strides, b, kv_heads, sk);
+  if (none || sq == 0) return fattn::done();
+  if (!out || !lse) return set_error(FATTN_EINVAL, "%s: null operand", kCross);
+  if (!aligned(out, 16)) return set_error(FATTN_EALIGN, "%s: rows must be 16-byte aligned", kCross);
+  const int B = static_cast<int>(b), H = static_cast<int>(heads), HK = static_cast<int>(kv_heads);
+  const int SQ = static_cast<int>(sq), SK = static_cast<int>(sk);
+  if (fattn::cross_splits(b, heads, kv_heads, sq, sk, d)) {
+    fattn::SplitArgs a{};
+    a.q = q, a.k = k, a.v = v, a.o = out, a.lse = lse;
+    a.qs[0] = c.q.sb, a.qs[1] = c.q.sh, a.qs[2] = c.q.ss;
+    a.ks[0] = c.k.sb, a.ks[1] = c.k.sh, a.ks[2] = c.k.ss;
+    a.vs[0] = c.v.sb, a.vs[1] = c.v.sh, a.vs[2] = c.v.ss;
+    a.lengths = key_lengths;
+    a.B = B, a.H = H, a.HK = HK, a.G = H / HK, a.SQ = SQ, a.SK = SK, a.scale = scale;
+    return run_split(kCross, a, FATTN_F32, FATTN_F32, d, sk, workspace, workspace_bytes, stream);
   }
-  if (negative(a.qs, 3) || negative(a.ks, 3) || negative(a.vs, 3)) {
-    return set_error(FATTN_EINVAL, "%s: negative strides", who);
+  const int err = fattn::launch_cross_forward(c.q, c.k, c.v, out, lse, B, H, HK, SQ, SK,
+                                              static_cast<int>(d), key_lengths, scale, stream);
+  if (err) return fattn::hip_error(err, kCross, "forward launch");
+  return fattn::done();
+}
+
+int fattn_cross_backward(const float* q, const int64_t q_strides[3], const float* k,
+                         const int64_t k_strides[3], const float* v, const int64_t v_strides[3],
+                         int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d,
+                         const int32_t* key_lengths, float scale, const float* out, const float* lse,
+                         const float* d_o, const int64_t do_strides[3], float* dq, float* dkv,
+                         void* stream) {
+  Cross c{};
+  bool none = false;
+  if (int rc = cross_operands(c, q, q_strides, k, k_strides, v, v_strides, b, heads, kv_heads, sq, sk, d,
+                              &none)) {
+    return rc;
   }
-  if (!aligned(q, 16) || !aligned(out, 16) || (sk > 0 && (!aligned(k, 16) || !aligned(v, 16))) ||
-      !multiples(a.qs, 4) || !multiples(a.ks, 4) || !multiples(a.vs, 4)) {
-    return set_error(FATTN_EALIGN, "%s: rows must be 16-byte aligned", who);
+  if (none || (sq == 0 && sk == 0)) return fattn::done();
+  if ((sq > 0 && (!out || !lse || !d_o || !do_strides || !dq)) || (sk > 0 && !dkv)) {
+    return set_error(FATTN_EINVAL, "%s: null operand", kCross);
   }
-  if (b > INT32_MAX || sq > INT32_MAX / kMaxHeads || sk > INT32_MAX - 64) {
-    return set_error(FATTN_ERANGE, "%s: the sizes exceed 32-bit indexing", who);
+  fattn::View g{d_o, 0, 0, 0};
+  if (sq > 0 && !view(g, d_o, do_strides, b, heads, sq)) return bad_view(kCross, do_strides);
+  if (!aligned(out, 16) || !aligned(dq, 16) || !aligned(dkv, 16)) {
+    return set_error(FATTN_EALIGN, "%s: rows must be 16-byte aligned", kCross);
   }
-  if (16 * 4 * a.ks[2] > INT32_MAX || 16 * 4 * a.vs[2] > INT32_MAX) {
-    return set_error(FATTN_ERANGE, "%s: 16 keys span more than 2 GiB", who);
+  if (!slice_fits(c.q, sq, d) || !slice_fits(g, sq, d) || sq * heads * d > int64_t{UINT32_MAX}) {
+    return set_error(FATTN_ERANGE, "%s: the queries of one sample span more than 4 GiB", kCross);
   }
-  a.q = q, a.k = k, a.v = v, a.o = out, a.lse = lse;
-  a.lengths = key_lengths;
-  a.B = static_cast<int>(b), a.H = static_cast<int>(heads), a.HK = static_cast<int>(kv_heads);
-  a.G = static_cast<int>(heads / kv_heads), a.SQ = static_cast<int>(sq), a.SK = static_cast<int>(sk);
-  a.scale = scale;
-  return run_split(who, a, FATTN_F32, FATTN_F32, d, sk, workspace, workspace_bytes, stream);
+  const int err = fattn::launch_cross_backward(
+      c.q, c.k, c.v, g, out, lse, dq, dkv, static_cast<int>(b), static_cast<int>(heads),
+      static_cast<int>(kv_heads), static_cast<int>(sq), static_cast<int>(sk), static_cast<int>(d),
+      key_lengths, scale, stream);
+  if (err) return fattn::hip_error(err, kCross, "backward launch");
+  return fattn::done();
 }
 
 }  // extern "C"

@@ -279,6 +279,17 @@ int fattn_cross_forward(const float* q, const int64_t q_strides[3], const float*
                         const int32_t* key_lengths, float scale, float* out, float* lse,
                         void* workspace, size_t workspace_bytes, void* stream);
 
+/* Its gradient, from out, lse and the output's gradient d_o ([b, heads, sq, d] by its strides {batch,
+ * head, seq}): dq [b, sq, heads, d] and dkv [b, sk, 2, kv_heads, d] (dK, then dV, in each row),
+ * contiguous, written whole: rows of keys that a sample does not see are 0, and those of a shared key
+ * head are summed over its query heads, all in a fixed order: reruns are bit-identical. */
+int fattn_cross_backward(const float* q, const int64_t q_strides[3], const float* k,
+                         const int64_t k_strides[3], const float* v, const int64_t v_strides[3],
+                         int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d,
+                         const int32_t* key_lengths, float scale, const float* out, const float* lse,
+                         const float* d_o, const int64_t do_strides[3], float* dq, float* dkv,
+                         void* stream);
+
 /* ------------------------------------------------------------------------------------------
  * Diagnostics (no counterpart in the reference).
  * ------------------------------------------------------------------------------------------ */

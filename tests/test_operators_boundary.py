@@ -140,7 +140,58 @@ def test_attention_refusals():
     assert L.fattn_paged_attention_workspace_bytes(4, 8, 2, 64, 16) == 0
     assert L.fattn_paged_attention_workspace_bytes(4, 8, 3, 64, 1 << 20) == 0
     assert L.fattn_paged_attention_workspace_bytes(4, 8, 2, 48, 1 << 20) == 0
-    assert attention(heads=0) == 0
+    refused(attention(heads=0), _lib.FATTN_EINVAL, "0 query heads")
+
+
+def cross(b=1, heads=1, hk=1, sq=1, sk=1, d=64, q=BAD, k=BAD, qst=ST, kst=ST, out=BAD, ws=BAD,
+          size=1 << 40):
+    return _lib.lib().fattn_cross_forward(q, qst, k, kst, k, kst, b, heads, hk, sq, sk, d, None, 1.0, out,
+                                          BAD, ws, size, None)
+
+
+def cross_bwd(b=1, heads=1, hk=1, sq=1, sk=1, d=64, q=BAD, k=BAD, qst=ST, kst=ST, out=BAD, g=BAD, gst=ST,
+              dq=BAD, dkv=BAD):
+    return _lib.lib().fattn_cross_backward(q, qst, k, kst, k, kst, b, heads, hk, sq, sk, d, None, 1.0, out,
+                                           BAD, g, gst, dq, dkv, None)
+
+
+@pytest.mark.parametrize("call", [cross, cross_bwd])
+def test_cross_refusals(call):
+    refused(call(b=-1), _lib.FATTN_EINVAL, "fused_cross_attention: negative size")
+    refused(call(sk=-1), _lib.FATTN_EINVAL, "negative size")
+    refused(call(d=48), _lib.FATTN_EHEADDIM, "32, 64 or 128, got 48")
+    refused(call(heads=3, hk=2), _lib.FATTN_EINVAL, "3 query heads are no multiple of 2 key heads")
+    refused(call(heads=0), _lib.FATTN_EINVAL, "0 query heads")
+    refused(call(hk=0), _lib.FATTN_EINVAL, "0 key heads")
+    refused(call(q=None), _lib.FATTN_EINVAL, "null operand")
+    refused(call(k=None), _lib.FATTN_EINVAL, "null operand")
+    refused(call(out=None), _lib.FATTN_EINVAL, "null operand")
+    refused(call(q=ODD), _lib.FATTN_EALIGN, "16-byte aligned")
+    refused(call(k=ODD), _lib.FATTN_EALIGN, "16-byte aligned")
+    refused(call(out=ODD), _lib.FATTN_EALIGN, "16-byte aligned")
+    refused(call(sk=2, kst=_lib.arr([0, 0, 66])), _lib.FATTN_EALIGN, "16-byte aligned")
+    refused(call(sk=2, kst=_lib.arr([0, 0, -4])), _lib.FATTN_EINVAL, "negative strides")
+    refused(call(sk=5, kst=_lib.arr([0, 0, 1 << 28])), _lib.FATTN_ERANGE, "4 GiB")
+    refused(call(b=1 << 16, heads=1 << 10, sq=1 << 10), _lib.FATTN_ERANGE, "32-bit")
+    refused(call(sk=(1 << 31) - 1), _lib.FATTN_ERANGE, "32-bit")
+    assert call(b=0, q=None) == 0 and call(heads=0, hk=0) == 0
+
+
+def test_cross_workspace_and_gradient_refusals():
+    L = _lib.lib()
+    need = L.fattn_cross_workspace_bytes(2, 4, 4, 1, 4096, 64)
+    assert need > 0
+    for ws, size in ((None, need), (ODD, need), (BAD, need - 1)):
+        refused(cross(b=2, heads=4, hk=4, sk=4096, ws=ws, size=size), _lib.FATTN_EWORKSPACE, str(need))
+    assert L.fattn_cross_workspace_bytes(2, 4, 4, 1000, 4096, 64) == 0
+    assert L.fattn_cross_workspace_bytes(2, 4, 3, 1, 4096, 64) == 0
+    refused(cross_bwd(g=None), _lib.FATTN_EINVAL, "null operand")
+    refused(cross_bwd(dq=None), _lib.FATTN_EINVAL, "null operand")
+    refused(cross_bwd(dkv=None), _lib.FATTN_EINVAL, "null operand")
+    refused(cross_bwd(g=ODD), _lib.FATTN_EALIGN, "16-byte aligned")
+    refused(cross_bwd(sq=2, gst=_lib.arr([0, 0, 2])), _lib.FATTN_EALIGN, "16-byte aligned")
+    refused(cross_bwd(sq=2, gst=_lib.arr([0, 0, -4])), _lib.FATTN_EINVAL, "negative strides")
+    refused(cross_bwd(sq=5, gst=_lib.arr([0, 0, 1 << 28])), _lib.FATTN_ERANGE, "4 GiB")
 
 
 # --- The Python layer ----------------------------------------------------------------------------

@@ -12,7 +12,7 @@
 
 namespace fattn {
 
-int64_t cross_blocks(int64_t pairs, int64_t s) { return pairs * ((s + 4 * kRows - 1) / (4 * kRows)); }
+int64_t cross_blocks(int64_t heads, int64_t s) { return heads * ((s + 4 * kRows - 1) / (4 * kRows)); }
 
 bool cross_splits(int64_t, int64_t h, int64_t hk, int64_t sq, int64_t, int64_t) {
   return h / hk * sq <= 32;
@@ -26,7 +26,7 @@ int launch_cross_forward(View q, View k, View v, float* o, float* lse, int b, in
   const void* fn = d == 32    ? reinterpret_cast<const void*>(fwd_pair_kernel<32, false, 1, 4, 4, true>)
                    : d == 128 ? reinterpret_cast<const void*>(fwd_pair_kernel<128, false, 1, 4, 2, true>)
                               : reinterpret_cast<const void*>(fwd_pair_kernel<64, false, 1, 4, 3, true>);
-  return static_cast<int>(hipLaunchKernel(fn, dim3(static_cast<unsigned>(nqb) * b * h), dim3(256), args, 0,
+  return static_cast<int>(hipLaunchKernel(fn, dim3(static_cast<unsigned>(cross_blocks(int64_t{b} * h, sq))), dim3(256), args, 0,
                                           static_cast<hipStream_t>(stream)));
 }
 
@@ -37,14 +37,14 @@ int launch_cross_backward(View q, View k, View v, View d_o, const float* o, cons
   BwdPairArgs a{};
   a.q = q, a.k = k, a.v = v, a.d_o = d_o, a.o = o, a.lse = lse, a.dq = dq, a.dkv = dkv;
   a.B = b, a.H = h, a.S = sq, a.SK = sk, a.G = h / hk, a.key_lengths = key_lengths, a.scale = scale;
-  a.nblk = nblk, a.nkv = nblk * b * hk, a.nblk_q = nblk_q, a.nqv = nblk_q * b * h;
+  a.nblk = nblk, a.nkv = nblk * b * hk, a.nblk_q = nblk_q;
   a.give_up_bh = -1;
   void* args[] = {&a};
   const void* fn = d == 32 ? reinterpret_cast<const void*>(bwd_pair_kernel<32, false, false, 4, 3, true>)
                    : d == 128
                        ? reinterpret_cast<const void*>(bwd_pair_kernel<128, false, false, 4, 1, true>)
                        : reinterpret_cast<const void*>(bwd_pair_kernel<64, false, false, 4, 2, true>);
-  return static_cast<int>(hipLaunchKernel(fn, dim3(static_cast<unsigned>(a.nkv + a.nqv)), dim3(256), args,
+  return static_cast<int>(hipLaunchKernel(fn, dim3(static_cast<unsigned>(a.nkv + nblk_q * b * h)), dim3(256), args,
                                           0, static_cast<hipStream_t>(stream)));
 }
 

@@ -232,7 +232,7 @@ int launch_cross_backward(View q, View k, View v, View d_o, const float* o, cons
                           const int32_t* key_lengths, float scale, void* stream);
 // Whether the forward takes the split kernel (few queries) and not blocks.
 bool cross_splits(int64_t b, int64_t h, int64_t hk, int64_t sq, int64_t sk, int64_t d);
-int64_t cross_blocks(int64_t pairs, int64_t s);  // workgroups over `pairs` (b, head) of s rows
+int64_t cross_blocks(int64_t heads, int64_t s);  // workgroups over `heads` (b, head) of s rows
 
 // Sets this thread's message (fattn_last_error) and returns `code`; done() clears it and returns 0.
 int set_error(int code, const char* format, ...) __attribute__((format(printf, 2, 3)));

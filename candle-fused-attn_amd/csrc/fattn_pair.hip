@@ -100,7 +100,7 @@ int launch_backward(View q, View k, View v, View d_o, const float* o, const floa
   const int waves = workgroup_waves(b * h, s, true), rows = kRows * waves, nblk = (s + rows - 1) / rows;
   BwdPairArgs a{q, k, v, d_o, o, lse, dqkv, part, done, epoch_slot, epoch, ctrl, b, h, s,
                 nblk * b * h, nblk, scale, causal ? 1 : 0, defer, last, give_up_bh,
-                nullptr, nullptr, s, 1, nullptr, 0, nblk};
+                nullptr, nullptr, s, 1, nullptr, nblk};
   void* args[] = {&a};
   const bool serial = causal && s <= kSerialLength && a.nkv <= kSerialBlocks;
   // Waves per SIMD: what the registers allow without spills to the loop. At d 32 the third fits once

@@ -7,25 +7,33 @@ import torch
 
 from ._lib import DTYPES, FusedAttentionError, check
 
-A2, A3, A9 = ctypes.c_int64 * 2, ctypes.c_int64 * 3, ctypes.c_int64 * 9
-P3 = ctypes.c_void_p * 3
+ALL = tuple(DTYPES)
+_ARRAYS = {n: ctypes.c_int64 * n for n in range(1, 40)}
 
 
-def require(who: str, name: str, t, rank: int, device: torch.device | None = None,
-            dtypes=None) -> None:
-    """A tensor of `rank` dimensions on a HIP device (that of the first operand), of a type the
-    operator takes."""
+def pack(*values):
+    """One int64 array of `values` (sizes, strides, addresses) and its address, which the C entries take
+    parts of: on small calls the host is the whole time, and an array per operand costs it 0.4 us each.
+    (Keep the array until the call returns.)"""
+    a = _ARRAYS[len(values)](*values)
+    return a, ctypes.addressof(a)
+
+
+def require(who: str, name: str, t, rank: int, like: torch.Tensor | None = None, dtypes=ALL) -> None:
+    """A tensor of `rank` dimensions on a HIP device (that of `like`), of a type the operator takes."""
+    if (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() == rank and t.is_cuda
+            and (like is None or t.get_device() == like.get_device())):
+        return
     if not isinstance(t, torch.Tensor):
         raise FusedAttentionError(f"{who}: {name} must be a tensor")
-    if t.dtype not in (DTYPES if dtypes is None else dtypes):
-        takes = ", ".join(str(d)[6:] for d in (DTYPES if dtypes is None else dtypes))
+    if t.dtype not in dtypes:
+        takes = ", ".join(str(d)[6:] for d in dtypes)
         raise FusedAttentionError(f"{who}: {name} must be {takes}, got {str(t.dtype)[6:]}")
     if t.dim() != rank:
         raise FusedAttentionError(f"{who}: {name} must have {rank} dimensions, got shape {list(t.shape)}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise FusedAttentionError(f"{who}: {name} is not on a HIP device (this operator has no CPU path)")
-    if device is not None and t.device != device:
-        raise FusedAttentionError(f"{who}: {name} is on {t.device}, the first operand on {device}")
+    raise FusedAttentionError(f"{who}: {name} is on {t.device}, the first operand on {like.device}")
 
 
 def rows(t: torch.Tensor) -> torch.Tensor:
@@ -34,17 +42,16 @@ def rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def aligned_rows(t: torch.Tensor) -> torch.Tensor:
-    """`t` itself where its rows are contiguous and 16-byte aligned, else a contiguous copy."""
-    per = 16 // t.element_size()
-    st = t.stride()
-    if st[-1] == 1 and t.data_ptr() % 16 == 0 and all(
-            s % per == 0 for s, n in zip(st[:-1], t.shape) if n > 1):
+    """A four-dimensional `t` itself where its rows are contiguous and 16-byte aligned, else a contiguous
+    copy."""
+    per = 15 // t.element_size()
+    s0, s1, s2, s3 = t.stride()
+    if s3 == 1 and not (s0 | s1 | s2) & per and not t.data_ptr() & 15:
+        return t
+    if s3 == 1 and not t.data_ptr() & 15 and not any(
+            s & per for s, n in zip((s0, s1, s2), t.shape) if n > 1):
         return t
     return t.clone(memory_format=torch.contiguous_format)
-
-
-def strides3(t: torch.Tensor):
-    return A3(*t.stride()[:3])
 
 
 def launch(t: torch.Tensor, fn, *args) -> None:

@@ -72,7 +72,6 @@ A3 = ctypes.POINTER(ctypes.c_int64)
 C_INT = ctypes.c_int
 C_FLOAT = ctypes.c_float
 C_DOUBLE = ctypes.c_double
-PP = ctypes.POINTER(ctypes.c_void_p)
 SIZE = ctypes.c_size_t
 
 
@@ -106,21 +105,21 @@ def _declare(L: ctypes.CDLL) -> None:
                                 P, P, P]
     L.fattn_backward.argtypes = [P, I64, A3, A3, P, I64, A3, A3, P, I64, A3, A3, C_FLOAT, C_INT,
                                  P, P, P, I64, A3, A3, P, P, SIZE, P]
-    L.fattn_rotary.argtypes = [C_INT, I64, I64, I64, A3, PP, PP, A3, A3, C_INT, P, C_INT, A3, P, I64,
-                               C_INT, C_DOUBLE, C_INT, P]
-    L.fattn_paged_append.argtypes = [C_INT, C_INT, I64, I64, I64, I64, I64, P, A3, P, A3, P, A3, P,
-                                     A3, P, A3, P, A3, I64, I64, P, I64, I64, P, P, P, I64, C_INT,
-                                     C_DOUBLE, P]
+    # (The operators around self-attention: sizes and strides as addresses into one array a call.)
+    L.fattn_rotary.argtypes = [C_INT, I64, I64, I64, P, P, P, P, P, C_INT, P, C_INT, P, P, I64, C_INT,
+                               C_DOUBLE, C_INT, P]
+    L.fattn_paged_append.argtypes = [C_INT, C_INT, I64, I64, I64, I64, I64, P, P, P, P, P, P, P, P, P,
+                                     P, P, P, I64, I64, P, I64, I64, P, P, P, I64, C_INT, C_DOUBLE, P]
     L.fattn_paged_attention_workspace_bytes.argtypes = [I64, I64, I64, I64, I64]
     L.fattn_paged_attention_workspace_bytes.restype = SIZE
-    L.fattn_paged_attention.argtypes = [C_INT, C_INT, I64, I64, I64, I64, P, A3, P, P, A3, P, A3,
-                                        I64, I64, P, I64, I64, P, C_FLOAT, P, SIZE, P]
+    L.fattn_paged_attention.argtypes = [C_INT, C_INT, I64, I64, I64, I64, P, P, P, P, P, P, P, I64, I64,
+                                        P, I64, I64, P, C_FLOAT, P, SIZE, P]
     L.fattn_cross_workspace_bytes.argtypes = [I64, I64, I64, I64, I64, I64]
     L.fattn_cross_workspace_bytes.restype = SIZE
-    L.fattn_cross_forward.argtypes = [P, A3, P, A3, P, A3, I64, I64, I64, I64, I64, I64, P, C_FLOAT,
-                                      P, P, P, SIZE, P]
-    L.fattn_cross_backward.argtypes = [P, A3, P, A3, P, A3, I64, I64, I64, I64, I64, I64, P, C_FLOAT,
-                                       P, P, P, A3, P, P, P]
+    L.fattn_cross_forward.argtypes = [P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, P, C_FLOAT, P, P,
+                                      P, SIZE, P]
+    L.fattn_cross_backward.argtypes = [P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, P, C_FLOAT, P, P,
+                                       P, P, P, P, P]
     L.fattn_bwd_status.argtypes = [P, SIZE, I64, I64, I64, P, ctypes.POINTER(C_INT)]
     for name in EXPORTS:
         if name not in ("fattn_last_error", "fattn_version") and "workspace" not in name:

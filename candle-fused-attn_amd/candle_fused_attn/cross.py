@@ -9,7 +9,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._call import A3, aligned_rows, launch, require, strides3
+from ._call import aligned_rows, launch, pack, require
 from ._lib import FusedAttentionError
 
 _F32 = (torch.float32,)
@@ -20,12 +20,11 @@ def _forward(q, k, v, scale, key_lengths):
     b, h, sq, d = q.shape
     hk, sk = k.shape[1], k.shape[2]
     L = _lib.lib()
-    out = torch.empty((b, sq, h, d), dtype=torch.float32, device=q.device)
-    lse = torch.empty((b, h, sq), dtype=torch.float32, device=q.device)
+    out, lse = q.new_empty((b, sq, h, d)), q.new_empty((b, h, sq))
     size = L.fattn_cross_workspace_bytes(b, h, hk, sq, sk, d)
     ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    launch(q, L.fattn_cross_forward, q.data_ptr(), strides3(q), k.data_ptr(), strides3(k),
-           v.data_ptr(), strides3(v), b, h, hk, sq, sk, d,
+    keep, p = pack(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+    launch(q, L.fattn_cross_forward, q.data_ptr(), p, k.data_ptr(), p + 24, v.data_ptr(), p + 48, b, h, hk, sq, sk, d,
            key_lengths.data_ptr() if key_lengths is not None else None, scale, out.data_ptr(),
            lse.data_ptr(), ws.data_ptr() if size else None, size)
     return out, lse
@@ -48,15 +47,15 @@ class _FusedCrossAttention(torch.autograd.Function):
         grad = aligned_rows(grad)
         b, h, sq, d = q.shape
         hk, sk = k.shape[1], k.shape[2]
-        dq = torch.empty((b, sq, h, d), dtype=torch.float32, device=q.device)
-        dkv = torch.empty((b, sk, 2, hk, d), dtype=torch.float32, device=q.device)
+        dq, dkv = q.new_empty((b, sq, h, d)), q.new_empty((b, sk, 2, hk, d))
         gb, gs, gh, _ = grad.stride()
-        launch(q, _lib.lib().fattn_cross_backward, q.data_ptr(), strides3(q), k.data_ptr(), strides3(k),
-               v.data_ptr(), strides3(v), b, h, hk, sq, sk, d,
+        keep, p = pack(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], gb, gh, gs)
+        launch(q, _lib.lib().fattn_cross_backward, q.data_ptr(), p, k.data_ptr(), p + 24, v.data_ptr(),
+               p + 48, b, h, hk, sq, sk, d,
                key_lengths.data_ptr() if key_lengths is not None else None, ctx.scale, out.data_ptr(),
-               lse.data_ptr(), grad.data_ptr(), A3(gb, gh, gs), dq.data_ptr(), dkv.data_ptr())
-        return (dq.transpose(1, 2), dkv[:, :, 0].transpose(1, 2), dkv[:, :, 1].transpose(1, 2), None,
-                None)
+               lse.data_ptr(), grad.data_ptr(), p + 72, dq.data_ptr(), dkv.data_ptr())
+        dk, dv = dkv.transpose(1, 3).unbind(2)  # [b, kv_heads, sk, d] each
+        return dq.transpose(1, 2), dk, dv, None, None
 
 
 def fused_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
@@ -71,14 +70,14 @@ def fused_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sca
     """
     who = "fused_cross_attention"
     require(who, "q", q, 4, None, _F32)
-    require(who, "k", k, 4, q.device, _F32)
-    require(who, "v", v, 4, q.device, _F32)
+    require(who, "k", k, 4, q, _F32)
+    require(who, "v", v, 4, q, _F32)
     b, h, _, d = q.shape
     if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
         raise FusedAttentionError(f"{who}: q [b, h, sq, d] and k, v [b, kv_heads, sk, d] expected, got "
                                   f"{list(q.shape)} {list(k.shape)} {list(v.shape)}")
     if key_lengths is not None:
-        require(who, "key_lengths", key_lengths, 1, q.device, _I32)
+        require(who, "key_lengths", key_lengths, 1, q, _I32)
         if key_lengths.shape[0] != b or not key_lengths.is_contiguous():
             raise FusedAttentionError(f"{who}: contiguous key_lengths [{b}] expected, got "
                                       f"{list(key_lengths.shape)}")

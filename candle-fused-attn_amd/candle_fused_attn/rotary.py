@@ -12,7 +12,7 @@ import math
 import torch
 
 from . import _lib
-from ._call import A2, A3, A9, P3, launch, require, rows
+from ._call import launch, pack, require, rows
 from ._lib import FusedAttentionError
 
 _SCALINGS = (None, "linear", "base", "ramp")
@@ -49,9 +49,13 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str | None = No
     return f.to(device) if device is not None else f
 
 
-def check_frequencies(who: str, frequencies, d: int, device: torch.device) -> int:
+_F64 = (torch.float64,)
+_INTS = (torch.int64, torch.int32)
+
+
+def check_frequencies(who: str, frequencies, d: int, like: torch.Tensor) -> int:
     """The rotated part of a head of d values."""
-    require(who, "frequencies", frequencies, 1, device, (torch.float64,))
+    require(who, "frequencies", frequencies, 1, like, _F64)
     dim = 2 * frequencies.shape[0]
     if dim > d or not frequencies.is_contiguous():
         raise FusedAttentionError(f"{who}: contiguous frequencies of at most {d // 2} pairs expected, "
@@ -59,41 +63,43 @@ def check_frequencies(who: str, frequencies, d: int, device: torch.device) -> in
     return dim
 
 
-def _turn(parts, rotated: int, positions, frequencies, interleaved: bool, magnitude: float,
-          inverse: bool) -> None:
-    """Launches on (x, y) pairs of [b, heads, s, d] views of one shape but for the heads."""
-    b, _, s, d = parts[0][0].shape
-    pos = positions
-    pst = (0, pos.stride(0)) if pos.dim() == 1 else (
-        pos.stride(0) if pos.shape[0] > 1 else 0, pos.stride(1))
-    none = [0] * (3 - len(parts))
-    xs, ys = [], []
-    for x, y in parts:
-        xs += x.stride()[:3]
-        ys += y.stride()[:3]
-    launch(parts[0][0], _lib.lib().fattn_rotary, _lib.DTYPES[parts[0][0].dtype], b, s, d,
-           A3(*[x.shape[1] for x, _ in parts], *none),
-           P3(*[x.data_ptr() for x, _ in parts], *none),
-           P3(*[y.data_ptr() for _, y in parts], *none), A9(*xs), A9(*ys), rotated, pos.data_ptr(),
-           pos.element_size() * 8, A2(*pst), frequencies.data_ptr(), 2 * frequencies.shape[0],
-           interleaved, magnitude, inverse)
-
-
-def _split_qkv(t: torch.Tensor, heads: int):
-    b, s, w = t.shape
-    v = t.view(b, s, 3, heads, w // 3 // heads)
-    return [v[:, :, i].transpose(1, 2) for i in range(3)]
-
-
 def _forward(xs, heads, positions, frequencies, interleaved, magnitude, inverse):
-    """heads 0: xs are [b, h, s, d] operands, all turned; else the one [b, s, 3 h d] projection, whose
-    q and k are turned and v copied."""
+    """heads 0: xs are one or two [b, h, s, d] operands, all turned; else the one [b, s, 3 h d]
+    projection, whose q and k are turned and v copied. New tensors."""
     ys = [torch.empty_like(x) for x in xs]
+    x, y = xs[0], ys[0]
+    xp, yp = x.data_ptr(), y.data_ptr()
     if heads:
-        parts, rotated = list(zip(_split_qkv(xs[0], heads), _split_qkv(ys[0], heads))), 0b011
+        b, s, w = x.shape
+        d = w // (3 * heads)
+        step = heads * d * x.element_size()
+        (xb, xs_, _), (yb, ys_, _) = x.stride(), y.stride()
+        sizes = (heads, heads, heads)
+        at = (xp, xp + step, xp + 2 * step, yp, yp + step, yp + 2 * step)
+        strides = (xb, d, xs_) * 3 + (yb, d, ys_) * 3
+        rotated = 0b011
     else:
-        parts, rotated = list(zip(xs, ys)), 0b111
-    _turn(parts, rotated, positions, frequencies, interleaved, magnitude, inverse)
+        b, h, s, d = x.shape
+        rotated = 0b111
+        if len(xs) == 2:
+            x2, y2 = xs[1], ys[1]
+            sizes = (h, x2.shape[1], 0)
+            at = (xp, x2.data_ptr(), 0, yp, y2.data_ptr(), 0)
+            strides = (*x.stride()[:3], *x2.stride()[:3], 0, 0, 0, *y.stride()[:3], *y2.stride()[:3],
+                       0, 0, 0)
+        else:
+            sizes, at = (h, 0, 0), (xp, 0, 0, yp, 0, 0)
+            strides = (*x.stride()[:3], *(0,) * 6, *y.stride()[:3], *(0,) * 6)
+    if positions.dim() == 1:
+        pb, ps = 0, positions.stride(0)
+    else:
+        pb, ps = positions.stride()
+        if positions.shape[0] == 1:
+            pb = 0
+    keep, p = pack(*sizes, *at, *strides, pb, ps)
+    launch(x, _lib.lib().fattn_rotary, _lib.DTYPES[x.dtype], b, s, d, p, p + 24, p + 48, p + 72, p + 144,
+           rotated, positions.data_ptr(), 64 if positions.dtype == torch.int64 else 32, p + 216,
+           frequencies.data_ptr(), 2 * frequencies.shape[0], interleaved, magnitude, inverse)
     return ys
 
 
@@ -130,10 +136,10 @@ def _apply(xs, heads, positions, frequencies, interleaved, magnitude, inverse):
     return _forward(xs, heads, positions, frequencies, interleaved, magnitude, inverse)
 
 
-def _check_positions(who: str, positions, b: int, s: int, device) -> None:
+def _check_positions(who: str, positions, b: int, s: int, like: torch.Tensor) -> None:
     if not isinstance(positions, torch.Tensor) or positions.dim() not in (1, 2):
         raise FusedAttentionError(f"{who}: positions must be a [s] or [b, s] tensor")
-    require(who, "positions", positions, positions.dim(), device, (torch.int64, torch.int32))
+    require(who, "positions", positions, positions.dim(), like, _INTS)
     if positions.shape[-1] != s or (positions.dim() == 2 and positions.shape[0] not in (1, b)):
         raise FusedAttentionError(f"{who}: positions [{s}] or [{b}, {s}] expected, got shape "
                                   f"{list(positions.shape)}")
@@ -151,13 +157,13 @@ def fused_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     """
     who = "fused_rotary"
     require(who, "q", q, 4)
-    require(who, "k", k, 4, q.device, (q.dtype,))
+    require(who, "k", k, 4, q, (q.dtype,))
     b, _, s, d = q.shape
-    if (k.shape[0], k.shape[2], k.shape[3]) != (b, s, d):
+    if k.shape[0] != b or k.shape[2:] != q.shape[2:]:
         raise FusedAttentionError(f"{who}: q and k must agree but for their heads, got {list(q.shape)} "
                                   f"and {list(k.shape)}")
-    _check_positions(who, positions, b, s, q.device)
-    check_frequencies(who, frequencies, d, q.device)
+    _check_positions(who, positions, b, s, q)
+    check_frequencies(who, frequencies, d, q)
     q2, k2 = _apply([rows(q), rows(k)], 0, positions, frequencies, bool(interleaved),
                     float(magnitude), False)
     return q2, k2
@@ -175,7 +181,7 @@ def fused_rotary_qkv(qkv: torch.Tensor, heads: int, positions: torch.Tensor,
     heads = int(heads)
     if heads <= 0 or w == 0 or w % (3 * heads) != 0:
         raise FusedAttentionError(f"{who}: last dimension {w} is not 3 x {heads} heads x head_dim")
-    _check_positions(who, positions, b, s, qkv.device)
-    check_frequencies(who, frequencies, w // 3 // heads, qkv.device)
+    _check_positions(who, positions, b, s, qkv)
+    check_frequencies(who, frequencies, w // 3 // heads, qkv)
     return _apply([rows(qkv)], heads, positions, frequencies, bool(interleaved), float(magnitude),
                   False)[0]

@@ -171,6 +171,21 @@ int static_scratch(void* stream, void** out);
 // --- Rotary positions and the paged cache (fattn_rotary.hip, fattn_paged.hip) --------------------
 // Element types of the C ABI (FATTN_F32, ..).
 constexpr int kF32 = 0, kF16 = 1, kBF16 = 2;
+// x / n for 0 <= x < 2^31, n >= 1 (n 0: not divided by): (hi32(x magic) + x) >> shift.
+struct Divider {
+  unsigned magic, shift;
+};
+inline Divider divider(int64_t n) {
+  Divider d{0, 0};
+  if (n <= 0) return d;
+  while ((int64_t{1} << d.shift) < n) ++d.shift;
+  d.magic = static_cast<unsigned>((static_cast<uint64_t>((uint64_t{1} << d.shift) - n) << 32) / n + 1);
+  return d;
+}
+__device__ __forceinline__ int divide(int x, Divider d) {
+  const unsigned u = static_cast<unsigned>(x);
+  return static_cast<int>((__umulhi(u, d.magic) + u) >> d.shift);
+}
 // One operand of a rotation: heads (0: absent) of a [b, heads, s, d] view x and of its result y,
 // (batch, head, seq) strides in elements, turned or copied.
 struct RotaryPart {
@@ -192,7 +207,9 @@ struct RotaryArgs {
   int B, S, D, pairs, interleaved, inverse;
   const int32_t *table, *lengths, *counts;
   int64_t table_stride, table_width, pages, page_size, page_strides[6];
-  int tokens;  // (the launcher's)
+  // The launcher's: tokens per workgroup; an operand's items per head, and its share of blockIdx.y.
+  int tokens, items[3], first_share[4];
+  Divider by_per[3], by_items[3], by_seq, by_pairs;
 };
 // vec: values per access, 8, 4 or 1 (2 interleaved): every pointer, stride and part of a head is a
 // multiple of it, where it is 4 or more.
@@ -210,15 +227,17 @@ struct SplitArgs {
   const int32_t *table, *lengths;  // lengths null: SK keys each
   int64_t table_stride;
   int page_size, pages;
-  unsigned div_magic, div_shift;  // x / (page_size / 16) = (hi32(x magic) + x) >> shift
+  Divider by_page;  // of halves of a tile: page_size / 16
   int B, H, HK, G, SQ, SK, RB;    // SK: the most keys a sequence can have; RB: blocks of rows
   float scale;
-  float* part;  // the workspace
-  int part_rows, wgs, min_run;  // wgs 0: one workgroup per key head and block of rows, no workspace
+  // The workspace: two parts per workgroup, and where each sequence's costs begin (B + 1 of them).
+  float* part;
+  int64_t* before;
+  int part_rows, wgs, min_run, begin;  // wgs 0: one workgroup per key head and block of rows, no workspace
 };
 struct SplitPlan {
-  int row_blocks, part_rows, wgs, min_run;
-  size_t bytes;
+  int row_blocks, part_rows, wgs, min_run, begin;
+  size_t before, bytes;  // where `before` lies in the workspace, its size
 };
 SplitPlan split_plan(int64_t b, int64_t hk, int64_t rows, int64_t d, int64_t capacity);
 int launch_split(const SplitArgs& a, int dtype, int cache_dtype, int d, void* stream);

@@ -99,14 +99,6 @@ bool fits(int64_t vec, const void* p, int64_t size, const int64_t st[3], int64_t
          (s <= 1 || st[2] % vec == 0);
 }
 
-// x / n for x below 2^31, n >= 1: (hi32(x magic) + x) >> shift.
-void divider(int64_t n, unsigned* magic, unsigned* shift) {
-  unsigned s = 0;
-  while ((int64_t{1} << s) < n) ++s;
-  *shift = s;
-  *magic = static_cast<unsigned>(((static_cast<uint64_t>(1) << 32) * ((uint64_t{1} << s) - n)) / n + 1);
-}
-
 int run_rotary(const char* who, fattn::RotaryArgs& a, int dtype, int cache_dtype, int64_t b, int64_t s,
                int64_t d, int64_t dim, void* stream) {
   const int64_t size = size_of(dtype);
@@ -156,7 +148,9 @@ int run_split(const char* who, fattn::SplitArgs& a, int dtype, int cache_dtype, 
                      who, plan.bytes);
   }
   a.RB = plan.row_blocks, a.part_rows = plan.part_rows, a.wgs = plan.wgs, a.min_run = plan.min_run;
+  a.begin = plan.begin;
   a.part = static_cast<float*>(workspace);
+  a.before = reinterpret_cast<int64_t*>(static_cast<char*>(workspace) + plan.before);
   const int err = fattn::launch_split(a, dtype, cache_dtype, static_cast<int>(d), stream);
   if (err) return fattn::hip_error(err, who, "launch");
   return fattn::done();
@@ -340,7 +334,7 @@ int fattn_paged_attention(int dtype, int cache_dtype, int64_t b, int64_t heads, 
   a.k = k_pages, a.v = v_pages;
   a.table = table, a.table_stride = table_stride, a.lengths = lengths;
   a.page_size = static_cast<int>(page_size), a.pages = static_cast<int>(pages);
-  divider(page_size / 16, &a.div_magic, &a.div_shift);
+  a.by_page = fattn::divider(page_size / 16);
   a.B = static_cast<int>(b), a.H = static_cast<int>(heads), a.HK = static_cast<int>(kv_heads);
   a.G = static_cast<int>(heads / kv_heads), a.SQ = 1, a.SK = static_cast<int>(capacity);
   a.scale = scale;

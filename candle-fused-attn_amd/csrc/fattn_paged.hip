@@ -93,32 +93,15 @@ __device__ __forceinline__ int seq_tiles(const SplitArgs& a, int b, int& len, bo
   len = bad ? 0 : min(max(len, 0), a.SK);
   return (len + kTile - 1) / kTile;
 }
-__device__ __forceinline__ int64_t block_sum(int64_t x, int64_t* sh, int waves) {
-  for (int i = 1; i < 64; i *= 2) x += __shfl_xor(static_cast<long long>(x), i);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
-  __syncthreads();
-  int64_t t = 0;
-  for (int w = 0; w < waves; ++w) t += sh[w];
-  return t;
+// A value that is one for the whole wave, in scalar registers.
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(x));
+  const unsigned hi = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(static_cast<uint64_t>(x) >> 32));
+  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
 }
-// Tiles before sequence `b` (times nothing), and of all.
-template <bool kPaged>
-__device__ __forceinline__ void tiles_before(const SplitArgs& a, int b, int64_t* sh, int64_t& before,
-                                             int64_t& all) {
-  int64_t x = 0, y = 0;
-  for (int i = threadIdx.x; i < a.B; i += blockDim.x) {
-    int len;
-    bool bad;
-    const int t = seq_tiles<kPaged>(a, i, len, bad);
-    y += t;
-    if (i < b) x += t;
-  }
-  const int waves = blockDim.x >> 6;
-  before = block_sum(x, sh, waves);
-  all = block_sum(y, sh, waves);
-}
-// Tiles of a run.
+// What a sequence of n tiles counts for per key head: its tiles, and what beginning a head costs.
+__device__ __forceinline__ int64_t cost(const SplitArgs& a, int n) { return n == 0 ? 0 : n + a.begin; }
+// The length of a run.
 __device__ __forceinline__ int64_t quota(const SplitArgs& a, int64_t units) {
   const int64_t q = (units + a.wgs - 1) / a.wgs;
   return q < a.min_run ? a.min_run : q;
@@ -366,67 +349,65 @@ struct Wave {
   }
 };
 
-template <typename Q, typename C, int D, bool kPaged, int WAVES>
-__global__ void __launch_bounds__(64 * kSplitWaves) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES)))
+// Waves per SIMD (so workgroups per CU) that the registers allow.
+template <typename Q, typename C, int D>
+constexpr int kOccupancy = D == 32    ? 4
+                           : D == 128 ? 2
+                           : std::is_same<C, _Float16>::value || (std::is_same<C, __bf16>::value &&
+                                                                  std::is_same<Q, C>::value)
+                               ? 4
+                               : 3;
+
+template <typename Q, typename C, int D, bool kPaged>
+__global__ void __launch_bounds__(64 * kSplitWaves)
+    __attribute__((amdgpu_waves_per_eu(kOccupancy<Q, C, D>, kOccupancy<Q, C, D>)))
 split_kernel(SplitArgs a) {
   typedef Wave<Q, C, D> W;
   constexpr int kPitch = D + 4;
   __shared__ __attribute__((aligned(16))) float so[kSplitWaves][kRowsMax][kPitch];
   __shared__ float sml[kSplitWaves][2][kRowsMax];
-  __shared__ int64_t sh[kSplitWaves + 2];
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int heads = a.HK * a.RB;
 
-  // This workgroup's run of tiles: [u, end) of the sequences end to end, from tile `off` of sequence b.
+  // This workgroup's run: `left` of the sequences' costs end to end, from `off` into sequence b's.
   int b = 0;
   int64_t off = 0, left = 0;
   if (a.wgs == 0) {  // one workgroup per key head and block of rows
     b = static_cast<int>(blockIdx.x) / heads;
-    int len;
-    bool bad;
-    const int n = seq_tiles<kPaged>(a, b, len, bad);
-    off = static_cast<int64_t>(static_cast<int>(blockIdx.x) % heads) * n;
-    left = n;
   } else {
-    int64_t x = 0;
-    for (int i = tid; i < a.B; i += 64 * kSplitWaves) {
+    // Each wave for itself, without LDS: a lane takes `each` sequences that follow one another.
+    const int each = (a.B + 63) / 64, from = min(lane * each, a.B), to = min(from + each, a.B);
+    auto costs = [&](int i) {
       int len;
       bool bad;
-      x += seq_tiles<kPaged>(a, i, len, bad);
+      return cost(a, seq_tiles<kPaged>(a, i, len, bad)) * heads;
+    };
+    long long mine = 0;
+    for (int i = from; i < to; ++i) mine += costs(i);
+    long long upto = mine;
+    for (int i = 1; i < 64; i *= 2) {
+      const long long y = __shfl_up(upto, i);
+      if (lane >= i) upto += y;
     }
-    const int64_t units = block_sum(x, sh, kSplitWaves) * heads, run = quota(a, units);
+    const int64_t units = uniform(__shfl(upto, 63)), run = uniform(quota(a, units));
     const int64_t u = static_cast<int64_t>(blockIdx.x) * run;
+    if (blockIdx.x == 0 && w == 0) {  // where each sequence begins, for the join
+      int64_t at = upto - mine;
+      for (int i = from; i < to; ++i) {
+        a.before[i] = at;
+        at += costs(i);
+      }
+      if (lane == 63) a.before[a.B] = units;
+    }
     if (u >= units) return;
     left = units - u < run ? units - u : run;
-    // The sequence that tile u is in.
-    int64_t base = 0;
-    for (int i0 = 0; i0 < a.B; i0 += 64 * kSplitWaves) {
-      int len;
-      bool bad;
-      const int64_t n = i0 + tid < a.B ? seq_tiles<kPaged>(a, i0 + tid, len, bad) * int64_t{heads} : 0;
-      long long s = n;
-      for (int i = 1; i < 64; i *= 2) {
-        const long long y = __shfl_up(s, i);
-        if (lane >= i) s += y;
-      }
-      __syncthreads();
-      if (lane == 63) sh[w] = s;
-      __syncthreads();
-      int64_t before = base;
-      for (int i = 0; i < kSplitWaves; ++i) {
-        if (i < w) before += sh[i];
-        base += sh[i];
-      }
-      if (u >= before + s - n && u < before + s) {
-        sh[kSplitWaves] = i0 + tid;
-        sh[kSplitWaves + 1] = u - (before + s - n);
-      }
-      if (base > u) break;
-    }
-    __syncthreads();
-    b = __builtin_amdgcn_readfirstlane(static_cast<int>(sh[kSplitWaves]));
-    off = sh[kSplitWaves + 1];
+    // The lane whose sequences u is in, and which of them.
+    const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(u < upto));
+    int64_t base = uniform(__shfl(upto - mine, at));
+    b = __builtin_amdgcn_readfirstlane(at * each);
+    for (int64_t c = uniform(costs(b)); u >= base + c; c = uniform(costs(b))) base += c, ++b;
+    off = u - base;
   }
 
   while (true) {
@@ -434,22 +415,26 @@ split_kernel(SplitArgs a) {
     bool bad;
     const int n = __builtin_amdgcn_readfirstlane(seq_tiles<kPaged>(a, b, len, bad));
     len = __builtin_amdgcn_readfirstlane(len);
-    int hh;
+    int hh, t0 = 0, t1 = n;
     if (a.wgs == 0) {
       hh = static_cast<int>(blockIdx.x) % heads;
-      off = 0;
     } else {
       if (left <= 0) return;
-      if (n == 0 || off >= static_cast<int64_t>(n) * heads) {
-        off -= static_cast<int64_t>(n) * heads;
+      const int64_t each = cost(a, n);
+      if (off >= each * heads) {
+        off -= each * heads;
         ++b;
         continue;
       }
-      hh = __builtin_amdgcn_readfirstlane(static_cast<int>(off / n));
-      off -= static_cast<int64_t>(hh) * n;
+      hh = __builtin_amdgcn_readfirstlane(static_cast<int>(off / each));
+      // The run's part of this head, [in, in + take) of begin + n: the tiles are what is past `begin`.
+      const int64_t in = off - each * hh, take = left < each - in ? left : each - in;
+      t0 = __builtin_amdgcn_readfirstlane(static_cast<int>(in > a.begin ? in - a.begin : 0));
+      t1 = __builtin_amdgcn_readfirstlane(static_cast<int>(in + take > a.begin ? in + take - a.begin : 0));
+      left -= take;
+      off += take;
+      if (t0 == t1) continue;
     }
-    const int t0 = __builtin_amdgcn_readfirstlane(static_cast<int>(off));
-    const int t1 = __builtin_amdgcn_readfirstlane(left < n - t0 ? t0 + static_cast<int>(left) : n);
     const int kvh = hh / a.RB, r0 = hh % a.RB * kRowsMax;
     const int rows = min(a.G * a.SQ - r0, kRowsMax);
 
@@ -476,8 +461,7 @@ split_kernel(SplitArgs a) {
       Half x;
       x.live = min(len - 16 * at, 16);
       if constexpr (kPaged) {
-        const unsigned pi = (__umulhi(static_cast<unsigned>(at), a.div_magic) + at) >> a.div_shift;
-        const int slot = 16 * (at - static_cast<int>(pi) * (a.page_size / 16));
+        const int pi = divide(at, a.by_page), slot = 16 * (at - pi * (a.page_size / 16));
         int page = __builtin_amdgcn_readfirstlane(a.table[b * a.table_stride + pi]);
         if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pages)) page = 0, wrong = 1;
         x.k = kp + page * a.ks[0] + slot * a.ks[2];
@@ -585,8 +569,6 @@ split_kernel(SplitArgs a) {
       return;
     }
     __syncthreads();
-    left -= t1 - t0;
-    off = static_cast<int64_t>(hh + 1) * n;
   }
 }
 
@@ -595,7 +577,6 @@ split_kernel(SplitArgs a) {
 template <typename Q, int D, bool kPaged>
 __global__ void __launch_bounds__(256) join_kernel(SplitArgs a) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
-  __shared__ int64_t sh[4];
   __shared__ __attribute__((aligned(16))) float so[kGroups][D];
   __shared__ float sm[kGroups], sl[kGroups];
   const int tid = threadIdx.x, d = tid % kLanes * 4, grp = tid / kLanes;
@@ -612,10 +593,8 @@ __global__ void __launch_bounds__(256) join_kernel(SplitArgs a) {
     if (tid == 0) put_lse(a, b, head, q, 0.0f, bad ? z : 0.0f);
     return;
   }
-  int64_t before, all;
-  tiles_before<kPaged>(a, b, sh, before, all);
-  const int64_t heads = static_cast<int64_t>(a.HK) * a.RB, run = quota(a, all * heads);
-  const int64_t u0 = before * heads + static_cast<int64_t>(hh) * n;
+  const int64_t run = quota(a, a.before[a.B]);
+  const int64_t u0 = a.before[b] + static_cast<int64_t>(hh) * (n + a.begin) + a.begin;
   const int w0 = static_cast<int>(u0 / run), w1 = static_cast<int>((u0 + n - 1) / run);
   if (w0 == w1) return;  // written by its one workgroup
   const int64_t pitch = static_cast<int64_t>(a.part_rows) * (D + 4);
@@ -623,15 +602,30 @@ __global__ void __launch_bounds__(256) join_kernel(SplitArgs a) {
   auto slot = [&](int w) { return row + (static_cast<int64_t>(w) * 2 + (w == w0 ? 1 : 0)) * pitch; };
   float m = kNegInf, l = 0.0f;
   f4 o{};
-  for (int w = w0 + grp; w <= w1; w += kGroups) {
-    const float* p = slot(w);
-    const float my = p[D], ly = p[D + 1];
-    const f4 oy = ld4(p + d);
-    const float to = fmaxf(m, my);
-    const float f = m == kNegInf ? 0.0f : exp2_hw(m - to), fy = my == kNegInf ? 0.0f : exp2_hw(my - to);
-    o = (f == 0.0f ? f4{} : o * f) + (fy == 0.0f ? f4{} : oy * fy);
-    l = (m == kNegInf ? l : l * f) + (my == kNegInf ? ly : ly * fy);
-    m = to;
+  constexpr int kAtOnce = 4;  // parts in flight
+  for (int w = w0 + grp; w <= w1; w += kGroups * kAtOnce) {
+    float ms[kAtOnce], ls[kAtOnce];
+    f4 os[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const float* p = slot(min(w + i * kGroups, w1));
+      ms[i] = p[D], ls[i] = p[D + 1], os[i] = ld4(p + d);
+    }
+    const float before = m;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (w + i * kGroups > w1) ms[i] = kNegInf, ls[i] = 0.0f;
+      m = fmaxf(m, ms[i]);
+    }
+    const float f = before == kNegInf ? 0.0f : exp2_hw(before - m);
+    o *= f, l *= before == kNegInf ? 1.0f : f;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      // (Sums without a score are 0; l may still be NaN, for a page.)
+      const float fi = ms[i] == kNegInf ? 0.0f : exp2_hw(ms[i] - m);
+      l += ms[i] == kNegInf ? ls[i] : ls[i] * fi;
+      o += fi == 0.0f ? f4{} : os[i] * fi;
+    }
   }
   st4(&so[grp][d], o);
   if (d == 0) sm[grp] = m, sl[grp] = l;
@@ -651,12 +645,12 @@ __global__ void __launch_bounds__(256) join_kernel(SplitArgs a) {
 
 template <typename Q, typename C, int D, bool kPaged>
 int run_split(const SplitArgs& a, hipStream_t stream) {
-  constexpr int kWaves = 2;
   const int64_t pairs = static_cast<int64_t>(a.B) * a.HK * a.RB;
   SplitArgs args = a;
+  if (args.wgs > 0) args.wgs = 256 * kOccupancy<Q, C, D>;
   void* kargs[] = {&args};
-  const unsigned grid = static_cast<unsigned>(a.wgs == 0 ? pairs : a.wgs);
-  hipError_t err = hipLaunchKernel(reinterpret_cast<const void*>(split_kernel<Q, C, D, kPaged, kWaves>),
+  const unsigned grid = static_cast<unsigned>(args.wgs == 0 ? pairs : args.wgs);
+  hipError_t err = hipLaunchKernel(reinterpret_cast<const void*>(split_kernel<Q, C, D, kPaged>),
                                    dim3(grid), dim3(64 * kSplitWaves), kargs, 0, stream);
   if (err != hipSuccess || a.wgs == 0) return static_cast<int>(err);
   const unsigned rows = static_cast<unsigned>(static_cast<int64_t>(a.B) * a.H * a.SQ);
@@ -678,10 +672,12 @@ SplitPlan split_plan(int64_t b, int64_t hk, int64_t rows, int64_t d, int64_t cap
   p.row_blocks = static_cast<int>((rows + kRowsMax - 1) / kRowsMax);
   p.part_rows = static_cast<int>(rows < kRowsMax ? rows : kRowsMax);
   const int64_t tiles = (capacity + kTile - 1) / kTile;
-  p.min_run = 2 * kSplitWaves;
+  p.min_run = kSplitWaves;
+  p.begin = kSplitWaves;
   // One workgroup per key head where no sequence can have more than a few tiles per wave.
   p.wgs = tiles <= 4 * kSplitWaves ? 0 : 1024;
-  p.bytes = static_cast<size_t>(p.wgs) * 2 * p.part_rows * static_cast<size_t>(d + 4) * sizeof(float);
+  p.before = static_cast<size_t>(p.wgs) * 2 * p.part_rows * static_cast<size_t>(d + 4) * sizeof(float);
+  p.bytes = p.wgs == 0 ? 0 : p.before + static_cast<size_t>(b + 1) * sizeof(int64_t);
   return p;
 }
 

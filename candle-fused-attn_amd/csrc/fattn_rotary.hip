@@ -11,6 +11,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "fattn_internal.h"
@@ -19,8 +20,8 @@ namespace fattn {
 namespace {
 
 constexpr int kRotThreads = 256;
-constexpr int kMaxTokens = 16;   // tokens of a workgroup
-constexpr int kMaxAngles = 1024; // angles of a workgroup (LDS: 8 bytes each)
+constexpr int kMaxTokens = 64;    // tokens of a workgroup
+constexpr int kMaxAngles = 2048;  // angles of a workgroup (LDS: 8 bytes each)
 constexpr int kUnroll = 4;       // items a thread has in flight
 
 // cos and sin of p f, times the magnitude. The angle is formed and reduced in 64 bits, since in 32 one
@@ -69,20 +70,60 @@ __device__ __forceinline__ float turned(float x, float c, float y) {
   return r;
 }
 
-// A workgroup: `tokens` tokens, and the share blockIdx.y of their items. An item is VEC pairs of a
-// rotated head in the half layout (two vectors, n apart), else VEC values. Items of a token, part by
-// part and head by head, run over a head's values, so a wave reads whole rows.
+// A workgroup: `tokens` tokens of one operand (blockIdx.y: the operand, and which share of the items). An
+// item is VEC pairs of a rotated head in the half layout (two vectors, n apart), else VEC values; a head's
+// items follow one another, so a wave moves whole rows. The first items are loaded before the angles
+// are formed, over whose latency they come in.
 template <typename T, typename C, int VEC, bool kInterleaved, bool kPaged>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotaryArgs a) {
   __shared__ float2 cs[kMaxAngles];
-  __shared__ int64_t pos_of[kMaxTokens], at_of[2][kMaxTokens];  // at: k's and v's place in the pages
-  __shared__ int seq_of[kMaxTokens], in_of[kMaxTokens];
+  __shared__ int64_t at_of[kMaxTokens];  // paged: the token's slot, -1: none
+  __shared__ int64_t pos_of[kMaxTokens];
   const int tid = threadIdx.x, n = a.pairs;
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens, all = static_cast<int64_t>(a.B) * a.S;
   const int nt = static_cast<int>(all - t0 < a.tokens ? all - t0 : a.tokens);
+  const int y = static_cast<int>(blockIdx.y);
+  const int pi = y < a.first_share[1] ? 0 : y < a.first_share[2] ? 1 : 2;
+  const RotaryPart& part = a.part[pi];
+  const bool to_pages = kPaged && pi != 0;  // (part 0 is q)
+  const bool turns = part.rotate != 0;
+  // A head's items: its turned values first, then the copies.
+  const int turned_items = kInterleaved ? 2 * n / VEC : n / VEC;
+  const int of = a.items[pi], per = of * part.heads, items = nt * per;
+  const int shares = a.first_share[pi + 1] - a.first_share[pi];
+  const int share = (items + shares - 1) / shares;
+  const int first = (y - a.first_share[pi]) * share;
+  const int last = first + share < items ? first + share : items;
+
+  typedef Vec<T, VEC> In;
+  struct Item {
+    In x[2];
+    int64_t to;     // (not the pages': the row's offset in y)
+    int t, e, head; // token, first value (-1: no item), head
+  };
+  Item it[kUnroll];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int item = base + u * kRotThreads;
+      it[u].e = -1;
+      if (item >= last) continue;
+      const int t = divide(item, a.by_per[pi]);
+      const int r = item - t * per, head = divide(r, a.by_items[pi]), c = r - head * of;
+      const int e = turns && c >= turned_items ? 2 * n + (c - turned_items) * VEC : c * VEC;
+      const int tok = static_cast<int>(t0) + t, b = divide(tok, a.by_seq), i = tok - b * a.S;
+      it[u].t = t, it[u].e = e, it[u].head = head;
+      it[u].to = b * part.ys[0] + head * part.ys[1] + i * part.ys[2];
+      const T* from = static_cast<const T*>(part.x) + b * part.xs[0] + head * part.xs[1] +
+                      i * part.xs[2] + e;
+      it[u].x[0] = *reinterpret_cast<const In*>(from);
+      if (!kInterleaved && turns && e < n) it[u].x[1] = *reinterpret_cast<const In*>(from + n);
+    }
+  };
+  load(first + tid);
+
   if (tid < nt) {
-    const int64_t t = t0 + tid;
-    const int b = static_cast<int>(t / a.S), i = static_cast<int>(t % a.S);
+    const int tok = static_cast<int>(t0) + tid, b = divide(tok, a.by_seq), i = tok - b * a.S;
     int64_t p;
     if constexpr (kPaged) {
       const int held = a.lengths[b];
@@ -94,112 +135,63 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotaryArgs a) {
       if (counted && held >= 0 && p / a.page_size < a.table_width) {
         page = a.table[b * a.table_stride + p / a.page_size];
       }
-      const bool live = page >= 0 && page < a.pages;
-      const int64_t slot = p % a.page_size;
-      at_of[0][tid] = live ? page * a.page_strides[0] + slot * a.page_strides[2] : -1;
-      at_of[1][tid] = live ? page * a.page_strides[3] + slot * a.page_strides[5] : -1;
+      const int64_t* st = a.page_strides + (pi == 2 ? 3 : 0);
+      at_of[tid] = page >= 0 && page < a.pages ? page * st[0] + p % a.page_size * st[2] : -1;
     } else {
       const int64_t at = b * a.pos_strides[0] + i * a.pos_strides[1];
       p = a.pos64 ? static_cast<const int64_t*>(a.positions)[at]
                   : static_cast<const int32_t*>(a.positions)[at];
     }
-    pos_of[tid] = p, seq_of[tid] = b, in_of[tid] = i;
+    pos_of[tid] = p;
   }
   __syncthreads();
-  for (int i = tid; i < nt * n; i += kRotThreads) {
-    float2 x = turn(static_cast<double>(pos_of[i / n]), a.frequencies[i % n], a.magnitude);
-    if (a.inverse) x.y = -x.y;
-    cs[i] = x;
+  if (turns) {
+    for (int i = tid; i < nt * n; i += kRotThreads) {
+      const int t = divide(i, a.by_pairs);
+      float2 x = turn(static_cast<double>(pos_of[t]), a.frequencies[i - t * n], a.magnitude);
+      if (a.inverse) x.y = -x.y;
+      cs[i] = x;
+    }
+    __syncthreads();
   }
-  __syncthreads();
 
-  typedef Vec<T, VEC> In;
-  // Items per head: rotated ones first, then copies of the rest.
-  const int turns = kInterleaved ? 2 * n / VEC : n / VEC, rest = (a.D - 2 * n) / VEC, plain = a.D / VEC;
-  const int n0 = a.part[0].heads * (a.part[0].rotate ? turns + rest : plain);
-  const int n1 = a.part[1].heads * (a.part[1].rotate ? turns + rest : plain);
-  const int n2 = a.part[2].heads * (a.part[2].rotate ? turns + rest : plain);
-  const int per = n0 + n1 + n2, items = nt * per;
-  const int share = (items + static_cast<int>(gridDim.y) - 1) / static_cast<int>(gridDim.y);
-  const int first = static_cast<int>(blockIdx.y) * share;
-  const int last = first + share < items ? first + share : items;
-
-  struct Item {
-    In x[2];
-    void* to;   // null: nothing to write
-    int angle;  // of the first pair, -1: a copy
-    bool own;   // the row is of the activations' type, not the cache's
+  auto store = [&](auto* base, const Item& x, int64_t at) {
+    typedef std::remove_pointer_t<decltype(base)> R;
+    R* out = base + at + x.e;
+    const float2* w = cs + x.t * n + (kInterleaved ? x.e / 2 : x.e);
+    Vec<R, VEC> y;
+    if (!turns || x.e >= (kInterleaved ? 2 * n : n)) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) y.v[i] = convert<R, T>(x.x[0].v[i]);
+    } else if constexpr (kInterleaved) {
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) {
+        const float p = static_cast<float>(x.x[0].v[2 * i]), q = static_cast<float>(x.x[0].v[2 * i + 1]);
+        y.v[2 * i] = static_cast<R>(turned(p, w[i].x, -(q * w[i].y)));
+        y.v[2 * i + 1] = static_cast<R>(turned(q, w[i].x, p * w[i].y));
+      }
+    } else {
+      Vec<R, VEC> z;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float p = static_cast<float>(x.x[0].v[i]), q = static_cast<float>(x.x[1].v[i]);
+        y.v[i] = static_cast<R>(turned(p, w[i].x, -(q * w[i].y)));
+        z.v[i] = static_cast<R>(turned(q, w[i].x, p * w[i].y));
+      }
+      *reinterpret_cast<Vec<R, VEC>*>(out + n) = z;
+    }
+    *reinterpret_cast<Vec<R, VEC>*>(out) = y;
   };
   for (int base = first + tid; base < last; base += kRotThreads * kUnroll) {
-    Item it[kUnroll];
+    if (base != first + tid) load(base);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int item = base + u * kRotThreads;
-      it[u].to = nullptr, it[u].angle = -1, it[u].own = true;
-      if (item >= last) continue;
-      const int t = item / per;
-      int r = item % per;
-      const int pi = r < n0 ? 0 : r < n0 + n1 ? 1 : 2;
-      r -= pi == 0 ? 0 : pi == 1 ? n0 : n0 + n1;
-      const RotaryPart& part = a.part[pi];
-      const int of = part.rotate ? turns + rest : plain, head = r / of, c = r % of;
-      const bool rotated = part.rotate && c < turns;
-      // The item's first value in its head.
-      const int e = part.rotate && !rotated ? 2 * n + (c - turns) * VEC : c * VEC;
-      const int64_t b = seq_of[t], i = in_of[t];
-      const T* from = static_cast<const T*>(part.x) + b * part.xs[0] + head * part.xs[1] +
-                      i * part.xs[2] + e;
-      if (kPaged && pi != 0) {
-        const int64_t at = at_of[pi - 1][t];
-        if (at < 0) continue;
-        it[u].to = static_cast<C*>(part.y) + at + head * a.page_strides[3 * pi - 2] + e;
-        it[u].own = false;
+      if (it[u].e < 0) continue;
+      if (to_pages) {
+        const int64_t at = at_of[it[u].t];
+        if (at >= 0) store(static_cast<C*>(part.y), it[u], at + it[u].head * a.page_strides[pi == 2 ? 4 : 1]);
       } else {
-        it[u].to = static_cast<T*>(part.y) + b * part.ys[0] + head * part.ys[1] + i * part.ys[2] + e;
-      }
-      it[u].x[0] = *reinterpret_cast<const In*>(from);
-      if (rotated) {
-        if constexpr (!kInterleaved) it[u].x[1] = *reinterpret_cast<const In*>(from + n);
-        it[u].angle = t * n + (kInterleaved ? e / 2 : e);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (it[u].to == nullptr) continue;
-      const int at = it[u].angle;
-      auto put = [&](auto* out) {
-        typedef std::remove_pointer_t<decltype(out)> R;
-        Vec<R, VEC> y;
-        if (at < 0) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) y.v[i] = convert<R, T>(it[u].x[0].v[i]);
-        } else if constexpr (kInterleaved) {
-#pragma unroll
-          for (int i = 0; i < VEC / 2; ++i) {
-            const float2 w = cs[at + i];
-            const float p = static_cast<float>(it[u].x[0].v[2 * i]);
-            const float q = static_cast<float>(it[u].x[0].v[2 * i + 1]);
-            y.v[2 * i] = static_cast<R>(turned(p, w.x, -(q * w.y)));
-            y.v[2 * i + 1] = static_cast<R>(turned(q, w.x, p * w.y));
-          }
-        } else {
-          Vec<R, VEC> z;
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float2 w = cs[at + i];
-            const float p = static_cast<float>(it[u].x[0].v[i]);
-            const float q = static_cast<float>(it[u].x[1].v[i]);
-            y.v[i] = static_cast<R>(turned(p, w.x, -(q * w.y)));
-            z.v[i] = static_cast<R>(turned(q, w.x, p * w.y));
-          }
-          *reinterpret_cast<Vec<R, VEC>*>(out + n) = z;
-        }
-        *reinterpret_cast<Vec<R, VEC>*>(out) = y;
-      };
-      if (!kPaged || it[u].own) {
-        put(static_cast<T*>(it[u].to));
-      } else {
-        put(static_cast<C*>(it[u].to));
+        store(static_cast<T*>(part.y), it[u], it[u].to);
       }
     }
   }
@@ -239,26 +231,32 @@ int launch_rotary(RotaryArgs a, int dtype, int cache_dtype, int vec, void* strea
     fn = dtype == kF16 ? rotary_fn<_Float16, _Float16, true>(vec, il)
                        : rotary_fn<__bf16, __bf16, true>(vec, il);
   }
-  // Tokens per workgroup: about two rounds of items per thread, angles within LDS, and no more than
-  // leave 1024 workgroups; few tokens share out their items over blockIdx.y.
+  // Tokens per workgroup: about two rounds of items per thread for the operand of most heads, angles
+  // within LDS, and no more than leave 1024 workgroups, but an item for every thread; few tokens share
+  // out an operand's items.
   const int64_t all = static_cast<int64_t>(a.B) * a.S;
-  int64_t per = 0;
-  for (const RotaryPart& p : a.part) {
-    const int pairs = a.interleaved ? a.pairs : a.pairs / 2;
-    per += static_cast<int64_t>(p.heads) * ((p.rotate ? a.D - 2 * a.pairs + 2 * pairs : a.D) / vec);
+  int64_t most = 1;
+  for (int i = 0; i < 3; ++i) {
+    const int turned = a.interleaved ? 2 * a.pairs / vec : a.pairs / vec;
+    a.items[i] = a.part[i].rotate ? turned + (a.D - 2 * a.pairs) / vec : a.D / vec;
+    most = std::max<int64_t>(most, static_cast<int64_t>(a.items[i]) * a.part[i].heads);
   }
-  if (per == 0) per = 1;
-  int64_t tokens = 2 * kUnroll * kRotThreads / per;
-  if (a.pairs > 0 && tokens > kMaxAngles / a.pairs) tokens = kMaxAngles / a.pairs;
-  if (tokens > kMaxTokens) tokens = kMaxTokens;
-  if (tokens > all / 1024) tokens = all / 1024;
-  if (tokens < 1) tokens = 1;
+  const int64_t fill = (kRotThreads + most - 1) / most;
+  int64_t tokens = std::min(std::max(fill, all / 1024), std::max(fill, 2 * kUnroll * kRotThreads / most));
+  if (a.pairs > 0) tokens = std::min<int64_t>(tokens, kMaxAngles / a.pairs);
+  tokens = std::min<int64_t>(tokens, kMaxTokens);
   a.tokens = static_cast<int>(tokens);
   const int64_t blocks = (all + tokens - 1) / tokens;
-  int64_t shares = (tokens * per + kRotThreads - 1) / kRotThreads;
-  const int64_t want = (1024 + blocks - 1) / blocks;
-  if (shares > want) shares = want;
-  // (A workgroup's share of items stays far inside 32 bits.)
+  a.first_share[0] = 0;
+  for (int i = 0; i < 3; ++i) {
+    const int64_t per = static_cast<int64_t>(a.items[i]) * a.part[i].heads;
+    const int64_t rounds = (tokens * per + kRotThreads - 1) / kRotThreads;
+    const int64_t shares = std::min(rounds, (512 + blocks - 1) / blocks);
+    a.first_share[i + 1] = a.first_share[i] + static_cast<int>(shares);
+    a.by_per[i] = divider(per), a.by_items[i] = divider(a.items[i]);
+  }
+  a.by_seq = divider(a.S), a.by_pairs = divider(a.pairs);
+  const int shares = a.first_share[3];
   void* args[] = {&a};
   return static_cast<int>(hipLaunchKernel(fn, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(shares)),
                                           dim3(kRotThreads), args, 0,

@@ -48,6 +48,7 @@ EXPORTS = (
     "fattn_paged_attention",
     "fattn_cross_workspace_bytes",
     "fattn_cross_forward",
+    "fattn_cross_backward_workspace_bytes",
     "fattn_cross_backward",
     "fattn_last_error",
     "fattn_version",
@@ -114,12 +115,13 @@ def _declare(L: ctypes.CDLL) -> None:
     L.fattn_paged_attention_workspace_bytes.restype = SIZE
     L.fattn_paged_attention.argtypes = [C_INT, C_INT, I64, I64, I64, I64, P, P, P, P, P, P, P, I64, I64,
                                         P, I64, I64, P, C_FLOAT, P, SIZE, P]
-    L.fattn_cross_workspace_bytes.argtypes = [I64, I64, I64, I64, I64, I64]
-    L.fattn_cross_workspace_bytes.restype = SIZE
+    for name in ("fattn_cross_workspace_bytes", "fattn_cross_backward_workspace_bytes"):
+        getattr(L, name).argtypes = [I64, I64, I64, I64, I64, I64]
+        getattr(L, name).restype = SIZE
     L.fattn_cross_forward.argtypes = [P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, P, C_FLOAT, P, P,
                                       P, SIZE, P]
     L.fattn_cross_backward.argtypes = [P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, P, C_FLOAT, P, P,
-                                       P, P, P, P, P]
+                                       P, P, P, P, P, SIZE, P]
     L.fattn_bwd_status.argtypes = [P, SIZE, I64, I64, I64, P, ctypes.POINTER(C_INT)]
     for name in EXPORTS:
         if name not in ("fattn_last_error", "fattn_version") and "workspace" not in name:

@@ -50,10 +50,14 @@ class _FusedCrossAttention(torch.autograd.Function):
         dq, dkv = q.new_empty((b, sq, h, d)), q.new_empty((b, sk, 2, hk, d))
         gb, gs, gh, _ = grad.stride()
         keep, p = pack(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], gb, gh, gs)
-        launch(q, _lib.lib().fattn_cross_backward, q.data_ptr(), p, k.data_ptr(), p + 24, v.data_ptr(),
+        L = _lib.lib()
+        size = L.fattn_cross_backward_workspace_bytes(b, h, hk, sq, sk, d)
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        launch(q, L.fattn_cross_backward, q.data_ptr(), p, k.data_ptr(), p + 24, v.data_ptr(),
                p + 48, b, h, hk, sq, sk, d,
                key_lengths.data_ptr() if key_lengths is not None else None, ctx.scale, out.data_ptr(),
-               lse.data_ptr(), grad.data_ptr(), p + 72, dq.data_ptr(), dkv.data_ptr())
+               lse.data_ptr(), grad.data_ptr(), p + 72, dq.data_ptr(), dkv.data_ptr(),
+               ws.data_ptr() if size else None, size)
         dk, dv = dkv.transpose(1, 3).unbind(2)  # [b, kv_heads, sk, d] each
         return dq.transpose(1, 2), dk, dv, None, None
 

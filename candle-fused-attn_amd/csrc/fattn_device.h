@@ -71,6 +71,10 @@ struct FwdArgs {
   // Cross attention: the keys' length, query heads per key head, each sample's keys (null: SK).
   int SK, G;
   const int32_t* key_lengths;
+  // Chunks of the keys (1: none), their tiles; with chunks o is [nc][b, s, h, d] of the workspace and L
+  // goes to l_part, [nc][b, h, s].
+  int nc, chunk;
+  double* l_part;
 };
 
 }  // namespace

@@ -153,6 +153,8 @@ void test_hook_state(int64_t out[3]);
 // and return a hipError_t value as int (0 = launched).
 int launch_forward(View q, View k, View v, float* o, float* lse, int b, int h, int s, int d,
                    float scale, int causal, void* stream);
+// Whether a forward in which every workgroup walks all keys takes 64 queries per wave, not 32.
+bool wide_queries(int64_t bh, int s, int d);
 // Backward, step 2 (fattn_pair.hip): dK, dV and dQ. part, done, epoch_slot (a split-size workspace,
 // else null): with `defer` dQ goes to `part` for step 3, else to its rows, and `done` takes `epoch`
 // per 16-query tile. last: no step 3 follows. give_up_bh: a test hook's pair (-1: none).
@@ -243,14 +245,27 @@ SplitPlan split_plan(int64_t b, int64_t hk, int64_t rows, int64_t d, int64_t cap
 int launch_split(const SplitArgs& a, int dtype, int cache_dtype, int d, void* stream);
 
 // Cross attention by blocks of 128 queries and 128 keys (fattn_cross.hip). dq [b, sq, h, d], dkv
-// [b, sk, 2, hk, d].
+// [b, sk, 2, hk, d]. The plans: whether the forward takes the split kernel (few queries) and not blocks;
+// into how many chunks the blocks' walks are cut (1: none) and their length, in tiles or steps of 32 rows;
+// the workspace that the chunks' outputs take (16-byte aligned), and where its second part begins.
+struct CrossForwardPlan {
+  bool split;
+  int nc, chunk;
+  size_t l_part, bytes;
+};
+struct CrossBackwardPlan {
+  int ncq, chq, nck, chk;
+  size_t k_part, bytes;
+};
+CrossForwardPlan cross_forward_plan(int64_t b, int64_t h, int64_t hk, int64_t sq, int64_t sk, int64_t d);
+CrossBackwardPlan cross_backward_plan(int64_t b, int64_t h, int64_t hk, int64_t sq, int64_t sk, int64_t d);
 int launch_cross_forward(View q, View k, View v, float* o, float* lse, int b, int h, int hk, int sq,
-                         int sk, int d, const int32_t* key_lengths, float scale, void* stream);
+                         int sk, int d, const int32_t* key_lengths, float scale,
+                         const CrossForwardPlan& plan, void* workspace, void* stream);
 int launch_cross_backward(View q, View k, View v, View d_o, const float* o, const float* lse, float* dq,
                           float* dkv, int b, int h, int hk, int sq, int sk, int d,
-                          const int32_t* key_lengths, float scale, void* stream);
-// Whether the forward takes the split kernel (few queries) and not blocks.
-bool cross_splits(int64_t b, int64_t h, int64_t hk, int64_t sq, int64_t sk, int64_t d);
+                          const int32_t* key_lengths, float scale, const CrossBackwardPlan& plan,
+                          void* workspace, void* stream);
 int64_t cross_blocks(int64_t heads, int64_t s);  // workgroups over `heads` (b, head) of s rows
 
 // Sets this thread's message (fattn_last_error) and returns `code`; done() clears it and returns 0.

@@ -134,6 +134,12 @@ int run_rotary(const char* who, fattn::RotaryArgs& a, int dtype, int cache_dtype
   return fattn::done();
 }
 
+int check_workspace(const char* who, const void* workspace, size_t bytes, size_t need) {
+  if (need == 0 || (workspace && aligned(workspace, 16) && bytes >= need)) return 0;
+  return set_error(FATTN_EWORKSPACE, "%s: a 16-byte aligned workspace of at least %zu bytes expected", who,
+                   need);
+}
+
 // Shared by the paged and the cross attention: the plan, the workspace, the launch.
 int run_split(const char* who, fattn::SplitArgs& a, int dtype, int cache_dtype, int64_t d,
               int64_t capacity, void* workspace, size_t workspace_bytes, void* stream) {
@@ -143,10 +149,7 @@ int run_split(const char* who, fattn::SplitArgs& a, int dtype, int cache_dtype, 
       static_cast<int64_t>(a.B) * a.H * a.SQ > kMaxGrid) {
     return set_error(FATTN_ERANGE, "%s: the grid exceeds the launch limit", who);
   }
-  if (plan.bytes > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < plan.bytes)) {
-    return set_error(FATTN_EWORKSPACE, "%s: a 16-byte aligned workspace of at least %zu bytes expected",
-                     who, plan.bytes);
-  }
+  if (int rc = check_workspace(who, workspace, workspace_bytes, plan.bytes)) return rc;
   a.RB = plan.row_blocks, a.part_rows = plan.part_rows, a.wgs = plan.wgs, a.min_run = plan.min_run;
   a.begin = plan.begin;
   a.part = static_cast<float*>(workspace);
@@ -344,8 +347,13 @@ int fattn_paged_attention(int dtype, int cache_dtype, int64_t b, int64_t heads, 
 size_t fattn_cross_workspace_bytes(int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk,
                                    int64_t d) {
   if (!split_shape(b, heads, kv_heads, d) || sq < 0 || sk < 0) return 0;
-  if (!fattn::cross_splits(b, heads, kv_heads, sq, sk, d)) return 0;
-  return fattn::split_plan(b, kv_heads, heads / kv_heads * sq, d, sk).bytes;
+  return fattn::cross_forward_plan(b, heads, kv_heads, sq, sk, d).bytes;
+}
+
+size_t fattn_cross_backward_workspace_bytes(int64_t b, int64_t heads, int64_t kv_heads, int64_t sq,
+                                            int64_t sk, int64_t d) {
+  if (!split_shape(b, heads, kv_heads, d) || sq < 0 || sk < 0) return 0;
+  return fattn::cross_backward_plan(b, heads, kv_heads, sq, sk, d).bytes;
 }
 
 int fattn_cross_forward(const float* q, const int64_t q_strides[3], const float* k,
@@ -364,7 +372,9 @@ int fattn_cross_forward(const float* q, const int64_t q_strides[3], const float*
   if (!aligned(out, 16)) return set_error(FATTN_EALIGN, "%s: rows must be 16-byte aligned", kCross);
   const int B = static_cast<int>(b), H = static_cast<int>(heads), HK = static_cast<int>(kv_heads);
   const int SQ = static_cast<int>(sq), SK = static_cast<int>(sk);
-  if (fattn::cross_splits(b, heads, kv_heads, sq, sk, d)) {
+  const fattn::CrossForwardPlan plan = fattn::cross_forward_plan(b, heads, kv_heads, sq, sk, d);
+  if (int rc = check_workspace(kCross, workspace, workspace_bytes, plan.bytes)) return rc;
+  if (plan.split) {
     fattn::SplitArgs a{};
     a.q = q, a.k = k, a.v = v, a.o = out, a.lse = lse;
     a.qs[0] = c.q.sb, a.qs[1] = c.q.sh, a.qs[2] = c.q.ss;
@@ -375,7 +385,8 @@ int fattn_cross_forward(const float* q, const int64_t q_strides[3], const float*
     return run_split(kCross, a, FATTN_F32, FATTN_F32, d, sk, workspace, workspace_bytes, stream);
   }
   const int err = fattn::launch_cross_forward(c.q, c.k, c.v, out, lse, B, H, HK, SQ, SK,
-                                              static_cast<int>(d), key_lengths, scale, stream);
+                                              static_cast<int>(d), key_lengths, scale, plan, workspace,
+                                              stream);
   if (err) return fattn::hip_error(err, kCross, "forward launch");
   return fattn::done();
 }
@@ -385,7 +396,7 @@ int fattn_cross_backward(const float* q, const int64_t q_strides[3], const float
                          int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d,
                          const int32_t* key_lengths, float scale, const float* out, const float* lse,
                          const float* d_o, const int64_t do_strides[3], float* dq, float* dkv,
-                         void* stream) {
+                         void* workspace, size_t workspace_bytes, void* stream) {
   Cross c{};
   bool none = false;
   if (int rc = cross_operands(c, q, q_strides, k, k_strides, v, v_strides, b, heads, kv_heads, sq, sk, d,
@@ -404,10 +415,12 @@ int fattn_cross_backward(const float* q, const int64_t q_strides[3], const float
   if (!slice_fits(c.q, sq, d) || !slice_fits(g, sq, d) || sq * heads * d > int64_t{UINT32_MAX}) {
     return set_error(FATTN_ERANGE, "%s: the queries of one sample span more than 4 GiB", kCross);
   }
+  const fattn::CrossBackwardPlan plan = fattn::cross_backward_plan(b, heads, kv_heads, sq, sk, d);
+  if (int rc = check_workspace(kCross, workspace, workspace_bytes, plan.bytes)) return rc;
   const int err = fattn::launch_cross_backward(
       c.q, c.k, c.v, g, out, lse, dq, dkv, static_cast<int>(b), static_cast<int>(heads),
       static_cast<int>(kv_heads), static_cast<int>(sq), static_cast<int>(sk), static_cast<int>(d),
-      key_lengths, scale, stream);
+      key_lengths, scale, plan, workspace, stream);
   if (err) return fattn::hip_error(err, kCross, "backward launch");
   return fattn::done();
 }

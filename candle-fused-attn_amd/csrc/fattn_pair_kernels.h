@@ -463,6 +463,9 @@ constexpr float kMaxScale = 0x1p127f;   // of a running scale, and where it star
 
 // Cross attention (kCross): keys and values of their own length and number of heads, of which sample b
 // sees its first key_count() and head h reads key_head(). Else every length is S and every head its own.
+// Where the blocks are too few to fill the chip their walks are cut into chunks, each a workgroup with an
+// output of its own in the workspace: the forward's O and L over a part of the keys, dQ of a part of the
+// keys, dK and dV of a part of the queries. Joins (fattn_cross.hip) sum them in order.
 template <bool kCross, typename Args>
 __device__ __forceinline__ int key_count(const Args& a, int b) {
   if constexpr (kCross) {
@@ -487,15 +490,24 @@ __device__ __forceinline__ int key_head(const Args& a, int h) {
   return kCross ? h / a.G : h;
 }
 
-// O and L of 32 queries from qg in fp32. `store` takes O's sums and their factor.
+// L of a row: of a chunk in 64 bits, since the join takes differences of it.
+template <bool kCross>
+__device__ __forceinline__ void put_l(const FwdArgs& a, int64_t at, double L) {
+  if (kCross && a.l_part != nullptr) {
+    a.l_part[at] = L;
+  } else {
+    __builtin_nontemporal_store(static_cast<float>(L), a.lse + at);
+  }
+}
+// O and L of 32 queries from qg over SK keys from key0, in fp32. `store` takes O's sums and their factor.
 template <int D, bool kCausal, bool kCross, typename Store>
-__device__ __forceinline__ void fwd_rows_fp32(const FwdArgs& a, int b, int h, int qg, float* so,
-                                              int lane, Store store) {
-  const int j = lane & 31, g = lane >> 5, S = a.S, SK = key_count<kCross>(a, b), qi = qg + j;
+__device__ __forceinline__ void fwd_rows_fp32(const FwdArgs& a, int b, int h, int qg, int key0, int SK,
+                                              float* so, int lane, Store store) {
+  const int j = lane & 31, g = lane >> 5, S = a.S, qi = qg + j;
   const int hk = key_head<kCross>(a, h);
   const float* qp = a.q.p + b * a.q.sb + h * a.q.sh + min(qi, S - 1) * a.q.ss;
-  const float* kp = a.k.p + b * a.k.sb + hk * a.k.sh;
-  const float* vp = a.v.p + b * a.v.sb + hk * a.v.sh;
+  const float* kp = a.k.p + b * a.k.sb + hk * a.k.sh + (kCross ? key0 * a.k.ss : 0);
+  const float* vp = a.v.p + b * a.v.sb + hk * a.v.sh + (kCross ? key0 * a.v.ss : 0);
   const float sign = a.scale < 0.0f ? -1.0f : 1.0f, c2 = fabsf(a.scale) * kLog2e;
   f16v acc[D / 32];
 #pragma unroll
@@ -531,7 +543,7 @@ __device__ __forceinline__ void fwd_rows_fp32(const FwdArgs& a, int b, int h, in
   l = pair_sum(l);
   store(acc, 1.0f / l);
   if (g == 0 && qi < S) {
-    a.lse[(static_cast<int64_t>(b) * a.H + h) * S + qi] = m * fabsf(a.scale) + logf(l);
+    put_l<kCross>(a, (static_cast<int64_t>(b) * a.H + h) * S + qi, m * fabsf(a.scale) + logf(l));
   }
 }
 
@@ -559,10 +571,12 @@ fwd_pair_kernel(FwdArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int S = a.S, BH = a.B * a.H;
-  int qb, bh;
+  int qb, bh, chunk = 0;
   if constexpr (kCross) {
     int in;
-    const int pair = spread(static_cast<int>(blockIdx.x), BH / a.G, a.nqb * a.G, in);
+    const int pair = spread(static_cast<int>(blockIdx.x), BH / a.G, a.nqb * a.G * a.nc, in);
+    chunk = in / (a.nqb * a.G);
+    in -= chunk * (a.nqb * a.G);
     qb = in / a.G;
     bh = pair * a.G + in % a.G;
   } else if (kCausal) {
@@ -574,12 +588,24 @@ fwd_pair_kernel(FwdArgs a) {
     bh = id / a.nqb;
   }
   const int b = bh / a.H, h = bh % a.H, hk = key_head<kCross>(a, h);
-  const int SK = key_count<kCross>(a, b);
+  // The keys: all, or a chunk of them (key0 on), as if there were no others.
+  int SK = key_count<kCross>(a, b);
+  const int key0 = kCross ? chunk * a.chunk * kRows : 0;
+  if constexpr (kCross) {
+    if (a.nc > 1) {
+      SK = min(SK - key0, a.chunk * kRows);
+      if (SK <= 0) return;  // (the join knows)
+      a.o += chunk * (static_cast<int64_t>(BH) * S * D);
+      a.l_part += chunk * (static_cast<int64_t>(BH) * S);
+    }
+  }
   const int q0 = qb * kQ, qw0 = q0 + w * kWaveQ;
   const float* qp = a.q.p + b * a.q.sb + h * a.q.sh;
-  const Operand kop{reinterpret_cast<const char*>(a.k.p + b * a.k.sb + hk * a.k.sh),
+  const Operand kop{reinterpret_cast<const char*>(a.k.p + b * a.k.sb + hk * a.k.sh +
+                                                  (kCross ? key0 * a.k.ss : 0)),
                     static_cast<unsigned>(a.k.ss) * 4u};
-  const Operand vop{reinterpret_cast<const char*>(a.v.p + b * a.v.sb + hk * a.v.sh),
+  const Operand vop{reinterpret_cast<const char*>(a.v.p + b * a.v.sb + hk * a.v.sh +
+                                                  (kCross ? key0 * a.v.ss : 0)),
                     static_cast<unsigned>(a.v.ss) * 4u};
 
   if constexpr (kCross) {
@@ -781,7 +807,7 @@ fwd_pair_kernel(FwdArgs a) {
     };
     if (__builtin_amdgcn_ballot_w64(qi < S && !(probe_finite<kDT>(acc[n], l * 0.0f) == 0.0f)) !=
         0) {
-      fwd_rows_fp32<D, kCausal, kCross>(a, b, h, qg, so, late(lane),
+      fwd_rows_fp32<D, kCausal, kCross>(a, b, h, qg, key0, SK, so, late(lane),
                                 [&](const f16v (&x)[kDT], float inv) { store(x, inv, 1.0f); });
       continue;
     }
@@ -792,7 +818,7 @@ fwd_pair_kernel(FwdArgs a) {
       float f = l * pow2(-le);  // [1, 2), then [0.75, 1.5)
       if (f > 1.5f) f *= 0.5f, ++le;
       const double L = fma(static_cast<double>(m[n]), mr, fma(le, 0.6931471805599453, logf(f)));
-      __builtin_nontemporal_store(static_cast<float>(L), a.lse + static_cast<int64_t>(bh) * S + qi);
+      put_l<kCross>(a, static_cast<int64_t>(bh) * S + qi, L);
     }
   }
 }
@@ -853,6 +879,9 @@ struct BwdPairArgs {
   int SK, G;
   const int32_t* key_lengths;
   int nblk_q;
+  // Chunks of the key blocks' walks and of the query blocks' (1: none), their steps, and where a chunk's
+  // outputs go (dq, dkv of chunk c at c times their size).
+  int nck, chk, ncq, chq;
 };
 // Where a new scale puts the largest weight: 9 bits of room before the next one moves it, which costs
 // a pass over the sums (with 5, inputs of deviation 2: d 128 b64 h6 s240 259 us against 242, d 32 56.0 /
@@ -896,14 +925,15 @@ __device__ __forceinline__ float shifted_l(float L, float k) {
 }
 __device__ __forceinline__ int half_log2(int s) { return (32 - __builtin_clz(s)) / 2; }
 
-// dK and dV of 32 keys from kw0, dQ of 32 queries from qw0, in fp32 (without the scale).
+// dK and dV of 32 keys from kw0 (crossing: over the steps u0 .. u1 of the group's heads' tiles), dQ of 32
+// queries from qw0 (over SK keys from key0), in fp32 (without the scale).
 template <int D, bool kCausal, bool kCross>
-__device__ __forceinline__ void bwd_keys_fp32(const BwdPairArgs& a, int b, int hk, int kw0, float* so,
-                                              f16v (&dk)[D / 32], f16v (&dv)[D / 32], int lane) {
+__device__ __forceinline__ void bwd_keys_fp32(const BwdPairArgs& a, int b, int hk, int kw0, int u0, int u1,
+                                              float* so, f16v (&dk)[D / 32], f16v (&dv)[D / 32], int lane) {
   const int j = lane & 31, g = lane >> 5, S = a.S, SK = key_count<kCross>(a, b), key = kw0 + j;
   const float* kr = a.k.p + b * a.k.sb + hk * a.k.sh + min(key, SK - 1) * a.k.ss;
   const float* vr = a.v.p + b * a.v.sb + hk * a.v.sh + min(key, SK - 1) * a.v.ss;
-  int h = kCross ? hk * a.G : hk;
+  const int ntiles = (S + kRows - 1) / kRows, h = kCross ? hk * a.G + u0 / ntiles : hk;
   const float* qp = a.q.p + b * a.q.sb + h * a.q.sh;
   const float* gp = a.d_o.p + b * a.d_o.sb + h * a.d_o.sh;
   const float* op = a.o + (static_cast<int64_t>(b) * S * a.H + h) * D;
@@ -934,35 +964,37 @@ __device__ __forceinline__ void bwd_keys_fp32(const BwdPairArgs& a, int b, int h
     sum_fp32<D, kFull>(s, gp, a.d_o.ss, q0, S, live, so, dv, j, g);
     sum_fp32<D, kFull>(dp, qp, a.q.ss, q0, S, live, so, dk, j, g);
   };
-  auto walk = [&] {
-    int q0 = kCausal ? kw0 : 0;
-    if (kCausal) tile(Const<0>{}, q0), q0 += kRows;
-    for (; q0 + kRows <= S; q0 += kRows) tile(Const<1>{}, q0);
-    if (q0 < S) tile(Const<0>{}, q0);
-  };
   if constexpr (kCross) {
-    for (; h < (hk + 1) * a.G; ++h) {  // each of the key head's query heads
-      walk();
-      qp += a.q.sh, gp += a.d_o.sh, op += D, lp += S;
+    for (int u = u0, q0 = u0 % ntiles * kRows; u < u1; ++u) {
+      if (q0 + kRows <= S) {
+        tile(Const<1>{}, q0);
+      } else {
+        tile(Const<0>{}, q0);
+      }
+      q0 += kRows;
+      if (q0 >= S) q0 = 0, qp += a.q.sh, gp += a.d_o.sh, op += D, lp += S;
     }
     if (key >= SK) {
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt) dk[dt] = zero16(), dv[dt] = zero16();
     }
   } else {
-    walk();
+    int q0 = kCausal ? kw0 : 0;
+    if (kCausal) tile(Const<0>{}, q0), q0 += kRows;
+    for (; q0 + kRows <= S; q0 += kRows) tile(Const<1>{}, q0);
+    if (q0 < S) tile(Const<0>{}, q0);
   }
 }
 template <int D, bool kCausal, bool kCross>
-__device__ __forceinline__ void bwd_queries_fp32(const BwdPairArgs& a, int b, int h, int qw0,
-                                                 float* so, f16v (&dq)[D / 32], int lane) {
-  const int j = lane & 31, g = lane >> 5, S = a.S, SK = key_count<kCross>(a, b), qi = qw0 + j;
+__device__ __forceinline__ void bwd_queries_fp32(const BwdPairArgs& a, int b, int h, int qw0, int key0,
+                                                 int SK, float* so, f16v (&dq)[D / 32], int lane) {
+  const int j = lane & 31, g = lane >> 5, S = a.S, qi = qw0 + j;
   const int hk = key_head<kCross>(a, h);
   const int64_t qc = min(qi, S - 1);
   const float* qr = a.q.p + b * a.q.sb + h * a.q.sh + qc * a.q.ss;
   const float* gr = a.d_o.p + b * a.d_o.sb + h * a.d_o.sh + qc * a.d_o.ss;
-  const float* kp = a.k.p + b * a.k.sb + hk * a.k.sh;
-  const float* vp = a.v.p + b * a.v.sb + hk * a.v.sh;
+  const float* kp = a.k.p + b * a.k.sb + hk * a.k.sh + (kCross ? key0 * a.k.ss : 0);
+  const float* vp = a.v.p + b * a.v.sb + hk * a.v.sh + (kCross ? key0 * a.v.ss : 0);
   const float* orow = a.o + ((static_cast<int64_t>(b) * S + qc) * a.H + h) * D;
   const float L = a.lse[(static_cast<int64_t>(b) * a.H + h) * S + qc];
   float dd = 0.0f;
@@ -1008,7 +1040,8 @@ struct BwdSmem {
 };
 
 template <int D, bool kCausal, bool kSerial, int W, bool kCross>
-__device__ __forceinline__ void bwd_keys(const BwdPairArgs& a, BwdSmem<D, W>& sm, int item) {
+__device__ __forceinline__ void bwd_keys(const BwdPairArgs& a, BwdSmem<D, W>& sm, int item,
+                                         int chunk = 0) {
   constexpr int kKS = D / 16, kDT = D / 32;
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1021,7 +1054,8 @@ __device__ __forceinline__ void bwd_keys(const BwdPairArgs& a, BwdSmem<D, W>& sm
   if constexpr (kCross) {
     if (k0 >= SK || S == 0) {  // keys that no query sees
       for (int i = tid; i < min(a.SK - k0, W * kRows) * (D / 4); i += 64 * W) {
-        float* row = a.dkv + ((static_cast<int64_t>(b) * a.SK + k0 + i / (D / 4)) * 2 * HK + hk) * D;
+        float* row = a.dkv + ((static_cast<int64_t>(chunk) * a.B + b) * a.SK + k0 + i / (D / 4)) * 2 * HK * D +
+                     static_cast<int64_t>(hk) * D;
         st4(row + i % (D / 4) * 4, f4{});
         st4(row + static_cast<int64_t>(HK) * D + i % (D / 4) * 4, f4{});
       }
@@ -1036,7 +1070,9 @@ __device__ __forceinline__ void bwd_keys(const BwdPairArgs& a, BwdSmem<D, W>& sm
   const float* lp = a.lse + (kCross ? static_cast<int64_t>(b) * a.H + h : bh) * S;
   // The walk: step u takes tile t0 + u (causal: from the block's diagonal, W tiles, on).
   const int ntiles = (S + kRows - 1) / kRows, t0 = kCausal ? k0 / kRows : 0;
-  const int nsteps = G * (ntiles - t0);
+  // (Crossing: steps u0 .. of the group's heads' tiles end to end.)
+  const int u0 = kCross ? chunk * a.chk : 0;
+  const int nsteps = kCross ? min(G * ntiles - u0, a.chk) : ntiles - t0;
 
   const int kp = half_log2(SK);
   Stage<D, W> st;
@@ -1044,8 +1080,8 @@ __device__ __forceinline__ void bwd_keys(const BwdPairArgs& a, BwdSmem<D, W>& sm
   float lreg;
   // Step u's query head (past the last step: the last) and its first row.
   auto place = [&](int u, int& hh) {
-    hh = kCross ? min(u / ntiles, G - 1) : 0;
-    return (kCross ? u - hh * ntiles : t0 + u) * kRows;
+    hh = kCross ? min((u + u0) / ntiles, G - 1) : 0;
+    return (kCross ? u + u0 - hh * ntiles : t0 + u) * kRows;
   };
   auto load = [&](int u) {
     int hh;
@@ -1204,13 +1240,13 @@ __device__ __forceinline__ void bwd_keys(const BwdPairArgs& a, BwdSmem<D, W>& sm
   __syncthreads();
   int u = 0;
   if constexpr (kCross) {
-    for (int hh = 0; hh < G; ++hh) {
-      int t = 0;
-      for (; t < full1; ++t, ++u) {
+    for (int t = u0 % ntiles; u < nsteps; t = 0) {  // one head's tiles, or what the chunk has of them
+      const int stop = min(ntiles, t + nsteps - u), stop1 = min(full1, stop);
+      for (; t < stop1; ++t, ++u) {
         tile(Const<1>{}, u, t * kRows);
         __syncthreads();
       }
-      for (; t < ntiles; ++t, ++u) masked(u, t * kRows);
+      for (; t < stop; ++t, ++u) masked(u, t * kRows);
     }
     if (kw0 >= a.SK) return;  // (rows past the sample's keys are written: 0)
   } else {
@@ -1228,13 +1264,14 @@ __device__ __forceinline__ void bwd_keys(const BwdPairArgs& a, BwdSmem<D, W>& sm
   float fk = pow2(-kTop) * a.scale, fk2 = pow2(-kp) / dsc, fv = pow2(-kTop - kp), fv2 = 1.0f / psc;
   const float z = probe_finite<kDT>(dk, probe_finite<kDT>(dv, fk * 0.0f));
   if (__builtin_amdgcn_ballot_w64(key < SK && !(z == 0.0f)) != 0) {
-    bwd_keys_fp32<D, kCausal, kCross>(a, b, hk, kw0, sm.o[w], dk, dv, late(lane));
+    bwd_keys_fp32<D, kCausal, kCross>(a, b, hk, kw0, u0, u0 + nsteps, sm.o[w], dk, dv, late(lane));
     fk = a.scale, fk2 = fv = fv2 = 1.0f;
   }
   const int64_t part = static_cast<int64_t>(HK) * D;
   const int lane_e = late(lane);
   if constexpr (kCross) {
-    float* row = a.dkv + (static_cast<int64_t>(b) * a.SK + kw0) * 2 * part + static_cast<int64_t>(hk) * D;
+    float* row = a.dkv + ((static_cast<int64_t>(chunk) * a.B + b) * a.SK + kw0) * 2 * part +
+                 static_cast<int64_t>(hk) * D;
     store_rows<D>(dk, fk, fk2, sm.o[w], row, 2 * part, a.SK - kw0, lane_e);
     store_rows<D>(dv, fv, fv2, sm.o[w], row + part, 2 * part, a.SK - kw0, lane_e);
     return;
@@ -1245,16 +1282,20 @@ __device__ __forceinline__ void bwd_keys(const BwdPairArgs& a, BwdSmem<D, W>& sm
 }
 
 template <int D, bool kCausal, int W, bool kCross>
-__device__ __forceinline__ void bwd_queries(const BwdPairArgs& a, BwdSmem<D, W>& sm, int item) {
+__device__ __forceinline__ void bwd_queries(const BwdPairArgs& a, BwdSmem<D, W>& sm, int item,
+                                            int chunk = 0) {
   constexpr int kKS = D / 16, kDT = D / 32;
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nblk = kCross ? a.nblk_q : a.nblk;
   const int S = a.S, bh = item / nblk, qb = item % nblk;
-  const int b = bh / a.H, h = bh % a.H, hk = key_head<kCross>(a, h), SK = key_count<kCross>(a, b);
+  const int b = bh / a.H, h = bh % a.H, hk = key_head<kCross>(a, h);
+  const int keys = key_count<kCross>(a, b), key0 = kCross ? chunk * a.chq * kRows : 0;
+  const int SK = kCross && a.ncq > 1 ? min(keys - key0, a.chq * kRows) : keys;
   const int q0 = qb * (W * kRows), qw0 = q0 + w * kRows, qi = qw0 + j;
   const bool wave_live = qw0 < S;
   if constexpr (kCross) {
+    if (a.ncq > 1 && SK <= 0) return;  // (the join knows)
     if (SK == 0) {  // no key was seen
       for (int i = tid; i < min(S - q0, W * kRows) * (D / 4); i += 64 * W) {
         const int64_t row = static_cast<int64_t>(b) * S + q0 + i / (D / 4);
@@ -1263,9 +1304,11 @@ __device__ __forceinline__ void bwd_queries(const BwdPairArgs& a, BwdSmem<D, W>&
       return;
     }
   }
-  const Operand kop{reinterpret_cast<const char*>(a.k.p + b * a.k.sb + hk * a.k.sh),
+  const Operand kop{reinterpret_cast<const char*>(a.k.p + b * a.k.sb + hk * a.k.sh +
+                                                  (kCross ? key0 * a.k.ss : 0)),
                     static_cast<unsigned>(a.k.ss) * 4u};
-  const Operand vop{reinterpret_cast<const char*>(a.v.p + b * a.v.sb + hk * a.v.sh),
+  const Operand vop{reinterpret_cast<const char*>(a.v.p + b * a.v.sb + hk * a.v.sh +
+                                                  (kCross ? key0 * a.v.ss : 0)),
                     static_cast<unsigned>(a.v.ss) * 4u};
   const int k_end = kCausal ? min(S, q0 + W * kRows) : SK;
   const int ntiles = (k_end + kRows - 1) / kRows;
@@ -1273,7 +1316,7 @@ __device__ __forceinline__ void bwd_queries(const BwdPairArgs& a, BwdSmem<D, W>&
 
   Stage<D, W> st;
   Pair qB[kKS], gB[kKS];
-  const int kp = half_log2(SK);
+  const int kp = half_log2(keys);
   float uq, ug, L, Dq;  // L: kp - L log2 e
   {
     OwnRows<D> oq, og, oo;
@@ -1389,10 +1432,11 @@ __device__ __forceinline__ void bwd_queries(const BwdPairArgs& a, BwdSmem<D, W>&
     if (!wave_live) return;
     float f = pow2(-kTop) * a.scale, f2 = pow2(-kp) / dsc;
     if (__builtin_amdgcn_ballot_w64(qi < S && !(probe_finite<kDT>(dq, f * 0.0f) == 0.0f)) != 0) {
-      bwd_queries_fp32<D, kCausal, kCross>(a, b, h, qw0, sm.o[w], dq, late(lane));
+      bwd_queries_fp32<D, kCausal, kCross>(a, b, h, qw0, key0, SK, sm.o[w], dq, late(lane));
       f = a.scale, f2 = 1.0f;
     }
-    store_rows<D>(dq, f, f2, sm.o[w], a.dq + ((static_cast<int64_t>(b) * S + qw0) * a.H + h) * D,
+    store_rows<D>(dq, f, f2, sm.o[w],
+                  a.dq + (((static_cast<int64_t>(chunk) * a.B + b) * S + qw0) * a.H + h) * D,
                   static_cast<int64_t>(a.H) * D, S - qw0, late(lane));
     return;
   }
@@ -1419,7 +1463,7 @@ __device__ __forceinline__ void bwd_queries(const BwdPairArgs& a, BwdSmem<D, W>&
     f = __builtin_nanf("");
   } else if (__builtin_amdgcn_ballot_w64(
                  qi < S && !(probe_finite<kDT>(dq, f * 0.0f) == 0.0f)) != 0) {
-    bwd_queries_fp32<D, kCausal, false>(a, b, h, qw0, sm.o[w], dq, late(lane));
+    bwd_queries_fp32<D, kCausal, false>(a, b, h, qw0, 0, S, sm.o[w], dq, late(lane));
     f = factor, f2 = 1.0f;
   }
   store_rows<D>(dq, f, f2, sm.o[w], row, stride, S - qw0, late(lane));
@@ -1435,11 +1479,13 @@ bwd_pair_kernel(BwdPairArgs a) {
     const int pairs = BH / a.G;
     int in;
     if (id < a.nkv) {
-      const int pair = spread(id, pairs, a.nblk, in);
-      bwd_keys<D, kCausal, kSerial, W, kCross>(a, sm, pair * a.nblk + in);
+      const int pair = spread(id, pairs, a.nblk * a.nck, in), chunk = in / a.nblk;
+      bwd_keys<D, kCausal, kSerial, W, kCross>(a, sm, pair * a.nblk + in - chunk * a.nblk, chunk);
     } else {
-      const int pair = spread(id - a.nkv, pairs, a.nblk_q * a.G, in);
-      bwd_queries<D, kCausal, W, kCross>(a, sm, (pair * a.G + in % a.G) * a.nblk_q + in / a.G);
+      const int per = a.nblk_q * a.G;
+      const int pair = spread(id - a.nkv, pairs, per * a.ncq, in), chunk = in / per;
+      in -= chunk * per;
+      bwd_queries<D, kCausal, W, kCross>(a, sm, (pair * a.G + in % a.G) * a.nblk_q + in / a.G, chunk);
     }
     return;
   }

@@ -270,7 +270,9 @@ int fattn_paged_attention(int dtype, int cache_dtype, int64_t b, int64_t heads, 
 /* Cross attention, fp32: q [b, heads, sq, d] to k, v [b, kv_heads, sk, d] (strides {batch, head, seq},
  * rows 16-byte aligned), of which sample b sees the first key_lengths[b] (NULL: all; a length outside
  * [0, sk] counts as the nearest). out [b, sq, heads, d] contiguous, lse [b, heads, sq]; a sample that
- * sees no key has out 0 and lse -infinity. Query head i reads key head i / (heads / kv_heads). */
+ * sees no key has out 0 and lse -infinity. Query head i reads key head i / (heads / kv_heads). The
+ * workspaces (16-byte aligned, nothing kept between calls; a size may be 0, then NULL) take the outputs
+ * of parts of a walk where there are few blocks. */
 size_t fattn_cross_workspace_bytes(int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk,
                                    int64_t d);
 int fattn_cross_forward(const float* q, const int64_t q_strides[3], const float* k,
@@ -283,12 +285,14 @@ int fattn_cross_forward(const float* q, const int64_t q_strides[3], const float*
  * head, seq}): dq [b, sq, heads, d] and dkv [b, sk, 2, kv_heads, d] (dK, then dV, in each row),
  * contiguous, written whole: rows of keys that a sample does not see are 0, and those of a shared key
  * head are summed over its query heads, all in a fixed order: reruns are bit-identical. */
+size_t fattn_cross_backward_workspace_bytes(int64_t b, int64_t heads, int64_t kv_heads, int64_t sq,
+                                            int64_t sk, int64_t d);
 int fattn_cross_backward(const float* q, const int64_t q_strides[3], const float* k,
                          const int64_t k_strides[3], const float* v, const int64_t v_strides[3],
                          int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d,
                          const int32_t* key_lengths, float scale, const float* out, const float* lse,
                          const float* d_o, const int64_t do_strides[3], float* dq, float* dkv,
-                         void* stream);
+                         void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Diagnostics (no counterpart in the reference).

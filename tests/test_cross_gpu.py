@@ -48,6 +48,11 @@ SHAPES = [  # b, h, hk, sq, sk, d, lengths
     (2, 4, 2, 3, 33, 32, [33, 7]), (3, 4, 1, 5, 700, 128, [0, 1, 700]), (1, 8, 8, 31, 64, 64, None),
     (2, 2, 2, 33, 31, 64, None), (2, 6, 3, 240, 333, 64, [333, 100]), (1, 4, 4, 128, 129, 128, None),
     (2, 8, 2, 257, 512, 32, [511, 0]), (4, 2, 1, 17, 65, 64, [65, 64, 33, 32]),
+    # Few blocks and long walks: cut into chunks, with samples that fill some of them or none.
+    (1, 2, 2, 130, 3000, 64, [2500]), (2, 16, 4, 100, 3000, 128, [3000, 10]), (1, 8, 1, 200, 600, 32, None),
+    (2, 2, 1, 40, 2000, 64, [0, 1999]), (1, 16, 1, 500, 64, 64, None), (1, 1, 1, 1, 4000, 64, [3999]),
+    (3, 1, 1, 2000, 1025, 32, [1025, 513, 256]),
+    (256, 4, 2, 256, 40, 64, None), (171, 3, 1, 512, 33, 32, None),  # 64 queries per wave
     (300, 1, 1, 20, 40, 64, None), (300, 1, 1, 64, 50, 32, None), (70, 4, 2, 70, 20, 128, None),
 ]
 
@@ -98,11 +103,11 @@ def test_gradients(cuda, b, h, hk, sq, sk, d, lengths):
     assert all(torch.equal(x, y) for x, y in zip(got, again))
 
 
-@pytest.mark.parametrize("sq", [3, 200])
-def test_garbage_behind_the_last_key(cuda, sq):
+@pytest.mark.parametrize("sq,sk", [(3, 150), (200, 150), (200, 1500)])
+def test_garbage_behind_the_last_key(cuda, sq, sk):
     """Infinities and NaN in keys that a sample does not see: no trace of them, their gradients 0."""
-    q, k, v, g = operands(cuda, 3, 4, 2, sq, 150, 64, seed=2)
-    lengths = [150, 90, 0]
+    q, k, v, g = operands(cuda, 3, 4, 2, sq, sk, 64, seed=2)
+    lengths = [sk, 90, 0]
     bad_k, bad_v = k.clone(), v.clone()
     for i, n in enumerate(lengths):
         bad_k[i, :, n:], bad_v[i, :, n:] = float("nan"), float("inf")
@@ -116,11 +121,11 @@ def test_garbage_behind_the_last_key(cuda, sq):
         assert torch.equal(x, y)
 
 
-@pytest.mark.parametrize("sq", [5, 130])
-def test_non_finite_values_that_are_seen(cuda, sq):
+@pytest.mark.parametrize("sq,sk", [(5, 70), (130, 70), (130, 1500)])
+def test_non_finite_values_that_are_seen(cuda, sq, sk):
     """What the formula gives of an infinity among the values and a NaN among the queries, and nothing of
     them in other rows."""
-    q, k, v, g = operands(cuda, 2, 2, 2, sq, 70, 64, seed=3)
+    q, k, v, g = operands(cuda, 2, 2, 2, sq, sk, 64, seed=3)
     v[0, 0, 3, 5], q[1, 1, 2, 7] = float("inf"), float("nan")
     leaves = [t.requires_grad_() for t in (q, k, v)]
     out = cfa.fused_cross_attention(q, k, v, 0.125)
@@ -163,7 +168,7 @@ def test_strides_and_broadcasts(cuda):
 
 def test_shared_heads_equal_repeated_ones(cuda):
     """A shared key head's gradient is the sum of its copies'."""
-    q, k, v, g = operands(cuda, 2, 6, 2, 70, 90, 64, seed=4)
+    q, k, v, g = operands(cuda, 2, 6, 2, 70, 90, 64, seed=4)  # (16 steps of a walk: not cut)
     a = [t.detach().requires_grad_() for t in (q, k, v)]
     b = [q.detach().requires_grad_(), *(t.repeat_interleave(3, 1).requires_grad_() for t in (k, v))]
     oa, ob = (cfa.fused_cross_attention(*x, 0.125) for x in (a, b))

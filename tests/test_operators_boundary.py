@@ -150,9 +150,9 @@ def cross(b=1, heads=1, hk=1, sq=1, sk=1, d=64, q=BAD, k=BAD, qst=ST, kst=ST, ou
 
 
 def cross_bwd(b=1, heads=1, hk=1, sq=1, sk=1, d=64, q=BAD, k=BAD, qst=ST, kst=ST, out=BAD, g=BAD, gst=ST,
-              dq=BAD, dkv=BAD):
+              dq=BAD, dkv=BAD, ws=BAD, size=1 << 40):
     return _lib.lib().fattn_cross_backward(q, qst, k, kst, k, kst, b, heads, hk, sq, sk, d, None, 1.0, out,
-                                           BAD, g, gst, dq, dkv, None)
+                                           BAD, g, gst, dq, dkv, ws, size, None)
 
 
 @pytest.mark.parametrize("call", [cross, cross_bwd])
@@ -183,7 +183,13 @@ def test_cross_workspace_and_gradient_refusals():
     assert need > 0
     for ws, size in ((None, need), (ODD, need), (BAD, need - 1)):
         refused(cross(b=2, heads=4, hk=4, sk=4096, ws=ws, size=size), _lib.FATTN_EWORKSPACE, str(need))
-    assert L.fattn_cross_workspace_bytes(2, 4, 4, 1000, 4096, 64) == 0
+    assert L.fattn_cross_workspace_bytes(64, 8, 8, 1000, 4096, 64) == 0
+    assert L.fattn_cross_backward_workspace_bytes(64, 8, 8, 1000, 4096, 64) == 0
+    need = L.fattn_cross_backward_workspace_bytes(2, 4, 4, 100, 4096, 64)
+    assert need > 0
+    for ws, size in ((None, need), (ODD, need), (BAD, need - 1)):
+        refused(cross_bwd(b=2, heads=4, hk=4, sq=100, sk=4096, ws=ws, size=size), _lib.FATTN_EWORKSPACE,
+                str(need))
     assert L.fattn_cross_workspace_bytes(2, 4, 3, 1, 4096, 64) == 0
     refused(cross_bwd(g=None), _lib.FATTN_EINVAL, "null operand")
     refused(cross_bwd(dq=None), _lib.FATTN_EINVAL, "null operand")

@@ -145,11 +145,11 @@ int launch_cross_forward(View q, View k, View v, float* o, float* lse, int b, in
   FwdArgs a{q, k, v, cut ? o_part : o, lse, b, h, sq, nqb, scale, 0, sk, h / hk, key_lengths, plan.nc,
             plan.chunk, cut ? l_part : nullptr};
   void* args[] = {&a};
-  const void* fn = wide && d == 32   ? reinterpret_cast<const void*>(fwd_pair_kernel<32, false, 2, 4, 3, true>)
-                   : wide && d == 64 ? reinterpret_cast<const void*>(fwd_pair_kernel<64, false, 2, 4, 2, true>)
-                   : d == 32  ? reinterpret_cast<const void*>(fwd_pair_kernel<32, false, 1, 4, 4, true>)
-                   : d == 128 ? reinterpret_cast<const void*>(fwd_pair_kernel<128, false, 1, 4, 2, true>)
-                              : reinterpret_cast<const void*>(fwd_pair_kernel<64, false, 1, 4, 3, true>);
+  const void* fn = wide && d == 32   ? reinterpret_cast<const void*>(fwd_cross_kernel<32, 2, 4, 3>)
+                   : wide && d == 64 ? reinterpret_cast<const void*>(fwd_cross_kernel<64, 2, 4, 2>)
+                   : d == 32         ? reinterpret_cast<const void*>(fwd_cross_kernel<32, 1, 4, 4>)
+                   : d == 128        ? reinterpret_cast<const void*>(fwd_cross_kernel<128, 1, 4, 2>)
+                                     : reinterpret_cast<const void*>(fwd_cross_kernel<64, 1, 4, 3>);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const unsigned grid = static_cast<unsigned>(int64_t{nqb} * b * h * plan.nc);
   const hipError_t err = hipLaunchKernel(fn, dim3(grid), dim3(256), args, 0, s);
@@ -180,10 +180,9 @@ int launch_cross_backward(View q, View k, View v, View d_o, const float* o, cons
   a.nblk = nblk, a.nkv = nblk * b * hk * plan.nck, a.nblk_q = nblk_q;
   a.give_up_bh = -1;
   void* args[] = {&a};
-  const void* fn = d == 32 ? reinterpret_cast<const void*>(bwd_pair_kernel<32, false, false, 4, 3, true>)
-                   : d == 128
-                       ? reinterpret_cast<const void*>(bwd_pair_kernel<128, false, false, 4, 1, true>)
-                       : reinterpret_cast<const void*>(bwd_pair_kernel<64, false, false, 4, 2, true>);
+  const void* fn = d == 32    ? reinterpret_cast<const void*>(bwd_cross_kernel<32, 4, 3>)
+                   : d == 128 ? reinterpret_cast<const void*>(bwd_cross_kernel<128, 4, 1>)
+                              : reinterpret_cast<const void*>(bwd_cross_kernel<64, 4, 2>);
   hipStream_t s = static_cast<hipStream_t>(stream);
   hipError_t err = hipLaunchKernel(fn, dim3(static_cast<unsigned>(a.nkv + nblk_q * b * h * plan.ncq)),
                                    dim3(256), args, 0, s);

@@ -547,9 +547,8 @@ __device__ __forceinline__ void fwd_rows_fp32(const FwdArgs& a, int b, int h, in
   }
 }
 
-template <int D, bool kCausal, int NQ, int W, int WAVES, bool kCross = false>
-__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES)))
-fwd_pair_kernel(FwdArgs a) {
+template <int D, bool kCausal, int NQ, int W, bool kCross>
+__device__ __forceinline__ void fwd_pair(FwdArgs a) {
   a.causal = kCausal ? 1 : 0;
   constexpr int kKS = D / 16;              // contraction steps of S
   constexpr int kDT = D / 32;              // 32-dim tiles of O
@@ -821,6 +820,17 @@ fwd_pair_kernel(FwdArgs a) {
       put_l<kCross>(a, static_cast<int64_t>(bh) * S + qi, L);
     }
   }
+}
+
+template <int D, bool kCausal, int NQ, int W, int WAVES>
+__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES)))
+fwd_pair_kernel(FwdArgs a) {
+  fwd_pair<D, kCausal, NQ, W, false>(a);
+}
+template <int D, int NQ, int W, int WAVES>
+__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES)))
+fwd_cross_kernel(FwdArgs a) {
+  fwd_pair<D, false, NQ, W, true>(a);
 }
 
 // --- Backward ----------------------------------------------------------------------------------
@@ -1469,9 +1479,8 @@ __device__ __forceinline__ void bwd_queries(const BwdPairArgs& a, BwdSmem<D, W>&
   store_rows<D>(dq, f, f2, sm.o[w], row, stride, S - qw0, late(lane));
 }
 
-template <int D, bool kCausal, bool kSerial, int W, int WAVES, bool kCross = false>
-__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES)))
-bwd_pair_kernel(BwdPairArgs a) {
+template <int D, bool kCausal, bool kSerial, int W, bool kCross>
+__device__ __forceinline__ void bwd_pair(BwdPairArgs a) {
   a.causal = kCausal ? 1 : 0;
   __shared__ __attribute__((aligned(16))) BwdSmem<D, W> sm;
   const int id = static_cast<int>(blockIdx.x), BH = a.B * a.H;
@@ -1509,6 +1518,17 @@ bwd_pair_kernel(BwdPairArgs a) {
     const int i = id - a.nkv;
     bwd_queries<D, kCausal, W, false>(a, sm, kCausal ? i % BH * a.nblk + a.nblk - 1 - i / BH : xcd_remap(i, a.nkv));
   }
+}
+
+template <int D, bool kCausal, bool kSerial, int W, int WAVES>
+__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES)))
+bwd_pair_kernel(BwdPairArgs a) {
+  bwd_pair<D, kCausal, kSerial, W, false>(a);
+}
+template <int D, int W, int WAVES>
+__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES)))
+bwd_cross_kernel(BwdPairArgs a) {
+  bwd_pair<D, false, false, W, true>(a);
 }
 
 }  // namespace

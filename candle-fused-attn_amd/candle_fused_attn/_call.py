@@ -2,9 +2,11 @@
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
+from . import _lib
 from ._lib import DTYPES, FusedAttentionError, check
 
 ALL = tuple(DTYPES)
@@ -64,3 +66,37 @@ def launch(t: torch.Tensor, fn, *args) -> None:
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         check(rc)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(query: str, *sizes: int) -> int:
+    """A C size query (a function of the sizes alone)."""
+    return getattr(_lib.lib(), query)(*sizes)
+
+
+def workspace(t: torch.Tensor, query: str, *sizes: int):
+    """The workspace of a call, from torch's allocator: (tensor, address, bytes), or (None, None, 0)."""
+    size = _workspace_bytes(query, *sizes)
+    if not size:
+        return None, None, 0
+    ws = torch.empty(size, dtype=torch.uint8, device=t.device)
+    return ws, ws.data_ptr(), size
+
+
+class _NotTwice(torch.autograd.Function):
+    """Gradients that were asked for with a graph: they are not differentiable, and say so when it is
+    tried (without this they would look like constants)."""
+
+    @staticmethod
+    def forward(ctx, who, n, *tensors):
+        ctx.who = who
+        return tuple(t.view_as(t) for t in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise FusedAttentionError(f"{ctx.who}: its gradient is not differentiable")
+
+
+def not_twice(who: str, inputs, grads):
+    """`grads` as results of a node on `inputs` that refuses to be differentiated."""
+    return _NotTwice.apply(who, len(grads), *grads, *inputs)

@@ -6,10 +6,9 @@ lengths in place of a mask.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._call import aligned_rows, launch, pack, require
+from ._call import aligned_rows, launch, not_twice, pack, require, workspace
 from ._lib import FusedAttentionError
 
 _F32 = (torch.float32,)
@@ -21,45 +20,45 @@ def _forward(q, k, v, scale, key_lengths):
     hk, sk = k.shape[1], k.shape[2]
     L = _lib.lib()
     out, lse = q.new_empty((b, sq, h, d)), q.new_empty((b, h, sq))
-    size = L.fattn_cross_workspace_bytes(b, h, hk, sq, sk, d)
-    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    ws, wp, size = workspace(q, "fattn_cross_workspace_bytes", b, h, hk, sq, sk, d)
     keep, p = pack(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
     launch(q, L.fattn_cross_forward, q.data_ptr(), p, k.data_ptr(), p + 24, v.data_ptr(), p + 48, b, h, hk, sq, sk, d,
            key_lengths.data_ptr() if key_lengths is not None else None, scale, out.data_ptr(),
-           lse.data_ptr(), ws.data_ptr() if size else None, size)
+           lse.data_ptr(), wp, size)
     return out, lse
 
 
 class _FusedCrossAttention(torch.autograd.Function):
-    """[b, h, sq, d] and [b, kv_heads, sk, d] in, the raw [b, sq, h, d] output out."""
+    """[b, h, sq, d] and [b, kv_heads, sk, d] in, the [b, h, sq, d] view of the output out."""
 
     @staticmethod
     def forward(ctx, q, k, v, scale, key_lengths):
         out, lse = _forward(q, k, v, scale, key_lengths)
         ctx.save_for_backward(q, k, v, key_lengths, out, lse)
         ctx.scale = scale
-        return out
+        return out.transpose(1, 2)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
         q, k, v, key_lengths, out, lse = ctx.saved_tensors
+        with_graph = torch.is_grad_enabled()
+        if with_graph:
+            inputs, grad = (q, k, v, grad), grad.detach()
         grad = aligned_rows(grad)
         b, h, sq, d = q.shape
         hk, sk = k.shape[1], k.shape[2]
         dq, dkv = q.new_empty((b, sq, h, d)), q.new_empty((b, sk, 2, hk, d))
-        gb, gs, gh, _ = grad.stride()
-        keep, p = pack(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], gb, gh, gs)
-        L = _lib.lib()
-        size = L.fattn_cross_backward_workspace_bytes(b, h, hk, sq, sk, d)
-        ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        launch(q, L.fattn_cross_backward, q.data_ptr(), p, k.data_ptr(), p + 24, v.data_ptr(),
+        keep, p = pack(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *grad.stride()[:3])
+        ws, wp, size = workspace(q, "fattn_cross_backward_workspace_bytes", b, h, hk, sq, sk, d)
+        launch(q, _lib.lib().fattn_cross_backward, q.data_ptr(), p, k.data_ptr(), p + 24, v.data_ptr(),
                p + 48, b, h, hk, sq, sk, d,
                key_lengths.data_ptr() if key_lengths is not None else None, ctx.scale, out.data_ptr(),
-               lse.data_ptr(), grad.data_ptr(), p + 72, dq.data_ptr(), dkv.data_ptr(),
-               ws.data_ptr() if size else None, size)
+               lse.data_ptr(), grad.data_ptr(), p + 72, dq.data_ptr(), dkv.data_ptr(), wp, size)
         dk, dv = dkv.transpose(1, 3).unbind(2)  # [b, kv_heads, sk, d] each
-        return dq.transpose(1, 2), dk, dv, None, None
+        grads = dq.transpose(1, 2), dk, dv
+        if with_graph:
+            grads = not_twice("fused_cross_attention", inputs, grads)
+        return *grads, None, None
 
 
 def fused_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
@@ -87,5 +86,5 @@ def fused_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sca
                                       f"{list(key_lengths.shape)}")
     q, k, v = aligned_rows(q), aligned_rows(k), aligned_rows(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _FusedCrossAttention.apply(q, k, v, float(scale), key_lengths).transpose(1, 2)
+        return _FusedCrossAttention.apply(q, k, v, float(scale), key_lengths)
     return _forward(q, k, v, float(scale), key_lengths)[0].transpose(1, 2)

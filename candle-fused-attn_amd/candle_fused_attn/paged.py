@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._call import aligned_rows, launch, pack, require, rows
+from ._call import aligned_rows, launch, pack, require, rows, workspace
 from ._lib import FusedAttentionError
 from .rotary import check_frequencies
 
@@ -84,6 +84,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
             raise FusedAttentionError(f"{who}: contiguous counts [{b}] expected, got "
                                       f"{list(counts.shape)}")
     dim = 0 if frequencies is None else check_frequencies(who, frequencies, d, k)
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if 0 in t.stride()[:3] and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+            raise FusedAttentionError(f"{who}: {name} is a broadcast view, whose slots share memory")
     k, v = rows(k), rows(v)
     keep, p = pack(*qst, *ost, *k.stride()[:3], *v.stride()[:3], *k_pages.stride()[:3],
                    *v_pages.stride()[:3])
@@ -116,14 +119,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise FusedAttentionError(f"{who}: not differentiable (call it under torch.no_grad())")
     q = aligned_rows(q)
-    L = _lib.lib()
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     page_size, width = k_pages.shape[2], page_table.shape[1]
-    size = L.fattn_paged_attention_workspace_bytes(b, h, hk, d, width * page_size)
-    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    ws, wp, size = workspace(q, "fattn_paged_attention_workspace_bytes", b, h, hk, d, width * page_size)
     keep, p = pack(*q.stride()[:2], *k_pages.stride()[:3], *v_pages.stride()[:3])
-    launch(q, L.fattn_paged_attention, _lib.DTYPES[q.dtype], _lib.DTYPES[k_pages.dtype], b, h, hk, d,
+    launch(q, _lib.lib().fattn_paged_attention, _lib.DTYPES[q.dtype], _lib.DTYPES[k_pages.dtype], b, h, hk, d,
            q.data_ptr(), p, out.data_ptr(), k_pages.data_ptr(), p + 16, v_pages.data_ptr(), p + 40, k_pages.shape[0], page_size, page_table.data_ptr(),
            page_table.stride(0), width, lengths.data_ptr(), float(scale),
-           ws.data_ptr() if size else None, size)
+           wp, size)
     return out

@@ -104,35 +104,37 @@ def _forward(xs, heads, positions, frequencies, interleaved, magnitude, inverse)
 
 
 class _Rotary(torch.autograd.Function):
-    """The turn; its gradient is the turn back, by the same Function (so it can be differentiated
-    again)."""
+    """The turn; its gradient is the turn back, by the same Function where a graph of it is asked for (so
+    it can be differentiated again)."""
 
     @staticmethod
     def forward(ctx, positions, frequencies, heads, interleaved, magnitude, inverse, *xs):
         ctx.save_for_backward(positions, frequencies)
         ctx.how = (heads, interleaved, magnitude, inverse)
         ctx.set_materialize_grads(False)
-        return tuple(_forward(xs, heads, positions, frequencies, interleaved, magnitude, inverse))
+        ys = _forward(xs, heads, positions, frequencies, interleaved, magnitude, inverse)
+        return ys[0] if len(ys) == 1 else tuple(ys)
 
     @staticmethod
     def backward(ctx, *grads):
         positions, frequencies = ctx.saved_tensors
         heads, interleaved, magnitude, inverse = ctx.how
-        need = ctx.needs_input_grad[6:]
-        at = [i for i, g in enumerate(grads) if g is not None and need[i]]
-        out = [None] * len(grads)
+        need = ctx.needs_input_grad
+        # (A projection's gradient is read by its heads: any strides but for the last dimension.)
+        at = [i for i, g in enumerate(grads) if g is not None and need[6 + i]]
+        out = [None] * (6 + len(grads))
         if at:
-            # (A projection's gradient is viewed by its heads.)
-            gs = [grads[i].contiguous() if heads else rows(grads[i]) for i in at]
-            for i, g in zip(at, _apply(gs, heads, positions, frequencies, interleaved, magnitude,
-                                       not inverse)):
-                out[i] = g
-        return (None,) * 6 + tuple(out)
+            turned = _apply([rows(grads[i]) for i in at], heads, positions, frequencies, interleaved,
+                            magnitude, not inverse)
+            for i, g in zip(at, turned):
+                out[6 + i] = g
+        return tuple(out)
 
 
 def _apply(xs, heads, positions, frequencies, interleaved, magnitude, inverse):
-    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
-        return _Rotary.apply(positions, frequencies, heads, interleaved, magnitude, inverse, *xs)
+    if torch.is_grad_enabled() and (xs[0].requires_grad or xs[-1].requires_grad):
+        ys = _Rotary.apply(positions, frequencies, heads, interleaved, magnitude, inverse, *xs)
+        return (ys,) if len(xs) == 1 else ys
     return _forward(xs, heads, positions, frequencies, interleaved, magnitude, inverse)
 
 

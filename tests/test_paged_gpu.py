@@ -339,3 +339,10 @@ def test_attention_side_streams(cuda):
                 got[i].append(cfa.paged_attention(qs[i], c.k, c.v, c.table, c.lengths, 0.125))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
+
+
+def test_append_refuses_broadcast_pages(cuda):
+    c = Cache(cuda, torch.float32, 1, 16, 32, [5], room=2, seed=17)
+    k = torch.randn(1, 2, 2, 32, device=cuda)
+    with pytest.raises(cfa.FusedAttentionError, match="broadcast"):
+        cfa.paged_append(k, k, c.k.expand(-1, 2, -1, -1), c.v.expand(-1, 2, -1, -1), c.table, c.lengths)

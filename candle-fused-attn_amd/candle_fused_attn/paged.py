@@ -107,8 +107,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     q: [b, h, 1, d], of the cache's type or f32, h a multiple of the cache's key heads (query head i
     reads key head i // (h // kv_heads)). Returns [b, h, 1, d] of q's type. A sequence of length 0
-    gives 0; one whose length the table cannot hold, or that names a page outside the cache, NaN (as
-    does an infinity among the keys or values it sees). Not differentiable.
+    gives 0; one whose length the table cannot hold, or that names a page outside the cache, NaN.
+    Infinities and NaN that a token sees give what the formula gives of them. Not differentiable.
     """
     who = "paged_attention"
     require(who, "q", q, 4)

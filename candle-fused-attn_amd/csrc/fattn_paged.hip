@@ -20,7 +20,7 @@
 // what is not of its type as a sum of 16-bit terms: fp32 queries as three bf16, or two f16 under a scale
 // of the row (22 bits of its largest, and an error in a score is one of its size anyway); weights, over
 // bf16 values, as two bf16 for a bf16 result (2^-17 of each weight, below its rounding) and three for an
-// fp32 one. Over f16 values the weights stay fp32 and the values are widened: f16 terms of a weight
+// fp32 one (2^-25). Over f16 values the weights stay fp32 and the values are widened: f16 terms of a weight
 // would end at 2^-24 of the largest one's size, and a key of all the weight but no value (an attention
 // sink) would take the bits of all the others.
 //
@@ -47,6 +47,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
 constexpr int kSplitWaves = 4;
+constexpr int kMostRuns = 1024;     // workgroups, with runs: 256 x kOccupancy
 constexpr int kTile = kSplitTile;   // keys of a tile: two halves of 16
 constexpr int kRowsMax = 16;        // rows of a block
 constexpr float kRoom = 4.0f;       // log2 of what a weight may pass its reference by
@@ -73,16 +74,31 @@ __device__ __forceinline__ float row_sum(float x) {
   return x + __shfl_xor(x, 32);
 }
 
-// x as N terms of type C, largest first: two values into one word per term.
-template <int N, typename C>
-__device__ __forceinline__ void terms2(float x, float y, unsigned (&w)[N]) {
-  typedef C c2v __attribute__((ext_vector_type(2)));
+// x and y as sums of N terms of type C, largest first, two values to a word. Each term but the last is
+// cut off towards 0 and none is 0 where x is not (a rest of nothing counts as 2^-30 of x): all have x's
+// sign, and an infinity that they multiply stays one.
+__device__ __forceinline__ float rest(float x, float least) { return fabsf(x) > fabsf(least) ? x : least; }
+template <int N>
+__device__ __forceinline__ void terms2(float x, float y, unsigned (&w)[N], __bf16) {
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  const float lx = x * 0x1p-30f, ly = y * 0x1p-30f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const c2v h{static_cast<C>(x), static_cast<C>(y)};
-    w[i] = __builtin_bit_cast(unsigned, h);
-    x -= static_cast<float>(h.x), y -= static_cast<float>(h.y);
+  for (int i = 0; i < N - 1; ++i) {
+    const unsigned hx = __float_as_uint(x) & 0xffff0000u, hy = __float_as_uint(y) & 0xffff0000u;
+    w[i] = __builtin_amdgcn_perm(hy, hx, 0x07060302u);
+    x = rest(x - __uint_as_float(hx), lx), y = rest(y - __uint_as_float(hy), ly);
   }
+  w[N - 1] = __builtin_bit_cast(unsigned, b2{static_cast<__bf16>(x), static_cast<__bf16>(y)});
+}
+template <int N>
+__device__ __forceinline__ void terms2(float x, float y, unsigned (&w)[N], _Float16) {
+  static_assert(N == 2, "two f16");
+  const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x, y));
+  w[0] = __builtin_bit_cast(unsigned, h);
+  // (The least f16 is 2^-24.)
+  const float lx = x == 0.0f ? 0.0f : copysignf(0x1p-24f, x), ly = y == 0.0f ? 0.0f : copysignf(0x1p-24f, y);
+  x = rest(x - static_cast<float>(h.x), lx), y = rest(y - static_cast<float>(h.y), ly);
+  w[1] = __builtin_bit_cast(unsigned, h2{static_cast<_Float16>(x), static_cast<_Float16>(y)});
 }
 
 // Tiles of sequence b, and its length; bad: a length that the cache cannot hold.
@@ -182,7 +198,7 @@ struct Wave {
         unsigned w[4][kQT];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          terms2<kQT, C>(x[i][e / 2][2 * (e % 2)] * sc, x[i][e / 2][2 * (e % 2) + 1] * sc, w[e]);
+          terms2(x[i][e / 2][2 * (e % 2)] * sc, x[i][e / 2][2 * (e % 2) + 1] * sc, w[e], C{});
         }
 #pragma unroll
         for (int t = 0; t < kQT; ++t) q[t][i] = u4{w[0][t], w[1][t], w[2][t], w[3][t]};
@@ -326,7 +342,7 @@ struct Wave {
       u4 b[kPT];
       unsigned w[4][kPT];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) terms2<kPT, C>(p[e / 2][2 * (e % 2)], p[e / 2][2 * (e % 2) + 1], w[e]);
+      for (int e = 0; e < 4; ++e) terms2(p[e / 2][2 * (e % 2)], p[e / 2][2 * (e % 2) + 1], w[e], C{});
 #pragma unroll
       for (int t = 0; t < kPT; ++t) b[t] = u4{w[0][t], w[1][t], w[2][t], w[3][t]};
 #pragma unroll
@@ -674,8 +690,12 @@ SplitPlan split_plan(int64_t b, int64_t hk, int64_t rows, int64_t d, int64_t cap
   const int64_t tiles = (capacity + kTile - 1) / kTile;
   p.min_run = kSplitWaves;
   p.begin = kSplitWaves;
-  // One workgroup per key head where no sequence can have more than a few tiles per wave.
-  p.wgs = tiles <= 4 * kSplitWaves ? 0 : 1024;
+  // One workgroup per key head, and no join, where no sequence can have more than four tiles a wave, or
+  // eight with a workgroup for every CU. Direct / in runs, us (with 6 us of a graph's launch): fp32 d 64,
+  // 384 heads of 1024 tokens 45.9 / 52.6, of 1 to 700 25.6 / 29.9; bf16 d 128, 256 of 1000 28.8 / 35.5;
+  // past it 384 of 1 to 2048 64.9 / 54.7, 48 of 1500 37.8 / 23.0.
+  const int64_t direct = b * hk * p.row_blocks >= 256 ? 8 * kSplitWaves : 4 * kSplitWaves;
+  p.wgs = tiles <= direct ? 0 : kMostRuns;
   p.before = static_cast<size_t>(p.wgs) * 2 * p.part_rows * static_cast<size_t>(d + 4) * sizeof(float);
   p.bytes = p.wgs == 0 ? 0 : p.before + static_cast<size_t>(b + 1) * sizeof(int64_t);
   return p;

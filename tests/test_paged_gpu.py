@@ -152,6 +152,31 @@ def test_attention_large_and_sinking_scores(cuda, types):
     assert rel(out, ref) <= bar(dt) + 1.1e-5 + least
 
 
+@pytest.mark.parametrize("types", PAIRS, ids="-".join)
+@pytest.mark.parametrize("n", [70, 1500])
+def test_attention_non_finite_values_that_are_seen(cuda, types, n):
+    """Infinities among the values, a key that scores minus infinity, a NaN among the keys: what the formula
+    gives, and nothing of them in other sequences, rows and columns. (The queries are halves of whole
+    numbers, exact in every type, and not 0, so that the infinite key's score is one.)"""
+    dt, ct = (TYPES[t] for t in types)
+    c = Cache(cuda, ct, 1, 16, 64, [n] * 4, seed=18)
+    q = ((torch.randint(1, 5, (4, 2, 1, 64), generator=torch.Generator().manual_seed(2)) / 2)
+         .to(dt).to(cuda))
+
+    def put(pages, i, t, e, value):
+        pages[int(c.table[i, t // 16]), 0, t % 16, e] = value
+
+    put(c.v, 0, 3, 5, float("inf")), put(c.v, 0, 40, 9, float("-inf"))
+    put(c.k, 1, 7, 11, float("-inf"))
+    put(c.k, 2, 9, 2, float("nan"))
+    out = cfa.paged_attention(q, c.k, c.v, c.table, c.lengths, 0.05).double().cpu()
+    ref = attend(q, c, [n] * 4, 0.05)
+    assert torch.equal(out.isnan(), ref.isnan()) and bool(out[2].isnan().all())
+    assert torch.equal(out.isinf(), ref.isinf()) and out[0, 0, 0, 5] > 0 > out[0, 0, 0, 9]
+    fine = ref.isfinite()
+    assert rel(out[fine][None], ref[fine][None]) <= bar(dt)
+
+
 def test_attention_strided_cache_and_queries(cuda):
     """Keys and values interleaved in one pool whose rows are padded and whose heads come after the
     slots; queries out of a wider buffer, misaligned ones copied."""

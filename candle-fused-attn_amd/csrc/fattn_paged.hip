@@ -27,7 +27,13 @@
 // Work: the sequences' 32-key tiles, end to end, are dealt in equal runs to a fixed number of
 // workgroups, whatever the lengths; a workgroup's run crosses heads and sequences. Where a run ends
 // inside a head the workgroup leaves its unnormalised sums in the workspace (at most two: its first
-// and its last head), and a second kernel joins them in order. Reruns are bit-identical.
+// and its last head), and a second kernel joins them in order. Reruns are bit-identical. A head counts
+// kSplitWaves tiles more than it has, which is what beginning one costs: without, the workgroup that the
+// shortest sequences fall to ends last (64 sequences of 1 to 2048, 6 heads, fp32 d 64: 79 us, 46 so).
+//
+// Measured (kernel and join): 4 contexts of 60000 to 131071, 32 heads in 8 groups, d 128 bf16, 273 + 5 us
+// (5.7 TB/s); that ragged batch 45 + 5 us (4.5 TB/s); 8 x 6 heads 1 x 1536 fp32 12.7 + 4.7 us (3.0 TB/s);
+// one sequence of 240, 6 heads, 8.2 us, the latency of one workgroup.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>

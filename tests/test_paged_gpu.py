@@ -371,3 +371,35 @@ def test_append_refuses_broadcast_pages(cuda):
     k = torch.randn(1, 2, 2, 32, device=cuda)
     with pytest.raises(cfa.FusedAttentionError, match="broadcast"):
         cfa.paged_append(k, k, c.k.expand(-1, 2, -1, -1), c.v.expand(-1, 2, -1, -1), c.table, c.lengths)
+
+
+def test_far_pages(cuda):
+    """A pool of more than 2^31 values, its last pages in use: as a small pool, bit for bit."""
+    far = torch.empty(2, 70000, 8, 64, 64, dtype=torch.bfloat16, device=cuda)
+    near = torch.zeros(2, 3, 8, 64, 64, dtype=torch.bfloat16, device=cuda)
+    far[:, -3:] = 0
+    k, v = (torch.randn(1, 8, 130, 64, device=cuda).bfloat16() for _ in range(2))
+    q = q_of(cuda, torch.bfloat16, 1, 16, 64, seed=19)
+    zero, n = (torch.tensor([i], dtype=torch.int32, device=cuda) for i in (0, 130))
+    out = []
+    for pool, first in ((far, 69997), (near, 0)):
+        table = torch.tensor([[first + 2, first, first + 1]], dtype=torch.int32, device=cuda)
+        cfa.paged_append(k, v, pool[0], pool[1], table, zero)
+        out.append(cfa.paged_attention(q, pool[0], pool[1], table, n, 0.125))
+    assert torch.equal(far[:, -3:], near) and torch.equal(*out)
+    assert bool(out[0].isfinite().all()) and float(out[0].abs().max()) > 0
+
+
+def test_append_side_stream(cuda):
+    """On another stream than the default one, ordered by events: as on the default."""
+    a, b = (Cache(cuda, torch.float32, 2, 16, 64, [9, 0], room=300, seed=20) for _ in range(2))
+    k, v, q = (torch.randn(2, n, 300, 64, device=cuda) for n in (2, 2, 4))
+    f = cfa.rotary_frequencies(64, device=cuda)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        x = cfa.paged_append(k, v, a.k, a.v, a.table, a.lengths, q=q, frequencies=f)
+    torch.cuda.current_stream().wait_stream(side)
+    y = cfa.paged_append(k, v, b.k, b.v, b.table, b.lengths, q=q, frequencies=f)
+    assert torch.equal(x, y)
+    assert all(torch.equal(s.nan_to_num(9.0), t.nan_to_num(9.0)) for s, t in ((a.k, b.k), (a.v, b.v)))

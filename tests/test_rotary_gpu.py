@@ -220,3 +220,16 @@ def test_scaled_frequencies(cuda, scaling):
     pos = torch.arange(70000, 70009, device=cuda)
     for x, y in zip((q, k), cfa.fused_rotary(q, k, pos, f, True)):
         near(y, formula(x, pos, f, True), x)
+
+
+def test_far_operands(cuda):
+    """Operands of more than 2^31 values: the last rows as those of a small call, bit for bit."""
+    s = 1 << 22
+    x = torch.empty(2, 1, s, 512, dtype=torch.float16, device=cuda)
+    x[:, :, -5:] = torch.randn(2, 1, 5, 512, device=cuda).half()
+    x[:, :, :5] = x[:, :, -5:]
+    f, pos = cfa.rotary_frequencies(512, device=cuda), torch.arange(s, device=cuda) % (s - 5)
+    y, z = cfa.fused_rotary(x, x, pos, f)
+    want = cfa.fused_rotary(x[:, :, :5], x[:, :, :5], pos[:5], f)[0]
+    for t in (y, z):
+        assert torch.equal(t[:, :, :5], want) and torch.equal(t[:, :, -5:], want)

@@ -21,7 +21,8 @@ REPO = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "lib"
 LIB = LIB_DIR / "libfattn.so"
-SOURCES = [CSRC / "fattn_pair.hip", CSRC / "fattn_cross.hip", CSRC / "fattn_paged.hip", CSRC / "fattn_rotary.hip",
+SOURCES = [CSRC / "fattn_pair.hip", CSRC / "fattn_cross.hip", CSRC / "fattn_paged.hip",
+           CSRC / "fattn_rotary.hip",
            CSRC / "fattn_kernels.hip", CSRC / "fattn_api.cpp", CSRC / "fattn_operators.cpp"]
 HEADERS = [REPO / "include" / "fattn.h", CSRC / "fattn_internal.h", CSRC / "fattn_device.h",
            CSRC / "fattn_pair_kernels.h"]

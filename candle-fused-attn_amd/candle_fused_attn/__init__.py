@@ -3,7 +3,9 @@ deterministic backward, head_dim 32, 64 or 128 (the reference's is 64), on hand-
 kernels (libfattn.so).
 
 The public surface mirrors the reference crate's (src/lib.rs:90-161): `fused_attention`,
-`fused_attention_qkv`, `CUDA_HEAD_DIM`.
+`fused_attention_qkv`, `CUDA_HEAD_DIM`. Around them, without a counterpart there: rotary positions
+(`fused_rotary`, `fused_rotary_qkv`, `rotary_frequencies`), a paged key-value cache (`paged_append`,
+`paged_attention`) and attention to states of another length (`fused_cross_attention`).
 """
 from ._lib import FusedAttentionError, LIB_PATH, version
 from .cross import fused_cross_attention

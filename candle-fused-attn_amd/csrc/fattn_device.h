@@ -1,4 +1,4 @@
-// Device helpers shared by the kernel files (fattn_kernels.hip, fattn_pair.hip).
+// Device helpers shared by the kernel files (fattn_kernels.hip, fattn_pair_kernels.h, fattn_paged.hip).
 #ifndef FATTN_DEVICE_H
 #define FATTN_DEVICE_H
 

@@ -1,5 +1,6 @@
 // Internal interface between the C-ABI layer (fattn_api.cpp) and the gfx950 kernels
-// (fattn_pair.hip, fattn_kernels.hip), all compiled by hipcc.
+// (fattn_pair.hip, fattn_cross.hip, fattn_paged.hip, fattn_rotary.hip, fattn_kernels.hip), all compiled
+// by hipcc.
 #ifndef FATTN_INTERNAL_H
 #define FATTN_INTERNAL_H
 

@@ -1,5 +1,5 @@
 // The backward's step 3, the library's static scratch, and the host's shape functions (the workspace
-// and schedule rules of the C ABI). The forward and step 2 are in fattn_pair.hip.
+// and schedule rules of the C ABI). The forward and step 2 are in fattn_pair_kernels.h.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -697,10 +697,11 @@ SplitPlan split_plan(int64_t b, int64_t hk, int64_t rows, int64_t d, int64_t cap
   p.min_run = kSplitWaves;
   p.begin = kSplitWaves;
   // One workgroup per key head, and no join, where no sequence can have more than four tiles a wave, or
-  // eight with a workgroup for every CU. Direct / in runs, us (with 6 us of a graph's launch): fp32 d 64,
-  // 384 heads of 1024 tokens 45.9 / 52.6, of 1 to 700 25.6 / 29.9; bf16 d 128, 256 of 1000 28.8 / 35.5;
-  // past it 384 of 1 to 2048 64.9 / 54.7, 48 of 1500 37.8 / 23.0.
-  const int64_t direct = b * hk * p.row_blocks >= 256 ? 8 * kSplitWaves : 4 * kSplitWaves;
+  // eight with a workgroup for most CUs. Direct / in runs, us (with 6 us of a graph's launch): fp32 d 64,
+  // 384 heads of 1024 tokens 45.9 / 52.6, of 1 to 700 25.6 / 29.9; bf16 d 128, 256 of 1000 28.8 / 35.5,
+  // 192 26.0 / 29.7; past it 384 of 1 to 2048 64.9 / 54.7, 48 of 1000 28.2 / 20.8, of 1500 37.8 / 23.0. (A
+  // wave alone takes 2 us a tile, the memory's latency twice; eight waves a workgroup change little.)
+  const int64_t direct = b * hk * p.row_blocks >= 192 ? 8 * kSplitWaves : 4 * kSplitWaves;
   p.wgs = tiles <= direct ? 0 : kMostRuns;
   p.before = static_cast<size_t>(p.wgs) * 2 * p.part_rows * static_cast<size_t>(d + 4) * sizeof(float);
   p.bytes = p.wgs == 0 ? 0 : p.before + static_cast<size_t>(b + 1) * sizeof(int64_t);

@@ -12,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
@@ -101,6 +102,30 @@ def build_host(verbose: bool = False) -> Path:
     return _run(host_command(tmp), tmp, HOST_LIB, verbose)
 
 
+# The operators around self-attention for Python (torch's C++ API over libfattn.so).
+OPERATORS_SRC = HOST / "torch_operators.cpp"
+OPERATORS = LIB_DIR / "torch_operators.so"
+
+
+def operators_command(out: Path = OPERATORS) -> list[str]:
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    abi = int(torch.compiled_with_cxx11_abi())
+    return [hipcc(), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden",
+            "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", f"-I{REPO / 'include'}",
+            f"-I{root / 'include'}", f"-I{root / 'include/torch/csrc/api/include'}",
+            f"-I{sysconfig.get_paths()['include']}", str(OPERATORS_SRC), f"-L{LIB_DIR}", "-lfattn",
+            f"-L{root / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
+            "-Wl,-rpath,$ORIGIN", "-o", str(out)]
+
+
+def build_operators(verbose: bool = False) -> Path:
+    """Compile lib/torch_operators.so (needs libfattn.so built first)."""
+    tmp = OPERATORS.with_suffix(".so.tmp")
+    return _run(operators_command(tmp), tmp, OPERATORS, verbose)
+
+
 STEP_BENCH_SRC = HOST / "step_bench.cpp"
 STEP_BENCH = LIB_DIR / "cfa_step_bench"
 
@@ -133,5 +158,6 @@ def build_host_test(verbose: bool = False) -> Path:
 
 if __name__ == "__main__":
     print(build(verbose="-v" in sys.argv))
+    print(build_operators(verbose="-v" in sys.argv))
     print(build_host(verbose="-v" in sys.argv))
     print(build_step_bench(verbose="-v" in sys.argv))

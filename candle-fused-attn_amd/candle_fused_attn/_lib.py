@@ -6,11 +6,14 @@ FusedAttentionError -- there is no CPU or composed fallback.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 from pathlib import Path
 
 import torch  # noqa: F401  -- loaded first, so libfattn binds to torch's HIP runtime
 
 LIB_PATH = Path(__file__).resolve().parent.parent / "lib" / "libfattn.so"
+OPERATORS_PATH = LIB_PATH.with_name("torch_operators.so")
 
 # Return codes (include/fattn.h).
 FATTN_EINVAL = -1
@@ -66,6 +69,7 @@ class FusedAttentionError(RuntimeError):
 
 
 _lib = None
+_operators = None
 
 I64 = ctypes.c_int64
 P = ctypes.c_void_p
@@ -143,6 +147,26 @@ def lib() -> ctypes.CDLL:
         _declare(L)
         _lib = L
     return _lib
+
+
+def operators():
+    """The loaded torch_operators.so (torch tensors to libfattn's operators around self-attention);
+    raises FusedAttentionError if it is not built."""
+    global _operators
+    if _operators is None:
+        lib()
+        if not OPERATORS_PATH.exists():
+            raise FusedAttentionError(
+                f"fused_attention: {OPERATORS_PATH} is not built (run __graft_entry__.build() or "
+                "python candle-fused-attn_amd/build.py); there is no fallback path")
+        loader = importlib.machinery.ExtensionFileLoader("torch_operators", str(OPERATORS_PATH))
+        try:
+            module = importlib.util.module_from_spec(
+                importlib.util.spec_from_loader("torch_operators", loader))
+        except ImportError as e:
+            raise FusedAttentionError(f"fused_attention: cannot load {OPERATORS_PATH}: {e}") from e
+        _operators = module
+    return _operators
 
 
 def last_error() -> str:

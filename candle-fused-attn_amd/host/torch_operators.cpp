@@ -1,0 +1,608 @@
+// torch_operators.cpp -- the operators around self-attention for Python: torch tensors to the C ABI
+// (include/fattn.h), with their checks and allocations.
+//
+// Their smallest calls, a decoding token's, are bound by the host, so what lies between Python and the
+// launch is compiled: fused_rotary of one token takes 7.9 us a call, 12.8 with these steps in Python;
+// paged_append 5.5 for 13.7; paged_attention over 240 tokens 7.8 for 11.2. What records a graph stays
+// with torch.autograd.Function in Python, which calls the unchecked entries below; the checked ones
+// return None where a graph has to be recorded.
+//
+// Every entry takes its positional arguments from candle_fused_attn/{rotary,paged,cross}.py, whose
+// docstrings say what they mean. A refused argument raises the package's FusedAttentionError.
+#include <Python.h>
+
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/empty_like.h>
+#include <ATen/ops/empty_strided.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <initializer_list>
+#include <stdexcept>
+#include <string>
+#include <vector>
+
+#include "fattn.h"
+
+namespace {
+
+using at::ScalarType;
+using at::Tensor;
+typedef std::vector<Tensor> Tensors;
+
+// A refused argument or a failed launch; `code` as the C ABI returned it (0: refused here).
+struct OpError : std::runtime_error {
+  explicit OpError(const std::string& msg, int c = 0) : std::runtime_error(msg), code(c) {}
+  int code;
+};
+
+std::string shape_of(at::IntArrayRef x) {
+  std::string out = "[";
+  for (size_t i = 0; i < x.size(); ++i) out += (i ? ", " : "") + std::to_string(x[i]);
+  return out + "]";
+}
+const char* name_of(ScalarType t) {
+  switch (t) {
+    case ScalarType::Float: return "float32";
+    case ScalarType::Half: return "float16";
+    case ScalarType::BFloat16: return "bfloat16";
+    case ScalarType::Double: return "float64";
+    case ScalarType::Int: return "int32";
+    case ScalarType::Long: return "int64";
+    default: return c10::toString(t);
+  }
+}
+
+// The element types an operand may have.
+typedef std::initializer_list<ScalarType> Types;
+constexpr ScalarType kF32 = ScalarType::Float, kF16 = ScalarType::Half, kBF16 = ScalarType::BFloat16;
+constexpr ScalarType kI32 = ScalarType::Int, kI64 = ScalarType::Long, kF64 = ScalarType::Double;
+
+// A tensor of `rank` dimensions on a HIP device (that of `like`), of one of `types`.
+void require(const char* who, const char* name, const Tensor& t, int64_t rank, const Tensor* like,
+             Types types) {
+  bool known = false;
+  for (ScalarType x : types) known = known || t.scalar_type() == x;
+  if (known && t.dim() == rank && t.is_cuda() && (!like || t.get_device() == like->get_device())) return;
+  const std::string what = std::string(who) + ": " + name;
+  if (!known) {
+    std::string takes;
+    for (ScalarType x : types) takes += (takes.empty() ? "" : ", ") + std::string(name_of(x));
+    throw OpError(what + " must be " + takes + ", got " + name_of(t.scalar_type()));
+  }
+  if (t.dim() != rank) {
+    throw OpError(what + " must have " + std::to_string(rank) + " dimensions, got shape " +
+                  shape_of(t.sizes()));
+  }
+  if (!t.is_cuda()) throw OpError(what + " is not on a HIP device (this operator has no CPU path)");
+  throw OpError(what + " is on " + t.device().str() + ", the first operand on " + like->device().str());
+}
+
+int type_code(const Tensor& t) {
+  return t.scalar_type() == kF32 ? FATTN_F32 : t.scalar_type() == kF16 ? FATTN_F16 : FATTN_BF16;
+}
+// `t` itself where its last dimension is contiguous, else a contiguous copy.
+Tensor rows(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+// A four-dimensional `t` itself where its rows are contiguous and 16-byte aligned, else a contiguous copy.
+Tensor aligned_rows(const Tensor& t) {
+  const int64_t per = 16 / t.element_size();
+  bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && (t.stride(i) % per == 0 || t.size(i) <= 1);
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// fn(stream) on torch's current stream of t's device, with that device current.
+template <typename F>
+void launch(const Tensor& t, F fn) {
+  const c10::OptionalDeviceGuard guard(t.device());
+  const int rc = fn(static_cast<void*>(c10::hip::getCurrentHIPStream(t.get_device()).stream()));
+  if (rc != 0) throw OpError(fattn_last_error(), rc);
+}
+// A workspace from torch's allocator (undefined for 0 bytes).
+Tensor workspace(const Tensor& t, size_t bytes) {
+  return bytes == 0 ? Tensor()
+                    : at::empty({static_cast<int64_t>(bytes)}, t.options().dtype(ScalarType::Byte));
+}
+void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// --- Rotary positions ------------------------------------------------------------------------------
+
+struct Turn {
+  Tensor positions, frequencies;
+  int64_t heads;  // 0: [b, h, s, d] operands; else of the one [b, s, 3 h d] projection
+  bool interleaved;
+  double magnitude;
+  bool inverse;
+};
+
+int64_t check_frequencies(const char* who, const Tensor& f, int64_t d, const Tensor& like) {
+  require(who, "frequencies", f, 1, &like, {kF64});
+  if (2 * f.size(0) > d || !f.is_contiguous()) {
+    throw OpError(std::string(who) + ": contiguous frequencies of at most " + std::to_string(d / 2) +
+                  " pairs expected, got " + std::to_string(f.size(0)));
+  }
+  return 2 * f.size(0);
+}
+void check_positions(const char* who, const Tensor& p, int64_t b, int64_t s, const Tensor& like) {
+  if (p.dim() != 1 && p.dim() != 2) {
+    throw OpError(std::string(who) + ": positions must be a [s] or [b, s] tensor");
+  }
+  require(who, "positions", p, p.dim(), &like, {kI64, kI32});
+  if (p.size(-1) != s || (p.dim() == 2 && p.size(0) != 1 && p.size(0) != b)) {
+    throw OpError(std::string(who) + ": positions [" + std::to_string(s) + "] or [" + std::to_string(b) +
+                  ", " + std::to_string(s) + "] expected, got shape " + shape_of(p.sizes()));
+  }
+}
+
+// The turned tensors: one or two operands, or the one projection, whose q and k are turned and v copied.
+Tensors turned(const Tensors& xs, const Turn& how) {
+  Tensors ys;
+  for (const Tensor& x : xs) ys.push_back(at::empty_like(x));
+  const Tensor& x = xs[0];
+  int64_t heads[3] = {0, 0, 0}, xst[9] = {}, yst[9] = {}, pst[2] = {};
+  const void* xp[3] = {};
+  void* yp[3] = {};
+  int64_t b, s, d;
+  int mask = 0b111;
+  if (how.heads > 0) {
+    b = x.size(0), s = x.size(1), d = x.size(2) / (3 * how.heads);
+    const int64_t step = how.heads * d * x.element_size();
+    for (int i = 0; i < 3; ++i) {
+      heads[i] = how.heads;
+      xp[i] = static_cast<const char*>(x.data_ptr()) + i * step;
+      yp[i] = static_cast<char*>(ys[0].data_ptr()) + i * step;
+      xst[3 * i] = x.stride(0), xst[3 * i + 1] = d, xst[3 * i + 2] = x.stride(1);
+      yst[3 * i] = ys[0].stride(0), yst[3 * i + 1] = d, yst[3 * i + 2] = ys[0].stride(1);
+    }
+    mask = 0b011;
+  } else {
+    b = x.size(0), s = x.size(2), d = x.size(3);
+    for (size_t i = 0; i < xs.size(); ++i) {
+      heads[i] = xs[i].size(1);
+      xp[i] = xs[i].data_ptr(), yp[i] = ys[i].data_ptr();
+      for (int k = 0; k < 3; ++k) xst[3 * i + k] = xs[i].stride(k), yst[3 * i + k] = ys[i].stride(k);
+    }
+  }
+  const Tensor& p = how.positions;
+  pst[0] = p.dim() == 1 || p.size(0) == 1 ? 0 : p.stride(0);
+  pst[1] = p.stride(-1);
+  launch(x, [&](void* stream) {
+    return fattn_rotary(type_code(x), b, s, d, heads, xp, yp, xst, yst, mask, p.data_ptr(),
+                        p.scalar_type() == kI64 ? 64 : 32, pst,
+                        static_cast<const double*>(how.frequencies.data_ptr()), 2 * how.frequencies.size(0),
+                        how.interleaved, how.magnitude, how.inverse, stream);
+  });
+  return ys;
+}
+
+bool records(std::initializer_list<const Tensor*> ts) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts) {
+    if (t->defined() && t->requires_grad()) return true;
+  }
+  return false;
+}
+
+// Empty where a graph has to be recorded.
+Tensors fused_rotary(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& f,
+                           bool interleaved, double magnitude) {
+  const char* who = "fused_rotary";
+  require(who, "q", q, 4, nullptr, {kF32, kF16, kBF16});
+  require(who, "k", k, 4, &q, {q.scalar_type()});
+  if (k.size(0) != q.size(0) || k.size(2) != q.size(2) || k.size(3) != q.size(3)) {
+    throw OpError(std::string(who) + ": q and k must agree but for their heads, got " + shape_of(q.sizes()) +
+                  " and " + shape_of(k.sizes()));
+  }
+  check_positions(who, positions, q.size(0), q.size(2), q);
+  check_frequencies(who, f, q.size(3), q);
+  if (records({&q, &k})) return {};
+  return turned({rows(q), rows(k)}, Turn{positions, f, 0, interleaved, magnitude, false});
+}
+
+Tensors fused_rotary_qkv(const Tensor& qkv, int64_t heads, const Tensor& positions, const Tensor& f,
+                        bool interleaved, double magnitude) {
+  const char* who = "fused_rotary_qkv";
+  require(who, "qkv", qkv, 3, nullptr, {kF32, kF16, kBF16});
+  const int64_t w = qkv.size(2);
+  if (heads <= 0 || w == 0 || w % (3 * heads) != 0) {
+    throw OpError(std::string(who) + ": last dimension " + std::to_string(w) + " is not 3 x " +
+                  std::to_string(heads) + " heads x head_dim");
+  }
+  check_positions(who, positions, qkv.size(0), qkv.size(1), qkv);
+  check_frequencies(who, f, w / 3 / heads, qkv);
+  if (records({&qkv})) return {};
+  return turned({rows(qkv)}, Turn{positions, f, heads, interleaved, magnitude, false});
+}
+
+// --- The paged cache -------------------------------------------------------------------------------
+
+void check_cache(const char* who, const Tensor& x, const Tensor& kp, const Tensor& vp, const Tensor& table,
+                 const Tensor& lengths, int64_t b, int64_t d) {
+  require(who, "k_pages", kp, 4, &x, {kF32, kF16, kBF16});
+  require(who, "v_pages", vp, 4, &x, {kp.scalar_type()});
+  if (vp.sizes() != kp.sizes() || kp.size(3) != d) {
+    throw OpError(std::string(who) + ": k_pages and v_pages [pages, kv_heads, page_size, " +
+                  std::to_string(d) + "] expected, got " + shape_of(kp.sizes()) + " and " +
+                  shape_of(vp.sizes()));
+  }
+  if (d > 1 && (kp.stride(3) != 1 || vp.stride(3) != 1)) {
+    throw OpError(std::string(who) + ": k_pages and v_pages must have a contiguous last dimension, strides " +
+                  shape_of(kp.strides()) + " and " + shape_of(vp.strides()));
+  }
+  require(who, "page_table", table, 2, &x, {kI32});
+  require(who, "lengths", lengths, 1, &x, {kI32});
+  if (table.size(0) != b || lengths.size(0) != b || !lengths.is_contiguous() ||
+      (table.stride(1) != 1 && table.size(1) > 1)) {
+    throw OpError(std::string(who) + ": a page table [" + std::to_string(b) +
+                  ", width] with contiguous rows and contiguous lengths [" + std::to_string(b) +
+                  "] expected, got " + shape_of(table.sizes()) + " and " + shape_of(lengths.sizes()));
+  }
+}
+const int32_t* ints(const Tensor& t) { return t.defined() ? static_cast<const int32_t*>(t.data_ptr()) : nullptr; }
+void no_graph(const char* who, std::initializer_list<const Tensor*> ts) {
+  if (records(ts)) throw OpError(std::string(who) + ": not differentiable (call it under torch.no_grad())");
+}
+bool broadcast(const Tensor& t) {
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    if (t.stride(i) == 0 && t.size(i) > 1) return true;
+  }
+  return false;
+}
+
+// counts, q, f: undefined where absent. The turned q, undefined without one.
+Tensor paged_append(const Tensor& k0, const Tensor& v0, const Tensor& kp, const Tensor& vp,
+                    const Tensor& table, const Tensor& lengths, const Tensor& counts, const Tensor& q0,
+                    const Tensor& f, bool interleaved, double magnitude) {
+  const char* who = "paged_append";
+  require(who, "k", k0, 4, nullptr, {kF32, kF16, kBF16});
+  require(who, "v", v0, 4, &k0, {k0.scalar_type()});
+  const int64_t b = k0.size(0), hk = k0.size(1), s = k0.size(2), d = k0.size(3);
+  if (v0.sizes() != k0.sizes()) {
+    throw OpError(std::string(who) + ": k and v must share one shape, got " + shape_of(k0.sizes()) +
+                  " and " + shape_of(v0.sizes()));
+  }
+  check_cache(who, k0, kp, vp, table, lengths, b, d);
+  if (kp.size(1) != hk) {
+    throw OpError(std::string(who) + ": the cache has " + std::to_string(kp.size(1)) + " key heads, k has " +
+                  std::to_string(hk));
+  }
+  no_graph(who, {&k0, &v0, &q0, &kp, &vp});
+  if (broadcast(kp) || broadcast(vp)) {
+    throw OpError(std::string(who) + ": k_pages or v_pages is a broadcast view, whose slots share memory");
+  }
+  Tensor q, out;
+  int64_t heads = 0;
+  if (q0.defined()) {
+    require(who, "q", q0, 4, &k0, {k0.scalar_type()});
+    if (q0.size(0) != b || q0.size(2) != s || q0.size(3) != d) {
+      throw OpError(std::string(who) + ": q and k must agree but for their heads, got " +
+                    shape_of(q0.sizes()) + " and " + shape_of(k0.sizes()));
+    }
+    q = rows(q0), out = at::empty_like(q), heads = q.size(1);
+  }
+  if (counts.defined()) {
+    require(who, "counts", counts, 1, &k0, {kI32});
+    if (counts.size(0) != b || !counts.is_contiguous()) {
+      throw OpError(std::string(who) + ": contiguous counts [" + std::to_string(b) + "] expected, got " +
+                    shape_of(counts.sizes()));
+    }
+  }
+  const int64_t dim = f.defined() ? check_frequencies(who, f, d, k0) : 0;
+  const Tensor k = rows(k0), v = rows(v0);
+  launch(k, [&](void* stream) {
+    return fattn_paged_append(
+        type_code(k), type_code(kp), b, heads, hk, s, d, address(q), heads ? q.strides().data() : nullptr,
+        address(out), heads ? out.strides().data() : nullptr, k.data_ptr(), k.strides().data(), v.data_ptr(),
+        v.strides().data(), kp.data_ptr(), kp.strides().data(), vp.data_ptr(), vp.strides().data(),
+        kp.size(0), kp.size(2), ints(table), table.stride(0), table.size(1), ints(lengths), ints(counts),
+        static_cast<const double*>(address(f)), dim, interleaved, magnitude, stream);
+  });
+  return out;
+}
+
+Tensor paged_attention(const Tensor& q0, const Tensor& kp, const Tensor& vp, const Tensor& table,
+                       const Tensor& lengths, double scale) {
+  const char* who = "paged_attention";
+  require(who, "q", q0, 4, nullptr, {kF32, kF16, kBF16});
+  const int64_t b = q0.size(0), h = q0.size(1), d = q0.size(3);
+  if (q0.size(2) != 1) {
+    throw OpError(std::string(who) + ": q [b, h, 1, d] expected, got shape " + shape_of(q0.sizes()));
+  }
+  check_cache(who, q0, kp, vp, table, lengths, b, d);
+  no_graph(who, {&q0, &kp, &vp});
+  const Tensor q = aligned_rows(q0);
+  Tensor out = at::empty_like(q, q.options(), at::MemoryFormat::Contiguous);
+  const int64_t hk = kp.size(1), page = kp.size(2), width = table.size(1);
+  const size_t bytes = fattn_paged_attention_workspace_bytes(b, h, hk, d, width * page);
+  const Tensor ws = workspace(q, bytes);
+  launch(q, [&](void* stream) {
+    return fattn_paged_attention(type_code(q), type_code(kp), b, h, hk, d, q.data_ptr(), q.strides().data(),
+                                 out.data_ptr(), kp.data_ptr(), kp.strides().data(), vp.data_ptr(),
+                                 vp.strides().data(), kp.size(0), page, ints(table), table.stride(0), width,
+                                 ints(lengths), static_cast<float>(scale), address(ws), bytes, stream);
+  });
+  return out;
+}
+
+// --- Cross attention -------------------------------------------------------------------------------
+
+const float* f32(const Tensor& t) { return static_cast<const float*>(t.data_ptr()); }
+
+// The output, [b, h, sq, d] over a contiguous [b, sq, h, d] buffer, and the [b, h, sq] log-sums.
+Tensors cross_forward(const Tensor& q, const Tensor& k, const Tensor& v, double scale, const Tensor& lengths) {
+  const int64_t b = q.size(0), h = q.size(1), sq = q.size(2), d = q.size(3), hk = k.size(1), sk = k.size(2);
+  Tensor out = at::empty_strided({b, h, sq, d}, {sq * h * d, d, h * d, 1}, q.options());
+  Tensor lse = at::empty({b, h, sq}, q.options());
+  const size_t bytes = fattn_cross_workspace_bytes(b, h, hk, sq, sk, d);
+  const Tensor ws = workspace(q, bytes);
+  launch(q, [&](void* stream) {
+    return fattn_cross_forward(f32(q), q.strides().data(), f32(k), k.strides().data(), f32(v),
+                               v.strides().data(), b, h, hk, sq, sk, d, ints(lengths),
+                               static_cast<float>(scale), static_cast<float*>(out.data_ptr()),
+                               static_cast<float*>(lse.data_ptr()), address(ws), bytes, stream);
+  });
+  return {out, lse};
+}
+
+// dq over a contiguous [b, sq, h, d] buffer, dk and dv over one contiguous [b, sk, 2, kv_heads, d].
+Tensors cross_backward(const Tensor& q, const Tensor& k, const Tensor& v, double scale, const Tensor& lengths,
+                       const Tensor& out, const Tensor& lse, const Tensor& grad) {
+  const int64_t b = q.size(0), h = q.size(1), sq = q.size(2), d = q.size(3), hk = k.size(1), sk = k.size(2);
+  const Tensor g = aligned_rows(grad);
+  Tensor dq = at::empty_strided({b, h, sq, d}, {sq * h * d, d, h * d, 1}, q.options());
+  Tensor dkv = at::empty({b, sk, 2, hk, d}, q.options());
+  const size_t bytes = fattn_cross_backward_workspace_bytes(b, h, hk, sq, sk, d);
+  const Tensor ws = workspace(q, bytes);
+  launch(q, [&](void* stream) {
+    return fattn_cross_backward(f32(q), q.strides().data(), f32(k), k.strides().data(), f32(v),
+                                v.strides().data(), b, h, hk, sq, sk, d, ints(lengths),
+                                static_cast<float>(scale), f32(out), f32(lse), f32(g), g.strides().data(),
+                                static_cast<float*>(dq.data_ptr()), static_cast<float*>(dkv.data_ptr()),
+                                address(ws), bytes, stream);
+  });
+  return {dq, dkv.select(2, 0).transpose(1, 2), dkv.select(2, 1).transpose(1, 2)};
+}
+
+// The output alone; empty where a graph has to be recorded.
+Tensors fused_cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, double scale,
+                              const Tensor& lengths) {
+  const char* who = "fused_cross_attention";
+  require(who, "q", q, 4, nullptr, {kF32});
+  require(who, "k", k, 4, &q, {kF32});
+  require(who, "v", v, 4, &q, {kF32});
+  const int64_t b = q.size(0);
+  if (k.sizes() != v.sizes() || k.size(0) != b || k.size(3) != q.size(3)) {
+    throw OpError(std::string(who) + ": q [b, h, sq, d] and k, v [b, kv_heads, sk, d] expected, got " +
+                  shape_of(q.sizes()) + " " + shape_of(k.sizes()) + " " + shape_of(v.sizes()));
+  }
+  if (lengths.defined()) {
+    require(who, "key_lengths", lengths, 1, &q, {kI32});
+    if (lengths.size(0) != b || !lengths.is_contiguous()) {
+      throw OpError(std::string(who) + ": contiguous key_lengths [" + std::to_string(b) +
+                    "] expected, got " + shape_of(lengths.sizes()));
+    }
+  }
+  if (records({&q, &k, &v})) return {};
+  Tensors out = cross_forward(aligned_rows(q), aligned_rows(k), aligned_rows(v), scale, lengths);
+  out.resize(1);
+  return out;
+}
+
+// --- Python ----------------------------------------------------------------------------------------
+
+PyObject* g_error = nullptr;  // candle_fused_attn.FusedAttentionError
+
+// The positional arguments of a call, read in turn.
+struct Args {
+  const char* who;
+  PyObject* const* at;
+  Py_ssize_t left;
+
+  PyObject* next() {
+    if (left == 0) throw OpError(std::string(who) + ": too few arguments");
+    --left;
+    return *at++;
+  }
+  const Tensor& tensor(const char* name, PyObject* x) const {
+    if (!THPVariable_Check(x)) throw OpError(std::string(who) + ": " + name + " must be a tensor");
+    return THPVariable_Unpack(x);
+  }
+  const Tensor& tensor(const char* name) { return tensor(name, next()); }
+  Tensor maybe(const char* name) {
+    PyObject* x = next();
+    return x == Py_None ? Tensor() : tensor(name, x);
+  }
+  bool truth() {
+    const int x = PyObject_IsTrue(next());
+    if (x < 0) throw python_error();
+    return x == 1;
+  }
+  double number() {
+    const double x = PyFloat_AsDouble(next());
+    if (x == -1.0 && PyErr_Occurred()) throw python_error();
+    return x;
+  }
+  int64_t integer() {
+    const long long x = PyLong_AsLongLong(next());
+    if (x == -1 && PyErr_Occurred()) throw python_error();
+    return x;
+  }
+};
+
+// Without the interpreter's lock while it lives, as every call of torch's is.
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
+// Undefined tensors, and no tensors at all, are None.
+PyObject* one(const Tensor& t) {
+  if (t.defined()) return THPVariable_Wrap(t);
+  Py_RETURN_NONE;
+}
+PyObject* all(const Tensors& ts) {
+  if (ts.empty()) Py_RETURN_NONE;
+  PyObject* out = PyTuple_New(static_cast<Py_ssize_t>(ts.size()));
+  if (!out) throw python_error();
+  for (size_t i = 0; i < ts.size(); ++i) PyTuple_SET_ITEM(out, i, THPVariable_Wrap(ts[i]));
+  return out;
+}
+
+// body(args) with what it throws as Python's exceptions: OpError as FusedAttentionError, torch's errors
+// as torch raises them.
+template <typename F>
+PyObject* entry(const char* who, PyObject* const* args, Py_ssize_t n, F body) {
+  HANDLE_TH_ERRORS
+  try {
+    Args a{who, args, n};
+    return body(a);
+  } catch (const OpError& e) {
+    PyObject* x = PyObject_CallFunction(g_error, "si", e.what(), e.code);
+    if (x) {
+      PyErr_SetObject(g_error, x);
+      Py_DECREF(x);
+    }
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return entry("fused_rotary", args, n, [](Args& a) {
+    const Tensor &q = a.tensor("q"), &k = a.tensor("k"), &p = a.tensor("positions"),
+                 &f = a.tensor("frequencies");
+    const bool interleaved = a.truth();
+    const double magnitude = a.number();
+    Tensors out;
+    {
+      const Unlocked unlocked;
+      out = fused_rotary(q, k, p, f, interleaved, magnitude);
+    }
+    return all(out);
+  });
+}
+
+PyObject* py_rotary_qkv(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return entry("fused_rotary_qkv", args, n, [](Args& a) {
+    const Tensor& x = a.tensor("qkv");
+    const int64_t heads = a.integer();
+    const Tensor &p = a.tensor("positions"), &f = a.tensor("frequencies");
+    const bool interleaved = a.truth();
+    const double magnitude = a.number();
+    Tensors out;
+    {
+      const Unlocked unlocked;
+      out = fused_rotary_qkv(x, heads, p, f, interleaved, magnitude);
+    }
+    return all(out);
+  });
+}
+
+// turn(positions, frequencies, heads, interleaved, magnitude, inverse, *xs)
+PyObject* py_turn(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return entry("fused_rotary", args, n, [](Args& a) {
+    Turn how;
+    how.positions = a.tensor("positions"), how.frequencies = a.tensor("frequencies");
+    how.heads = a.integer(), how.interleaved = a.truth(), how.magnitude = a.number();
+    how.inverse = a.truth();
+    Tensors xs;
+    do xs.push_back(rows(a.tensor("x")));
+    while (a.left > 0 && xs.size() < 2);
+    Tensors out;
+    {
+      const Unlocked unlocked;
+      out = turned(xs, how);
+    }
+    return all(out);
+  });
+}
+
+PyObject* py_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return entry("paged_append", args, n, [](Args& a) {
+    const Tensor &k = a.tensor("k"), &v = a.tensor("v"), &kp = a.tensor("k_pages"),
+                 &vp = a.tensor("v_pages"), &table = a.tensor("page_table"), &lengths = a.tensor("lengths");
+    const Tensor counts = a.maybe("counts"), q = a.maybe("q"), f = a.maybe("frequencies");
+    const bool interleaved = a.truth();
+    const double magnitude = a.number();
+    Tensor out;
+    {
+      const Unlocked unlocked;
+      out = paged_append(k, v, kp, vp, table, lengths, counts, q, f, interleaved, magnitude);
+    }
+    return one(out);
+  });
+}
+
+PyObject* py_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return entry("paged_attention", args, n, [](Args& a) {
+    const Tensor &q = a.tensor("q"), &kp = a.tensor("k_pages"), &vp = a.tensor("v_pages"),
+                 &table = a.tensor("page_table"), &lengths = a.tensor("lengths");
+    const double scale = a.number();
+    Tensor out;
+    {
+      const Unlocked unlocked;
+      out = paged_attention(q, kp, vp, table, lengths, scale);
+    }
+    return one(out);
+  });
+}
+
+template <bool kChecked>
+PyObject* py_cross(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return entry("fused_cross_attention", args, n, [](Args& a) {
+    const Tensor &q = a.tensor("q"), &k = a.tensor("k"), &v = a.tensor("v");
+    const double scale = a.number();
+    const Tensor lengths = a.maybe("key_lengths");
+    Tensors out;
+    {
+      const Unlocked unlocked;
+      out = (kChecked ? fused_cross_attention : cross_forward)(q, k, v, scale, lengths);
+    }
+    return kChecked ? one(out.empty() ? Tensor() : out[0]) : all(out);
+  });
+}
+
+PyObject* py_cross_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return entry("fused_cross_attention", args, n, [](Args& a) {
+    const Tensor &q = a.tensor("q"), &k = a.tensor("k"), &v = a.tensor("v");
+    const double scale = a.number();
+    const Tensor lengths = a.maybe("key_lengths");
+    const Tensor &out = a.tensor("out"), &lse = a.tensor("lse"), &grad = a.tensor("grad");
+    Tensors grads;
+    {
+      const Unlocked unlocked;
+      grads = cross_backward(q, k, v, scale, lengths, out, lse, grad);
+    }
+    return all(grads);
+  });
+}
+
+PyMethodDef g_methods[] = {
+#define ENTRY(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL, ""}
+    ENTRY("rotary", py_rotary),
+    ENTRY("rotary_qkv", py_rotary_qkv),
+    ENTRY("turn", py_turn),
+    ENTRY("paged_append", py_append),
+    ENTRY("paged_attention", py_paged_attention),
+    ENTRY("cross", py_cross<true>),
+    ENTRY("cross_forward", py_cross<false>),
+    ENTRY("cross_backward", py_cross_backward),
+#undef ENTRY
+    {nullptr, nullptr, 0, nullptr}};
+
+PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "torch_operators", nullptr, -1, g_methods,
+                        nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit_torch_operators() {
+  PyObject* package = PyImport_ImportModule("candle_fused_attn._lib");
+  if (!package) return nullptr;
+  g_error = PyObject_GetAttrString(package, "FusedAttentionError");
+  Py_DECREF(package);
+  return g_error ? PyModule_Create(&g_module) : nullptr;
+}

@@ -219,3 +219,28 @@ def test_python_refusals():
     ]:
         with pytest.raises(cfa.FusedAttentionError, match=text):
             call()
+
+
+def test_missing_binding_is_an_error(monkeypatch, tmp_path):
+    monkeypatch.setattr(_lib, "_operators", None)
+    monkeypatch.setattr(_lib, "OPERATORS_PATH", tmp_path / "absent.so")
+    with pytest.raises(cfa.FusedAttentionError, match="not built"):
+        cfa.fused_cross_attention(torch.zeros(1), torch.zeros(1), torch.zeros(1), 1.0)
+    monkeypatch.setattr(_lib, "OPERATORS_PATH", tmp_path / "broken.so")
+    (tmp_path / "broken.so").write_bytes(b"no library")
+    with pytest.raises(cfa.FusedAttentionError, match="cannot load"):
+        cfa.fused_cross_attention(torch.zeros(1), torch.zeros(1), torch.zeros(1), 1.0)
+
+
+def test_binding_arguments():
+    q, f = torch.randn(1, 2, 3, 64), cfa.rotary_frequencies(64)
+    pos = torch.arange(3)
+    with pytest.raises(cfa.FusedAttentionError, match="too few arguments"):
+        _lib.operators().rotary(q, q, pos)
+    with pytest.raises(TypeError):
+        cfa.fused_rotary(q, q, pos, f, False, "one")
+    with pytest.raises(TypeError):
+        cfa.fused_cross_attention(q, q, q, None)
+    with pytest.raises(cfa.FusedAttentionError) as e:
+        cfa.fused_cross_attention(q, q, q, 1.0)
+    assert e.value.code == 0

@@ -26,8 +26,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     lengths[b] + i; so is `q` ([b, h, s, d], of k's type), every row of it, and the call returns it (a
     new tensor; None without q). f32 keys and values are rounded to the cache's type. A token whose
     page the table or the cache does not have is not written (its sequence's attention gives NaN), and
-    no slot that holds no new token is touched. Two new tokens must not share a slot. Not
-    differentiable.
+    no slot that holds no new token is touched. Two new tokens must not share a slot, and k, v and q must
+    not lie in the cache. Not differentiable.
     """
     return operators().paged_append(k, v, k_pages, v_pages, page_table, lengths, counts, q, frequencies,
                                     interleaved, magnitude)

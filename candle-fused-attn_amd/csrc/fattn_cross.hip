@@ -116,6 +116,8 @@ CrossForwardPlan cross_forward_plan(int64_t b, int64_t h, int64_t hk, int64_t sq
 
 CrossBackwardPlan cross_backward_plan(int64_t b, int64_t h, int64_t hk, int64_t sq, int64_t sk, int64_t d) {
   CrossBackwardPlan p{};
+  p.ncq = p.nck = 1, p.chq = static_cast<int>(ceil_div(sk, kRows)), p.chk = 1;
+  if (sq == 0 || sk == 0) return p;  // (nothing to walk, and nothing to join)
   const int64_t slots = 256 * (d == 32 ? 3 : d == 64 ? 2 : 1);
   const int64_t tq = ceil_div(sq, kRows), tk = ceil_div(sk, kRows), g = h / hk;
   // A step of a key block takes four products, of a query block three. Chunks as in the forward, of 20

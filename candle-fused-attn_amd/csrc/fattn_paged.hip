@@ -567,16 +567,17 @@ split_kernel(SplitArgs a) {
 #pragma unroll
       for (int y = 0; y < kSplitWaves; ++y) {
         const float my = sml[y][0][row], ly = sml[y][1][row];
-        // (A wave without a score left no sums; its l may still be NaN, for a page.)
+        // (A wave without a finite score has sums of 0, or NaN for infinite values; its l may still be NaN,
+        // for a page.)
         const float f = my == kNegInf ? 0.0f : my == m ? 1.0f : exp2_hw(my - m);
         l += my == kNegInf ? ly : ly * f;
-        const f4 oy = ld4(&so[y][row][d]);
-        if (f != 0.0f) o += oy * f;
+        o += ld4(&so[y][row][d]) * f;
       }
       if (whole) {
         int head, q;
         row_of(a, kvh, r0 + row, head, q);
-        put4(out_row<Q>(a, b, head, q, D) + d, l == 0.0f ? f4{} : o * (1.0f / l));
+        // (l is 0 where every score is minus infinity: NaN, as the formula.)
+        put4(out_row<Q>(a, b, head, q, D) + d, o * (1.0f / l));
         if (d == 0) put_lse(a, b, head, q, m, l);
       } else {
         st4(part + row * (D + 4) + d, o);
@@ -643,17 +644,17 @@ __global__ void __launch_bounds__(256) join_kernel(SplitArgs a) {
     const float before = m;
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
-      if (w + i * kGroups > w1) ms[i] = kNegInf, ls[i] = 0.0f;
+      if (w + i * kGroups > w1) ms[i] = kNegInf, ls[i] = 0.0f, os[i] = f4{};
       m = fmaxf(m, ms[i]);
     }
     const float f = before == kNegInf ? 0.0f : exp2_hw(before - m);
     o *= f, l *= before == kNegInf ? 1.0f : f;
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
-      // (Sums without a score are 0; l may still be NaN, for a page.)
+      // (As for the waves' sums.)
       const float fi = ms[i] == kNegInf ? 0.0f : exp2_hw(ms[i] - m);
       l += ms[i] == kNegInf ? ls[i] : ls[i] * fi;
-      o += fi == 0.0f ? f4{} : os[i] * fi;
+      o += os[i] * fi;
     }
   }
   st4(&so[grp][d], o);
@@ -666,9 +667,9 @@ __global__ void __launch_bounds__(256) join_kernel(SplitArgs a) {
   for (int y = 0; y < kGroups; ++y) {
     const float f = sm[y] == kNegInf ? 0.0f : exp2_hw(sm[y] - mm);
     l += sm[y] == kNegInf ? sl[y] : sl[y] * f;
-    if (f != 0.0f) o += ld4(&so[y][d]) * f;
+    o += ld4(&so[y][d]) * f;
   }
-  put4(out_row<Q>(a, b, head, q, D) + d, l == 0.0f ? f4{} : o * (1.0f / l));
+  put4(out_row<Q>(a, b, head, q, D) + d, o * (1.0f / l));
   if (tid == 0) put_lse(a, b, head, q, mm, l);
 }
 

@@ -541,7 +541,9 @@ __device__ __forceinline__ void fwd_rows_fp32(const FwdArgs& a, int b, int h, in
   for (; k0 + kRows <= (kCausal ? min(SK, qg + 1) : SK); k0 += kRows) tile(Const<1>{}, k0);
   for (; k0 < kend; k0 += kRows) tile(Const<0>{}, k0);
   l = pair_sum(l);
-  store(acc, 1.0f / l);
+  // (A chunk whose scores are all minus infinity weighs nothing beside others: its sums as they are. A row
+  // of such is NaN, as its formula is: 0 / 0.)
+  store(acc, kCross && a.l_part != nullptr && l == 0.0f ? 1.0f : 1.0f / l);
   if (g == 0 && qi < S) {
     put_l<kCross>(a, (static_cast<int64_t>(b) * a.H + h) * S + qi, m * fabsf(a.scale) + logf(l));
   }

@@ -208,7 +208,7 @@ Tensors fused_rotary_qkv(const Tensor& qkv, int64_t heads, const Tensor& positio
   const char* who = "fused_rotary_qkv";
   require(who, "qkv", qkv, 3, nullptr, {kF32, kF16, kBF16});
   const int64_t w = qkv.size(2);
-  if (heads <= 0 || w == 0 || w % (3 * heads) != 0) {
+  if (heads <= 0 || heads > w / 3 || w % (3 * heads) != 0) {
     throw OpError(std::string(who) + ": last dimension " + std::to_string(w) + " is not 3 x " +
                   std::to_string(heads) + " heads x head_dim");
   }
@@ -273,6 +273,9 @@ Tensor paged_append(const Tensor& k0, const Tensor& v0, const Tensor& kp, const 
   no_graph(who, {&k0, &v0, &q0, &kp, &vp});
   if (broadcast(kp) || broadcast(vp)) {
     throw OpError(std::string(who) + ": k_pages or v_pages is a broadcast view, whose slots share memory");
+  }
+  if (kp.numel() > 0 && kp.data_ptr() == vp.data_ptr()) {
+    throw OpError(std::string(who) + ": k_pages and v_pages are the same memory");
   }
   Tensor q, out;
   int64_t heads = 0;

@@ -140,6 +140,28 @@ def test_non_finite_values_that_are_seen(cuda, sq, sk):
         assert rel(x[fine], y[fine]) <= TOL, name
 
 
+@pytest.mark.parametrize("sq,sk", [(5, 70), (5, 1500), (130, 70), (130, 1500)])
+def test_scores_of_minus_infinity(cuda, sq, sk):
+    """Keys that score minus infinity, whole tiles and chunks of them: no weight; a sample of nothing else:
+    NaN, as the formula. (Positive queries, so that no infinite score is of another sign.)"""
+    q, k, v, g = operands(cuda, 2, 2, 2, sq, sk, 64, seed=14)
+    q = q.abs() + 0.5
+    k[0, :, : sk * 2 // 3, 5] = -float("inf")
+    k[1, 1, :, 5] = -float("inf")
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = cfa.fused_cross_attention(q, k, v, 0.125)
+    got = [out.detach(), *torch.autograd.grad(out, leaves, g)]
+    exact = [t.detach().double().cpu().requires_grad_() for t in leaves]
+    ref = formula(*exact, 0.125)
+    want = [ref.detach(), *torch.autograd.grad(ref, exact, g.double().cpu())]
+    assert bool(want[0][1, 1].isnan().all()) and bool(want[0][0].isfinite().all())
+    for name, x, y in zip(("o", "dq", "dk", "dv"), got, want):
+        x = x.double().cpu()
+        fine = y.isfinite()
+        assert torch.equal(fine, x.isfinite()), name
+        assert rel(x[fine], y[fine]) <= TOL, name
+
+
 def test_strides_and_broadcasts(cuda):
     """Head views of fused projections, padded rows, odd offsets and broadcast keys: as contiguous ones."""
     b, h, sq, sk, d = 2, 4, 37, 50, 64
@@ -214,7 +236,8 @@ def test_some_gradients_only(cuda):
         dq.sum().backward()
 
 
-@pytest.mark.parametrize("shape", [(0, 2, 2, 5, 5), (2, 2, 2, 0, 5), (2, 2, 2, 5, 0), (2, 0, 0, 5, 5)])
+@pytest.mark.parametrize("shape", [(0, 2, 2, 5, 5), (2, 2, 2, 0, 5), (2, 2, 2, 5, 0), (2, 0, 0, 5, 5),
+                                   (2, 2, 2, 0, 900), (2, 2, 2, 900, 0), (1, 2, 1, 900, 0)])
 def test_empty(cuda, shape):
     q, k, v, g = operands(cuda, *shape, 64)
     leaves = [t.requires_grad_() for t in (q, k, v)]

@@ -177,6 +177,27 @@ def test_attention_non_finite_values_that_are_seen(cuda, types, n):
     assert rel(out[fine][None], ref[fine][None]) <= bar(dt)
 
 
+@pytest.mark.parametrize("types", PAIRS, ids="-".join)
+@pytest.mark.parametrize("n", [70, 1500])
+def test_attention_scores_of_minus_infinity(cuda, types, n):
+    """Keys that score minus infinity have no weight, whole tiles and runs of them; an infinite value of one
+    gives NaN (0 times infinity), and a sequence of nothing else is NaN, as the formula."""
+    dt, ct = (TYPES[t] for t in types)
+    c = Cache(cuda, ct, 1, 16, 64, [n] * 4, seed=19)
+    q = ((torch.randint(1, 5, (4, 2, 1, 64), generator=torch.Generator().manual_seed(3)) / 2)
+         .to(dt).to(cuda))
+    for i, last in ((1, n * 2 // 3), (2, n), (3, n * 2 // 3)):
+        for t in range(last):
+            c.k[int(c.table[i, t // 16]), 0, t % 16, 9] = -float("inf")
+    c.v[int(c.table[3, 2]), 0, 5, 4] = float("inf")
+    out = cfa.paged_attention(q, c.k, c.v, c.table, c.lengths, 0.05).double().cpu()
+    ref = attend(q, c, [n] * 4, 0.05)
+    assert torch.equal(out.isnan(), ref.isnan()) and bool(ref[2].isnan().all())
+    assert ref[3].isnan().sum() == 2 and bool(ref[1].isfinite().all())
+    fine = ref.isfinite()
+    assert rel(out[fine][None], ref[fine][None]) <= bar(dt)
+
+
 def test_attention_strided_cache_and_queries(cuda):
     """Keys and values interleaved in one pool whose rows are padded and whose heads come after the
     slots; queries out of a wider buffer, misaligned ones copied."""
@@ -364,6 +385,13 @@ def test_attention_side_streams(cuda):
                 got[i].append(cfa.paged_attention(qs[i], c.k, c.v, c.table, c.lengths, 0.125))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
+
+
+def test_append_refuses_one_cache_for_both(cuda):
+    c = Cache(cuda, torch.float32, 2, 16, 64, [3])
+    x = torch.zeros(1, 2, 1, 64, device=cuda)
+    with pytest.raises(cfa.FusedAttentionError, match="same memory"):
+        cfa.paged_append(x, x, c.k, c.k, c.table, c.lengths)
 
 
 def test_append_refuses_broadcast_pages(cuda):

@@ -233,3 +233,10 @@ def test_far_operands(cuda):
     want = cfa.fused_rotary(x[:, :, :5], x[:, :, :5], pos[:5], f)[0]
     for t in (y, z):
         assert torch.equal(t[:, :, :5], want) and torch.equal(t[:, :, -5:], want)
+
+
+def test_impossible_heads_refused(cuda):
+    qkv, f = torch.zeros(1, 2, 192, device=cuda), cfa.rotary_frequencies(64, device=cuda)
+    for heads in (0, -1, 5, 65, (2 ** 64 - 1) // 3):
+        with pytest.raises(cfa.FusedAttentionError, match="is not 3 x"):
+            cfa.fused_rotary_qkv(qkv, heads, torch.arange(2, device=cuda), f)

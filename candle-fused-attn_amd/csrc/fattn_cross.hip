@@ -85,6 +85,9 @@ __global__ void __launch_bounds__(256) join_sum_kernel(const float* part, float*
 }  // namespace
 
 int64_t cross_blocks(int64_t heads, int64_t s) { return heads * ceil_div(s, kBlockRows); }
+int64_t cross_query_blocks(int64_t pairs, int64_t g, int64_t s, int wave_rows) {
+  return pairs * ceil_div(g * ceil_div(s, wave_rows), 4);
+}
 
 CrossForwardPlan cross_forward_plan(int64_t b, int64_t h, int64_t hk, int64_t sq, int64_t sk, int64_t d) {
   CrossForwardPlan p{};
@@ -103,7 +106,7 @@ CrossForwardPlan cross_forward_plan(int64_t b, int64_t h, int64_t hk, int64_t sq
   // Chunks of the keys where the blocks do not fill the chip, of 8 tiles or more: d 128 2 x 16 heads
   // 100 x 3000 58 us (202 whole), 4 heads 2048 x 4096 60 (164). A grid that fills it loses by them: b 64
   // h 6 240 x 1024 116 in two chunks, 80 whole.
-  const int64_t slots = 256 * (d == 32 ? 4 : d == 64 ? 3 : 2), blocks = cross_blocks(b * h, sq);
+  const int64_t slots = 256 * (d == 32 ? 4 : d == 64 ? 3 : 2), blocks = cross_query_blocks(b * hk, h / hk, sq);
   const int64_t steps = ceil_div(sk, kRows);
   chunks(steps, std::max<int64_t>(8, ceil_div(blocks * steps, slots)), &p.nc, &p.chunk);
   if (p.nc > 1) {
@@ -124,7 +127,7 @@ CrossBackwardPlan cross_backward_plan(int64_t b, int64_t h, int64_t hk, int64_t 
   // products or more: forward and backward, us, 4 x 8 heads 1 x 4096 82 (235 whole), d 128 2 x 16 heads
   // 100 x 3000 221 (320), 1 head 500 x 500 45 (63); of 32 57, of 12 42, but d 128 4 x 8 heads in 2
   // groups 12 x 1000 74, 68 and 69.
-  const int64_t all = cross_blocks(b * hk, sk) * g * tq * 4 + cross_blocks(b * h, sq) * tk * 3;
+  const int64_t all = cross_blocks(b * hk, sk) * g * tq * 4 + cross_query_blocks(b * hk, g, sq) * tk * 3;
   const int64_t target = std::max<int64_t>(20, ceil_div(all, slots));
   chunks(g * tq, ceil_div(target, 4), &p.nck, &p.chk);
   chunks(tk, ceil_div(target, 3), &p.ncq, &p.chq);
@@ -139,8 +142,10 @@ int launch_cross_forward(View q, View k, View v, float* o, float* lse, int b, in
                          int sk, int d, const int32_t* key_lengths, float scale,
                          const CrossForwardPlan& plan, void* workspace, void* stream) {
   // 64 queries per wave where self-attention takes them.
-  const bool wide = wide_queries(int64_t{b} * h, sq, d);
-  const int rows = wide ? 2 * kBlockRows : kBlockRows, nqb = (sq + rows - 1) / rows;
+  const int64_t pairs = int64_t{b} * hk;
+  const bool wide = wide_queries(cross_query_blocks(pairs, h / hk, sq, 2 * kRows),
+                                 cross_query_blocks(pairs, h / hk, sq), sq, d);
+  const int nqb = static_cast<int>(cross_query_blocks(1, h / hk, sq, wide ? 2 * kRows : kRows));
   float* o_part = static_cast<float*>(workspace);
   double* l_part = reinterpret_cast<double*>(static_cast<char*>(workspace) + plan.l_part);
   const bool cut = plan.nc > 1;
@@ -153,7 +158,7 @@ int launch_cross_forward(View q, View k, View v, float* o, float* lse, int b, in
                    : d == 128        ? reinterpret_cast<const void*>(fwd_cross_kernel<128, 1, 4, 2>)
                                      : reinterpret_cast<const void*>(fwd_cross_kernel<64, 1, 4, 3>);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const unsigned grid = static_cast<unsigned>(int64_t{nqb} * b * h * plan.nc);
+  const unsigned grid = static_cast<unsigned>(pairs * nqb * plan.nc);
   const hipError_t err = hipLaunchKernel(fn, dim3(grid), dim3(256), args, 0, s);
   if (err != hipSuccess || !cut) return static_cast<int>(err);
   const float* op = o_part;
@@ -171,7 +176,7 @@ int launch_cross_backward(View q, View k, View v, View d_o, const float* o, cons
                           float* dkv, int b, int h, int hk, int sq, int sk, int d,
                           const int32_t* key_lengths, float scale, const CrossBackwardPlan& plan,
                           void* workspace, void* stream) {
-  const int nblk = (sk + kBlockRows - 1) / kBlockRows, nblk_q = (sq + kBlockRows - 1) / kBlockRows;
+  const int nblk = (sk + kBlockRows - 1) / kBlockRows, nblk_q = static_cast<int>(cross_query_blocks(1, h / hk, sq));
   float* q_part = static_cast<float*>(workspace);
   float* k_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.k_part);
   BwdPairArgs a{};
@@ -186,7 +191,7 @@ int launch_cross_backward(View q, View k, View v, View d_o, const float* o, cons
                    : d == 128 ? reinterpret_cast<const void*>(bwd_cross_kernel<128, 4, 1>)
                               : reinterpret_cast<const void*>(bwd_cross_kernel<64, 4, 2>);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipError_t err = hipLaunchKernel(fn, dim3(static_cast<unsigned>(a.nkv + nblk_q * b * h * plan.ncq)),
+  hipError_t err = hipLaunchKernel(fn, dim3(static_cast<unsigned>(a.nkv + nblk_q * b * hk * plan.ncq)),
                                    dim3(256), args, 0, s);
   auto sum = [&](const float* part, float* out, int64_t per, const int32_t* lengths, int nc, int chunk) {
     void* jargs[] = {&part, &out, &per, &sk, &lengths, &nc, &chunk};

@@ -154,8 +154,9 @@ void test_hook_state(int64_t out[3]);
 // and return a hipError_t value as int (0 = launched).
 int launch_forward(View q, View k, View v, float* o, float* lse, int b, int h, int s, int d,
                    float scale, int causal, void* stream);
-// Whether a forward in which every workgroup walks all keys takes 64 queries per wave, not 32.
-bool wide_queries(int64_t bh, int s, int d);
+// Whether a forward in which every workgroup walks all keys takes 64 queries per wave, not 32: `wide` and
+// `narrow`, its workgroups of either kind.
+bool wide_queries(int64_t wide, int64_t narrow, int s, int d);
 // Backward, step 2 (fattn_pair.hip): dK, dV and dQ. part, done, epoch_slot (a split-size workspace,
 // else null): with `defer` dQ goes to `part` for step 3, else to its rows, and `done` takes `epoch`
 // per 16-query tile. last: no step 3 follows. give_up_bh: a test hook's pair (-1: none).
@@ -267,7 +268,9 @@ int launch_cross_backward(View q, View k, View v, View d_o, const float* o, cons
                           float* dkv, int b, int h, int hk, int sq, int sk, int d,
                           const int32_t* key_lengths, float scale, const CrossBackwardPlan& plan,
                           void* workspace, void* stream);
-int64_t cross_blocks(int64_t heads, int64_t s);  // workgroups over `heads` (b, head) of s rows
+// Workgroups over `heads` (b, head) of s rows; over the queries of `pairs` (b, key head) with groups of g.
+int64_t cross_blocks(int64_t heads, int64_t s);
+int64_t cross_query_blocks(int64_t pairs, int64_t g, int64_t s, int wave_rows = 32);
 
 // Sets this thread's message (fattn_last_error) and returns `code`; done() clears it and returns 0.
 int set_error(int code, const char* format, ...) __attribute__((format(printf, 2, 3)));

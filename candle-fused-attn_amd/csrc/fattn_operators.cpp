@@ -191,7 +191,7 @@ int cross_operands(Cross& c, const float* q, const int64_t q_strides[3], const f
   const int64_t lim = INT32_MAX - 256;
   if (b > lim || sq > lim || sk > lim || b * heads > lim || b * heads * sq > lim ||
       b * kv_heads * sk > lim ||
-      fattn::cross_blocks(b * heads, sq) + fattn::cross_blocks(b * kv_heads, sk) > kMaxGrid) {
+      fattn::cross_query_blocks(b * kv_heads, heads / kv_heads, sq) + fattn::cross_blocks(b * kv_heads, sk) > kMaxGrid) {
     return set_error(FATTN_ERANGE, "%s: the sizes exceed 32-bit indexing or the launch limit", kCross);
   }
   if ((sq > 0 && (!q || !q_strides)) || (sk > 0 && (!k || !v || !k_strides || !v_strides))) {

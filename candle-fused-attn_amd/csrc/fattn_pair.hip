@@ -62,7 +62,7 @@ const void* bwd_pair_fn(int causal, bool serial, int waves) {
 
 }  // namespace
 
-bool wide_queries(int64_t bh, int s, int d) {
+bool wide_queries(int64_t wide, int64_t narrow, int s, int d) {
   // 64 queries per wave (256 per workgroup) halve what a query pays for reading, splitting and
   // waiting for the key tiles, but hold 2 waves per SIMD instead of 3 (D 64; 3 instead of 4 at D 32)
   // and halve the workgroups. Taken where every workgroup walks all keys, 1024 of them keep every CU
@@ -72,14 +72,16 @@ bool wide_queries(int64_t bh, int s, int d) {
   // 119 / 108, 256 x 256 26 / 23; padded, 1024 x 300 140 / 121, 1024 x 640 425 / 419, and below s 128
   // half of it is (1536 x 32: 29 / 17). D 32, 256 x 1024 145 / 150, 512 x 512 81 / 81, but 1024 x 200
   // 46 / 43: from s 257 on. At D 128 their registers do not fit.
-  const int64_t wide = static_cast<int64_t>((s + 255) / 256) * bh;
-  const bool filled = 8 * 2 * ((s + 255) / 256) <= 9 * ((s + 127) / 128) && (d == 64 || s > 256);
+  const bool filled = 8 * 2 * wide <= 9 * narrow && (d == 64 || s > 256);
   return d != 128 && wide >= 1024 && filled;
 }
 
 int launch_forward(View q, View k, View v, float* o, float* lse, int b, int h, int s, int d,
                    float scale, int causal, void* stream) {
-  const int nq = !causal && wide_queries(int64_t{b} * h, s, d) ? 2 : 1;
+  const int nq = !causal && wide_queries(int64_t{b} * h * ((s + 255) / 256), int64_t{b} * h * ((s + 127) / 128),
+                                           s, d)
+                     ? 2
+                     : 1;
   const int waves = workgroup_waves(b * h, s, d != 128), qb = kRows * waves * nq, nqb = (s + qb - 1) / qb;
   FwdArgs a{q, k, v, o, lse, b, h, s, nqb, scale, causal ? 1 : 0, s, 1, nullptr,
             1, 0, nullptr};

@@ -490,6 +490,17 @@ __device__ __forceinline__ int key_head(const Args& a, int h) {
   return kCross ? h / a.G : h;
 }
 
+// A wave's query rows where key heads are shared: the tiles of `rows` queries of a group's heads follow one
+// another, and tile `at` is one wave's, so a workgroup's waves may have rows of several heads, whose keys
+// are the same, and only a group's last workgroup has waves without any. (Blocks of one head each / so,
+// forward and backward, us: 64 x 16 heads in 4 groups, 300 x 700, d 64 235 + 740 / 203 + 718; 64 x 12 in 4,
+// 129 x 400 70 + 195 / 61 + 173.) The head in the group, and the first row (S for a wave without).
+__device__ __forceinline__ int group_rows(int S, int G, int rows, int at, int& q0) {
+  const int tiles = (S + rows - 1) / rows, h = min(at / tiles, G - 1);
+  q0 = at < G * tiles ? (at - h * tiles) * rows : S;
+  return h;
+}
+
 // L of a row: of a chunk in 64 bits, since the join takes differences of it.
 template <bool kCross>
 __device__ __forceinline__ void put_l(const FwdArgs& a, int64_t at, double L) {
@@ -572,14 +583,13 @@ __device__ __forceinline__ void fwd_pair(FwdArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int S = a.S, BH = a.B * a.H;
-  int qb, bh, chunk = 0;
+  int qb, bh, chunk = 0, qw0;
   if constexpr (kCross) {
     int in;
-    const int pair = spread(static_cast<int>(blockIdx.x), BH / a.G, a.nqb * a.G * a.nc, in);
-    chunk = in / (a.nqb * a.G);
-    in -= chunk * (a.nqb * a.G);
-    qb = in / a.G;
-    bh = pair * a.G + in % a.G;
+    const int pair = spread(static_cast<int>(blockIdx.x), BH / a.G, a.nqb * a.nc, in);
+    chunk = in / a.nqb;
+    qb = in - chunk * a.nqb;
+    bh = pair * a.G + group_rows(S, a.G, kWaveQ, qb * W + w, qw0);
   } else if (kCausal) {
     qb = a.nqb - 1 - static_cast<int>(blockIdx.x) / BH;  // the most expensive first
     bh = static_cast<int>(blockIdx.x) % BH;
@@ -600,7 +610,8 @@ __device__ __forceinline__ void fwd_pair(FwdArgs a) {
       a.l_part += chunk * (static_cast<int64_t>(BH) * S);
     }
   }
-  const int q0 = qb * kQ, qw0 = q0 + w * kWaveQ;
+  const int q0 = qb * kQ;
+  if constexpr (!kCross) qw0 = q0 + w * kWaveQ;
   const float* qp = a.q.p + b * a.q.sb + h * a.q.sh;
   const Operand kop{reinterpret_cast<const char*>(a.k.p + b * a.k.sb + hk * a.k.sh +
                                                   (kCross ? key0 * a.k.ss : 0)),
@@ -611,13 +622,11 @@ __device__ __forceinline__ void fwd_pair(FwdArgs a) {
 
   if constexpr (kCross) {
     if (SK == 0) {  // no key to see: O is 0, L -infinity
-      for (int i = tid; i < min(S - q0, kQ) * (D / 4); i += 64 * W) {
-        const int64_t row = static_cast<int64_t>(b) * S + q0 + i / (D / 4);
+      for (int i = lane; i < min(S - qw0, kWaveQ) * (D / 4); i += 64) {
+        const int64_t row = static_cast<int64_t>(b) * S + qw0 + i / (D / 4);
         st4(a.o + (row * a.H + h) * D + i % (D / 4) * 4, f4{});
       }
-      for (int i = q0 + tid; i < min(S, q0 + kQ); i += 64 * W) {
-        a.lse[static_cast<int64_t>(bh) * S + i] = kNegInf;
-      }
+      if (lane < min(S - qw0, kWaveQ)) a.lse[static_cast<int64_t>(bh) * S + qw0 + lane] = kNegInf;
       return;
     }
   }
@@ -886,7 +895,7 @@ struct BwdPairArgs {
   float scale;
   int causal, defer, last, give_up_bh;
   // Cross attention: dQ [b, S, H, D], dK and dV in one [b, SK, 2, H / G, D]; the keys' length, query heads
-  // per key head, each sample's keys (null: SK); query blocks per (b, h).
+  // per key head, each sample's keys (null: SK); query blocks per (b, key head).
   float *dq, *dkv;
   int SK, G;
   const int32_t* key_lengths;
@@ -1300,17 +1309,19 @@ __device__ __forceinline__ void bwd_queries(const BwdPairArgs& a, BwdSmem<D, W>&
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nblk = kCross ? a.nblk_q : a.nblk;
-  const int S = a.S, bh = item / nblk, qb = item % nblk;
+  const int S = a.S, qb = item % nblk, q0 = qb * (W * kRows);  // (item: of the (b, key head), crossing)
+  int bh = item / nblk, qw0 = q0 + w * kRows;
+  if constexpr (kCross) bh = bh * a.G + group_rows(S, a.G, kRows, qb * W + w, qw0);
   const int b = bh / a.H, h = bh % a.H, hk = key_head<kCross>(a, h);
   const int keys = key_count<kCross>(a, b), key0 = kCross ? chunk * a.chq * kRows : 0;
   const int SK = kCross && a.ncq > 1 ? min(keys - key0, a.chq * kRows) : keys;
-  const int q0 = qb * (W * kRows), qw0 = q0 + w * kRows, qi = qw0 + j;
+  const int qi = qw0 + j;
   const bool wave_live = qw0 < S;
   if constexpr (kCross) {
     if (a.ncq > 1 && SK <= 0) return;  // (the join knows)
     if (SK == 0) {  // no key was seen
-      for (int i = tid; i < min(S - q0, W * kRows) * (D / 4); i += 64 * W) {
-        const int64_t row = static_cast<int64_t>(b) * S + q0 + i / (D / 4);
+      for (int i = lane; i < min(S - qw0, kRows) * (D / 4); i += 64) {
+        const int64_t row = static_cast<int64_t>(b) * S + qw0 + i / (D / 4);
         st4(a.dq + (row * a.H + h) * D + i % (D / 4) * 4, f4{});
       }
       return;
@@ -1493,10 +1504,8 @@ __device__ __forceinline__ void bwd_pair(BwdPairArgs a) {
       const int pair = spread(id, pairs, a.nblk * a.nck, in), chunk = in / a.nblk;
       bwd_keys<D, kCausal, kSerial, W, kCross>(a, sm, pair * a.nblk + in - chunk * a.nblk, chunk);
     } else {
-      const int per = a.nblk_q * a.G;
-      const int pair = spread(id - a.nkv, pairs, per * a.ncq, in), chunk = in / per;
-      in -= chunk * per;
-      bwd_queries<D, kCausal, W, kCross>(a, sm, (pair * a.G + in % a.G) * a.nblk_q + in / a.G, chunk);
+      const int pair = spread(id - a.nkv, pairs, a.nblk_q * a.ncq, in), chunk = in / a.nblk_q;
+      bwd_queries<D, kCausal, W, kCross>(a, sm, pair * a.nblk_q + in - chunk * a.nblk_q, chunk);
     }
     return;
   }

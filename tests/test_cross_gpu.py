@@ -53,6 +53,9 @@ SHAPES = [  # b, h, hk, sq, sk, d, lengths
     (2, 2, 1, 40, 2000, 64, [0, 1999]), (1, 16, 1, 500, 64, 64, None), (1, 1, 1, 1, 4000, 64, [3999]),
     (3, 1, 1, 2000, 1025, 32, [1025, 513, 256]),
     (256, 4, 2, 256, 40, 64, None), (171, 3, 1, 512, 33, 32, None),  # 64 queries per wave
+    # Tiles of several heads in one workgroup, with lengths.
+    (40, 6, 2, 33, 200, 64, [0, 77, 200, 31] * 10), (20, 10, 2, 65, 300, 32, [300, 0] * 10),
+    (9, 12, 4, 97, 260, 128, None),
     (300, 1, 1, 20, 40, 64, None), (300, 1, 1, 64, 50, 32, None), (70, 4, 2, 70, 20, 128, None),
 ]
 

@@ -7,27 +7,7 @@ from __future__ import annotations
 
 import torch
 
-from ._call import aligned_rows, not_twice
 from ._lib import operators
-
-
-class _FusedCrossAttention(torch.autograd.Function):
-    """Operands the kernels can read in place."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, scale, key_lengths):
-        out, lse = operators().cross_forward(q, k, v, scale, key_lengths)
-        ctx.save_for_backward(q, k, v, key_lengths, out, lse)
-        ctx.scale = scale
-        return out
-
-    @staticmethod
-    def backward(ctx, grad):
-        q, k, v, key_lengths, out, lse = ctx.saved_tensors
-        grads = operators().cross_backward(q, k, v, ctx.scale, key_lengths, out, lse, grad)
-        if torch.is_grad_enabled():
-            grads = not_twice("fused_cross_attention", (q, k, v, grad), grads)
-        return *grads, None, None
 
 
 def fused_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
@@ -40,8 +20,4 @@ def fused_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sca
     nearest). Returns [b, h, sq, d], laid out as a contiguous [b, sq, h, d] buffer; a sample that sees no
     key gives 0.
     """
-    out = operators().cross(q, k, v, scale, key_lengths)
-    if out is None:  # (q, k or v requires a gradient)
-        out = _FusedCrossAttention.apply(aligned_rows(q), aligned_rows(k), aligned_rows(v), float(scale),
-                                         key_lengths)
-    return out
+    return operators().cross_attention(q, k, v, scale, key_lengths)

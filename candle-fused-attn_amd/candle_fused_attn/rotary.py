@@ -47,36 +47,6 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str | None = No
     return f.to(device) if device is not None else f
 
 
-class _Rotary(torch.autograd.Function):
-    """The turn; its gradient is the turn back, by the same Function where a graph of it is asked for (so
-    it can be differentiated again)."""
-
-    @staticmethod
-    def forward(ctx, positions, frequencies, heads, interleaved, magnitude, inverse, *xs):
-        ctx.save_for_backward(positions, frequencies)
-        ctx.how = (heads, interleaved, magnitude, inverse)
-        ctx.set_materialize_grads(False)
-        ys = operators().turn(positions, frequencies, heads, interleaved, magnitude, inverse, *xs)
-        return ys[0] if len(ys) == 1 else ys
-
-    @staticmethod
-    def backward(ctx, *grads):
-        positions, frequencies = ctx.saved_tensors
-        heads, interleaved, magnitude, inverse = ctx.how
-        need = ctx.needs_input_grad
-        # (A projection's gradient is read by its heads: any strides but for the last dimension.)
-        at = [i for i, g in enumerate(grads) if g is not None and need[6 + i]]
-        out = [None] * (6 + len(grads))
-        if at:
-            given = [grads[i] for i in at]
-            records = torch.is_grad_enabled() and any(g.requires_grad for g in given)
-            turned = (_Rotary.apply if records else operators().turn)(
-                positions, frequencies, heads, interleaved, magnitude, not inverse, *given)
-            for i, g in zip(at, turned if isinstance(turned, tuple) else (turned,)):
-                out[6 + i] = g
-        return tuple(out)
-
-
 def fused_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
                  frequencies: torch.Tensor, interleaved: bool = False,
                  magnitude: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
@@ -87,10 +57,7 @@ def fused_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     one per pair of the rotated part of a head (rotary_frequencies). The results have the operands'
     shapes and types.
     """
-    out = operators().rotary(q, k, positions, frequencies, interleaved, magnitude)
-    if out is None:  # (q or k requires a gradient)
-        out = _Rotary.apply(positions, frequencies, 0, bool(interleaved), float(magnitude), False, q, k)
-    return out
+    return operators().rotary(q, k, positions, frequencies, interleaved, magnitude)
 
 
 def fused_rotary_qkv(qkv: torch.Tensor, heads: int, positions: torch.Tensor,
@@ -99,9 +66,4 @@ def fused_rotary_qkv(qkv: torch.Tensor, heads: int, positions: torch.Tensor,
     """fused_rotary on the q and k of a fused [b, s, 3 h d] projection laid out [q | k | v]: a new
     projection, v copied, which fused_attention_qkv takes; differentiable, with one gradient shaped
     like qkv."""
-    heads = int(heads)
-    out = operators().rotary_qkv(qkv, heads, positions, frequencies, interleaved, magnitude)
-    if out is None:  # (qkv requires a gradient)
-        return _Rotary.apply(positions, frequencies, heads, bool(interleaved), float(magnitude), False,
-                             qkv)
-    return out[0]
+    return operators().rotary_qkv(qkv, int(heads), positions, frequencies, interleaved, magnitude)

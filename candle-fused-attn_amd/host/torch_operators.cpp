@@ -1,11 +1,11 @@
 // torch_operators.cpp -- the operators around self-attention for Python: torch tensors to the C ABI
-// (include/fattn.h), with their checks and allocations.
+// (include/fattn.h), with their checks, allocations and autograd nodes.
 //
 // Their smallest calls, a decoding token's, are bound by the host, so what lies between Python and the
-// launch is compiled: fused_rotary of one token takes 7.9 us a call, 12.8 with these steps in Python;
-// paged_append 5.5 for 13.7; paged_attention over 240 tokens 7.8 for 11.2. What records a graph stays
-// with torch.autograd.Function in Python, which calls the unchecked entries below; the checked ones
-// return None where a graph has to be recorded.
+// launch is compiled: fused_rotary of one token takes 7.5 us a call, 12.8 with these steps in Python;
+// paged_append 5.1 for 13.7; paged_attention over 240 tokens 7.7 for 11.2. With the nodes in
+// Python a small training call takes 15 us more: fused_rotary and its gradient 77 us, 60 so, where an
+// elementwise product and its gradient take 52; fused_cross_attention 78, 62.
 //
 // Every entry takes its positional arguments from candle_fused_attn/{rotary,paged,cross}.py, whose
 // docstrings say what they mean. A refused argument raises the package's FusedAttentionError.
@@ -19,6 +19,7 @@
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <initializer_list>
@@ -32,13 +33,46 @@ namespace {
 
 using at::ScalarType;
 using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
 typedef std::vector<Tensor> Tensors;
+
+PyObject* g_error = nullptr;  // candle_fused_attn.FusedAttentionError
 
 // A refused argument or a failed launch; `code` as the C ABI returned it (0: refused here).
 struct OpError : std::runtime_error {
   explicit OpError(const std::string& msg, int c = 0) : std::runtime_error(msg), code(c) {}
   int code;
 };
+
+void set_python(const OpError& e) {
+  PyObject* x = PyObject_CallFunction(g_error, "si", e.what(), e.code);
+  if (!x) return;  // (with that call's own error set)
+  PyErr_SetObject(g_error, x);
+  Py_DECREF(x);
+}
+// fn() inside a backward, which may be any thread without the interpreter's lock: an OpError leaves as
+// the Python exception that the engine hands to its caller.
+template <typename F>
+auto in_backward(F fn) -> decltype(fn()) {
+  try {
+    return fn();
+  } catch (const OpError& e) {
+    const PyGILState_STATE state = PyGILState_Ensure();
+    set_python(e);
+    python_error error;
+    error.persist();
+    PyGILState_Release(state);
+    throw error;
+  }
+}
+bool records(std::initializer_list<const Tensor*> ts) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts) {
+    if (t->defined() && t->requires_grad()) return true;
+  }
+  return false;
+}
 
 std::string shape_of(at::IntArrayRef x) {
   std::string out = "[";
@@ -179,15 +213,63 @@ Tensors turned(const Tensors& xs, const Turn& how) {
   return ys;
 }
 
-bool records(std::initializer_list<const Tensor*> ts) {
-  if (!c10::GradMode::is_enabled()) return false;
-  for (const Tensor* t : ts) {
-    if (t->defined() && t->requires_grad()) return true;
+// The turn as a node, of one operand or two; its gradient is the turn back, the same node again where a
+// graph of it is asked for (so it can be differentiated again).
+void remember(AutogradContext* ctx, const Turn& how) {
+  ctx->save_for_backward({how.positions, how.frequencies});
+  ctx->saved_data["heads"] = how.heads;
+  ctx->saved_data["interleaved"] = how.interleaved;
+  ctx->saved_data["magnitude"] = how.magnitude;
+  ctx->saved_data["inverse"] = how.inverse;
+  ctx->set_materialize_grads(false);
+}
+Turn turn_back(AutogradContext* ctx) {
+  const Tensors saved = ctx->get_saved_variables();
+  return Turn{saved[0],
+              saved[1],
+              ctx->saved_data["heads"].toInt(),
+              ctx->saved_data["interleaved"].toBool(),
+              ctx->saved_data["magnitude"].toDouble(),
+              !ctx->saved_data["inverse"].toBool()};
+}
+Tensor turn_one(const Tensor& x, const Turn& how);
+Tensors turn_two(const Tensor& q, const Tensor& k, const Turn& how);
+
+struct TurnOne : Function<TurnOne> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Turn& how) {
+    remember(ctx, how);
+    return turned({rows(x)}, how)[0];
   }
-  return false;
+  static Tensors backward(AutogradContext* ctx, const Tensors& grads) {
+    if (!grads[0].defined()) return {Tensor(), Tensor()};
+    return in_backward([&]() -> Tensors { return {turn_one(grads[0], turn_back(ctx)), Tensor()}; });
+  }
+};
+struct TurnTwo : Function<TurnTwo> {
+  static Tensors forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Turn& how) {
+    remember(ctx, how);
+    return turned({rows(q), rows(k)}, how);
+  }
+  static Tensors backward(AutogradContext* ctx, const Tensors& grads) {
+    const bool gq = grads[0].defined() && ctx->needs_input_grad(0);
+    const bool gk = grads[1].defined() && ctx->needs_input_grad(1);
+    return in_backward([&]() -> Tensors {
+      if (gq && gk) {
+        const Tensors both = turn_two(grads[0], grads[1], turn_back(ctx));
+        return {both[0], both[1], Tensor()};
+      }
+      return {gq ? turn_one(grads[0], turn_back(ctx)) : Tensor(),
+              gk ? turn_one(grads[1], turn_back(ctx)) : Tensor(), Tensor()};
+    });
+  }
+};
+Tensor turn_one(const Tensor& x, const Turn& how) {
+  return records({&x}) ? TurnOne::apply(x, how) : turned({rows(x)}, how)[0];
+}
+Tensors turn_two(const Tensor& q, const Tensor& k, const Turn& how) {
+  return records({&q, &k}) ? TurnTwo::apply(q, k, how) : turned({rows(q), rows(k)}, how);
 }
 
-// Empty where a graph has to be recorded.
 Tensors fused_rotary(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& f,
                            bool interleaved, double magnitude) {
   const char* who = "fused_rotary";
@@ -199,11 +281,10 @@ Tensors fused_rotary(const Tensor& q, const Tensor& k, const Tensor& positions, 
   }
   check_positions(who, positions, q.size(0), q.size(2), q);
   check_frequencies(who, f, q.size(3), q);
-  if (records({&q, &k})) return {};
-  return turned({rows(q), rows(k)}, Turn{positions, f, 0, interleaved, magnitude, false});
+  return turn_two(q, k, Turn{positions, f, 0, interleaved, magnitude, false});
 }
 
-Tensors fused_rotary_qkv(const Tensor& qkv, int64_t heads, const Tensor& positions, const Tensor& f,
+Tensor fused_rotary_qkv(const Tensor& qkv, int64_t heads, const Tensor& positions, const Tensor& f,
                         bool interleaved, double magnitude) {
   const char* who = "fused_rotary_qkv";
   require(who, "qkv", qkv, 3, nullptr, {kF32, kF16, kBF16});
@@ -214,8 +295,7 @@ Tensors fused_rotary_qkv(const Tensor& qkv, int64_t heads, const Tensor& positio
   }
   check_positions(who, positions, qkv.size(0), qkv.size(1), qkv);
   check_frequencies(who, f, w / 3 / heads, qkv);
-  if (records({&qkv})) return {};
-  return turned({rows(qkv)}, Turn{positions, f, heads, interleaved, magnitude, false});
+  return turn_one(qkv, Turn{positions, f, heads, interleaved, magnitude, false});
 }
 
 // --- The paged cache -------------------------------------------------------------------------------
@@ -370,8 +450,47 @@ Tensors cross_backward(const Tensor& q, const Tensor& k, const Tensor& v, double
   return {dq, dkv.select(2, 0).transpose(1, 2), dkv.select(2, 1).transpose(1, 2)};
 }
 
-// The output alone; empty where a graph has to be recorded.
-Tensors fused_cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, double scale,
+// Gradients that were asked for with a graph: they are not differentiable, and say so when it is tried
+// (without this they would look like constants).
+struct NotTwice : Function<NotTwice> {
+  static Tensors forward(AutogradContext*, const Tensor& dq, const Tensor& dk, const Tensor& dv,
+                         const Tensor&, const Tensor&, const Tensor&, const Tensor&) {
+    return {dq.view_as(dq), dk.view_as(dk), dv.view_as(dv)};
+  }
+  static Tensors backward(AutogradContext*, const Tensors&) {
+    return in_backward([]() -> Tensors {
+      throw OpError("fused_cross_attention: its gradient is not differentiable");
+    });
+  }
+};
+struct How {
+  double scale;
+  Tensor lengths;  // (may be undefined: not among a node's tensors)
+};
+struct CrossNode : Function<CrossNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                        const How& how) {
+    const Tensors out = cross_forward(q, k, v, how.scale, how.lengths);
+    ctx->save_for_backward({q, k, v, how.lengths, out[0], out[1]});
+    ctx->saved_data["scale"] = how.scale;
+    return out[0];
+  }
+  static Tensors backward(AutogradContext* ctx, const Tensors& grads) {
+    const Tensors s = ctx->get_saved_variables();
+    return in_backward([&]() -> Tensors {
+      Tensors to;
+      {
+        const c10::AutoGradMode off(false);
+        to = cross_backward(s[0], s[1], s[2], ctx->saved_data["scale"].toDouble(), s[3], s[4], s[5], grads[0]);
+      }
+      if (c10::GradMode::is_enabled()) to = NotTwice::apply(to[0], to[1], to[2], s[0], s[1], s[2], grads[0]);
+      to.resize(4);  // (none for `how`)
+      return to;
+    });
+  }
+};
+
+Tensor fused_cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, double scale,
                               const Tensor& lengths) {
   const char* who = "fused_cross_attention";
   require(who, "q", q, 4, nullptr, {kF32});
@@ -389,15 +508,12 @@ Tensors fused_cross_attention(const Tensor& q, const Tensor& k, const Tensor& v,
                     "] expected, got " + shape_of(lengths.sizes()));
     }
   }
-  if (records({&q, &k, &v})) return {};
-  Tensors out = cross_forward(aligned_rows(q), aligned_rows(k), aligned_rows(v), scale, lengths);
-  out.resize(1);
-  return out;
+  const Tensor qa = aligned_rows(q), ka = aligned_rows(k), va = aligned_rows(v);
+  return records({&qa, &ka, &va}) ? CrossNode::apply(qa, ka, va, How{scale, lengths})
+                                  : cross_forward(qa, ka, va, scale, lengths)[0];
 }
 
 // --- Python ----------------------------------------------------------------------------------------
-
-PyObject* g_error = nullptr;  // candle_fused_attn.FusedAttentionError
 
 // The positional arguments of a call, read in turn.
 struct Args {
@@ -442,13 +558,12 @@ struct Unlocked {
   ~Unlocked() { PyEval_RestoreThread(state); }
 };
 
-// Undefined tensors, and no tensors at all, are None.
+// (Undefined: None.)
 PyObject* one(const Tensor& t) {
   if (t.defined()) return THPVariable_Wrap(t);
   Py_RETURN_NONE;
 }
 PyObject* all(const Tensors& ts) {
-  if (ts.empty()) Py_RETURN_NONE;
   PyObject* out = PyTuple_New(static_cast<Py_ssize_t>(ts.size()));
   if (!out) throw python_error();
   for (size_t i = 0; i < ts.size(); ++i) PyTuple_SET_ITEM(out, i, THPVariable_Wrap(ts[i]));
@@ -464,11 +579,7 @@ PyObject* entry(const char* who, PyObject* const* args, Py_ssize_t n, F body) {
     Args a{who, args, n};
     return body(a);
   } catch (const OpError& e) {
-    PyObject* x = PyObject_CallFunction(g_error, "si", e.what(), e.code);
-    if (x) {
-      PyErr_SetObject(g_error, x);
-      Py_DECREF(x);
-    }
+    set_python(e);
     return nullptr;
   }
   END_HANDLE_TH_ERRORS
@@ -496,31 +607,12 @@ PyObject* py_rotary_qkv(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor &p = a.tensor("positions"), &f = a.tensor("frequencies");
     const bool interleaved = a.truth();
     const double magnitude = a.number();
-    Tensors out;
+    Tensor out;
     {
       const Unlocked unlocked;
       out = fused_rotary_qkv(x, heads, p, f, interleaved, magnitude);
     }
-    return all(out);
-  });
-}
-
-// turn(positions, frequencies, heads, interleaved, magnitude, inverse, *xs)
-PyObject* py_turn(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  return entry("fused_rotary", args, n, [](Args& a) {
-    Turn how;
-    how.positions = a.tensor("positions"), how.frequencies = a.tensor("frequencies");
-    how.heads = a.integer(), how.interleaved = a.truth(), how.magnitude = a.number();
-    how.inverse = a.truth();
-    Tensors xs;
-    do xs.push_back(rows(a.tensor("x")));
-    while (a.left > 0 && xs.size() < 2);
-    Tensors out;
-    {
-      const Unlocked unlocked;
-      out = turned(xs, how);
-    }
-    return all(out);
+    return one(out);
   });
 }
 
@@ -554,33 +646,17 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
-template <bool kChecked>
-PyObject* py_cross(PyObject*, PyObject* const* args, Py_ssize_t n) {
+PyObject* py_cross_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return entry("fused_cross_attention", args, n, [](Args& a) {
     const Tensor &q = a.tensor("q"), &k = a.tensor("k"), &v = a.tensor("v");
     const double scale = a.number();
     const Tensor lengths = a.maybe("key_lengths");
-    Tensors out;
+    Tensor out;
     {
       const Unlocked unlocked;
-      out = (kChecked ? fused_cross_attention : cross_forward)(q, k, v, scale, lengths);
+      out = fused_cross_attention(q, k, v, scale, lengths);
     }
-    return kChecked ? one(out.empty() ? Tensor() : out[0]) : all(out);
-  });
-}
-
-PyObject* py_cross_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  return entry("fused_cross_attention", args, n, [](Args& a) {
-    const Tensor &q = a.tensor("q"), &k = a.tensor("k"), &v = a.tensor("v");
-    const double scale = a.number();
-    const Tensor lengths = a.maybe("key_lengths");
-    const Tensor &out = a.tensor("out"), &lse = a.tensor("lse"), &grad = a.tensor("grad");
-    Tensors grads;
-    {
-      const Unlocked unlocked;
-      grads = cross_backward(q, k, v, scale, lengths, out, lse, grad);
-    }
-    return all(grads);
+    return one(out);
   });
 }
 
@@ -588,12 +664,9 @@ PyMethodDef g_methods[] = {
 #define ENTRY(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL, ""}
     ENTRY("rotary", py_rotary),
     ENTRY("rotary_qkv", py_rotary_qkv),
-    ENTRY("turn", py_turn),
     ENTRY("paged_append", py_append),
     ENTRY("paged_attention", py_paged_attention),
-    ENTRY("cross", py_cross<true>),
-    ENTRY("cross_forward", py_cross<false>),
-    ENTRY("cross_backward", py_cross_backward),
+    ENTRY("cross_attention", py_cross_attention),
 #undef ENTRY
     {nullptr, nullptr, 0, nullptr}};
 

@@ -239,6 +239,55 @@ def test_some_gradients_only(cuda):
         dq.sum().backward()
 
 
+def test_errors_of_a_backward(cuda):
+    """What a backward refuses reaches the caller as the package's error or torch's own."""
+    q, k, v, g = operands(cuda, 1, 2, 2, 20, 30, 64, seed=15)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = cfa.fused_cross_attention(*leaves, 0.125)
+    (dq,) = torch.autograd.grad(out, q, g, create_graph=True)
+    with pytest.raises(cfa.FusedAttentionError, match="not differentiable"):
+        dq.sum().backward()
+    out = cfa.fused_cross_attention(*leaves, 0.125)
+    torch.autograd.grad(out, q, g)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(out, q, g)
+    x = q.detach().clone().requires_grad_() * 1.0
+    out = cfa.fused_cross_attention(x, k, v, 0.125)
+    x.mul_(2.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(out, k, g)
+
+
+def test_threads(cuda):
+    """Calls and their gradients from several threads at once: as one after the other."""
+    import threading
+
+    ops = [operands(cuda, 2, 4, 2, 3 + 40 * i, 300, 64, seed=16 + i) for i in range(4)]
+    f, pos = cfa.rotary_frequencies(64, device=cuda), torch.arange(200, device=cuda)
+
+    def step(q, k, v, g):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        a, b = cfa.fused_rotary(leaves[0], leaves[0] * 2.0, pos[: q.shape[2]], f)
+        out = cfa.fused_cross_attention(a + b, leaves[1], leaves[2], 0.125)
+        return [out.detach(), *torch.autograd.grad(out, leaves, g)]
+
+    want, got = [step(*x) for x in ops], [None] * 4
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] = [step(*ops[i]) for _ in range(10)]
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for outs, ref in zip(got, want):
+        assert all(torch.equal(x, y) for o in outs for x, y in zip(o, ref))
+
+
 @pytest.mark.parametrize("shape", [(0, 2, 2, 5, 5), (2, 2, 2, 0, 5), (2, 2, 2, 5, 0), (2, 0, 0, 5, 5),
                                    (2, 2, 2, 0, 900), (2, 2, 2, 900, 0), (1, 2, 1, 900, 0)])
 def test_empty(cuda, shape):

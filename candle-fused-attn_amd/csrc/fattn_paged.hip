@@ -31,9 +31,9 @@
 // kSplitWaves tiles more than it has, which is what beginning one costs: without, the workgroup that the
 // shortest sequences fall to ends last (64 sequences of 1 to 2048, 6 heads, fp32 d 64: 79 us, 46 so).
 //
-// Measured (kernel and join): 4 contexts of 60000 to 131071, 32 heads in 8 groups, d 128 bf16, 273 + 5 us
-// (5.7 TB/s); that ragged batch 45 + 5 us (4.5 TB/s); 8 x 6 heads 1 x 1536 fp32 12.7 + 4.7 us (3.0 TB/s);
-// one sequence of 240, 6 heads, 8.2 us, the latency of one workgroup.
+// Measured (kernel and join): 4 contexts of 60000 to 131071, 32 heads in 8 groups, d 128 bf16, 263 + 5 us
+// (5.9 TB/s); that ragged batch 45 + 5 us (4.5 TB/s); 8 x 6 heads 1 x 1536 fp32 12.4 + 3.9 us (3.0 TB/s);
+// one sequence of 240, 6 heads, 7.8 us, the latency of one workgroup.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -400,8 +400,17 @@ split_kernel(SplitArgs a) {
   // This workgroup's run: `left` of the sequences' costs end to end, from `off` into sequence b's.
   int b = 0;
   int64_t off = 0, left = 0;
+  int early[2] = {};  // the pages of the wave's first tile
   if (a.wgs == 0) {  // one workgroup per key head and block of rows
     b = static_cast<int>(blockIdx.x) / heads;
+    if constexpr (kPaged) {
+      // Read beside the length, which says whether the tile is there: one load's latency less before the
+      // first keys (one sequence of 240: 8.1 us without, 7.8 so).
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        early[h] = a.table[b * a.table_stride + divide(min(2 * w + h, a.SK / 16 - 1), a.by_page)];
+      }
+    }
   } else {
     // Each wave for itself, without LDS: a lane takes `each` sequences that follow one another.
     const int each = (a.B + 63) / 64, from = min(lane * each, a.B), to = min(from + each, a.B);
@@ -489,7 +498,8 @@ split_kernel(SplitArgs a) {
       x.live = min(len - 16 * at, 16);
       if constexpr (kPaged) {
         const int pi = divide(at, a.by_page), slot = 16 * (at - pi * (a.page_size / 16));
-        int page = __builtin_amdgcn_readfirstlane(a.table[b * a.table_stride + pi]);
+        const bool had = a.wgs == 0 && at == 2 * w + h;
+        int page = __builtin_amdgcn_readfirstlane(had ? early[h] : a.table[b * a.table_stride + pi]);
         if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pages)) page = 0, wrong = 1;
         x.k = kp + page * a.ks[0] + slot * a.ks[2];
         x.v = vp + page * a.vs[0] + slot * a.vs[2];

@@ -3,7 +3,7 @@
 //
 // Their smallest calls, a decoding token's, are bound by the host, so what lies between Python and the
 // launch is compiled: fused_rotary of one token takes 7.5 us a call, 12.8 with these steps in Python;
-// paged_append 5.1 for 13.7; paged_attention over 240 tokens 7.7 for 11.2. With the nodes in
+// paged_append 5.1 for 13.7; paged_attention over 240 tokens 7.5 for 11.2. With the nodes in
 // Python a small training call takes 15 us more: fused_rotary and its gradient 77 us, 60 so, where an
 // elementwise product and its gradient take 52; fused_cross_attention 78, 62.
 //

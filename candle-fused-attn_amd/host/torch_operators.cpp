@@ -136,6 +136,10 @@ void launch(const Tensor& t, F fn) {
   const int rc = fn(static_cast<void*>(c10::hip::getCurrentHIPStream(t.get_device()).stream()));
   if (rc != 0) throw OpError(fattn_last_error(), rc);
 }
+// An empty tensor laid out like t. (A contiguous one by one call of the dispatcher instead of two.)
+Tensor like(const Tensor& t) {
+  return t.is_contiguous() ? at::empty(t.sizes(), t.options()) : at::empty_like(t);
+}
 // A workspace from torch's allocator (undefined for 0 bytes).
 Tensor workspace(const Tensor& t, size_t bytes) {
   return bytes == 0 ? Tensor()
@@ -175,7 +179,7 @@ void check_positions(const char* who, const Tensor& p, int64_t b, int64_t s, con
 // The turned tensors: one or two operands, or the one projection, whose q and k are turned and v copied.
 Tensors turned(const Tensors& xs, const Turn& how) {
   Tensors ys;
-  for (const Tensor& x : xs) ys.push_back(at::empty_like(x));
+  for (const Tensor& x : xs) ys.push_back(like(x));
   const Tensor& x = xs[0];
   int64_t heads[3] = {0, 0, 0}, xst[9] = {}, yst[9] = {}, pst[2] = {};
   const void* xp[3] = {};
@@ -365,7 +369,7 @@ Tensor paged_append(const Tensor& k0, const Tensor& v0, const Tensor& kp, const 
       throw OpError(std::string(who) + ": q and k must agree but for their heads, got " +
                     shape_of(q0.sizes()) + " and " + shape_of(k0.sizes()));
     }
-    q = rows(q0), out = at::empty_like(q), heads = q.size(1);
+    q = rows(q0), out = like(q), heads = q.size(1);
   }
   if (counts.defined()) {
     require(who, "counts", counts, 1, &k0, {kI32});
@@ -398,7 +402,7 @@ Tensor paged_attention(const Tensor& q0, const Tensor& kp, const Tensor& vp, con
   check_cache(who, q0, kp, vp, table, lengths, b, d);
   no_graph(who, {&q0, &kp, &vp});
   const Tensor q = aligned_rows(q0);
-  Tensor out = at::empty_like(q, q.options(), at::MemoryFormat::Contiguous);
+  Tensor out = at::empty(q.sizes(), q.options());
   const int64_t hk = kp.size(1), page = kp.size(2), width = table.size(1);
   const size_t bytes = fattn_paged_attention_workspace_bytes(b, h, hk, d, width * page);
   const Tensor ws = workspace(q, bytes);

@@ -275,7 +275,7 @@ Tensors turn_two(const Tensor& q, const Tensor& k, const Turn& how) {
 }
 
 Tensors fused_rotary(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& f,
-                           bool interleaved, double magnitude) {
+                     bool interleaved, double magnitude) {
   const char* who = "fused_rotary";
   require(who, "q", q, 4, nullptr, {kF32, kF16, kBF16});
   require(who, "k", k, 4, &q, {q.scalar_type()});

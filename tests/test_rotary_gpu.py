@@ -240,3 +240,53 @@ def test_impossible_heads_refused(cuda):
     for heads in (0, -1, 5, 65, (2 ** 64 - 1) // 3):
         with pytest.raises(cfa.FusedAttentionError, match="is not 3 x"):
             cfa.fused_rotary_qkv(qkv, heads, torch.arange(2, device=cuda), f)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d", [64, 10])
+def test_in_place_through_the_c_abi(cuda, d, interleaved):
+    """y may be x itself."""
+    import ctypes
+
+    from candle_fused_attn import _lib
+
+    b, h, hk, s = 3, 5, 2, 70
+    q, k = (t.contiguous() for t in operands(cuda, torch.float32, b, h, hk, s, d, seed=13))
+    f, pos = cfa.rotary_frequencies(d, device=cuda), torch.arange(s, device=cuda)
+    want = cfa.fused_rotary(q, k, pos, f, interleaved)
+    at = (ctypes.c_void_p * 3)(q.data_ptr(), k.data_ptr(), None)
+    st = _lib.arr([*q.stride()[:3], *k.stride()[:3], 0, 0, 0])
+    _lib.check(_lib.lib().fattn_rotary(0, b, s, d, _lib.arr([h, hk, 0]), at, at, st, st, 0b11, pos.data_ptr(),
+                                       64, _lib.arr([0, 1]), f.data_ptr(), d, int(interleaved), 1.0, 0,
+                                       torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+def test_training_captured(cuda):
+    """A rotated projection's attention and its gradient, replayed with other values and positions, eager
+    steps between: bit for bit the eager results."""
+    b, s, h, d = 2, 50, 3, 64
+    qkv = torch.randn(b, s, 3 * h * d, device=cuda, requires_grad=True)
+    g, pos = torch.randn(b, s, h * d, device=cuda), torch.arange(s, device=cuda)
+    f = cfa.rotary_frequencies(d, device=cuda)
+
+    def step():
+        out = cfa.fused_attention_qkv(cfa.fused_rotary_qkv(qkv, h, pos, f), h, 0.125, True)
+        return [out.detach(), *torch.autograd.grad(out, qkv, g)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(4):
+        with torch.no_grad():
+            qkv.normal_(), g.normal_(), pos.add_(1000 * i)
+        graph.replay()
+        out = [t.clone() for t in got]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, want)), i

@@ -110,7 +110,7 @@ def _declare(L: ctypes.CDLL) -> None:
                                 P, P, P]
     L.fattn_backward.argtypes = [P, I64, A3, A3, P, I64, A3, A3, P, I64, A3, A3, C_FLOAT, C_INT,
                                  P, P, P, I64, A3, A3, P, P, SIZE, P]
-    # (The operators around self-attention: sizes and strides as addresses into one array a call.)
+    # (The operators around self-attention, which torch_operators.so calls: arrays by their addresses.)
     L.fattn_rotary.argtypes = [C_INT, I64, I64, I64, P, P, P, P, P, C_INT, P, C_INT, P, P, I64, C_INT,
                                C_DOUBLE, C_INT, P]
     L.fattn_paged_append.argtypes = [C_INT, C_INT, I64, I64, I64, I64, I64, P, P, P, P, P, P, P, P, P,

@@ -18,9 +18,12 @@
 //   head_dims that it has loaded of those keys (kC of them, one per instruction): D: row j again.
 // Types: an fp32 cache takes the fp32 instruction. A 16-bit one takes the 16-bit instructions, with
 // what is not of its type as a sum of 16-bit terms: fp32 queries as three bf16, or two f16 under a scale
-// of the row (22 bits of its largest, and an error in a score is one of its size anyway); weights, over
-// bf16 values, as two bf16 for a bf16 result (2^-17 of each weight, below its rounding) and three for an
-// fp32 one (2^-25). Over f16 values the weights stay fp32 and the values are widened: f16 terms of a weight
+// of the row (22 bits of its largest, and an error in a score is one of its size anyway; a third f16 term
+// changed fp32 results' error from 7.3e-7 to 7.2e-7); weights, over bf16 values, as three bf16, which hold
+// their 24 bits. (Two are off by 2^-17 of a weight, and a bf16 result that lies near a tie then rounds to
+// the wrong side: 86 of 16384 results over 60000 to 131071 tokens, 15 so, where sums in fp32 give 46. Two /
+// three, bf16, us: those contexts, d 128, 279.4 / 279.9; 64 sequences of 1 to 2048, d 64, 27.1 / 27.5.)
+// Over f16 values the weights stay fp32 and the values are widened: f16 terms of a weight
 // would end at 2^-24 of the largest one's size, and a key of all the weight but no value (an attention
 // sink) would take the bits of all the others.
 //
@@ -170,7 +173,7 @@ struct Wave {
   // Terms of the queries and of the weights (1: as they are).
   static constexpr bool kSame = std::is_same<Q, C>::value;
   static constexpr int kQT = kF32 || kSame ? 1 : std::is_same<C, __bf16>::value ? 3 : 2;
-  static constexpr int kPT = kSame ? 2 : 3;  // (bf16)
+  static constexpr int kPT = 3;  // (bf16)
 
   u4 k[2][kKLoads];
   unsigned v[2][4][kBlocks][kVWords];

@@ -431,3 +431,36 @@ def test_append_side_stream(cuda):
     y = cfa.paged_append(k, v, b.k, b.v, b.table, b.lengths, q=q, frequencies=f)
     assert torch.equal(x, y)
     assert all(torch.equal(s.nan_to_num(9.0), t.nan_to_num(9.0)) for s, t in ((a.k, b.k), (a.v, b.v)))
+
+
+@pytest.mark.parametrize("width", [1, 100])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_attention_16_bit_results_are_rounded_once(cuda, dtype, width):
+    """A 16-bit result is off by half a step of its own and an error of fp32 sums, no more: as far from the
+    exact value as its rounding, but where that lies within 2^-19 of the values' size of a tie. Tables as
+    wide as the sequences, and far wider.
+
+    Scores are exact (halves times halves, a scale of 2^-8, so at most 1/2 and 0.72 in log2 units). In
+    units of 2^-24: log2 e and the exponent are off by 0.72 each and their difference by 1.44, by ln 2 of a
+    weight: 2; the exponential by 2; so 8 for the weights above and below the line, 16 for the sum of 4 keys
+    on the matrix instructions, 5 for that of the weights, 3 for the quotient: 32, 2^-19."""
+    b, h, d, n, dt = 128, 16, 128, 4, TYPES[dtype]
+    gen = torch.Generator().manual_seed(22)
+    halves = lambda *shape: (torch.randint(0, 4, shape, generator=gen) - 1.5).sign() * (
+        torch.randint(1, 3, shape, generator=gen) / 2)
+    q, k = halves(b, h, 1, d), halves(b, h, n, d)
+    v = torch.randn(b, h, n, d, generator=gen).to(dt)
+    kp, vp = (torch.full((b, h, 16, d), float("nan"), dtype=dt) for _ in range(2))
+    kp[:, :, :n], vp[:, :, :n] = k.to(dt), v
+    table = torch.full((b, width), -1, dtype=torch.int32)
+    table[:, 0] = torch.arange(b)
+    out = cfa.paged_attention(q.to(dt).to(cuda), kp.to(cuda), vp.to(cuda), table.to(cuda),
+                              torch.full((b,), n, dtype=torch.int32, device=cuda), 2.0 ** -8)
+    p = torch.softmax(torch.matmul(q.double(), k.double().transpose(2, 3).contiguous()) * 2.0 ** -8, -1)
+    ref, size = torch.matmul(p, v.double()), torch.matmul(p, v.double().abs())
+    room = 2.0 ** -19 * size
+    # Half a step at the value (the least normal f16 is 2^-14).
+    least = 2.0 ** -14 if dt == torch.float16 else 2.0 ** -126
+    half = torch.exp2(torch.floor(torch.log2((ref.abs() + room).clamp_min(least)))) * (torch.finfo(dt).eps / 2)
+    over = (out.double().cpu() - ref).abs() - half - room
+    assert int((over > 0).sum()) == 0, (int((over > 0).sum()), float((over / size).max()))

@@ -136,9 +136,15 @@ void launch(const Tensor& t, F fn) {
   const int rc = fn(static_cast<void*>(c10::hip::getCurrentHIPStream(t.get_device()).stream()));
   if (rc != 0) throw OpError(fattn_last_error(), rc);
 }
-// An empty tensor laid out like t. (A contiguous one by one call of the dispatcher instead of two.)
+// An empty tensor laid out like t, whose rows are contiguous, and its own contiguous too. (A contiguous one
+// by one call of the dispatcher instead of two. Where rows of t overlap, in windows of a longer row, torch
+// may order the dimensions otherwise.)
 Tensor like(const Tensor& t) {
-  return t.is_contiguous() ? at::empty(t.sizes(), t.options()) : at::empty_like(t);
+  if (!t.is_contiguous()) {
+    Tensor y = at::empty_like(t);
+    if (y.stride(-1) == 1) return y;
+  }
+  return at::empty(t.sizes(), t.options());
 }
 // A workspace from torch's allocator (undefined for 0 bytes).
 Tensor workspace(const Tensor& t, size_t bytes) {

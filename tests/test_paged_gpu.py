@@ -464,3 +464,19 @@ def test_attention_16_bit_results_are_rounded_once(cuda, dtype, width):
     half = torch.exp2(torch.floor(torch.log2((ref.abs() + room).clamp_min(least)))) * (torch.finfo(dt).eps / 2)
     over = (out.double().cpu() - ref).abs() - half - room
     assert int((over > 0).sum()) == 0, (int((over > 0).sum()), float((over / size).max()))
+
+
+@pytest.mark.parametrize("types", PAIRS, ids="-".join)
+def test_append_overlapping_operands(cuda, types):
+    """New keys, values and queries whose rows overlap (windows of a longer row): as of contiguous copies,
+    bit for bit."""
+    dt, ct = (TYPES[t] for t in types)
+    buf = torch.randn(4096, generator=torch.Generator().manual_seed(23)).to(dt).to(cuda)
+    k, v, q = (buf.as_strided((2, n, 20, 64), (700, 100, 1, 1), i) for i, n in enumerate((2, 2, 4)))
+    f = cfa.rotary_frequencies(64, device=cuda)
+    a, b = (Cache(cuda, ct, 2, 16, 64, [5, 30], room=20, seed=24) for _ in range(2))
+    x = cfa.paged_append(k, v, a.k, a.v, a.table, a.lengths, q=q, frequencies=f)
+    y = cfa.paged_append(k.contiguous(), v.contiguous(), b.k, b.v, b.table, b.lengths, q=q.contiguous(),
+                         frequencies=f)
+    assert torch.equal(x, y)
+    assert all(torch.equal(s.nan_to_num(9.0), t.nan_to_num(9.0)) for s, t in ((a.k, b.k), (a.v, b.v)))

@@ -290,3 +290,32 @@ def test_training_captured(cuda):
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(out, want)), i
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_overlapping_views(cuda, dtype, interleaved):
+    """Operands, projections and output gradients whose rows overlap (windows of a longer row: the stride
+    of head_dim is another dimension's too): as of contiguous copies, bit for bit."""
+    gen = torch.Generator().manual_seed(16)
+    buf = torch.randn(4096, generator=gen).to(dtype).to(cuda)
+    f, pos = cfa.rotary_frequencies(64, device=cuda), torch.arange(37, device=cuda)
+    q = buf[:800].view(2, 4, 100).unfold(2, 64, 1)               # rows
+    k = buf.as_strided((2, 3, 37, 64), (1000, 1, 20, 1), 3)      # heads
+    x = buf.as_strided((2, 37, 3 * 64), (1000, 1, 1), 5)
+    r = buf.as_strided((2, 37, 3 * 128), (1, 40, 1), 7)          # samples
+    assert q.shape == (2, 4, 37, 64) and q.stride()[2:] == (1, 1)
+    got = cfa.fused_rotary(q, k, pos, f, interleaved)
+    want = cfa.fused_rotary(q.contiguous(), k.contiguous(), pos, f, interleaved)
+    for a, b, t in zip(got, want, (q, k)):
+        assert torch.equal(a, b)
+        near(a, formula(t, pos, f, interleaved), t)
+    for t, heads in ((x, 1), (r, 2)):
+        assert torch.equal(cfa.fused_rotary_qkv(t, heads, pos, f, interleaved),
+                           cfa.fused_rotary_qkv(t.contiguous(), heads, pos, f, interleaved))
+    leaves = [t.contiguous().requires_grad_() for t in (q, k, x)]
+    outs = [*cfa.fused_rotary(*leaves[:2], pos, f, interleaved),
+            cfa.fused_rotary_qkv(leaves[2], 1, pos, f, interleaved)]
+    grads = [torch.autograd.grad(outs, leaves, g, retain_graph=True)
+             for g in ((q, k, x), (q.contiguous(), k.contiguous(), x.contiguous()))]
+    assert all(torch.equal(a, b) for a, b in zip(*grads))

@@ -27,7 +27,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     new tensor; None without q). f32 keys and values are rounded to the cache's type. A token whose
     page the table or the cache does not have is not written (its sequence's attention gives NaN), and
     no slot that holds no new token is touched. Two new tokens must not share a slot, and k, v and q must
-    not lie in the cache. Not differentiable.
+    not lie in the cache. Not differentiable; a graph that saved the pages before refuses its backward, as
+    after any operation in place.
     """
     return operators().paged_append(k, v, k_pages, v_pages, page_table, lengths, counts, q, frequencies,
                                     interleaved, magnitude)

@@ -336,6 +336,11 @@ const int32_t* ints(const Tensor& t) { return t.defined() ? static_cast<const in
 void no_graph(const char* who, std::initializer_list<const Tensor*> ts) {
   if (records(ts)) throw OpError(std::string(who) + ": not differentiable (call it under torch.no_grad())");
 }
+// The pages were written: a graph that saved them before must not run on them. (Tensors of inference mode
+// have no versions.)
+void wrote(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 bool broadcast(const Tensor& t) {
   for (int64_t i = 0; i < t.dim(); ++i) {
     if (t.stride(i) == 0 && t.size(i) > 1) return true;
@@ -394,6 +399,7 @@ Tensor paged_append(const Tensor& k0, const Tensor& v0, const Tensor& kp, const 
         kp.size(0), kp.size(2), ints(table), table.stride(0), table.size(1), ints(lengths), ints(counts),
         static_cast<const double*>(address(f)), dim, interleaved, magnitude, stream);
   });
+  wrote(kp), wrote(vp);
   return out;
 }
 

@@ -480,3 +480,26 @@ def test_append_overlapping_operands(cuda, types):
                          frequencies=f)
     assert torch.equal(x, y)
     assert all(torch.equal(s.nan_to_num(9.0), t.nan_to_num(9.0)) for s, t in ((a.k, b.k), (a.v, b.v)))
+
+
+def test_append_counts_as_a_write_of_the_pages(cuda):
+    """The pages' versions move with an append, and nothing else's: a graph that saved pages before it
+    refuses its backward, which would run on other values. Pages without versions (inference mode) are
+    written all the same."""
+    c = Cache(cuda, torch.float32, 2, 16, 64, [3, 0], room=2, seed=21)
+    k, v, q = (torch.randn(2, n, 2, 64, device=cuda) for n in (2, 2, 4))
+    f = cfa.rotary_frequencies(64, device=cuda)
+    w = torch.ones((), device=cuda, requires_grad=True)
+    losses = [(w * pages[:1]).sum() for pages in (c.k, c.v)]
+    others = (k, v, q, f, c.table, c.lengths)
+    before = [t._version for t in (c.k, c.v, *others)]
+    cfa.paged_append(k, v, c.k, c.v, c.table, c.lengths, q=q, frequencies=f)
+    after = [t._version for t in (c.k, c.v, *others)]
+    assert after == [before[0] + 1, before[1] + 1, *before[2:]]
+    for loss in losses:
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+    with torch.inference_mode():
+        kp, vp = c.k.nan_to_num(0.0), c.v.nan_to_num(0.0)
+        cfa.paged_append(2.0 * k, v, kp, vp, c.table, c.lengths)
+        assert torch.equal(kp[int(c.table[1, 0]), :, :2], 2.0 * k[1])

@@ -18,6 +18,6 @@ def fused_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sca
     the kernels cannot read them in place), d 32, 64 or 128, h a multiple of kv_heads (query head i
     reads key head i // (h // kv_heads)); key_lengths: [b] int32 (one outside [0, sk] counts as the
     nearest). Returns [b, h, sq, d], laid out as a contiguous [b, sq, h, d] buffer; a sample that sees no
-    key gives 0.
+    key gives 0. Differentiable once, in reverse mode (a forward-mode tangent is refused).
     """
     return operators().cross_attention(q, k, v, scale, key_lengths)

@@ -50,7 +50,8 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str | None = No
 def fused_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
                  frequencies: torch.Tensor, interleaved: bool = False,
                  magnitude: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
-    """q and k with their positions turned into them, in one launch; differentiable in q and k.
+    """q and k with their positions turned into them, in one launch; differentiable in q and k (in reverse
+    mode: a forward-mode tangent is refused).
 
     q: [b, h, s, d], k: [b, kv_heads, s, d], of one type (f32, f16 or bf16), any strides (copied first
     where head_dim is not contiguous); positions: [s] or [b, s], int64 or int32; frequencies: float64,

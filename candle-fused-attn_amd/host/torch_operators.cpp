@@ -73,6 +73,15 @@ bool records(std::initializer_list<const Tensor*> ts) {
   }
   return false;
 }
+// No operand may have a tangent of forward-mode differentiation: a result without one would be a derivative
+// of 0. (Tensors that are absent have none.)
+void no_tangents(const char* who, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts) {
+    if (t->defined() && t->_fw_grad(0).defined()) {
+      throw OpError(std::string(who) + ": no forward-mode derivative");
+    }
+  }
+}
 
 std::string shape_of(at::IntArrayRef x) {
   std::string out = "[";
@@ -252,7 +261,11 @@ struct TurnOne : Function<TurnOne> {
   }
   static Tensors backward(AutogradContext* ctx, const Tensors& grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor()};
-    return in_backward([&]() -> Tensors { return {turn_one(grads[0], turn_back(ctx)), Tensor()}; });
+    return in_backward([&]() -> Tensors {
+      const Turn how = turn_back(ctx);
+      no_tangents(how.heads > 0 ? "fused_rotary_qkv" : "fused_rotary", {&grads[0]});
+      return {turn_one(grads[0], how), Tensor()};
+    });
   }
 };
 struct TurnTwo : Function<TurnTwo> {
@@ -264,12 +277,13 @@ struct TurnTwo : Function<TurnTwo> {
     const bool gq = grads[0].defined() && ctx->needs_input_grad(0);
     const bool gk = grads[1].defined() && ctx->needs_input_grad(1);
     return in_backward([&]() -> Tensors {
+      const Turn how = turn_back(ctx);
+      no_tangents("fused_rotary", {&grads[0], &grads[1]});
       if (gq && gk) {
-        const Tensors both = turn_two(grads[0], grads[1], turn_back(ctx));
+        const Tensors both = turn_two(grads[0], grads[1], how);
         return {both[0], both[1], Tensor()};
       }
-      return {gq ? turn_one(grads[0], turn_back(ctx)) : Tensor(),
-              gk ? turn_one(grads[1], turn_back(ctx)) : Tensor(), Tensor()};
+      return {gq ? turn_one(grads[0], how) : Tensor(), gk ? turn_one(grads[1], how) : Tensor(), Tensor()};
     });
   }
 };
@@ -283,6 +297,7 @@ Tensors turn_two(const Tensor& q, const Tensor& k, const Turn& how) {
 Tensors fused_rotary(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& f,
                      bool interleaved, double magnitude) {
   const char* who = "fused_rotary";
+  no_tangents(who, {&q, &k, &f});
   require(who, "q", q, 4, nullptr, {kF32, kF16, kBF16});
   require(who, "k", k, 4, &q, {q.scalar_type()});
   if (k.size(0) != q.size(0) || k.size(2) != q.size(2) || k.size(3) != q.size(3)) {
@@ -297,6 +312,7 @@ Tensors fused_rotary(const Tensor& q, const Tensor& k, const Tensor& positions, 
 Tensor fused_rotary_qkv(const Tensor& qkv, int64_t heads, const Tensor& positions, const Tensor& f,
                         bool interleaved, double magnitude) {
   const char* who = "fused_rotary_qkv";
+  no_tangents(who, {&qkv, &f});
   require(who, "qkv", qkv, 3, nullptr, {kF32, kF16, kBF16});
   const int64_t w = qkv.size(2);
   if (heads <= 0 || heads > w / 3 || w % (3 * heads) != 0) {
@@ -353,6 +369,7 @@ Tensor paged_append(const Tensor& k0, const Tensor& v0, const Tensor& kp, const 
                     const Tensor& table, const Tensor& lengths, const Tensor& counts, const Tensor& q0,
                     const Tensor& f, bool interleaved, double magnitude) {
   const char* who = "paged_append";
+  no_tangents(who, {&k0, &v0, &kp, &vp, &q0, &f});
   require(who, "k", k0, 4, nullptr, {kF32, kF16, kBF16});
   require(who, "v", v0, 4, &k0, {k0.scalar_type()});
   const int64_t b = k0.size(0), hk = k0.size(1), s = k0.size(2), d = k0.size(3);
@@ -406,6 +423,7 @@ Tensor paged_append(const Tensor& k0, const Tensor& v0, const Tensor& kp, const 
 Tensor paged_attention(const Tensor& q0, const Tensor& kp, const Tensor& vp, const Tensor& table,
                        const Tensor& lengths, double scale) {
   const char* who = "paged_attention";
+  no_tangents(who, {&q0, &kp, &vp});
   require(who, "q", q0, 4, nullptr, {kF32, kF16, kBF16});
   const int64_t b = q0.size(0), h = q0.size(1), d = q0.size(3);
   if (q0.size(2) != 1) {
@@ -429,6 +447,7 @@ Tensor paged_attention(const Tensor& q0, const Tensor& kp, const Tensor& vp, con
 
 // --- Cross attention -------------------------------------------------------------------------------
 
+constexpr const char* kCross = "fused_cross_attention";
 const float* f32(const Tensor& t) { return static_cast<const float*>(t.data_ptr()); }
 
 // The output, [b, h, sq, d] over a contiguous [b, sq, h, d] buffer, and the [b, h, sq] log-sums.
@@ -475,7 +494,7 @@ struct NotTwice : Function<NotTwice> {
   }
   static Tensors backward(AutogradContext*, const Tensors&) {
     return in_backward([]() -> Tensors {
-      throw OpError("fused_cross_attention: its gradient is not differentiable");
+      throw OpError(std::string(kCross) + ": its gradient is not differentiable");
     });
   }
 };
@@ -494,6 +513,7 @@ struct CrossNode : Function<CrossNode> {
   static Tensors backward(AutogradContext* ctx, const Tensors& grads) {
     const Tensors s = ctx->get_saved_variables();
     return in_backward([&]() -> Tensors {
+      no_tangents(kCross, {&grads[0]});
       Tensors to;
       {
         const c10::AutoGradMode off(false);
@@ -508,7 +528,8 @@ struct CrossNode : Function<CrossNode> {
 
 Tensor fused_cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, double scale,
                               const Tensor& lengths) {
-  const char* who = "fused_cross_attention";
+  const char* who = kCross;
+  no_tangents(who, {&q, &k, &v});
   require(who, "q", q, 4, nullptr, {kF32});
   require(who, "k", k, 4, &q, {kF32});
   require(who, "v", v, 4, &q, {kF32});

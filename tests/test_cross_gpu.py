@@ -400,3 +400,21 @@ def test_decoder_layer(cuda):
             out = cross(x.transpose(1, 2).reshape(b, 1, h * d))
             # Two fp32 attentions and a product of 256 terms on either side.
             assert rel(out, want[:, :, t:t + 1]) <= 4 * TOL
+
+
+@pytest.mark.parametrize("sq", [1, 150])
+def test_forward_mode_refused(cuda, sq):
+    """A tangent of an operand, or of the gradient that the backward is given."""
+    import torch.autograd.forward_ad as forward_ad
+
+    q, k, v, g = operands(cuda, 1, 2, 2, sq, 30, 64, seed=20)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    out = cfa.fused_cross_attention(*leaves, 0.125)
+    with forward_ad.dual_level():
+        for i in range(3):
+            x = [q, k, v]
+            x[i] = forward_ad.make_dual(x[i], torch.ones_like(x[i]))
+            with pytest.raises(cfa.FusedAttentionError, match="no forward-mode derivative"):
+                cfa.fused_cross_attention(*x, 0.125)
+        with pytest.raises(cfa.FusedAttentionError, match="no forward-mode derivative"):
+            torch.autograd.grad(out, leaves, forward_ad.make_dual(g, g))

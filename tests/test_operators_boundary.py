@@ -244,3 +244,35 @@ def test_binding_arguments():
     with pytest.raises(cfa.FusedAttentionError) as e:
         cfa.fused_cross_attention(q, q, q, 1.0)
     assert e.value.code == 0
+
+
+def test_forward_mode_refused():
+    """An operand with a tangent of forward-mode differentiation: a result without one would be a
+    derivative of 0."""
+    import torch.autograd.forward_ad as forward_ad
+
+    x, f, pos = torch.randn(1, 2, 3, 64), cfa.rotary_frequencies(64), torch.arange(3)
+    ints = torch.zeros(1, dtype=torch.int32)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        turning = forward_ad.make_dual(f, torch.ones_like(f))
+        for call in (lambda: cfa.fused_rotary(dual, x, pos, f), lambda: cfa.fused_rotary(x, dual, pos, f),
+                     lambda: cfa.fused_rotary(x, x, pos, turning),
+                     lambda: cfa.fused_rotary_qkv(dual[0], 2, pos[:2], f),
+                     lambda: cfa.fused_rotary_qkv(x[0], 2, pos[:2], turning),
+                     lambda: cfa.paged_append(dual, x, x, x, ints[None], ints),
+                     lambda: cfa.paged_append(x, dual, x, x, ints[None], ints),
+                     lambda: cfa.paged_append(x, x, dual, x, ints[None], ints),
+                     lambda: cfa.paged_append(x, x, x, dual, ints[None], ints),
+                     lambda: cfa.paged_append(x, x, x, x, ints[None], ints, q=dual),
+                     lambda: cfa.paged_append(x, x, x, x, ints[None], ints, frequencies=turning),
+                     lambda: cfa.paged_attention(dual[:, :, :1], x, x, ints[None], ints, 1.0),
+                     lambda: cfa.paged_attention(x[:, :, :1], dual, x, ints[None], ints, 1.0),
+                     lambda: cfa.paged_attention(x[:, :, :1], x, dual, ints[None], ints, 1.0),
+                     lambda: cfa.fused_cross_attention(dual, x, x, 1.0),
+                     lambda: cfa.fused_cross_attention(x, dual, x, 1.0),
+                     lambda: cfa.fused_cross_attention(x, x, dual, 1.0)):
+            with pytest.raises(cfa.FusedAttentionError, match="no forward-mode derivative"):
+                call()
+            with torch.no_grad(), pytest.raises(cfa.FusedAttentionError, match="no forward-mode derivative"):
+                call()

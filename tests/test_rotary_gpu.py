@@ -319,3 +319,26 @@ def test_overlapping_views(cuda, dtype, interleaved):
     grads = [torch.autograd.grad(outs, leaves, g, retain_graph=True)
              for g in ((q, k, x), (q.contiguous(), k.contiguous(), x.contiguous()))]
     assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_forward_mode_refused(cuda):
+    """A tangent of an operand, or of the gradient that a backward is given."""
+    import torch.autograd.forward_ad as forward_ad
+
+    q, k = operands(cuda, torch.float32, 1, 2, 2, 5, 32, seed=14)
+    f, pos = cfa.rotary_frequencies(32, device=cuda), torch.arange(5, device=cuda)
+    x = torch.randn(1, 5, 3 * 64, device=cuda, requires_grad=True)
+    leaves = [t.clone().requires_grad_() for t in (q, k)]
+    outs = [*cfa.fused_rotary(*leaves, pos, f), cfa.fused_rotary_qkv(x, 2, pos, f)]
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, k)
+        with pytest.raises(cfa.FusedAttentionError, match="no forward-mode derivative"):
+            cfa.fused_rotary(dual, k, pos, f)
+        grads = [forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)) for y in outs]
+        for y, leaf, g in zip(outs, (*leaves, x), grads):
+            with pytest.raises(cfa.FusedAttentionError, match="no forward-mode derivative"):
+                torch.autograd.grad(y, leaf, g, retain_graph=True)
+        with pytest.raises(cfa.FusedAttentionError, match="no forward-mode derivative"):
+            torch.autograd.grad(outs[:2], leaves, grads[:2], retain_graph=True)
+    for y, leaf in zip(outs, (*leaves, x)):
+        assert torch.autograd.grad(y, leaf, torch.ones_like(y), retain_graph=True)[0].shape == leaf.shape

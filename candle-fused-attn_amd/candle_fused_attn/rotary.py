@@ -55,8 +55,8 @@ def fused_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
 
     q: [b, h, s, d], k: [b, kv_heads, s, d], of one type (f32, f16 or bf16), any strides (copied first
     where head_dim is not contiguous); positions: [s] or [b, s], int64 or int32; frequencies: float64,
-    one per pair of the rotated part of a head (rotary_frequencies). The results have the operands'
-    shapes and types.
+    one per pair of the rotated part of a head (rotary_frequencies), constants: ones that require a
+    gradient are refused where a graph is recorded. The results have the operands' shapes and types.
     """
     return operators().rotary(q, k, positions, frequencies, interleaved, magnitude)
 

@@ -172,6 +172,13 @@ struct Turn {
   bool inverse;
 };
 
+// The frequencies get no gradient: those that ask for one are refused where a graph would be recorded.
+void not_learned(const char* who, const Tensor& f) {
+  if (records({&f})) {
+    throw OpError(std::string(who) + ": no gradient of the frequencies (detach them, or call it under "
+                  "torch.no_grad())");
+  }
+}
 int64_t check_frequencies(const char* who, const Tensor& f, int64_t d, const Tensor& like) {
   require(who, "frequencies", f, 1, &like, {kF64});
   if (2 * f.size(0) > d || !f.is_contiguous()) {
@@ -298,6 +305,7 @@ Tensors fused_rotary(const Tensor& q, const Tensor& k, const Tensor& positions, 
                      bool interleaved, double magnitude) {
   const char* who = "fused_rotary";
   no_tangents(who, {&q, &k, &f});
+  not_learned(who, f);
   require(who, "q", q, 4, nullptr, {kF32, kF16, kBF16});
   require(who, "k", k, 4, &q, {q.scalar_type()});
   if (k.size(0) != q.size(0) || k.size(2) != q.size(2) || k.size(3) != q.size(3)) {
@@ -313,6 +321,7 @@ Tensor fused_rotary_qkv(const Tensor& qkv, int64_t heads, const Tensor& position
                         bool interleaved, double magnitude) {
   const char* who = "fused_rotary_qkv";
   no_tangents(who, {&qkv, &f});
+  not_learned(who, f);
   require(who, "qkv", qkv, 3, nullptr, {kF32, kF16, kBF16});
   const int64_t w = qkv.size(2);
   if (heads <= 0 || heads > w / 3 || w % (3 * heads) != 0) {
@@ -370,6 +379,7 @@ Tensor paged_append(const Tensor& k0, const Tensor& v0, const Tensor& kp, const 
                     const Tensor& f, bool interleaved, double magnitude) {
   const char* who = "paged_append";
   no_tangents(who, {&k0, &v0, &kp, &vp, &q0, &f});
+  not_learned(who, f);
   require(who, "k", k0, 4, nullptr, {kF32, kF16, kBF16});
   require(who, "v", v0, 4, &k0, {k0.scalar_type()});
   const int64_t b = k0.size(0), hk = k0.size(1), s = k0.size(2), d = k0.size(3);

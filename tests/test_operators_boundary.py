@@ -276,3 +276,17 @@ def test_forward_mode_refused():
                 call()
             with torch.no_grad(), pytest.raises(cfa.FusedAttentionError, match="no forward-mode derivative"):
                 call()
+
+
+def test_learned_frequencies_refused():
+    """Frequencies that require a gradient would get none: refused, unless no graph is recorded or they are
+    detached."""
+    x, pos, ints = torch.randn(1, 2, 3, 64), torch.arange(3), torch.zeros(1, dtype=torch.int32)
+    f = cfa.rotary_frequencies(64).requires_grad_()
+    for call in (lambda f: cfa.fused_rotary(x, x, pos, f), lambda f: cfa.fused_rotary_qkv(x[0], 2, pos[:2], f),
+                 lambda f: cfa.paged_append(x, x, x, x, ints[None], ints, frequencies=f)):
+        with pytest.raises(cfa.FusedAttentionError, match="no gradient of the frequencies"):
+            call(f)
+        for fine in (lambda: call(f.detach()), lambda: torch.no_grad()(call)(f)):
+            with pytest.raises(cfa.FusedAttentionError, match="not on a HIP device"):
+                fine()

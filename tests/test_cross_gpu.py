@@ -418,3 +418,21 @@ def test_forward_mode_refused(cuda, sq):
                 cfa.fused_cross_attention(*x, 0.125)
         with pytest.raises(cfa.FusedAttentionError, match="no forward-mode derivative"):
             torch.autograd.grad(out, leaves, forward_ad.make_dual(g, g))
+
+
+@pytest.mark.parametrize("sq", [1, 150])
+def test_far_keys(cuda, sq):
+    """Samples more than 2^31 values apart: as contiguous ones, bit for bit, gradients too."""
+    b, h, sk, d = 2, 2, 70, 64
+    q, k, v, g = operands(cuda, b, h, h, sq, sk, d, seed=21)
+    k, v = (t.contiguous() for t in (k, v))
+    far = torch.empty(2 ** 31 + 2 ** 16, device=cuda)
+    at = [far.as_strided(k.shape, (2 ** 31 + 64, sk * d, d, 1), i * h * sk * d) for i in range(2)]
+    at[0].copy_(k), at[1].copy_(v)
+    out = []
+    for x in ((q, k, v), (q, *at)):
+        leaves = [t.detach().requires_grad_() for t in x]
+        o = cfa.fused_cross_attention(*leaves, 0.125, ints(cuda, [70, 33]))
+        out.append([o.detach(), *torch.autograd.grad(o, leaves, g)])
+    assert all(torch.equal(x, y) for x, y in zip(*out))
+    assert bool(out[0][0].isfinite().all()) and float(out[0][0].abs().max()) > 0

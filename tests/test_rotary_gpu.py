@@ -342,3 +342,15 @@ def test_forward_mode_refused(cuda):
             torch.autograd.grad(outs[:2], leaves, grads[:2], retain_graph=True)
     for y, leaf in zip(outs, (*leaves, x)):
         assert torch.autograd.grad(y, leaf, torch.ones_like(y), retain_graph=True)[0].shape == leaf.shape
+
+
+def test_gradient_records_a_graph(cuda):
+    """A gradient with a graph of it has one where the output's gradient does, and none where nothing in it
+    can be differentiated (the rotation is linear)."""
+    q, k = operands(cuda, torch.float32, 1, 2, 2, 5, 32, seed=15)
+    f, pos = cfa.rotary_frequencies(32, device=cuda), torch.arange(5, device=cuda)
+    q.requires_grad_()
+    out = cfa.fused_rotary(q, k, pos, f)[0]
+    for g in (torch.ones_like(out), torch.ones_like(out).requires_grad_()):
+        (dq,) = torch.autograd.grad(out, q, g, create_graph=True)
+        assert dq.requires_grad == g.requires_grad and (dq.grad_fn is not None) == g.requires_grad

@@ -67,10 +67,10 @@ def link_command(objects: list[Path], out: Path = LIB) -> list[str]:
             str(out)]
 
 
-def _run(cmd: list[str], tmp: Path, out: Path, verbose: bool) -> Path:
+def _run(cmd: list[str], tmp: Path, out: Path, verbose: bool, cwd: Path | None = None) -> Path:
     if verbose:
         print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
+    res = subprocess.run(cmd, capture_output=True, text=True, cwd=cwd)
     if res.returncode != 0:
         raise RuntimeError(f"hipcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
     if tmp != out:
@@ -78,16 +78,24 @@ def _run(cmd: list[str], tmp: Path, out: Path, verbose: bool) -> Path:
     return out
 
 
+def compile_objects(sources: list[Path], folder: Path, verbose: bool = False) -> list[Path]:
+    """One object file in `folder` per source, compiled at once. The commands name them without the
+    folder: hipcc puts a hash of its command into the object, and a library of the same sources has to
+    be the same file wherever it was built (bench.py knows by its hash which one was measured)."""
+    outs = [Path(s.name + ".o") for s in sources]
+    with ThreadPoolExecutor(len(sources)) as pool:
+        # (list() waits for every source and raises what a compilation raised.)
+        list(pool.map(lambda so: _run(compile_command(*so), so[1], so[1], verbose, folder),
+                      zip(sources, outs)))
+    return [folder / o for o in outs]
+
+
 def build(verbose: bool = False) -> Path:
     """Compile libfattn.so in-tree (always; the caller decides when to rebuild)."""
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     tmp = LIB.with_suffix(".so.tmp")
-    with tempfile.TemporaryDirectory() as d, ThreadPoolExecutor(len(SOURCES)) as pool:
-        objects = [Path(d) / (s.name + ".o") for s in SOURCES]
-        # (list() waits for every source and raises what a compilation raised.)
-        list(pool.map(lambda so: _run(compile_command(*so), so[1], so[1], verbose),
-                      zip(SOURCES, objects)))
-        return _run(link_command(objects, tmp), tmp, LIB, verbose)
+    with tempfile.TemporaryDirectory() as d:
+        return _run(link_command(compile_objects(SOURCES, Path(d), verbose), tmp), tmp, LIB, verbose)
 
 
 def host_command(out: Path = HOST_LIB) -> list[str]:

@@ -249,14 +249,23 @@ void remember(AutogradContext* ctx, const Turn& how) {
   ctx->saved_data["inverse"] = how.inverse;
   ctx->set_materialize_grads(false);
 }
-Turn turn_back(AutogradContext* ctx) {
+Turn turn_back(AutogradContext* ctx, const Tensor& grad) {
   const Tensors saved = ctx->get_saved_variables();
-  return Turn{saved[0],
-              saved[1],
-              ctx->saved_data["heads"].toInt(),
-              ctx->saved_data["interleaved"].toBool(),
-              ctx->saved_data["magnitude"].toDouble(),
-              !ctx->saved_data["inverse"].toBool()};
+  const Turn how{saved[0],
+                 saved[1],
+                 ctx->saved_data["heads"].toInt(),
+                 ctx->saved_data["interleaved"].toBool(),
+                 ctx->saved_data["magnitude"].toDouble(),
+                 !ctx->saved_data["inverse"].toBool()};
+  // (Hooks on saved tensors may have replaced them.)
+  if (how.heads > 0) {
+    check_positions("fused_rotary_qkv", how.positions, grad.size(0), grad.size(1), grad);
+    check_frequencies("fused_rotary_qkv", how.frequencies, grad.size(2) / 3 / how.heads, grad);
+  } else {
+    check_positions("fused_rotary", how.positions, grad.size(0), grad.size(2), grad);
+    check_frequencies("fused_rotary", how.frequencies, grad.size(3), grad);
+  }
+  return how;
 }
 Tensor turn_one(const Tensor& x, const Turn& how);
 Tensors turn_two(const Tensor& q, const Tensor& k, const Turn& how);
@@ -269,7 +278,7 @@ struct TurnOne : Function<TurnOne> {
   static Tensors backward(AutogradContext* ctx, const Tensors& grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor()};
     return in_backward([&]() -> Tensors {
-      const Turn how = turn_back(ctx);
+      const Turn how = turn_back(ctx, grads[0]);
       no_tangents(how.heads > 0 ? "fused_rotary_qkv" : "fused_rotary", {&grads[0]});
       return {turn_one(grads[0], how), Tensor()};
     });
@@ -283,8 +292,9 @@ struct TurnTwo : Function<TurnTwo> {
   static Tensors backward(AutogradContext* ctx, const Tensors& grads) {
     const bool gq = grads[0].defined() && ctx->needs_input_grad(0);
     const bool gk = grads[1].defined() && ctx->needs_input_grad(1);
+    if (!gq && !gk) return {Tensor(), Tensor(), Tensor()};
     return in_backward([&]() -> Tensors {
-      const Turn how = turn_back(ctx);
+      const Turn how = turn_back(ctx, gq ? grads[0] : grads[1]);
       no_tangents("fused_rotary", {&grads[0], &grads[1]});
       if (gq && gk) {
         const Tensors both = turn_two(grads[0], grads[1], how);
@@ -460,6 +470,30 @@ Tensor paged_attention(const Tensor& q0, const Tensor& kp, const Tensor& vp, con
 constexpr const char* kCross = "fused_cross_attention";
 const float* f32(const Tensor& t) { return static_cast<const float*>(t.data_ptr()); }
 
+void check_cross(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths) {
+  require(kCross, "q", q, 4, nullptr, {kF32});
+  require(kCross, "k", k, 4, &q, {kF32});
+  require(kCross, "v", v, 4, &q, {kF32});
+  const int64_t b = q.size(0);
+  if (k.sizes() != v.sizes() || k.size(0) != b || k.size(3) != q.size(3)) {
+    throw OpError(std::string(kCross) + ": q [b, h, sq, d] and k, v [b, kv_heads, sk, d] expected, got " +
+                  shape_of(q.sizes()) + " " + shape_of(k.sizes()) + " " + shape_of(v.sizes()));
+  }
+  if (!lengths.defined()) return;
+  require(kCross, "key_lengths", lengths, 1, &q, {kI32});
+  if (lengths.size(0) != b || !lengths.is_contiguous()) {
+    throw OpError(std::string(kCross) + ": contiguous key_lengths [" + std::to_string(b) +
+                  "] expected, got " + shape_of(lengths.sizes()));
+  }
+}
+// A [b, h, s, d] tensor itself where it lies over a contiguous [b, s, h, d] buffer, else a copy that does.
+Tensor merged(const Tensor& t) {
+  const int64_t h = t.size(1), s = t.size(2), d = t.size(3);
+  const bool ok = t.stride(3) == 1 && (h <= 1 || t.stride(1) == d) && (s <= 1 || t.stride(2) == h * d) &&
+                  (t.size(0) <= 1 || t.stride(0) == s * h * d);
+  return ok ? t : t.transpose(1, 2).contiguous().transpose(1, 2);
+}
+
 // The output, [b, h, sq, d] over a contiguous [b, sq, h, d] buffer, and the [b, h, sq] log-sums.
 Tensors cross_forward(const Tensor& q, const Tensor& k, const Tensor& v, double scale, const Tensor& lengths) {
   const int64_t b = q.size(0), h = q.size(1), sq = q.size(2), d = q.size(3), hk = k.size(1), sk = k.size(2);
@@ -524,10 +558,19 @@ struct CrossNode : Function<CrossNode> {
     const Tensors s = ctx->get_saved_variables();
     return in_backward([&]() -> Tensors {
       no_tangents(kCross, {&grads[0]});
+      // (Hooks on saved tensors may have replaced them: save_on_cpu brings them back in another layout.)
+      check_cross(s[0], s[1], s[2], s[3]);
+      require(kCross, "the saved output", s[4], 4, &s[0], {kF32});
+      require(kCross, "the saved log-sums", s[5], 3, &s[0], {kF32});
+      if (s[4].sizes() != s[0].sizes() || s[5].sizes() != s[0].sizes().slice(0, 3) ||
+          grads[0].sizes() != s[0].sizes()) {
+        throw OpError(std::string(kCross) + ": saved tensors came back in other shapes");
+      }
       Tensors to;
       {
         const c10::AutoGradMode off(false);
-        to = cross_backward(s[0], s[1], s[2], ctx->saved_data["scale"].toDouble(), s[3], s[4], s[5], grads[0]);
+        to = cross_backward(aligned_rows(s[0]), aligned_rows(s[1]), aligned_rows(s[2]),
+                            ctx->saved_data["scale"].toDouble(), s[3], merged(s[4]), s[5].contiguous(), grads[0]);
       }
       if (c10::GradMode::is_enabled()) to = NotTwice::apply(to[0], to[1], to[2], s[0], s[1], s[2], grads[0]);
       to.resize(4);  // (none for `how`)
@@ -538,23 +581,8 @@ struct CrossNode : Function<CrossNode> {
 
 Tensor fused_cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, double scale,
                               const Tensor& lengths) {
-  const char* who = kCross;
-  no_tangents(who, {&q, &k, &v});
-  require(who, "q", q, 4, nullptr, {kF32});
-  require(who, "k", k, 4, &q, {kF32});
-  require(who, "v", v, 4, &q, {kF32});
-  const int64_t b = q.size(0);
-  if (k.sizes() != v.sizes() || k.size(0) != b || k.size(3) != q.size(3)) {
-    throw OpError(std::string(who) + ": q [b, h, sq, d] and k, v [b, kv_heads, sk, d] expected, got " +
-                  shape_of(q.sizes()) + " " + shape_of(k.sizes()) + " " + shape_of(v.sizes()));
-  }
-  if (lengths.defined()) {
-    require(who, "key_lengths", lengths, 1, &q, {kI32});
-    if (lengths.size(0) != b || !lengths.is_contiguous()) {
-      throw OpError(std::string(who) + ": contiguous key_lengths [" + std::to_string(b) +
-                    "] expected, got " + shape_of(lengths.sizes()));
-    }
-  }
+  no_tangents(kCross, {&q, &k, &v});
+  check_cross(q, k, v, lengths);
   const Tensor qa = aligned_rows(q), ka = aligned_rows(k), va = aligned_rows(v);
   return records({&qa, &ka, &va}) ? CrossNode::apply(qa, ka, va, How{scale, lengths})
                                   : cross_forward(qa, ka, va, scale, lengths)[0];

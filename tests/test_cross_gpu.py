@@ -436,3 +436,30 @@ def test_far_keys(cuda, sq):
         out.append([o.detach(), *torch.autograd.grad(o, leaves, g)])
     assert all(torch.equal(x, y) for x, y in zip(*out))
     assert bool(out[0][0].isfinite().all()) and float(out[0][0].abs().max()) > 0
+
+
+@pytest.mark.parametrize("sq,sk,lengths", [(1, 300, None), (40, 70, [70, 3]), (150, 600, None)])
+def test_saved_tensors_elsewhere(cuda, sq, sk, lengths):
+    """What the node saves may come back in other memory and another layout (activations kept on the host):
+    the same gradients, bit for bit; of another type or shape: an error."""
+    q, k, v, g = operands(cuda, 2, 4, 2, sq, sk, 64, seed=22)
+    q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+    n = ints(cuda, lengths)
+
+    def step(context):
+        with context:
+            out = cfa.fused_cross_attention(q, k, v, 0.125, n)
+        return torch.autograd.grad(out, (q, k, v), g)
+
+    hooks = torch.autograd.graph.saved_tensors_hooks
+    want = step(hooks(lambda t: t, lambda t: t))
+    for context in (torch.autograd.graph.save_on_cpu(pin_memory=True), torch.autograd.graph.save_on_cpu(),
+                    hooks(lambda t: t, lambda t: t.clone(memory_format=torch.contiguous_format)),
+                    hooks(lambda t: t, lambda t: t.transpose(0, -1).contiguous().transpose(0, -1))):
+        assert all(torch.equal(x, y) for x, y in zip(step(context), want))
+    for context in (hooks(lambda t: t, lambda t: t.half() if t.is_floating_point() else t),
+                    hooks(lambda t: t, lambda t: t[..., :-1] if t.dim() == 3 else t),
+                    hooks(lambda t: t, lambda t: t[:1]),
+                    hooks(lambda t: t.cpu(), lambda t: t)):
+        with pytest.raises(cfa.FusedAttentionError, match="fused_cross_attention: "):
+            step(context)

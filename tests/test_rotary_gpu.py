@@ -354,3 +354,29 @@ def test_gradient_records_a_graph(cuda):
     for g in (torch.ones_like(out), torch.ones_like(out).requires_grad_()):
         (dq,) = torch.autograd.grad(out, q, g, create_graph=True)
         assert dq.requires_grad == g.requires_grad and (dq.grad_fn is not None) == g.requires_grad
+
+
+def test_saved_tensors_elsewhere(cuda):
+    """Positions and frequencies that the node saves may come back in other memory (activations kept on the
+    host): the same gradients, bit for bit; of another type or shape: an error."""
+    q, k = operands(cuda, torch.float32, 2, 4, 2, 9, 64, seed=17)
+    gq, gk = operands(cuda, torch.float32, 2, 4, 2, 9, 64, seed=18)
+    x, gx = (torch.randn(2, 9, 3 * 128, device=cuda) for _ in range(2))
+    q, k, x = (t.detach().requires_grad_() for t in (q, k, x))
+    f, pos = cfa.rotary_frequencies(64, device=cuda), torch.randint(0, 999, (9, 2), device=cuda).t()
+
+    def step(context, two):
+        with context:
+            outs = cfa.fused_rotary(q, k, pos, f) if two else [cfa.fused_rotary_qkv(x, 2, pos, f)]
+        return torch.autograd.grad(outs, (q, k) if two else x, (gq, gk) if two else gx)
+
+    hooks = torch.autograd.graph.saved_tensors_hooks
+    for two in (True, False):
+        want = step(hooks(lambda t: t, lambda t: t), two)
+        for context in (torch.autograd.graph.save_on_cpu(pin_memory=True), torch.autograd.graph.save_on_cpu(),
+                        hooks(lambda t: t, lambda t: t.clone(memory_format=torch.contiguous_format))):
+            assert all(torch.equal(a, b) for a, b in zip(step(context, two), want))
+        for context in (hooks(lambda t: t, lambda t: t.float()), hooks(lambda t: t, lambda t: t[:1, :1]
+                        if t.dim() == 2 else t), hooks(lambda t: t.cpu(), lambda t: t)):
+            with pytest.raises(cfa.FusedAttentionError, match="fused_rotary"):
+                step(context, two)

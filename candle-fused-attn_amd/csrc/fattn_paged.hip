@@ -36,7 +36,9 @@
 //
 // Measured (kernel and join): 4 contexts of 60000 to 131071, 32 heads in 8 groups, d 128 bf16, 263 + 5 us
 // (5.9 TB/s); that ragged batch 45 + 5 us (4.5 TB/s); 8 x 6 heads 1 x 1536 fp32 12.4 + 3.9 us (3.0 TB/s);
-// one sequence of 240, 6 heads, 7.8 us, the latency of one workgroup.
+// one sequence of 240, 6 heads, 7.8 us, the latency of one workgroup, where the table has room for little
+// more (split_plan); under one for 4096 or 131072 tokens the same sequence takes runs and a join, 10.5 us
+// for 7.3 from a graph, 64 such sequences 20.1 for 12.6.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -718,7 +720,8 @@ SplitPlan split_plan(int64_t b, int64_t hk, int64_t rows, int64_t d, int64_t cap
   p.min_run = kSplitWaves;
   p.begin = kSplitWaves;
   // One workgroup per key head, and no join, where no sequence can have more than four tiles a wave, or
-  // eight with a workgroup for most CUs. Direct / in runs, us (with 6 us of a graph's launch): fp32 d 64,
+  // eight with a workgroup for most CUs: by what the tables have room for, since the lengths are on the
+  // device. Direct / in runs, us (with 6 us of a graph's launch): fp32 d 64,
   // 384 heads of 1024 tokens 45.9 / 52.6, of 1 to 700 25.6 / 29.9; bf16 d 128, 256 of 1000 28.8 / 35.5,
   // 192 26.0 / 29.7; past it 384 of 1 to 2048 64.9 / 54.7, 48 of 1000 28.2 / 20.8, of 1500 37.8 / 23.0. (A
   // wave alone takes 2 us a tile, the memory's latency twice; eight waves a workgroup change little.)

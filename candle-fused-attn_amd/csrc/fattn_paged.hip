@@ -34,11 +34,11 @@
 // kSplitWaves tiles more than it has, which is what beginning one costs: without, the workgroup that the
 // shortest sequences fall to ends last (64 sequences of 1 to 2048, 6 heads, fp32 d 64: 79 us, 46 so).
 //
-// Measured (kernel and join): 4 contexts of 60000 to 131071, 32 heads in 8 groups, d 128 bf16, 263 + 5 us
-// (5.9 TB/s); that ragged batch 45 + 5 us (4.5 TB/s); 8 x 6 heads 1 x 1536 fp32 12.4 + 3.9 us (3.0 TB/s);
-// one sequence of 240, 6 heads, 7.8 us, the latency of one workgroup, where the table has room for little
-// more (split_plan); under one for 4096 or 131072 tokens the same sequence takes runs and a join, 10.5 us
-// for 7.3 from a graph, 64 such sequences 20.1 for 12.6.
+// Measured (kernel and join): 4 contexts of 60000 to 131071, 32 heads in 8 groups, d 128 bf16, 263 to 273 + 5
+// us (5.7 to 5.9 TB/s, by card); that ragged batch 45 + 5 us (4.5 TB/s); 8 x 6 heads 1 x 1536 fp32 12.4 + 3.9
+// us (3.0 TB/s); one sequence of 240, 6 heads, 7.8 us, the latency of one workgroup, where the table has room
+// for little more (split_plan); under one for 4096 or 131072 tokens the same sequence takes runs and a join,
+// 10.5 us for 7.3 from a graph, 64 such sequences 20.1 for 12.6.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>

@@ -4,8 +4,8 @@ kernels (libfattn.so).
 
 The public surface mirrors the reference crate's (src/lib.rs:90-161): `fused_attention`,
 `fused_attention_qkv`, `CUDA_HEAD_DIM`. Around them, without a counterpart there: rotary positions
-(`fused_rotary`, `fused_rotary_qkv`, `rotary_frequencies`), a paged key-value cache (`paged_append`,
-`paged_attention`) and attention to states of another length (`fused_cross_attention`).
+(`fused_rotary`, `fused_rotary_qkv`, `rotary_frequencies`), a paged key-value cache, in 4 bits too
+(`paged_append`, `paged_attention`, `paged_read`, `fp4_row_bytes`) and attention to states of another length (`fused_cross_attention`).
 """
 from ._lib import FusedAttentionError, LIB_PATH, version
 from .cross import fused_cross_attention
@@ -21,7 +21,7 @@ from .ops import (
     set_dq_sum,
     set_projection_route,
 )
-from .paged import paged_append, paged_attention
+from .paged import fp4_row_bytes, paged_append, paged_attention, paged_read
 from .rotary import fused_rotary, fused_rotary_qkv, rotary_frequencies
 
 __all__ = [
@@ -31,6 +31,7 @@ __all__ = [
     "FusedAttentionError",
     "LIB_PATH",
     "float4_aligned",
+    "fp4_row_bytes",
     "fused_attention",
     "fused_attention_qkv",
     "fused_cross_attention",
@@ -38,6 +39,7 @@ __all__ = [
     "fused_rotary_qkv",
     "paged_append",
     "paged_attention",
+    "paged_read",
     "qkv_projection_of",
     "reads_in_place",
     "rotary_frequencies",

@@ -24,6 +24,7 @@ FATTN_EWORKSPACE = -5
 
 # Element types.
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+FP4 = 3  # (of a cache: uint8 tensors)
 
 # Every entry point include/fattn.h declares.
 EXPORTS = (
@@ -49,6 +50,8 @@ EXPORTS = (
     "fattn_paged_append",
     "fattn_paged_attention_workspace_bytes",
     "fattn_paged_attention",
+    "fattn_paged_scored_attention",
+    "fattn_paged_read",
     "fattn_cross_workspace_bytes",
     "fattn_cross_forward",
     "fattn_cross_backward_workspace_bytes",
@@ -119,6 +122,10 @@ def _declare(L: ctypes.CDLL) -> None:
     L.fattn_paged_attention_workspace_bytes.restype = SIZE
     L.fattn_paged_attention.argtypes = [C_INT, C_INT, I64, I64, I64, I64, P, P, P, P, P, P, P, I64, I64,
                                         P, I64, I64, P, C_FLOAT, P, SIZE, P]
+    L.fattn_paged_scored_attention.argtypes = [C_INT, C_INT, I64, I64, I64, I64, P, P, P, P, P, P, P, I64, I64,
+                                               P, I64, I64, P, C_FLOAT, C_FLOAT, P, P, SIZE, P]
+    L.fattn_paged_read.argtypes = [C_INT, C_INT, I64, I64, I64, I64, P, P, P, P, I64, I64, P, I64, I64, P,
+                                   P, P, P, P]
     for name in ("fattn_cross_workspace_bytes", "fattn_cross_backward_workspace_bytes"):
         getattr(L, name).argtypes = [I64, I64, I64, I64, I64, I64]
         getattr(L, name).restype = SIZE

@@ -174,7 +174,14 @@ int static_scratch(void* stream, void** out);
 
 // --- Rotary positions and the paged cache (fattn_rotary.hip, fattn_paged.hip) --------------------
 // Element types of the C ABI (FATTN_F32, ..).
-constexpr int kF32 = 0, kF16 = 1, kBF16 = 2;
+constexpr int kF32 = 0, kF16 = 1, kBF16 = 2, kFP4 = 3;
+// A cache's row of d values in 4 bits: two to a byte, the first in the low bits, then a byte per 32 values
+// with their scale's exponent + 127, up to a multiple of 4 bytes. (32 values' codes: a sign, then 0, .5, 1,
+// 1.5, 2, 3, 4, 6 in order; scale byte 255: NaN.)
+struct four {
+  unsigned char bits;
+};
+__host__ __device__ constexpr int four_row(int d) { return d / 2 + (d < 128 ? 4 : d / 32); }
 // x / n for 0 <= x < 2^31, n >= 1 (n 0: not divided by): (hi32(x magic) + x) >> shift.
 struct Divider {
   unsigned magic, shift;
@@ -216,8 +223,23 @@ struct RotaryArgs {
   Divider by_per[3], by_items[3], by_seq, by_pairs;
 };
 // vec: values per access, 8, 4 or 1 (2 interleaved): every pointer, stride and part of a head is a
-// multiple of it, where it is 4 or more.
+// multiple of it, where it is 4 or more. (To a 4-bit cache: 8, of accesses of 16 bytes, or less.)
 int launch_rotary(RotaryArgs a, int dtype, int cache_dtype, int vec, void* stream);
+
+// Tokens starts[b] + i (starts null: i), i < S, of a paged cache, to k and v, [B, HK, S, d] contiguous: 0
+// past lengths[b], NaN where the table or the cache has no page. ks, vs: (page, head, slot).
+struct PagedReadArgs {
+  const void *k_pages, *v_pages;
+  void *k, *v;
+  int64_t ks[3], vs[3];
+  const int32_t *table, *lengths, *starts;
+  int64_t table_stride;
+  int table_width, pages, page_size, B, HK, S;
+  int blocks;  // the launcher's: workgroups of one (b, head), and the division by page_size
+  Divider by_page;
+};
+int launch_paged_read(PagedReadArgs a, int cache_dtype, int dtype, int d, void* stream);
+int64_t paged_read_blocks(int64_t s, int64_t d);
 
 // Attention of few queries per key head, split over the keys (fattn_paged.hip). Rows of one key head:
 // the G query heads of its group times SQ queries, in blocks of 16.
@@ -234,6 +256,10 @@ struct SplitArgs {
   Divider by_page;  // of halves of a tile: page_size / 16
   int B, H, HK, G, SQ, SK, RB;    // SK: the most keys a sequence can have; RB: blocks of rows
   float scale;
+  // Scores x (of one query, over a page table) as cap tanh(x / cap), less slopes[head] times the distance;
+  // cap2: cap log2 e (0: not capped), cap_inv its inverse; slopes null: none.
+  const float* slopes;
+  float cap2, cap_inv;
   // The workspace: two parts per workgroup, and where each sequence's costs begin (B + 1 of them).
   float* part;
   int64_t* before;

@@ -17,7 +17,7 @@ constexpr int64_t kMaxGrid = (int64_t{1} << 24) - 1;
 constexpr int64_t kMaxHeads = 65535;
 
 bool known(int dtype) { return dtype == FATTN_F32 || dtype == FATTN_F16 || dtype == FATTN_BF16; }
-int64_t size_of(int dtype) { return dtype == FATTN_F32 ? 4 : 2; }
+int64_t size_of(int dtype) { return dtype == FATTN_F32 ? 4 : dtype == FATTN_FP4 ? 1 : 2; }
 bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 void copy3(int64_t to[3], const int64_t from[3]) {
   for (int i = 0; i < 3; ++i) to[i] = from[i];
@@ -42,10 +42,10 @@ int check_dim(const char* who, int64_t d) {
                    static_cast<long long>(d));
 }
 int check_types(const char* who, int dtype, int cache_dtype) {
-  if (!known(dtype) || !known(cache_dtype)) {
+  if (!known(dtype) || !(known(cache_dtype) || cache_dtype == FATTN_FP4)) {
     return set_error(FATTN_EINVAL, "%s: f32, f16 or bf16 only", who);
   }
-  if (dtype != FATTN_F32 && cache_dtype != dtype) {
+  if (dtype != FATTN_F32 && cache_dtype != dtype && cache_dtype != FATTN_FP4) {
     return set_error(FATTN_EINVAL, "%s: a cache of another type than 16-bit activations", who);
   }
   return 0;
@@ -61,6 +61,13 @@ int check_heads(const char* who, int64_t heads, int64_t kv_heads, bool none) {
                      static_cast<long long>(heads), static_cast<long long>(kv_heads));
   }
   return 0;
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+// The cap of scores: 0 (none), or such that it and its inverse are floats in units of log2 e too.
+int check_cap(const char* who, float cap) {
+  if (cap == 0.0f || (cap >= 1e-30f && cap <= 1e30f)) return 0;
+  return set_error(FATTN_EINVAL, "%s: a cap from 1e-30 to 1e30 expected, got %g", who, static_cast<double>(cap));
 }
 
 // The pages, their table and the lengths of a cache; ks, vs: the strides that its indices use.
@@ -80,12 +87,13 @@ int check_cache(const char* who, int cache_dtype, const void* k, const int64_t k
   if (pages > INT32_MAX || page_size > INT32_MAX / 2 || table_width > INT32_MAX) {
     return set_error(FATTN_ERANGE, "%s: the cache exceeds 32-bit indexing", who);
   }
-  const int64_t size = size_of(cache_dtype), per = 16 / size;
+  // (4-bit rows are words of 4 bytes, 68 of d 128.)
+  const int64_t size = size_of(cache_dtype), unit = cache_dtype == FATTN_FP4 ? 4 : 16, per = unit / size;
   used3(ks, k_strides, pages, kv_heads, page_size);
   used3(vs, v_strides, pages, kv_heads, page_size);
   if (negative(ks, 3) || negative(vs, 3)) return set_error(FATTN_EINVAL, "%s: negative strides", who);
-  if (!aligned(k, 16) || !aligned(v, 16) || !multiples(ks, per) || !multiples(vs, per)) {
-    return set_error(FATTN_EALIGN, "%s: the cache's rows must be 16-byte aligned", who);
+  if (!aligned(k, unit) || !aligned(v, unit) || !multiples(ks, per) || !multiples(vs, per)) {
+    return set_error(FATTN_EALIGN, "%s: the cache's rows must be %d-byte aligned", who, static_cast<int>(unit));
   }
   if (16 * ks[2] * size > INT32_MAX || 16 * vs[2] * size > INT32_MAX) {
     return set_error(FATTN_ERANGE, "%s: 16 slots of the cache span more than 2 GiB", who);
@@ -115,6 +123,19 @@ int run_rotary(const char* who, fattn::RotaryArgs& a, int dtype, int cache_dtype
   a.B = static_cast<int>(b), a.S = static_cast<int>(s), a.D = static_cast<int>(d);
   a.pairs = static_cast<int>(dim / 2);
   int64_t vec = 16 / size;
+  if (cache_dtype == FATTN_FP4) {
+    // Eight values at a time, in accesses of 16 bytes, or one by one.
+    bool wide = a.interleaved || dim / 2 % 8 == 0;
+    for (int i = 0; i < 3; ++i) {
+      const fattn::RotaryPart& p = a.part[i];
+      if (p.heads == 0) continue;
+      wide = wide && fits(vec, p.x, size, p.xs, b, p.heads, s);
+      if (i == 0) wide = wide && fits(vec, p.y, size, p.ys, b, p.heads, s);
+    }
+    const int err = fattn::launch_rotary(a, dtype, cache_dtype, wide ? 8 : 1, stream);
+    if (err) return fattn::hip_error(err, who, "launch");
+    return fattn::done();
+  }
   auto allowed = [&](int64_t v) {
     if (d % v != 0 || (a.interleaved ? dim : dim / 2) % v != 0) return false;
     for (int i = 0; i < 3; ++i) {
@@ -278,6 +299,9 @@ int fattn_paged_append(int dtype, int cache_dtype, int64_t b, int64_t heads, int
   if (!k || !v || !k_strides || !v_strides || (heads > 0 && (!q || !q_out || !q_strides || !q_out_strides))) {
     return set_error(FATTN_EINVAL, "%s: null operand", who);
   }
+  if (cache_dtype == FATTN_FP4 && heads > 0 && q == q_out) {
+    return set_error(FATTN_EINVAL, "%s: q_out must not be q with a 4-bit cache", who);
+  }
   const int turned = frequencies != nullptr ? 1 : 0;
   a.part[0].heads = static_cast<int>(heads), a.part[0].rotate = turned;
   if (heads > 0) {
@@ -311,11 +335,26 @@ int fattn_paged_attention(int dtype, int cache_dtype, int64_t b, int64_t heads, 
                           const int32_t* table, int64_t table_stride, int64_t table_width,
                           const int32_t* lengths, float scale, void* workspace,
                           size_t workspace_bytes, void* stream) {
+  return fattn_paged_scored_attention(dtype, cache_dtype, b, heads, kv_heads, d, q, q_strides, out, k_pages,
+                                      k_page_strides, v_pages, v_page_strides, pages, page_size, table,
+                                      table_stride, table_width, lengths, scale, 0.0f, nullptr, workspace,
+                                      workspace_bytes, stream);
+}
+
+int fattn_paged_scored_attention(int dtype, int cache_dtype, int64_t b, int64_t heads, int64_t kv_heads,
+                                 int64_t d, const void* q, const int64_t q_strides[2], void* out,
+                                 const void* k_pages, const int64_t k_page_strides[3],
+                                 const void* v_pages, const int64_t v_page_strides[3], int64_t pages,
+                                 int64_t page_size, const int32_t* table, int64_t table_stride,
+                                 int64_t table_width, const int32_t* lengths, float scale, float cap,
+                                 const float* slopes, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
   const char* who = "paged_attention";
   if (int rc = check_types(who, dtype, cache_dtype)) return rc;
   if (b < 0) return set_error(FATTN_EINVAL, "%s: negative size", who);
   if (int rc = check_heads(who, heads, kv_heads, b == 0)) return rc;
   if (int rc = check_dim(who, d)) return rc;
+  if (int rc = check_cap(who, cap)) return rc;
   if (b == 0) return fattn::done();
   fattn::SplitArgs a{};
   if (int rc = check_cache(who, cache_dtype, k_pages, k_page_strides, v_pages, v_page_strides, pages,
@@ -341,7 +380,46 @@ int fattn_paged_attention(int dtype, int cache_dtype, int64_t b, int64_t heads, 
   a.B = static_cast<int>(b), a.H = static_cast<int>(heads), a.HK = static_cast<int>(kv_heads);
   a.G = static_cast<int>(heads / kv_heads), a.SQ = 1, a.SK = static_cast<int>(capacity);
   a.scale = scale;
+  a.slopes = slopes, a.cap2 = cap * kLog2e, a.cap_inv = cap == 0.0f ? 0.0f : 1.0f / a.cap2;
   return run_split(who, a, dtype, cache_dtype, d, capacity, workspace, workspace_bytes, stream);
+}
+
+int fattn_paged_read(int cache_dtype, int dtype, int64_t b, int64_t kv_heads, int64_t s, int64_t d,
+                     const void* k_pages, const int64_t k_page_strides[3], const void* v_pages,
+                     const int64_t v_page_strides[3], int64_t pages, int64_t page_size,
+                     const int32_t* table, int64_t table_stride, int64_t table_width,
+                     const int32_t* lengths, const int32_t* starts, void* k, void* v, void* stream) {
+  const char* who = "paged_read";
+  if (!known(dtype) || !(known(cache_dtype) || cache_dtype == FATTN_FP4)) {
+    return set_error(FATTN_EINVAL, "%s: f32, f16 or bf16 only", who);
+  }
+  if (b < 0 || s < 0) return set_error(FATTN_EINVAL, "%s: negative size", who);
+  if (kv_heads < 0 || kv_heads > kMaxHeads) {
+    return set_error(FATTN_ERANGE, "%s: at most %lld heads", who, static_cast<long long>(kMaxHeads));
+  }
+  if (int rc = check_dim(who, d)) return rc;
+  if (b == 0 || s == 0 || kv_heads == 0) return fattn::done();
+  fattn::PagedReadArgs a{};
+  if (int rc = check_cache(who, cache_dtype, k_pages, k_page_strides, v_pages, v_page_strides, pages,
+                           kv_heads, page_size, table, table_stride, table_width, lengths, a.ks, a.vs)) {
+    return rc;
+  }
+  if (!k || !v) return set_error(FATTN_EINVAL, "%s: null operand", who);
+  if (!aligned(k, 16) || !aligned(v, 16)) {
+    return set_error(FATTN_EALIGN, "%s: rows must be 16-byte aligned", who);
+  }
+  if (b > kMaxGrid || s > (int64_t{1} << 26) ||
+      b * kv_heads > kMaxGrid / fattn::paged_read_blocks(s, d)) {
+    return set_error(FATTN_ERANGE, "%s: the sizes exceed 32-bit indexing or the launch limit", who);
+  }
+  a.k_pages = k_pages, a.v_pages = v_pages, a.k = k, a.v = v;
+  a.table = table, a.lengths = lengths, a.starts = starts, a.table_stride = table_stride;
+  a.table_width = static_cast<int>(table_width), a.pages = static_cast<int>(pages);
+  a.page_size = static_cast<int>(page_size);
+  a.B = static_cast<int>(b), a.HK = static_cast<int>(kv_heads), a.S = static_cast<int>(s);
+  const int err = fattn::launch_paged_read(a, cache_dtype, dtype, static_cast<int>(d), stream);
+  if (err) return fattn::hip_error(err, who, "launch");
+  return fattn::done();
 }
 
 size_t fattn_cross_workspace_bytes(int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk,

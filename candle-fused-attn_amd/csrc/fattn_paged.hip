@@ -25,7 +25,9 @@
 // three, bf16, us: those contexts, d 128, 279.4 / 279.9; 64 sequences of 1 to 2048, d 64, 27.1 / 27.5.)
 // Over f16 values the weights stay fp32 and the values are widened: f16 terms of a weight
 // would end at 2^-24 of the largest one's size, and a key of all the weight but no value (an attention
-// sink) would take the bits of all the others.
+// sink) would take the bits of all the others. A 4-bit cache's values, two bits of significand times a power
+// of two, are bf16 values: an instruction makes two of them from their codes and scale where they are
+// multiplied, and the rest is as over bf16.
 //
 // Work: the sequences' 32-key tiles, end to end, are dealt in equal runs to a fixed number of
 // workgroups, whatever the lengths; a workgroup's run crosses heads and sequences. Where a run ends
@@ -163,26 +165,56 @@ __device__ __forceinline__ void put4(Q* p, f4 x) {
   *reinterpret_cast<q4*>(p) = y;
 }
 
-// The registers of one wave: a tile's keys and values, the rows, the sums.
-template <typename Q, typename C, int D>
+// Codes 2 i and 2 i + 1 of a word of eight, as bf16 of a scale 2^(byte - 127) (255: NaN).
+// (i: known once its loop is unrolled.)
+__device__ __forceinline__ unsigned four_pair(unsigned word, int i, float scale) {
+  const auto x = i == 0   ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 0)
+                 : i == 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 1)
+                 : i == 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 2)
+                          : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 3);
+  return __builtin_bit_cast(unsigned, x);
+}
+__device__ __forceinline__ float four_scale(unsigned byte) { return __uint_as_float(byte << 23); }
+
+// The registers of one wave: a tile's keys and values, the rows, the sums. kMods: scores capped, or less a
+// slope times the distance.
+template <typename Q, typename C, int D, bool kMods>
 struct Wave {
+  static constexpr bool kFour = std::is_same<C, four>::value;
+  typedef std::conditional_t<kFour, __bf16, C> M;  // what is multiplied
   static constexpr bool kF32 = std::is_same<C, float>::value;
   static constexpr int kC = kF32 ? (D == 32 ? 2 : 4) : D / 16;  // head_dims of V per load
   static constexpr int kBlocks = D / (16 * kC);                 // loads of a V row
   static constexpr int kKLoads = kF32 ? D / 16 : D / 32;        // loads of a K row, 16 bytes a lane
+  // (4 bits: one load of D / 32 words, and the scale: lane g has the row's g-th quarter.)
   static constexpr int kVWords = kF32 ? kC : kC / 2;
   static constexpr int kAcc = D / 16;
   // Terms of the queries and of the weights (1: as they are).
-  static constexpr bool kSame = std::is_same<Q, C>::value;
-  static constexpr int kQT = kF32 || kSame ? 1 : std::is_same<C, __bf16>::value ? 3 : 2;
+  static constexpr bool kSame = std::is_same<Q, M>::value;
+  // (f16 queries over bf16 keys: two bf16 hold their 11 bits.)
+  static constexpr int kQT = kF32 || kSame                                                     ? 1
+                             : std::is_same<M, __bf16>::value && std::is_same<Q, float>::value ? 3
+                                                                                               : 2;
   static constexpr int kPT = 3;  // (bf16)
 
-  u4 k[2][kKLoads];
-  unsigned v[2][4][kBlocks][kVWords];
+  struct Raw {
+    u4 k[2][kKLoads];
+    unsigned v[2][4][kBlocks][kVWords];
+  };
+  struct Raw4 {
+    unsigned k[2][kKLoads], k_scale[2], v[2][4], v_scale[2][4];
+  };
+  std::conditional_t<kFour, Raw4, Raw> raw;
   u4 q[kQT][kKLoads];
   f4 o[kAcc];  // register r of o[kC T + n]: head_dim 16 kC T + kC (4 g + r) + n of row j
   float c2;    // scale log2 e over the row's scale
   float m, l;
+  float slope2;  // (kMods) the row's slope times log2 e
+
+  // The first head_dim of the eight that lane g has in contraction step i.
+  static __device__ __forceinline__ int step_dim(int i, int g) {
+    return kFour ? D / 4 * g + 8 * i : 32 * i + 8 * g;
+  }
 
   __device__ __forceinline__ void load_q(const Q* row, float scale, int g) {
     c2 = scale * kLog2e;
@@ -191,19 +223,25 @@ struct Wave {
       for (int i = 0; i < kKLoads; ++i) q[0][i] = *reinterpret_cast<const u4*>(row + 16 * i + 4 * g);
     } else if constexpr (kSame) {
 #pragma unroll
-      for (int i = 0; i < kKLoads; ++i) q[0][i] = *reinterpret_cast<const u4*>(row + 32 * i + 8 * g);
+      for (int i = 0; i < kKLoads; ++i) q[0][i] = *reinterpret_cast<const u4*>(row + step_dim(i, g));
     } else {
       f4 x[kKLoads][2];
       float top = 0.0f;
 #pragma unroll
       for (int i = 0; i < kKLoads; ++i) {
-        x[i][0] = ld4(row + 32 * i + 8 * g);
-        x[i][1] = ld4(row + 32 * i + 8 * g + 4);
+        if constexpr (std::is_same<Q, float>::value) {
+          x[i][0] = ld4(row + step_dim(i, g));
+          x[i][1] = ld4(row + step_dim(i, g) + 4);
+        } else {
+          const h8 y = *reinterpret_cast<const h8*>(row + step_dim(i, g));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[i][e / 4][e % 4] = static_cast<float>(y[e]);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[i][e / 4][e % 4]));
       }
       float sc = 1.0f;
-      if constexpr (std::is_same<C, _Float16>::value) {
+      if constexpr (std::is_same<M, _Float16>::value) {
         // The row's largest magnitude at 2^13: 22 bits of each value down to 2^-17 of it.
         const int e = min(max(static_cast<int>(__float_as_uint(row_max(top)) >> 23) - 127, -113), 126);
         sc = __int_as_float((13 - e + 127) << 23);
@@ -214,7 +252,7 @@ struct Wave {
         unsigned w[4][kQT];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          terms2(x[i][e / 2][2 * (e % 2)] * sc, x[i][e / 2][2 * (e % 2) + 1] * sc, w[e], C{});
+          terms2(x[i][e / 2][2 * (e % 2)] * sc, x[i][e / 2][2 * (e % 2) + 1] * sc, w[e], M{});
         }
 #pragma unroll
         for (int t = 0; t < kQT; ++t) q[t][i] = u4{w[0][t], w[1][t], w[2][t], w[3][t]};
@@ -230,30 +268,68 @@ struct Wave {
   // offset of the lane); `live` of its 16 keys are there (the others repeat the last).
   __device__ __forceinline__ void load_k(int h, const C* p, unsigned ss, int live, int j, int g) {
     const char* base = reinterpret_cast<const char*>(p);
-    const unsigned at = static_cast<unsigned>(min(j, live - 1)) * ss + 16u * g;
+    const unsigned row = static_cast<unsigned>(min(j, live - 1)) * ss;
+    if constexpr (kFour) {
+      struct alignas(4) Words {
+        unsigned w[kKLoads];
+      };
+      const Words x = *reinterpret_cast<const Words*>(base + (row + static_cast<unsigned>(D / 8) * g));
 #pragma unroll
-    for (int i = 0; i < kKLoads; ++i) k[h][i] = *reinterpret_cast<const u4*>(base + (at + 64u * i));
+      for (int i = 0; i < kKLoads; ++i) raw.k[h][i] = x.w[i];
+      raw.k_scale[h] = *reinterpret_cast<const unsigned char*>(base + (row + D / 2 + D / 4 * g / 32));
+    } else {
+      const unsigned at = row + 16u * g;
+#pragma unroll
+      for (int i = 0; i < kKLoads; ++i) raw.k[h][i] = *reinterpret_cast<const u4*>(base + (at + 64u * i));
+    }
   }
   __device__ __forceinline__ void load_v(int h, const C* p, unsigned ss, int live, int j, int g) {
     const char* base = reinterpret_cast<const char*>(p);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const unsigned at =
-          static_cast<unsigned>(min(4 * g + r, live - 1)) * ss + static_cast<unsigned>(kC * sizeof(C)) * j;
+      const unsigned first = static_cast<unsigned>(min(4 * g + r, live - 1)) * ss;
+      if constexpr (kFour) {
+        typedef std::conditional_t<kC == 8, unsigned, std::conditional_t<kC == 4, unsigned short, unsigned char>>
+            Codes;
+        raw.v[h][r] = *reinterpret_cast<const Codes*>(base + (first + static_cast<unsigned>(kC / 2) * j));
+        raw.v_scale[h][r] =
+            *reinterpret_cast<const unsigned char*>(base + (first + D / 2 + static_cast<unsigned>(kC) * j / 32));
+        continue;
+      } else {
+        const unsigned at = first + static_cast<unsigned>(kC * sizeof(C)) * j;
 #pragma unroll
-      for (int t = 0; t < kBlocks; ++t) {
-        const char* row = base + (at + static_cast<unsigned>(16 * kC * sizeof(C)) * t);
-        if constexpr (kVWords == 4) {
-          const u4 x = *reinterpret_cast<const u4*>(row);
+        for (int t = 0; t < kBlocks; ++t) {
+          const char* row = base + (at + static_cast<unsigned>(16 * kC * sizeof(C)) * t);
+          if constexpr (kVWords == 4) {
+            const u4 x = *reinterpret_cast<const u4*>(row);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[h][r][t][i] = x[i];
-        } else if constexpr (kVWords == 2) {
-          const u2 x = *reinterpret_cast<const u2*>(row);
-          v[h][r][t][0] = x[0], v[h][r][t][1] = x[1];
-        } else {
-          v[h][r][t][0] = *reinterpret_cast<const unsigned*>(row);
+            for (int i = 0; i < 4; ++i) raw.v[h][r][t][i] = x[i];
+          } else if constexpr (kVWords == 2) {
+            const u2 x = *reinterpret_cast<const u2*>(row);
+            raw.v[h][r][t][0] = x[0], raw.v[h][r][t][1] = x[1];
+          } else {
+            raw.v[h][r][t][0] = *reinterpret_cast<const unsigned*>(row);
+          }
         }
       }
+    }
+  }
+  // Half h's operand of contraction step i.
+  __device__ __forceinline__ u4 key_step(int h, int i) const {
+    if constexpr (kFour) {
+      const float sc = four_scale(raw.k_scale[h]);
+      const unsigned w = raw.k[h][i];
+      return u4{four_pair(w, 0, sc), four_pair(w, 1, sc), four_pair(w, 2, sc), four_pair(w, 3, sc)};
+    } else {
+      return raw.k[h][i];
+    }
+  }
+  // Head_dims 2 i and 2 i + 1 (16-bit values), of the lane's, of key 16 h + 4 g + r.
+  __device__ __forceinline__ unsigned value_pair(int h, int r, int i) const {
+    if constexpr (kFour) {
+      return four_pair(raw.v[h][r], i, four_scale(raw.v_scale[h][r]));
+    } else {
+      return raw.v[h][r][0][i];
     }
   }
   __device__ __forceinline__ void scores(f4 (&s)[2]) const {
@@ -265,7 +341,7 @@ struct Wave {
         for (int e = 0; e < 4; ++e) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            s[h] = mma_f32(__uint_as_float(k[h][i][e]), __uint_as_float(q[0][i][e]), s[h]);
+            s[h] = mma_f32(__uint_as_float(raw.k[h][i][e]), __uint_as_float(q[0][i][e]), s[h]);
           }
         }
       }
@@ -275,19 +351,25 @@ struct Wave {
 #pragma unroll
         for (int i = 0; i < kKLoads; ++i) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) s[h] = mma_16(k[h][i], q[t][i], s[h], C{});
+          for (int h = 0; h < 2; ++h) s[h] = mma_16(key_step(h, i), q[t][i], s[h], M{});
         }
       }
     }
   }
-  // Weights from scores, `live` keys of the tile.
-  __device__ __forceinline__ void weights(f4 (&s)[2], int live, int g) {
+  // Weights from scores, `live` keys of the tile (the last of them, over a page table, the query's own).
+  __device__ __forceinline__ void weights(f4 (&s)[2], int live, int g, float cap2, float cap_inv) {
     float top = kNegInf;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        s[h][r] = 16 * h + 4 * g + r < live ? s[h][r] * c2 : kNegInf;
+        float x = s[h][r] * c2;
+        if constexpr (kMods) {
+          float d;
+          if (cap2 != 0.0f) x = cap2 * tanh_any(x * cap_inv, d);
+          x = fmaf(-slope2, static_cast<float>(live - 1 - 16 * h - 4 * g - r), x);
+        }
+        s[h][r] = 16 * h + 4 * g + r < live ? x : kNegInf;
         top = fmaxf(top, s[h][r]);
       }
     }
@@ -318,10 +400,14 @@ struct Wave {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           if (16 * h + 4 * g + r >= live) {
+            if constexpr (kFour) {
+              raw.v[h][r] = raw.v_scale[h][r] = 0;
+            } else {
 #pragma unroll
-            for (int t = 0; t < kBlocks; ++t) {
+              for (int t = 0; t < kBlocks; ++t) {
 #pragma unroll
-              for (int i = 0; i < kVWords; ++i) v[h][r][t][i] = 0;
+                for (int i = 0; i < kVWords; ++i) raw.v[h][r][t][i] = 0;
+              }
             }
           }
         }
@@ -336,19 +422,19 @@ struct Wave {
           for (int t = 0; t < kBlocks; ++t) {
 #pragma unroll
             for (int n = 0; n < kC; ++n) {
-              o[kC * t + n] = mma_f32(__uint_as_float(v[h][r][t][n]), p[h][r], o[kC * t + n]);
+              o[kC * t + n] = mma_f32(__uint_as_float(raw.v[h][r][t][n]), p[h][r], o[kC * t + n]);
             }
           }
         }
       }
-    } else if constexpr (std::is_same<C, _Float16>::value) {
+    } else if constexpr (std::is_same<M, _Float16>::value) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
 #pragma unroll
           for (int i = 0; i < kVWords; ++i) {
-            const h2 x = __builtin_bit_cast(h2, v[h][r][0][i]);
+            const h2 x = __builtin_bit_cast(h2, raw.v[h][r][0][i]);
             o[2 * i] = mma_f32(static_cast<float>(x.x), p[h][r], o[2 * i]);
             o[2 * i + 1] = mma_f32(static_cast<float>(x.y), p[h][r], o[2 * i + 1]);
           }
@@ -358,7 +444,7 @@ struct Wave {
       u4 b[kPT];
       unsigned w[4][kPT];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) terms2(p[e / 2][2 * (e % 2)], p[e / 2][2 * (e % 2) + 1], w[e], C{});
+      for (int e = 0; e < 4; ++e) terms2(p[e / 2][2 * (e % 2)], p[e / 2][2 * (e % 2) + 1], w[e], M{});
 #pragma unroll
       for (int t = 0; t < kPT; ++t) b[t] = u4{w[0][t], w[1][t], w[2][t], w[3][t]};
 #pragma unroll
@@ -367,14 +453,14 @@ struct Wave {
         u4 lo, hi;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const unsigned x = v[e / 2][2 * (e % 2)][0][i], y = v[e / 2][2 * (e % 2) + 1][0][i];
+          const unsigned x = value_pair(e / 2, 2 * (e % 2), i), y = value_pair(e / 2, 2 * (e % 2) + 1, i);
           lo[e] = __builtin_amdgcn_perm(y, x, 0x05040100u);
           hi[e] = __builtin_amdgcn_perm(y, x, 0x07060302u);
         }
 #pragma unroll
         for (int t = kPT - 1; t >= 0; --t) {
-          o[2 * i] = mma_16(lo, b[t], o[2 * i], C{});
-          o[2 * i + 1] = mma_16(hi, b[t], o[2 * i + 1], C{});
+          o[2 * i] = mma_16(lo, b[t], o[2 * i], M{});
+          o[2 * i + 1] = mma_16(hi, b[t], o[2 * i + 1], M{});
         }
       }
     }
@@ -384,17 +470,18 @@ struct Wave {
 // Waves per SIMD (so workgroups per CU) that the registers allow.
 template <typename Q, typename C, int D>
 constexpr int kOccupancy = D == 32    ? 4
+                           : std::is_same<C, four>::value ? (std::is_same<Q, float>::value ? (D == 64 ? 3 : 2) : D == 64 ? 4 : 3)
                            : D == 128 ? 2
                            : std::is_same<C, _Float16>::value || (std::is_same<C, __bf16>::value &&
                                                                   std::is_same<Q, C>::value)
                                ? 4
                                : 3;
 
-template <typename Q, typename C, int D, bool kPaged>
+template <typename Q, typename C, int D, bool kPaged, bool kMods>
 __global__ void __launch_bounds__(64 * kSplitWaves)
     __attribute__((amdgpu_waves_per_eu(kOccupancy<Q, C, D>, kOccupancy<Q, C, D>)))
 split_kernel(SplitArgs a) {
-  typedef Wave<Q, C, D> W;
+  typedef Wave<Q, C, D, kMods> W;
   constexpr int kPitch = D + 4;
   __shared__ __attribute__((aligned(16))) float so[kSplitWaves][kRowsMax][kPitch];
   __shared__ float sml[kSplitWaves][2][kRowsMax];
@@ -487,6 +574,7 @@ split_kernel(SplitArgs a) {
       int head, i;
       row_of(a, kvh, r0 + min(j, rows - 1), head, i);
       x.load_q(static_cast<const Q*>(a.q) + b * a.qs[0] + head * a.qs[1] + i * a.qs[2], a.scale, g);
+      if constexpr (kMods) x.slope2 = a.slopes != nullptr ? a.slopes[head] * kLog2e : 0.0f;
     }
     const C* kp = static_cast<const C*>(a.k) + kvh * a.ks[1];
     const C* vp = static_cast<const C*>(a.v) + kvh * a.vs[1];
@@ -541,7 +629,7 @@ split_kernel(SplitArgs a) {
           x.load_k(h, at[h].k, kss, at[h].live, j, g);
         }
       }
-      x.weights(s, live, g);
+      x.weights(s, live, g, a.cap2, a.cap_inv);
       x.sums(s, live, g);
       if (more) {
 #pragma unroll
@@ -688,14 +776,14 @@ __global__ void __launch_bounds__(256) join_kernel(SplitArgs a) {
   if (tid == 0) put_lse(a, b, head, q, mm, l);
 }
 
-template <typename Q, typename C, int D, bool kPaged>
+template <typename Q, typename C, int D, bool kPaged, bool kMods>
 int run_split(const SplitArgs& a, hipStream_t stream) {
   const int64_t pairs = static_cast<int64_t>(a.B) * a.HK * a.RB;
   SplitArgs args = a;
   if (args.wgs > 0) args.wgs = 256 * kOccupancy<Q, C, D>;
   void* kargs[] = {&args};
   const unsigned grid = static_cast<unsigned>(args.wgs == 0 ? pairs : args.wgs);
-  hipError_t err = hipLaunchKernel(reinterpret_cast<const void*>(split_kernel<Q, C, D, kPaged>),
+  hipError_t err = hipLaunchKernel(reinterpret_cast<const void*>(split_kernel<Q, C, D, kPaged, kMods>),
                                    dim3(grid), dim3(64 * kSplitWaves), kargs, 0, stream);
   if (err != hipSuccess || a.wgs == 0) return static_cast<int>(err);
   const unsigned rows = static_cast<unsigned>(static_cast<int64_t>(a.B) * a.H * a.SQ);
@@ -703,11 +791,24 @@ int run_split(const SplitArgs& a, hipStream_t stream) {
                                           dim3(rows), dim3(256), kargs, 0, stream));
 }
 
-template <typename Q, typename C, bool kPaged>
+template <typename Q, typename C, bool kPaged, bool kMods>
 int by_dim(const SplitArgs& a, int d, hipStream_t s) {
-  return d == 32   ? run_split<Q, C, 32, kPaged>(a, s)
-         : d == 64 ? run_split<Q, C, 64, kPaged>(a, s)
-                   : run_split<Q, C, 128, kPaged>(a, s);
+  return d == 32   ? run_split<Q, C, 32, kPaged, kMods>(a, s)
+         : d == 64 ? run_split<Q, C, 64, kPaged, kMods>(a, s)
+                   : run_split<Q, C, 128, kPaged, kMods>(a, s);
+}
+template <bool kMods>
+int by_type(const SplitArgs& a, int dtype, int cache_dtype, int d, hipStream_t s) {
+  if (cache_dtype == kFP4) {
+    return dtype == kF16    ? by_dim<_Float16, four, true, kMods>(a, d, s)
+           : dtype == kBF16 ? by_dim<__bf16, four, true, kMods>(a, d, s)
+                            : by_dim<float, four, true, kMods>(a, d, s);
+  }
+  if (dtype == kF16) return by_dim<_Float16, _Float16, true, kMods>(a, d, s);
+  if (dtype == kBF16) return by_dim<__bf16, __bf16, true, kMods>(a, d, s);
+  return cache_dtype == kF16    ? by_dim<float, _Float16, true, kMods>(a, d, s)
+         : cache_dtype == kBF16 ? by_dim<float, __bf16, true, kMods>(a, d, s)
+                                : by_dim<float, float, true, kMods>(a, d, s);
 }
 
 }  // namespace
@@ -734,12 +835,9 @@ SplitPlan split_plan(int64_t b, int64_t hk, int64_t rows, int64_t d, int64_t cap
 
 int launch_split(const SplitArgs& a, int dtype, int cache_dtype, int d, void* stream) {
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a.table == nullptr) return by_dim<float, float, false>(a, d, s);
-  if (dtype == kF16) return by_dim<_Float16, _Float16, true>(a, d, s);
-  if (dtype == kBF16) return by_dim<__bf16, __bf16, true>(a, d, s);
-  return cache_dtype == kF16    ? by_dim<float, _Float16, true>(a, d, s)
-         : cache_dtype == kBF16 ? by_dim<float, __bf16, true>(a, d, s)
-                                : by_dim<float, float, true>(a, d, s);
+  if (a.table == nullptr) return by_dim<float, float, false, false>(a, d, s);
+  return a.slopes != nullptr || a.cap2 != 0.0f ? by_type<true>(a, dtype, cache_dtype, d, s)
+                                               : by_type<false>(a, dtype, cache_dtype, d, s);
 }
 
 }  // namespace fattn

@@ -201,6 +201,338 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotaryArgs a) {
   }
 }
 
+// --- The append to a 4-bit cache ---------------------------------------------------------------------
+// 32 values share a scale 2^e, e the least with none of them past 7 2^e (so 6, the largest magnitude, is the
+// nearest to each that passes it), and are stored as the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6, the even code
+// where two are as near: what the conversion instruction gives, times 2^-e. Which code is nearest is decided
+// by the exact value: of a rotated key by its value in 64 bits (its angle p f rounded once, reduced in two
+// terms of pi / 2), brought to 32 bits by rounding to odd, so that no second rounding moves a value across
+// the border between two codes, and a token has the same codes on whatever path it came.
+//
+// Bound: memory, and for few tokens the launch. A thread has 8 values, so that four neighbours share a scale
+// and a head's scales are one word; the values that a rotation pairs with them are read by the neighbours too.
+
+// cos and sin of the angle p f (rounded once), times the magnitude, in 64 bits: less q quarter turns, |y| <=
+// pi / 4, where the Taylor series to y^17 and y^16 are exact to 1e-17.
+__device__ __forceinline__ double2 turn64(double p, double f, double magnitude) {
+  const double a = p * f, q = rint(a * 0.63661977236758134308);
+  const double y = fma(q, -6.123233995736766036e-17, fma(q, -1.57079632679489661923, a)), z = y * y;
+  double s = 1.0 / 355687428096000.0, c = 1.0 / 20922789888000.0;
+  s = fma(s, z, -1.0 / 1307674368000.0), c = fma(c, z, -1.0 / 87178291200.0);
+  s = fma(s, z, 1.0 / 6227020800.0), c = fma(c, z, 1.0 / 479001600.0);
+  s = fma(s, z, -1.0 / 39916800.0), c = fma(c, z, -1.0 / 3628800.0);
+  s = fma(s, z, 1.0 / 362880.0), c = fma(c, z, 1.0 / 40320.0);
+  s = fma(s, z, -1.0 / 5040.0), c = fma(c, z, -1.0 / 720.0);
+  s = fma(s, z, 1.0 / 120.0), c = fma(c, z, 1.0 / 24.0);
+  s = fma(s, z, -1.0 / 6.0), c = fma(c, z, -0.5);
+  s = fma(s * z, y, y), c = fma(c, z, 1.0);
+  const int k = static_cast<int>(q - 4.0 * floor(0.25 * q));
+  const double cc = (k & 1) ? s : c, ss = (k & 1) ? c : s;
+  return double2{((k == 1 || k == 2) ? -cc : cc) * magnitude, (k >= 2 ? -ss : ss) * magnitude};
+}
+// x in 32 bits, rounded to odd: where it is not exact, towards 0 and with the last bit set.
+__device__ __forceinline__ float to_odd(double x) {
+  const float r = static_cast<float>(x);
+  const double back = static_cast<double>(r);
+  if (!(back != x) || x != x) return r;
+  const unsigned u = __float_as_uint(r) - (fabs(back) > fabs(x) ? 1u : 0u);
+  return __uint_as_float(u | 1u);
+}
+// Eight values, of a group of 32 that four neighbouring lanes have: their codes, and the group's scale byte.
+__device__ __forceinline__ unsigned codes_of(const float (&x)[8], unsigned& scale) {
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  top = max(top, static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0xB1, 0xF, 0xF, true)));
+  top = max(top, static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0x4E, 0xF, 0xF, true)));
+  // (1.m 2^E <= 7 2^(E - 2) up to 1.75.)
+  const int e = static_cast<int>(top >> 23) - 2 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+  const bool finite = top < 0x7f800000u;
+  scale = finite ? static_cast<unsigned>(max(e, 0)) : 255u;
+  const float s = __uint_as_float(scale << 23);
+  unsigned w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
+  // No negative zeros: a token has one code for 0.
+  const unsigned some = (w | w >> 1 | w >> 2) & 0x11111111u;
+  w &= 0x77777777u | some << 3;
+  return finite ? w : 0u;
+}
+
+constexpr int kMaxAngles64 = 1024;
+
+// As rotary_kernel, an item 8 values of a head: of part 0 (q) written turned, of parts 1 and 2 as codes.
+// kWide: an operand's values are moved 8 at a time.
+template <typename T, bool kWide, bool kInterleaved>
+__global__ void __launch_bounds__(kRotThreads) append_four_kernel(RotaryArgs a) {
+  __shared__ double2 cs[kMaxAngles64];
+  __shared__ int64_t at_of[kMaxTokens];
+  __shared__ int pos_of[kMaxTokens];
+  const int tid = threadIdx.x, n = a.pairs, D = a.D;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens, all = static_cast<int64_t>(a.B) * a.S;
+  const int nt = static_cast<int>(all - t0 < a.tokens ? all - t0 : a.tokens);
+  const int y = static_cast<int>(blockIdx.y);
+  const int pi = y < a.first_share[1] ? 0 : y < a.first_share[2] ? 1 : 2;
+  const RotaryPart& part = a.part[pi];
+  const bool turns = part.rotate != 0 && n > 0;
+  const int of = a.items[pi], per = of * part.heads, items = nt * per;
+  const int shares = a.first_share[pi + 1] - a.first_share[pi];
+  const int share = (items / of + shares - 1) / shares * of;  // (whole heads)
+  const int first = (y - a.first_share[pi]) * share;
+  const int last = first + share < items ? first + share : items;
+  constexpr int kInFlight = 2;
+
+  struct Item {
+    T x[8], z[8];  // the values, and those that they turn with
+    int64_t to;
+    int t, e, head, low;  // token, first value (-1: no item), head; low: (half layout) the first of the pairs
+  };
+  Item it[kInFlight];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const int item = base + u * kRotThreads;
+      it[u].e = -1;
+      if (item >= last) continue;
+      const int t = divide(item, a.by_per[pi]);
+      const int r = item - t * per, head = divide(r, a.by_items[pi]), e = 8 * (r - head * of);
+      const int tok = static_cast<int>(t0) + t, b = divide(tok, a.by_seq), i = tok - b * a.S;
+      it[u].t = t, it[u].e = e, it[u].head = head;
+      it[u].to = pi == 0 ? b * part.ys[0] + head * part.ys[1] + i * part.ys[2] : 0;
+      const T* row = static_cast<const T*>(part.x) + b * part.xs[0] + head * part.xs[1] + i * part.xs[2];
+      if constexpr (kWide) {
+        typedef Vec<T, 16 / sizeof(T)> In;
+        constexpr int kIn = 16 / sizeof(T);
+#pragma unroll
+        for (int k = 0; k < 8; k += kIn) {
+          const In x = *reinterpret_cast<const In*>(row + e + k);
+#pragma unroll
+          for (int c = 0; c < kIn; ++c) it[u].x[k + c] = x.v[c];
+        }
+        if (!kInterleaved && turns && e < 2 * n) {
+          const T* other = row + (e < n ? e + n : e - n);
+#pragma unroll
+          for (int k = 0; k < 8; k += kIn) {
+            const In x = *reinterpret_cast<const In*>(other + k);
+#pragma unroll
+            for (int c = 0; c < kIn; ++c) it[u].z[k + c] = x.v[c];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int c = e + k;
+          it[u].x[k] = row[c];
+          if (!kInterleaved && turns && c < 2 * n) it[u].z[k] = row[c < n ? c + n : c - n];
+        }
+      }
+    }
+  };
+  load(first + tid);
+
+  if (tid < nt) {
+    const int tok = static_cast<int>(t0) + tid, b = divide(tok, a.by_seq), i = tok - b * a.S;
+    const int held = a.lengths[b];
+    const int64_t p = static_cast<int64_t>(held) + i;
+    // (As in rotary_kernel.)
+    int64_t page = -1;
+    const bool counted = a.counts == nullptr || i < a.counts[b];
+    if (counted && held >= 0 && p / a.page_size < a.table_width) {
+      page = a.table[b * a.table_stride + p / a.page_size];
+    }
+    const int64_t* st = a.page_strides + (pi == 2 ? 3 : 0);
+    at_of[tid] = page >= 0 && page < a.pages ? page * st[0] + p % a.page_size * st[2] : -1;
+    pos_of[tid] = held;
+  }
+  __syncthreads();
+  // Angles: q's in 32 bits, as fused_rotary's.
+  float2* cs32 = reinterpret_cast<float2*>(cs);
+  if (turns) {
+    for (int i = tid; i < nt * n; i += kRotThreads) {
+      const int t = divide(i, a.by_pairs);
+      const int tok = static_cast<int>(t0) + t, b = divide(tok, a.by_seq);
+      const double p = static_cast<double>(static_cast<int64_t>(pos_of[t]) + (tok - b * a.S));
+      const double f = a.frequencies[i - t * n];
+      if (pi == 0) {
+        cs32[i] = turn(p, f, a.magnitude);
+      } else {
+        cs[i] = turn64(p, f, a.magnitude);
+      }
+    }
+    __syncthreads();
+  }
+
+  // fn(k, value, its partner, whether it is the first of the pair, its pair) of an item's turned values.
+  auto each = [&](const Item& x, auto turned_value, auto plain_value) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int c = x.e + k;
+      if (!turns || c >= 2 * n) {
+        plain_value(k);
+      } else if (kInterleaved) {
+        turned_value(k, x.x[k], x.x[k ^ 1], (k & 1) == 0, x.t * n + c / 2);
+      } else {
+        turned_value(k, x.x[k], x.z[k], c < n, x.t * n + (c < n ? c : c - n));
+      }
+    }
+  };
+  for (int base = first + tid; base < last; base += kRotThreads * kInFlight) {
+    if (base != first + tid) load(base);
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const Item& x = it[u];
+      if (x.e < 0) continue;
+      if (pi == 0) {
+        T out[8];
+        each(
+            x,
+            [&](int k, T v, T o, bool low, int at) {
+              const float2 w = cs32[at];
+              const float fv = static_cast<float>(v), fo = static_cast<float>(o);
+              out[k] = static_cast<T>(turned(fv, w.x, low ? -(fo * w.y) : fo * w.y));
+            },
+            [&](int k) { out[k] = x.x[k]; });
+        T* to = static_cast<T*>(part.y) + x.to + x.e;
+        if constexpr (kWide) {
+          constexpr int kOut = 16 / sizeof(T);
+#pragma unroll
+          for (int k = 0; k < 8; k += kOut) {
+            Vec<T, kOut> v;
+#pragma unroll
+            for (int c = 0; c < kOut; ++c) v.v[c] = out[k + c];
+            *reinterpret_cast<Vec<T, kOut>*>(to + k) = v;
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) to[k] = out[k];
+        }
+      } else {
+        float v[8];
+        each(
+            x,
+            [&](int k, T p, T o, bool low, int at) {
+              const double2 w = cs[at];
+              const double dp = static_cast<double>(static_cast<float>(p));
+              const double dq = static_cast<double>(static_cast<float>(o)) * w.y;
+              v[k] = to_odd(fma(dp, w.x, low ? -dq : dq));
+            },
+            [&](int k) { v[k] = static_cast<float>(x.x[k]); });
+        unsigned scale;
+        const unsigned codes = codes_of(v, scale);
+        // The head's scale bytes, in order, from its groups' lanes.
+        unsigned word = scale << (x.e / 32 * 8);
+        if (D >= 64) word |= static_cast<unsigned>(__shfl_xor(static_cast<int>(word), 4));
+        if (D == 128) word |= static_cast<unsigned>(__shfl_xor(static_cast<int>(word), 8));
+        const int64_t at = at_of[x.t];
+        if (at >= 0) {
+          unsigned char* row = static_cast<unsigned char*>(part.y) + at + x.head * a.page_strides[pi == 2 ? 4 : 1];
+          *reinterpret_cast<unsigned*>(row + x.e / 2) = codes;
+          if (x.e == 0) *reinterpret_cast<unsigned*>(row + D / 2) = word;
+        }
+      }
+    }
+  }
+}
+
+// --- Tokens back out of a paged cache ------------------------------------------------------------------
+// Bound: memory, each row read and each result written once. A thread has 8 values of a token's head; the
+// results of one (sample, head) are contiguous, and those of neighbouring tokens lie in one page, so a wave
+// reads and writes whole rows one after the other.
+template <typename C, typename O, int D>
+__global__ void __launch_bounds__(256) read_kernel(PagedReadArgs a) {
+  constexpr int kOf = D / 8, kInFlight = 4;
+  const int pair = static_cast<int>(blockIdx.x) / a.blocks, in = static_cast<int>(blockIdx.x) - pair * a.blocks;
+  const int b = pair / a.HK, head = pair - b * a.HK, which = static_cast<int>(blockIdx.y);
+  const int64_t* st = which == 0 ? a.ks : a.vs;
+  const C* pages = static_cast<const C*>(which == 0 ? a.k_pages : a.v_pages) + head * st[1];
+  O* out = static_cast<O*>(which == 0 ? a.k : a.v) + static_cast<int64_t>(pair) * a.S * D;
+  const int len = a.lengths[b];
+  const int64_t start = a.starts != nullptr ? a.starts[b] : 0;
+  const int item0 = in * (256 * kInFlight) + static_cast<int>(threadIdx.x), items = a.S * kOf;
+  const C* row[kInFlight];  // (null: zeros; with `bad`: NaN)
+  bool bad[kInFlight];
+#pragma unroll
+  for (int u = 0; u < kInFlight; ++u) {
+    const int item = item0 + 256 * u;
+    row[u] = nullptr, bad[u] = false;
+    const int64_t t = start + item / kOf;
+    if (item >= items || t < 0 || t >= len) continue;
+    const int at = divide(static_cast<int>(t), a.by_page);
+    bad[u] = true;
+    if (at >= a.table_width) continue;
+    const int page = a.table[b * a.table_stride + at];
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pages)) continue;
+    bad[u] = false;
+    row[u] = pages + page * st[0] + (static_cast<int>(t) - at * a.page_size) * st[2];
+  }
+  struct alignas(16) Values {
+    C v[8];
+  };
+  struct Codes {
+    unsigned w, scale;
+  };
+  std::conditional_t<std::is_same<C, four>::value, Codes, Values> x[kInFlight];
+#pragma unroll
+  for (int u = 0; u < kInFlight; ++u) {
+    const int e = (item0 + 256 * u) % kOf * 8;
+    if (row[u] == nullptr) continue;
+    if constexpr (std::is_same<C, four>::value) {
+      const char* p = reinterpret_cast<const char*>(row[u]);
+      x[u].w = *reinterpret_cast<const unsigned*>(p + e / 2);
+      x[u].scale = *reinterpret_cast<const unsigned char*>(p + D / 2 + e / 32);
+    } else {
+      x[u] = *reinterpret_cast<const Values*>(row[u] + e);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kInFlight; ++u) {
+    const int item = item0 + 256 * u;
+    if (item >= items) continue;
+    struct alignas(16) Out {
+      O v[8];
+    } y;
+    if (row[u] == nullptr) {
+      const O z = static_cast<O>(bad[u] ? __builtin_nanf("") : 0.0f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y.v[k] = z;
+    } else if constexpr (std::is_same<C, four>::value) {
+      typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+      const float s = __uint_as_float(x[u].scale << 23);
+      const b2 p[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x[u].w, s, 0),
+                       __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x[u].w, s, 1),
+                       __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x[u].w, s, 2),
+                       __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x[u].w, s, 3)};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y.v[k] = convert<O, __bf16>(p[k / 2][k % 2]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y.v[k] = convert<O, C>(x[u].v[k]);
+    }
+    *reinterpret_cast<Out*>(out + static_cast<int64_t>(item) * 8) = y;
+  }
+}
+
+template <typename C, typename O>
+const void* read_fn(int d) {
+  return d == 32    ? reinterpret_cast<const void*>(read_kernel<C, O, 32>)
+         : d == 128 ? reinterpret_cast<const void*>(read_kernel<C, O, 128>)
+                    : reinterpret_cast<const void*>(read_kernel<C, O, 64>);
+}
+template <typename C>
+const void* read_fn(int dtype, int d) {
+  return dtype == kF16 ? read_fn<C, _Float16>(d) : dtype == kBF16 ? read_fn<C, __bf16>(d) : read_fn<C, float>(d);
+}
+
+template <typename T>
+const void* append_four_fn(bool wide, bool interleaved) {
+  return wide ? (interleaved ? reinterpret_cast<const void*>(append_four_kernel<T, true, true>)
+                             : reinterpret_cast<const void*>(append_four_kernel<T, true, false>))
+              : (interleaved ? reinterpret_cast<const void*>(append_four_kernel<T, false, true>)
+                             : reinterpret_cast<const void*>(append_four_kernel<T, false, false>));
+}
+
 template <typename T, typename C, bool kPaged>
 const void* rotary_fn(int vec, bool interleaved) {
   auto fn = [&](auto v) {
@@ -220,10 +552,16 @@ const void* rotary_fn(int vec, bool interleaved) {
 }  // namespace
 
 int launch_rotary(RotaryArgs a, int dtype, int cache_dtype, int vec, void* stream) {
-  const bool paged = a.table != nullptr;
+  const bool paged = a.table != nullptr, to_four = cache_dtype == kFP4;
   const void* fn = nullptr;
   const bool il = a.interleaved != 0;
-  if (!paged) {
+  if (to_four) {
+    const bool wide = vec == 8;
+    fn = dtype == kF32   ? append_four_fn<float>(wide, il)
+         : dtype == kF16 ? append_four_fn<_Float16>(wide, il)
+                         : append_four_fn<__bf16>(wide, il);
+    vec = 8;
+  } else if (!paged) {
     fn = dtype == kF32   ? rotary_fn<float, float, false>(vec, il)
          : dtype == kF16 ? rotary_fn<_Float16, _Float16, false>(vec, il)
                          : rotary_fn<__bf16, __bf16, false>(vec, il);
@@ -242,12 +580,12 @@ int launch_rotary(RotaryArgs a, int dtype, int cache_dtype, int vec, void* strea
   int64_t most = 1;
   for (int i = 0; i < 3; ++i) {
     const int turned = a.interleaved ? 2 * a.pairs / vec : a.pairs / vec;
-    a.items[i] = a.part[i].rotate ? turned + (a.D - 2 * a.pairs) / vec : a.D / vec;
+    a.items[i] = a.part[i].rotate && !to_four ? turned + (a.D - 2 * a.pairs) / vec : a.D / vec;
     most = std::max<int64_t>(most, static_cast<int64_t>(a.items[i]) * a.part[i].heads);
   }
   const int64_t fill = (kRotThreads + most - 1) / most;
   int64_t tokens = std::min(std::max(fill, all / 1024), std::max(fill, 2 * kUnroll * kRotThreads / most));
-  if (a.pairs > 0) tokens = std::min<int64_t>(tokens, kMaxAngles / a.pairs);
+  if (a.pairs > 0) tokens = std::min<int64_t>(tokens, (to_four ? kMaxAngles64 : kMaxAngles) / a.pairs);
   tokens = std::min<int64_t>(tokens, kMaxTokens);
   a.tokens = static_cast<int>(tokens);
   const int64_t blocks = (all + tokens - 1) / tokens;
@@ -266,5 +604,18 @@ int launch_rotary(RotaryArgs a, int dtype, int cache_dtype, int vec, void* strea
                                           dim3(kRotThreads), args, 0,
                                           static_cast<hipStream_t>(stream)));
 }
+
+int launch_paged_read(PagedReadArgs a, int cache_dtype, int dtype, int d, void* stream) {
+  const void* fn = cache_dtype == kF32    ? read_fn<float>(dtype, d)
+                   : cache_dtype == kF16  ? read_fn<_Float16>(dtype, d)
+                   : cache_dtype == kBF16 ? read_fn<__bf16>(dtype, d)
+                                          : read_fn<four>(dtype, d);
+  a.blocks = static_cast<int>(paged_read_blocks(a.S, d));
+  a.by_page = divider(a.page_size);
+  void* args[] = {&a};
+  return static_cast<int>(hipLaunchKernel(fn, dim3(static_cast<unsigned>(a.B) * a.HK * a.blocks, 2), dim3(256),
+                                          args, 0, static_cast<hipStream_t>(stream)));
+}
+int64_t paged_read_blocks(int64_t s, int64_t d) { return (s * (d / 8) + 1023) / 1024; }
 
 }  // namespace fattn

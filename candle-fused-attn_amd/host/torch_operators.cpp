@@ -7,7 +7,7 @@
 // Python a small training call takes 15 us more: fused_rotary and its gradient 77 us, 60 so, where an
 // elementwise product and its gradient take 52; fused_cross_attention 78, 62.
 //
-// Every entry takes its positional arguments from candle_fused_attn/{rotary,paged,cross}.py, whose
+// Every entry takes its positional arguments from candle_fused_attn/{rotary,paged,cross,scored}.py, whose
 // docstrings say what they mean. A refused argument raises the package's FusedAttentionError.
 #include <Python.h>
 
@@ -96,6 +96,7 @@ const char* name_of(ScalarType t) {
     case ScalarType::Double: return "float64";
     case ScalarType::Int: return "int32";
     case ScalarType::Long: return "int64";
+    case ScalarType::Byte: return "uint8";
     default: return c10::toString(t);
   }
 }
@@ -104,6 +105,7 @@ const char* name_of(ScalarType t) {
 typedef std::initializer_list<ScalarType> Types;
 constexpr ScalarType kF32 = ScalarType::Float, kF16 = ScalarType::Half, kBF16 = ScalarType::BFloat16;
 constexpr ScalarType kI32 = ScalarType::Int, kI64 = ScalarType::Long, kF64 = ScalarType::Double;
+constexpr ScalarType kFP4 = ScalarType::Byte;  // (of a cache: rows of 4-bit floats)
 
 // A tensor of `rank` dimensions on a HIP device (that of `like`), of one of `types`.
 void require(const char* who, const char* name, const Tensor& t, int64_t rank, const Tensor* like,
@@ -125,9 +127,10 @@ void require(const char* who, const char* name, const Tensor& t, int64_t rank, c
   throw OpError(what + " is on " + t.device().str() + ", the first operand on " + like->device().str());
 }
 
-int type_code(const Tensor& t) {
-  return t.scalar_type() == kF32 ? FATTN_F32 : t.scalar_type() == kF16 ? FATTN_F16 : FATTN_BF16;
+int type_code(ScalarType t) {
+  return t == kF32 ? FATTN_F32 : t == kF16 ? FATTN_F16 : t == kFP4 ? FATTN_FP4 : FATTN_BF16;
 }
+int type_code(const Tensor& t) { return type_code(t.scalar_type()); }
 // `t` itself where its last dimension is contiguous, else a contiguous copy.
 Tensor rows(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 // A four-dimensional `t` itself where its rows are contiguous and 16-byte aligned, else a contiguous copy.
@@ -347,11 +350,12 @@ Tensor fused_rotary_qkv(const Tensor& qkv, int64_t heads, const Tensor& position
 
 void check_cache(const char* who, const Tensor& x, const Tensor& kp, const Tensor& vp, const Tensor& table,
                  const Tensor& lengths, int64_t b, int64_t d) {
-  require(who, "k_pages", kp, 4, &x, {kF32, kF16, kBF16});
+  require(who, "k_pages", kp, 4, &x, {kF32, kF16, kBF16, kFP4});
   require(who, "v_pages", vp, 4, &x, {kp.scalar_type()});
-  if (vp.sizes() != kp.sizes() || kp.size(3) != d) {
+  const int64_t row = kp.scalar_type() == kFP4 ? FATTN_FP4_ROW(d) : d;
+  if (vp.sizes() != kp.sizes() || kp.size(3) != row) {
     throw OpError(std::string(who) + ": k_pages and v_pages [pages, kv_heads, page_size, " +
-                  std::to_string(d) + "] expected, got " + shape_of(kp.sizes()) + " and " +
+                  std::to_string(row) + "] expected, got " + shape_of(kp.sizes()) + " and " +
                   shape_of(vp.sizes()));
   }
   if (d > 1 && (kp.stride(3) != 1 || vp.stride(3) != 1)) {
@@ -440,16 +444,39 @@ Tensor paged_append(const Tensor& k0, const Tensor& v0, const Tensor& kp, const 
   return out;
 }
 
+// A cap of scores, 0 for None.
+float check_cap(const char* who, double cap) {
+  const float c = static_cast<float>(cap);
+  if (c == 0.0f && cap != 0.0) throw OpError(std::string(who) + ": a cap from 1e-30 to 1e30 expected");
+  return c;
+}
+// Slopes of `heads` heads (may be undefined): constants, as frequencies are.
+void check_slopes(const char* who, const Tensor& slopes, int64_t heads, const Tensor& like) {
+  if (!slopes.defined()) return;
+  if (records({&slopes})) {
+    throw OpError(std::string(who) + ": no gradient of the slopes (detach them, or call it under "
+                  "torch.no_grad())");
+  }
+  require(who, "slopes", slopes, 1, &like, {kF32});
+  if (slopes.size(0) != heads || !slopes.is_contiguous()) {
+    throw OpError(std::string(who) + ": contiguous slopes [" + std::to_string(heads) + "] expected, got " +
+                  shape_of(slopes.sizes()));
+  }
+}
+
+// slopes: undefined where absent; cap 0: none.
 Tensor paged_attention(const Tensor& q0, const Tensor& kp, const Tensor& vp, const Tensor& table,
-                       const Tensor& lengths, double scale) {
+                       const Tensor& lengths, double scale, double cap, const Tensor& slopes) {
   const char* who = "paged_attention";
-  no_tangents(who, {&q0, &kp, &vp});
+  no_tangents(who, {&q0, &kp, &vp, &slopes});
   require(who, "q", q0, 4, nullptr, {kF32, kF16, kBF16});
   const int64_t b = q0.size(0), h = q0.size(1), d = q0.size(3);
   if (q0.size(2) != 1) {
     throw OpError(std::string(who) + ": q [b, h, 1, d] expected, got shape " + shape_of(q0.sizes()));
   }
   check_cache(who, q0, kp, vp, table, lengths, b, d);
+  const float c = check_cap(who, cap);
+  check_slopes(who, slopes, h, q0);
   no_graph(who, {&q0, &kp, &vp});
   const Tensor q = aligned_rows(q0);
   Tensor out = at::empty(q.sizes(), q.options());
@@ -457,12 +484,50 @@ Tensor paged_attention(const Tensor& q0, const Tensor& kp, const Tensor& vp, con
   const size_t bytes = fattn_paged_attention_workspace_bytes(b, h, hk, d, width * page);
   const Tensor ws = workspace(q, bytes);
   launch(q, [&](void* stream) {
-    return fattn_paged_attention(type_code(q), type_code(kp), b, h, hk, d, q.data_ptr(), q.strides().data(),
-                                 out.data_ptr(), kp.data_ptr(), kp.strides().data(), vp.data_ptr(),
-                                 vp.strides().data(), kp.size(0), page, ints(table), table.stride(0), width,
-                                 ints(lengths), static_cast<float>(scale), address(ws), bytes, stream);
+    return fattn_paged_scored_attention(
+        type_code(q), type_code(kp), b, h, hk, d, q.data_ptr(), q.strides().data(), out.data_ptr(),
+        kp.data_ptr(), kp.strides().data(), vp.data_ptr(), vp.strides().data(), kp.size(0), page, ints(table),
+        table.stride(0), width, ints(lengths), static_cast<float>(scale), c,
+        static_cast<const float*>(address(slopes)), address(ws), bytes, stream);
   });
   return out;
+}
+
+// starts: undefined where absent; type: FATTN_F32, .., or -1: the cache's, bf16 of a 4-bit one.
+Tensors paged_read(const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& lengths, int64_t s,
+                   const Tensor& starts, int64_t type) {
+  const char* who = "paged_read";
+  no_tangents(who, {&kp, &vp});
+  require(who, "k_pages", kp, 4, nullptr, {kF32, kF16, kBF16, kFP4});
+  require(who, "lengths", lengths, 1, &kp, {kI32});
+  const int64_t row = kp.size(3), b = lengths.size(0), hk = kp.size(1);
+  int64_t d = row;
+  if (kp.scalar_type() == kFP4) {
+    for (d = 32; d < 128 && FATTN_FP4_ROW(d) != row; d *= 2) {
+    }
+  }
+  check_cache(who, kp, kp, vp, table, lengths, b, d);
+  no_graph(who, {&kp, &vp});
+  if (s < 0) throw OpError(std::string(who) + ": a number of tokens expected, got " + std::to_string(s));
+  if (starts.defined()) {
+    require(who, "starts", starts, 1, &kp, {kI32});
+    if (starts.size(0) != b || !starts.is_contiguous()) {
+      throw OpError(std::string(who) + ": contiguous starts [" + std::to_string(b) + "] expected, got " +
+                    shape_of(starts.sizes()));
+    }
+  }
+  const ScalarType to = type == FATTN_F32                               ? kF32
+                        : type == FATTN_F16                             ? kF16
+                        : type == FATTN_BF16 || kp.scalar_type() == kFP4 ? kBF16
+                                                                         : kp.scalar_type();
+  Tensor k = at::empty({b, hk, s, d}, kp.options().dtype(to)), v = at::empty({b, hk, s, d}, k.options());
+  launch(kp, [&](void* stream) {
+    return fattn_paged_read(type_code(kp), type_code(to), b, hk, s, d, kp.data_ptr(), kp.strides().data(),
+                            vp.data_ptr(), vp.strides().data(), kp.size(0), kp.size(2), ints(table),
+                            table.stride(0), table.size(1), ints(lengths), ints(starts), k.data_ptr(),
+                            v.data_ptr(), stream);
+  });
+  return {k, v};
 }
 
 // --- Cross attention -------------------------------------------------------------------------------
@@ -620,6 +685,15 @@ struct Args {
     if (x == -1.0 && PyErr_Occurred()) throw python_error();
     return x;
   }
+  // A cap of scores: None is 0, and 0 itself is refused.
+  double maybe_cap() {
+    PyObject* x = next();
+    if (x == Py_None) return 0.0;
+    const double c = PyFloat_AsDouble(x);
+    if (c == -1.0 && PyErr_Occurred()) throw python_error();
+    if (!(c > 0.0)) throw OpError(std::string(who) + ": a cap from 1e-30 to 1e30 expected, got " + std::to_string(c));
+    return c;
+  }
   int64_t integer() {
     const long long x = PyLong_AsLongLong(next());
     if (x == -1 && PyErr_Occurred()) throw python_error();
@@ -711,13 +785,30 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return entry("paged_attention", args, n, [](Args& a) {
     const Tensor &q = a.tensor("q"), &kp = a.tensor("k_pages"), &vp = a.tensor("v_pages"),
                  &table = a.tensor("page_table"), &lengths = a.tensor("lengths");
-    const double scale = a.number();
+    const double scale = a.number(), cap = a.maybe_cap();
+    const Tensor slopes = a.maybe("slopes");
     Tensor out;
     {
       const Unlocked unlocked;
-      out = paged_attention(q, kp, vp, table, lengths, scale);
+      out = paged_attention(q, kp, vp, table, lengths, scale, cap, slopes);
     }
     return one(out);
+  });
+}
+
+PyObject* py_paged_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return entry("paged_read", args, n, [](Args& a) {
+    const Tensor &kp = a.tensor("k_pages"), &vp = a.tensor("v_pages"), &table = a.tensor("page_table"),
+                 &lengths = a.tensor("lengths");
+    const int64_t s = a.integer();
+    const Tensor starts = a.maybe("starts");
+    const int64_t type = a.integer();
+    Tensors out;
+    {
+      const Unlocked unlocked;
+      out = paged_read(kp, vp, table, lengths, s, starts, type);
+    }
+    return all(out);
   });
 }
 
@@ -741,6 +832,7 @@ PyMethodDef g_methods[] = {
     ENTRY("rotary_qkv", py_rotary_qkv),
     ENTRY("paged_append", py_append),
     ENTRY("paged_attention", py_paged_attention),
+    ENTRY("paged_read", py_paged_read),
     ENTRY("cross_attention", py_cross_attention),
 #undef ENTRY
     {nullptr, nullptr, 0, nullptr}};

@@ -219,6 +219,14 @@ int fattn_backward(const float* q, int64_t q_offset, const int64_t q_shape[4],
 #define FATTN_F32 0
 #define FATTN_F16 1
 #define FATTN_BF16 2
+/* Of a cache only: 4-bit floats. A row of d values is FATTN_FP4_ROW(d) bytes (its strides count bytes,
+ * rows 4-byte aligned): d / 2 of codes, value 2 i in the low bits of byte i, then a scale byte per 32
+ * values, then zeros. A code is a sign and the index of a magnitude among 0, .5, 1, 1.5, 2, 3, 4, 6 (no
+ * negative 0); a scale byte e means times 2^(e - 127), 255 NaN. An append takes the least scale (byte 0 at
+ * least) under which none of the 32 values passes 7, and the nearest code, the even one of two; a group
+ * with a value that is not finite is NaN. The values are bf16 values. */
+#define FATTN_FP4 3
+#define FATTN_FP4_ROW(d) ((d) / 2 + ((d) < 128 ? 4 : (d) / 32))
 
 /* Rotary positions on up to three [b, heads, s, d] operands of one type (d even, at most 1024;
  * heads[i] 0: absent; strides {batch, head, seq}, three of each operand): y = x, but with bit i of
@@ -235,7 +243,8 @@ int fattn_rotary(int dtype, int64_t b, int64_t s, int64_t d, const int64_t heads
 /* Appends up to s new tokens per sequence to a paged cache: token i < counts[b] (counts NULL: all s)
  * is token lengths[b] + i of sequence b, and goes to slot t % page_size of page
  * table[b][t / page_size] of k_pages and v_pages ([pages, kv_heads, page_size, d], page_strides
- * {page, head, slot}), rounded to cache_dtype (the activations' type, or any for fp32 ones). Keys are
+ * {page, head, slot}), rounded to cache_dtype (the activations' type or FATTN_FP4, or any for fp32
+ * ones; with FATTN_FP4 q_out is not q, and the codes are those of the keys turned in 64 bits). Keys are
  * turned as by fattn_rotary at position t (frequencies NULL: not), and so is q ([b, heads, s, d],
  * heads 0: absent) into q_out, in all s rows. A token whose page the table ([b, table_width], row
  * stride table_stride) or the cache does not have is not written; nor is anything else. page_size is
@@ -266,6 +275,27 @@ int fattn_paged_attention(int dtype, int cache_dtype, int64_t b, int64_t heads, 
                           const int32_t* table, int64_t table_stride, int64_t table_width,
                           const int32_t* lengths, float scale, void* workspace,
                           size_t workspace_bytes, void* stream);
+
+/* The same, of scores x = scale q.k taken as cap tanh(x / cap) (cap 0: as they are; else 1e-30 to 1e30),
+ * less slopes[head] times the distance lengths[b] - 1 - j to cached token j (slopes NULL: none; [heads]
+ * finite floats on the device). The workspace is fattn_paged_attention's. */
+int fattn_paged_scored_attention(int dtype, int cache_dtype, int64_t b, int64_t heads, int64_t kv_heads,
+                                 int64_t d, const void* q, const int64_t q_strides[2], void* out,
+                                 const void* k_pages, const int64_t k_page_strides[3],
+                                 const void* v_pages, const int64_t v_page_strides[3], int64_t pages,
+                                 int64_t page_size, const int32_t* table, int64_t table_stride,
+                                 int64_t table_width, const int32_t* lengths, float scale, float cap,
+                                 const float* slopes, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+
+/* Tokens starts[b] + i, i < s (starts NULL: from 0), out of a paged cache into k and v, [b, kv_heads, s, d]
+ * contiguous, of type dtype (rounded once where it is narrower): 0 before token 0 and from token lengths[b]
+ * on, NaN where the table or the cache has no page for a token that the sequence holds. */
+int fattn_paged_read(int cache_dtype, int dtype, int64_t b, int64_t kv_heads, int64_t s, int64_t d,
+                     const void* k_pages, const int64_t k_page_strides[3], const void* v_pages,
+                     const int64_t v_page_strides[3], int64_t pages, int64_t page_size,
+                     const int32_t* table, int64_t table_stride, int64_t table_width,
+                     const int32_t* lengths, const int32_t* starts, void* k, void* v, void* stream);
 
 /* Cross attention, fp32: q [b, heads, sq, d] to k, v [b, kv_heads, sk, d] (strides {batch, head, seq},
  * rows 16-byte aligned), of which sample b sees the first key_lengths[b] (NULL: all; a length outside

@@ -5,7 +5,8 @@ kernels (libfattn.so).
 The public surface mirrors the reference crate's (src/lib.rs:90-161): `fused_attention`,
 `fused_attention_qkv`, `CUDA_HEAD_DIM`. Around them, without a counterpart there: rotary positions
 (`fused_rotary`, `fused_rotary_qkv`, `rotary_frequencies`), a paged key-value cache, in 4 bits too
-(`paged_append`, `paged_attention`, `paged_read`, `fp4_row_bytes`) and attention to states of another length (`fused_cross_attention`).
+(`paged_append`, `paged_attention`, `paged_read`, `fp4_row_bytes`), attention to states of another length
+(`fused_cross_attention`) and attention of capped, biased and masked scores (`fused_scored_attention`).
 """
 from ._lib import FusedAttentionError, LIB_PATH, version
 from .cross import fused_cross_attention
@@ -23,6 +24,7 @@ from .ops import (
 )
 from .paged import fp4_row_bytes, paged_append, paged_attention, paged_read
 from .rotary import fused_rotary, fused_rotary_qkv, rotary_frequencies
+from .scored import fused_scored_attention
 
 __all__ = [
     "CUDA_HEAD_DIM",
@@ -37,6 +39,7 @@ __all__ = [
     "fused_cross_attention",
     "fused_rotary",
     "fused_rotary_qkv",
+    "fused_scored_attention",
     "paged_append",
     "paged_attention",
     "paged_read",

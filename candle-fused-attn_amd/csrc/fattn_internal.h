@@ -298,6 +298,34 @@ int launch_cross_backward(View q, View k, View v, View d_o, const float* o, cons
 int64_t cross_blocks(int64_t heads, int64_t s);
 int64_t cross_query_blocks(int64_t pairs, int64_t g, int64_t s, int wave_rows = 32);
 
+// Attention of capped, biased and masked scores (fattn_scored.hip): out [b, sq, h, d], lse [b, h, sq], dq
+// [b, sq, h, d], dkv [b, sk, 2, h / g, d].
+struct ScoredArgs {
+  View q, k, v, d_o;
+  const float* o;  // the backward's: the forward's out
+  float *out, *lse, *dq, *dkv;
+  int B, H, G, SQ, SK;  // G: query heads per key head; queries are the last SQ of SK positions
+  float scale;
+  int causal;
+  float cap2, unit;  // cap log2 e (0: none), and its inverse (1: none)
+  const float* slopes;
+  const int32_t *documents, *prefix;
+  int64_t document_stride;
+  // The launchers': blocks of 128 queries and keys, chunks of the forward's walks and their tiles, and where
+  // the chunks' O and L go.
+  int nqb, nkb, nc, chunk;
+  float* o_part;
+  double* l_part;
+};
+struct ScoredPlan {
+  int nc, chunk;
+  size_t l_part, bytes;
+};
+ScoredPlan scored_plan(int64_t b, int64_t h, int64_t sq, int64_t sk, int64_t d);
+int64_t scored_blocks(int64_t b, int64_t heads, int64_t rows);
+int launch_scored_forward(ScoredArgs a, int d, const ScoredPlan& plan, void* workspace, void* stream);
+int launch_scored_backward(ScoredArgs a, int d, void* stream);
+
 // Sets this thread's message (fattn_last_error) and returns `code`; done() clears it and returns 0.
 int set_error(int code, const char* format, ...) __attribute__((format(printf, 2, 3)));
 int hip_error(int err, const char* who, const char* what);

@@ -227,6 +227,47 @@ int cross_operands(Cross& c, const float* q, const int64_t q_strides[3], const f
   return 0;
 }
 
+// --- Scored attention's operands --------------------------------------------------------------------
+constexpr const char* kScored = "fused_scored_attention";
+int scored_operands(fattn::ScoredArgs& a, const float* q, const int64_t q_strides[3], const float* k,
+                    const int64_t k_strides[3], const float* v, const int64_t v_strides[3], int64_t b,
+                    int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d, float scale, int causal,
+                    float cap, const float* slopes, const int32_t* documents, int64_t document_stride,
+                    const int32_t* prefix, bool* none) {
+  if (b < 0 || sq < 0 || sk < 0) return set_error(FATTN_EINVAL, "%s: negative size", kScored);
+  if (sq > sk) {
+    return set_error(FATTN_EINVAL, "%s: %lld queries are more than the %lld positions", kScored,
+                     static_cast<long long>(sq), static_cast<long long>(sk));
+  }
+  if (heads == 0 && kv_heads == 0) b = 0;
+  if (int rc = check_heads(kScored, heads, kv_heads, b == 0)) return rc;
+  if (int rc = check_dim(kScored, d)) return rc;
+  if (int rc = check_cap(kScored, cap)) return rc;
+  *none = b == 0 || sk == 0;
+  if (*none) return 0;
+  const int64_t lim = INT32_MAX - 256;
+  if (b > lim || sk > lim || b * heads > lim || b * heads * sk > lim ||
+      fattn::scored_blocks(b, heads, sq) + fattn::scored_blocks(b, kv_heads, sk) > kMaxGrid) {
+    return set_error(FATTN_ERANGE, "%s: the sizes exceed 32-bit indexing or the launch limit", kScored);
+  }
+  if ((sq > 0 && (!q || !q_strides)) || !k || !v || !k_strides || !v_strides) {
+    return set_error(FATTN_EINVAL, "%s: null operand", kScored);
+  }
+  if (documents && document_stride < 0) return set_error(FATTN_EINVAL, "%s: negative strides", kScored);
+  if (sq > 0 && !view(a.q, q, q_strides, b, heads, sq)) return bad_view(kScored, q_strides);
+  if (!view(a.k, k, k_strides, b, kv_heads, sk)) return bad_view(kScored, k_strides);
+  if (!view(a.v, v, v_strides, b, kv_heads, sk)) return bad_view(kScored, v_strides);
+  if (!slice_fits(a.k, sk, d) || !slice_fits(a.v, sk, d)) {
+    return set_error(FATTN_ERANGE, "%s: the keys of one (batch, head) span more than 4 GiB", kScored);
+  }
+  a.B = static_cast<int>(b), a.H = static_cast<int>(heads), a.G = static_cast<int>(heads / kv_heads);
+  a.SQ = static_cast<int>(sq), a.SK = static_cast<int>(sk);
+  a.scale = scale, a.causal = causal ? 1 : 0;
+  a.cap2 = cap * kLog2e, a.unit = cap == 0.0f ? 1.0f : 1.0f / a.cap2;
+  a.slopes = slopes, a.documents = documents, a.document_stride = document_stride, a.prefix = prefix;
+  return 0;
+}
+
 bool split_shape(int64_t b, int64_t heads, int64_t kv_heads, int64_t d) {
   return b >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && fattn::head_dim_supported(d);
 }
@@ -500,6 +541,68 @@ int fattn_cross_backward(const float* q, const int64_t q_strides[3], const float
       static_cast<int>(kv_heads), static_cast<int>(sq), static_cast<int>(sk), static_cast<int>(d),
       key_lengths, scale, plan, workspace, stream);
   if (err) return fattn::hip_error(err, kCross, "backward launch");
+  return fattn::done();
+}
+
+size_t fattn_scored_workspace_bytes(int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk,
+                                    int64_t d) {
+  if (!split_shape(b, heads, kv_heads, d) || sq < 0 || sk < sq) return 0;
+  return fattn::scored_plan(b, heads, sq, sk, d).bytes;
+}
+
+int fattn_scored_forward(const float* q, const int64_t q_strides[3], const float* k,
+                         const int64_t k_strides[3], const float* v, const int64_t v_strides[3],
+                         int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d,
+                         float scale, int causal, float cap, const float* slopes,
+                         const int32_t* documents, int64_t document_stride, const int32_t* prefix,
+                         float* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  fattn::ScoredArgs a{};
+  bool none = false;
+  if (int rc = scored_operands(a, q, q_strides, k, k_strides, v, v_strides, b, heads, kv_heads, sq, sk, d, scale,
+                               causal, cap, slopes, documents, document_stride, prefix, &none)) {
+    return rc;
+  }
+  if (none || sq == 0) return fattn::done();
+  if (!out || !lse) return set_error(FATTN_EINVAL, "%s: null operand", kScored);
+  if (!aligned(out, 16)) return set_error(FATTN_EALIGN, "%s: rows must be 16-byte aligned", kScored);
+  const fattn::ScoredPlan plan = fattn::scored_plan(b, heads, sq, sk, d);
+  if (fattn::scored_blocks(b, heads, sq) * plan.nc > kMaxGrid) {
+    return set_error(FATTN_ERANGE, "%s: the grid exceeds the launch limit", kScored);
+  }
+  if (int rc = check_workspace(kScored, workspace, workspace_bytes, plan.bytes)) return rc;
+  a.out = out, a.lse = lse;
+  const int err = fattn::launch_scored_forward(a, static_cast<int>(d), plan, workspace, stream);
+  if (err) return fattn::hip_error(err, kScored, "forward launch");
+  return fattn::done();
+}
+
+int fattn_scored_backward(const float* q, const int64_t q_strides[3], const float* k,
+                          const int64_t k_strides[3], const float* v, const int64_t v_strides[3],
+                          int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d,
+                          float scale, int causal, float cap, const float* slopes,
+                          const int32_t* documents, int64_t document_stride, const int32_t* prefix,
+                          const float* out, const float* lse, const float* d_o,
+                          const int64_t do_strides[3], float* dq, float* dkv, void* stream) {
+  fattn::ScoredArgs a{};
+  bool none = false;
+  if (int rc = scored_operands(a, q, q_strides, k, k_strides, v, v_strides, b, heads, kv_heads, sq, sk, d, scale,
+                               causal, cap, slopes, documents, document_stride, prefix, &none)) {
+    return rc;
+  }
+  if (none) return fattn::done();
+  if ((sq > 0 && (!out || !lse || !d_o || !do_strides || !dq)) || !dkv) {
+    return set_error(FATTN_EINVAL, "%s: null operand", kScored);
+  }
+  if (sq > 0 && !view(a.d_o, d_o, do_strides, b, heads, sq)) return bad_view(kScored, do_strides);
+  if (!aligned(out, 16) || !aligned(dq, 16) || !aligned(dkv, 16)) {
+    return set_error(FATTN_EALIGN, "%s: rows must be 16-byte aligned", kScored);
+  }
+  if (!slice_fits(a.q, sq, d) || !slice_fits(a.d_o, sq, d) || sq * heads * d > int64_t{UINT32_MAX}) {
+    return set_error(FATTN_ERANGE, "%s: the queries of one sample span more than 4 GiB", kScored);
+  }
+  a.o = out, a.lse = const_cast<float*>(lse), a.dq = dq, a.dkv = dkv;
+  const int err = fattn::launch_scored_backward(a, static_cast<int>(d), stream);
+  if (err) return fattn::hip_error(err, kScored, "backward launch");
   return fattn::done();
 }
 

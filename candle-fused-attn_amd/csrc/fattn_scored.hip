@@ -1,0 +1,1083 @@
+// Attention of scores of other forms, forward and backward: queries the last SQ of SK positions, key heads
+// shared by groups of query heads. With x = scale q.k, i the query's position and j the key's:
+//   y = cap tanh(x / cap) - slope_h |i - j|        (or x itself; no slope)
+//   i sees j where (j <= i, or j < prefix_b, or it is not causal) and documents[b][i] = documents[b][j] >= 0
+//   P = softmax(y) over what is seen, O = P V; a row that sees nothing is 0.
+//   dV = P^T dO, dY = P o (dO V^T - rowsum(dO o O)), dX = dY (1 - tanh^2(x / cap)), dQ = scale dX K,
+//   dK = scale dX^T Q.
+// The products, scales, staging and sums are those of fattn_pair_kernels.h (fp32 as pairs of f16, blocks of
+// four waves of 32 rows, a backward of two kinds of workgroup that share no sum); here are the scores and
+// the walks. What a block can see is a range of tiles: from its positions, and, with documents, from the
+// first to the last place of the ids between its least and its largest (so ids in order, as packed
+// documents have them, leave only their own tiles; other orders are walked over and masked). A tile's ids
+// are staged beside it: a wave passes over a tile in which it sees nothing, and takes one in which it sees
+// everything without a mask.
+#include <hip/hip_runtime.h>
+#include <limits.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "fattn_internal.h"
+#include "fattn_pair_kernels.h"
+
+namespace fattn {
+namespace {
+
+constexpr int kW = 4;                    // waves of a workgroup
+constexpr int kBlock = kW * kRows;       // its rows
+constexpr double kLn2 = 0.69314718055994530942;
+constexpr double kUnseen = -__builtin_inf();  // L of a row that sees nothing
+constexpr double kVanished = -1e308;          // of one whose every score is minus infinity
+enum { kNone, kSome, kAll };                  // what a wave sees of a tile
+
+// --- Who sees whom -----------------------------------------------------------------------------
+__device__ __forceinline__ int wave_least(int x) {
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) x = min(x, __shfl_xor(x, i));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ int wave_most(int x) {
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) x = max(x, __shfl_xor(x, i));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+// LDS of the ids: those of the staged tiles, and what the waves find.
+struct IdSmem {
+  int tile[2][kRows];
+  int found[2][kW][2];
+};
+// A wave's ids (one per lane j, both halves alike) and its block's.
+struct Ids {
+  int mine;          // of the lane's row
+  int least, most;   // of the wave's rows that have a document; most -1: none
+  bool one;          // all 32 rows have the same
+  __device__ __forceinline__ void take(int id) {
+    mine = id;
+    least = wave_least(id >= 0 ? id : INT_MAX);
+    most = wave_most(id);
+    one = most >= 0 && __builtin_amdgcn_ballot_w64(id != most) == 0;
+  }
+};
+// The block's rows' ids lie in [*lo, *hi]; the first and the last + 1 of ids[from .. to) that do (none:
+// first >= last). For the whole workgroup.
+__device__ __forceinline__ void find_ids(IdSmem& sm, const Ids& ids, const int32_t* all, int from, int to, int w,
+                                         int tid, int& first, int& last) {
+  if ((tid & 63) == 0) sm.found[0][w][0] = ids.least, sm.found[0][w][1] = ids.most;
+  __syncthreads();
+  int lo = sm.found[0][0][0], hi = sm.found[0][0][1];
+#pragma unroll
+  for (int i = 1; i < kW; ++i) lo = min(lo, sm.found[0][i][0]), hi = max(hi, sm.found[0][i][1]);
+  int f = INT_MAX, l = -1;
+#pragma unroll 4
+  for (int i = from + tid; i < to; i += 64 * kW) {
+    const int id = all[i];
+    if (id >= lo && id <= hi) f = min(f, i), l = i;
+  }
+  f = wave_least(f), l = wave_most(l);
+  if ((tid & 63) == 0) sm.found[1][w][0] = f, sm.found[1][w][1] = l;
+  __syncthreads();
+  first = sm.found[1][0][0], last = sm.found[1][0][1];
+#pragma unroll
+  for (int i = 1; i < kW; ++i) first = min(first, sm.found[1][i][0]), last = max(last, sm.found[1][i][1]);
+  last += 1;
+  first = __builtin_amdgcn_readfirstlane(first), last = __builtin_amdgcn_readfirstlane(last);
+}
+// What a wave with `ids` sees of a tile with id `id` in lane j, where positions let it see `sees` of it.
+__device__ __forceinline__ int among(int id, const Ids& ids, int sees) {
+  if (__builtin_amdgcn_ballot_w64(id >= ids.least && id <= ids.most) == 0) return kNone;
+  return ids.one && __builtin_amdgcn_ballot_w64(id != ids.most) == 0 ? sees : kSome;
+}
+// The last key that the query at position p sees (but for documents).
+__device__ __forceinline__ int last_key(const ScoredArgs& a, int p, int prefix) {
+  return a.causal ? max(p, prefix - 1) : a.SK - 1;
+}
+__device__ __forceinline__ int prefix_of(const ScoredArgs& a, int b) {
+  return a.prefix != nullptr ? min(max(a.prefix[b], 0), a.SK) : 0;
+}
+__device__ __forceinline__ const int32_t* ids_of(const ScoredArgs& a, int b) {
+  return a.documents != nullptr ? a.documents + b * a.document_stride : nullptr;
+}
+__device__ __forceinline__ float slope_of(const ScoredArgs& a, int h) {
+  return a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.0f;
+}
+
+// --- Scores ------------------------------------------------------------------------------------
+// One score in units of log2 e from x (in those units; with a cap in units of the cap), `far` the distance:
+// CAP 0: no cap, 1: every |x| of the wave's tile is at most kTanhSmall, 2: any. `slope`: dy / dx.
+template <int CAP>
+__device__ __forceinline__ float score(float x, float cap2, float slope2, float far, float& slope) {
+  float y = x;
+  if constexpr (CAP == 1) {
+    const float t = tanh_small(x);
+    slope = fmaf(-t, t, 1.0f);
+    y = cap2 * t;
+  } else if constexpr (CAP == 2) {
+    y = cap2 * tanh_any(x, slope);
+  } else {
+    slope = 1.0f;
+  }
+  return fmaf(-slope2, fabsf(far), y);
+}
+// One score by its definition, for the rows in fp32.
+__device__ __forceinline__ float score_fp32(const ScoredArgs& a, float dot, float slope2, int far, float& slope) {
+  const float x = dot * (a.scale * kLog2e * a.unit);
+  return a.cap2 != 0.0f ? score<2>(x, a.cap2, slope2, static_cast<float>(far), slope)
+                        : score<0>(x, 0.0f, slope2, static_cast<float>(far), slope);
+}
+template <typename F>
+__device__ __forceinline__ void by_cap(const ScoredArgs& a, const f16v& x, F fn) {
+  if (a.cap2 == 0.0f) {
+    fn(Const<0>{});
+  } else if (__builtin_amdgcn_ballot_w64(max_weight(x) > kTanhSmall) == 0) {
+    fn(Const<1>{});
+  } else {
+    fn(Const<2>{});
+  }
+}
+
+// --- Rows in fp32 (see fattn_pair_kernels.h) -----------------------------------------------------
+// L of a row; of a chunk in 64 bits, since the join takes differences of it.
+__device__ __forceinline__ void put_l(const ScoredArgs& a, int chunk, int64_t at, double L) {
+  if (a.nc > 1) {
+    a.l_part[chunk * (static_cast<int64_t>(a.B) * a.H * a.SQ) + at] = L;
+  } else {
+    __builtin_nontemporal_store(static_cast<float>(L), a.lse + at);
+  }
+}
+// O and L of 32 queries from qg over the tiles from t0 to t1.
+template <int D, typename Store>
+__device__ __forceinline__ void scored_rows_fp32(const ScoredArgs& a, int b, int h, int qg, int t0, int t1,
+                                                 int chunk, float* so, int lane, Store store) {
+  const int j = lane & 31, g = lane >> 5, qc = min(qg + j, a.SQ - 1), p = qc + a.SK - a.SQ, hk = h / a.G;
+  const float* qp = a.q.p + b * a.q.sb + h * a.q.sh + qc * a.q.ss;
+  const float* kp = a.k.p + b * a.k.sb + hk * a.k.sh;
+  const float* vp = a.v.p + b * a.v.sb + hk * a.v.sh;
+  const int lim = last_key(a, p, prefix_of(a, b));
+  const int32_t* ids = ids_of(a, b);
+  const int id = ids != nullptr ? ids[p] : 0;
+  const float slope2 = slope_of(a, h);
+  f16v acc[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) acc[dt] = zero16();
+  float m = kNegInf, l = 0.0f;
+  bool seen = false;
+  auto live = [&](int key) {
+    return key <= lim && id >= 0 && (ids == nullptr || ids[min(key, a.SK - 1)] == id);
+  };
+#pragma clang loop unroll(disable)
+  for (int t = t0; t < t1; ++t) {
+    const int k0 = t * kRows;
+    f16v s = dots_fp32<D>(kp + min(k0 + j, a.SK - 1) * a.k.ss, qp, g);
+    float mn = m;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int key = k0 + tile_row(r, g);
+      const bool is = live(key);
+      float d;
+      s[r] = is ? score_fp32(a, s[r], slope2, p - key, d) : kNegInf;
+      seen = seen || is;
+      mn = fmaxf(mn, s[r]);
+    }
+    mn = pair_max(fmaxf(mn, kNegInf));
+    const float alpha = mn == m ? 1.0f : m == kNegInf ? 0.0f : exp2_hw(m - mn);
+    m = mn;
+    l *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) acc[dt] *= alpha;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[r] = s[r] == kNegInf ? 0.0f : exp2_hw(s[r] - mn);
+      l += s[r];
+    }
+    sum_fp32<D, false>(s, vp, a.v.ss, k0, a.SK, live, so, acc, j, g);
+  }
+  l = pair_sum(l);
+  seen = pair_max(seen ? 1.0f : 0.0f) > 0.0f;
+  // (A row whose every score is minus infinity is NaN, as its formula: 0 / 0; a chunk of such weighs nothing.)
+  store(acc, !seen || (a.nc > 1 && l == 0.0f) ? 1.0f : 1.0f / l);
+  if (g == 0 && qg + j < a.SQ) {
+    const double L = !seen ? kUnseen : l == 0.0f ? kVanished : static_cast<double>(m) * kLn2 + logf(l);
+    put_l(a, chunk, (static_cast<int64_t>(b) * a.H + h) * a.SQ + qg + j, L);
+  }
+}
+
+// dK and dV of 32 keys from kw0 (walking the tiles t0 .. t1 of the G query heads' queries), in fp32.
+template <int D>
+__device__ __forceinline__ void scored_keys_fp32(const ScoredArgs& a, int b, int hk, int kw0, int t0, int t1,
+                                                 float* so, f16v (&dk)[D / 32], f16v (&dv)[D / 32], int lane) {
+  const int j = lane & 31, g = lane >> 5, key = kw0 + j, kc = min(key, a.SK - 1), off = a.SK - a.SQ;
+  const float* kr = a.k.p + b * a.k.sb + hk * a.k.sh + kc * a.k.ss;
+  const float* vr = a.v.p + b * a.v.sb + hk * a.v.sh + kc * a.v.ss;
+  const int prefix = prefix_of(a, b);
+  const int32_t* ids = ids_of(a, b);
+  const int id = key < a.SK ? (ids != nullptr ? ids[kc] : 0) : -1;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) dk[dt] = zero16(), dv[dt] = zero16();
+  auto live = [&](int qi) {
+    return qi < a.SQ && id >= 0 && key <= last_key(a, qi + off, prefix) &&
+           (ids == nullptr || ids[min(qi, a.SQ - 1) + off] == id);
+  };
+#pragma clang loop unroll(disable)
+  for (int u = 0; u < a.G * (t1 - t0); ++u) {
+    const int h = hk * a.G + u / (t1 - t0), q0 = (t0 + u % (t1 - t0)) * kRows;
+    const float* qp = a.q.p + b * a.q.sb + h * a.q.sh;
+    const float* gp = a.d_o.p + b * a.d_o.sb + h * a.d_o.sh;
+    const float* op = a.o + (static_cast<int64_t>(b) * a.SQ * a.H + h) * D;
+    const float* lp = a.lse + (static_cast<int64_t>(b) * a.H + h) * a.SQ;
+    const float slope2 = slope_of(a, h);
+    const int64_t qr = min(q0 + j, a.SQ - 1);
+    f16v s = dots_fp32<D>(qp + qr * a.q.ss, kr, g), dp = dots_fp32<D>(gp + qr * a.d_o.ss, vr, g);
+    float dd = 0.0f;
+#pragma clang loop unroll(disable)
+    for (int c = 4 * g; c < D; c += 8) {
+      const f4 x = ld4(gp + qr * a.d_o.ss + c), y = ld4(op + qr * a.H * D + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dd = fmaf(x[e], y[e], dd);
+    }
+    dd = pair_sum(dd);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int t = tile_row(r, g), qi = min(q0 + t, a.SQ - 1);
+      float slope;
+      const float y = score_fp32(a, s[r], slope2, qi + off - key, slope);
+      const float p = exp2_hw(y + shifted_l(lp[qi], 0.0f));
+      const float w = p * (dp[r] - __shfl(dd, t)) * slope;  // (every lane takes part in the shuffle)
+      const bool is = live(q0 + t);
+      s[r] = is ? p : 0.0f;
+      dp[r] = is ? w : 0.0f;
+    }
+    sum_fp32<D, false>(s, gp, a.d_o.ss, q0, a.SQ, live, so, dv, j, g);
+    sum_fp32<D, false>(dp, qp, a.q.ss, q0, a.SQ, live, so, dk, j, g);
+  }
+}
+// dQ of 32 queries from qw0 over the tiles t0 .. t1, in fp32 (without the scale).
+template <int D>
+__device__ __forceinline__ void scored_queries_fp32(const ScoredArgs& a, int b, int h, int qw0, int t0, int t1,
+                                                    float* so, f16v (&dq)[D / 32], int lane) {
+  const int j = lane & 31, g = lane >> 5, hk = h / a.G, off = a.SK - a.SQ;
+  const int64_t qc = min(qw0 + j, a.SQ - 1);
+  const int p = static_cast<int>(qc) + off;
+  const float* qr = a.q.p + b * a.q.sb + h * a.q.sh + qc * a.q.ss;
+  const float* gr = a.d_o.p + b * a.d_o.sb + h * a.d_o.sh + qc * a.d_o.ss;
+  const float* kp = a.k.p + b * a.k.sb + hk * a.k.sh;
+  const float* vp = a.v.p + b * a.v.sb + hk * a.v.sh;
+  const float* orow = a.o + ((static_cast<int64_t>(b) * a.SQ + qc) * a.H + h) * D;
+  const float L = shifted_l(a.lse[(static_cast<int64_t>(b) * a.H + h) * a.SQ + qc], 0.0f);
+  const int lim = last_key(a, p, prefix_of(a, b));
+  const int32_t* ids = ids_of(a, b);
+  const int id = ids != nullptr ? ids[p] : 0;
+  const float slope2 = slope_of(a, h);
+  float dd = 0.0f;
+#pragma clang loop unroll(disable)
+  for (int c = 4 * g; c < D; c += 8) {
+    const f4 x = ld4(gr + c), y = ld4(orow + c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) dd = fmaf(x[e], y[e], dd);
+  }
+  dd = pair_sum(dd);
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) dq[dt] = zero16();
+  auto live = [&](int key) {
+    return key <= lim && id >= 0 && (ids == nullptr || ids[min(key, a.SK - 1)] == id);
+  };
+#pragma clang loop unroll(disable)
+  for (int t = t0; t < t1; ++t) {
+    const int64_t kr = min(t * kRows + j, a.SK - 1);
+    const f16v s = dots_fp32<D>(kp + kr * a.k.ss, qr, g);
+    f16v dp = dots_fp32<D>(vp + kr * a.v.ss, gr, g);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int key = t * kRows + tile_row(r, g);
+      float slope;
+      const float y = score_fp32(a, s[r], slope2, p - key, slope);
+      const float w = exp2_hw(y + L) * (dp[r] - dd) * slope;
+      dp[r] = live(key) ? w : 0.0f;
+    }
+    sum_fp32<D, false>(dp, kp, a.k.ss, t * kRows, a.SK, live, so, dq, j, g);
+  }
+}
+
+// --- Forward -----------------------------------------------------------------------------------
+// A workgroup: 128 queries of one head, over a range of key tiles; where the blocks are too few for the
+// chip the tiles are cut into chunks, whose O and L a second kernel joins in order.
+template <int D, bool kMods>
+__device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
+  constexpr int kKS = D / 16, kDT = D / 32, kOPitch = (D < 64 ? D : 64) + 4;
+  struct Kv {
+    Tile<D> k, v;
+  };
+  union Tiles {
+    Kv kv[2];
+    float o[kW][kRows * kOPitch];
+  };
+  struct Smem {
+    Tiles t;
+    float uk[2][kRows], uv[2][kRows];
+    IdSmem ids;
+  };
+  __shared__ __attribute__((aligned(16))) Smem sm;
+  const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, g = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int BH = a.B * a.H, off = a.SK - a.SQ;
+  // (Causal: the blocks that see most first.)
+  const int id = static_cast<int>(blockIdx.x), per = a.nqb * a.nc;
+  const int item = a.causal ? id % BH * per + per - 1 - id / BH : xcd_remap(id, per * BH);
+  const int bh = item / per, in = item - bh * per, qb = in / a.nc, chunk = in - qb * a.nc;
+  const int b = bh / a.H, h = bh % a.H, hk = h / a.G;
+  const int qw0 = qb * kBlock + w * kRows, qi = qw0 + j, pos = min(qi, a.SQ - 1) + off;
+  const int prefix = prefix_of(a, b);
+  const int32_t* all_ids = ids_of(a, b);
+  // The keys: of the block to `end`, of the wave's first and last query to `lo` and `hi`.
+  const int end = last_key(a, min(qb * kBlock + kBlock, a.SQ) - 1 + off, prefix) + 1;
+  const int lim = last_key(a, pos, prefix);
+  const int lo = last_key(a, min(qw0, a.SQ - 1) + off, prefix);
+  const int hi = last_key(a, min(qw0 + kRows, a.SQ) - 1 + off, prefix);
+  const bool wave_live = qw0 < a.SQ;
+  int t0 = 0, t1 = (end + kRows - 1) / kRows;
+  Ids ids{0, 0, 0, true};
+  if (all_ids != nullptr) {
+    ids.take(all_ids[pos]);
+    int first, last;
+    find_ids(sm.ids, ids, all_ids, 0, end, w, tid, first, last);
+    t0 = first / kRows, t1 = first < last ? (last + kRows - 1) / kRows : t0;
+  }
+  if (a.nc > 1) t0 = max(t0, chunk * a.chunk), t1 = min(t1, (chunk + 1) * a.chunk);
+  float* out = a.nc > 1 ? a.o_part + chunk * (static_cast<int64_t>(BH) * a.SQ * D) : a.out;
+  if (t0 >= t1) {  // no key to see: O is 0, L -infinity (a chunk: L alone)
+    if (a.nc == 1) {
+      for (int i = lane; i < min(a.SQ - qw0, kRows) * (D / 4); i += 64) {
+        const int64_t row = static_cast<int64_t>(b) * a.SQ + qw0 + i / (D / 4);
+        st4(out + (row * a.H + h) * D + i % (D / 4) * 4, f4{});
+      }
+    }
+    if (lane < min(a.SQ - qw0, kRows)) put_l(a, chunk, static_cast<int64_t>(bh) * a.SQ + qw0 + lane, kUnseen);
+    return;
+  }
+  const float* qp = a.q.p + b * a.q.sb + h * a.q.sh;
+  const Operand kop{reinterpret_cast<const char*>(a.k.p + b * a.k.sb + hk * a.k.sh),
+                    static_cast<unsigned>(a.k.ss) * 4u};
+  const Operand vop{reinterpret_cast<const char*>(a.v.p + b * a.v.sb + hk * a.v.sh),
+                    static_cast<unsigned>(a.v.ss) * 4u};
+
+  Stage<D, kW> st;
+  int id_next = 0;
+  auto load = [&](int t) {
+    st.load(kop, vop, t * kRows, a.SK - 1, w, lane);
+    if (all_ids != nullptr && w == 0) id_next = all_ids[min(t * kRows + j, a.SK - 1)];
+  };
+  auto store = [&](int t) {
+    const int put = t & 1;
+    st.store(sm.t.kv[put].k, sm.t.kv[put].v, sm.uk[put], sm.uv[put], w, lane);
+    if (all_ids != nullptr && w == 0) sm.ids.tile[put][j] = t * kRows + j < a.SK ? id_next : -1;
+  };
+  Pair q[kKS];
+  float cq;  // |scale| log2 e over the query's scale, with a cap over that too
+  {
+    OwnRows<D> own;
+    load(t0);
+    own.load(qp + min(qi, a.SQ - 1) * a.q.ss, g);
+    store(t0);
+    load(t0 + 1);
+    cq = own.split(a.scale < 0.0f ? -1.0f : 1.0f, q) * (fabsf(a.scale) * kLog2e * (kMods ? a.unit : 1.0f));
+  }
+  const float slope2 = kMods ? slope_of(a, h) : 0.0f, fpos = static_cast<float>(pos - 4 * g);
+  f16v acc[kDT];  // O^T, in units of p / wsc and 2^-kTop
+  float m = kNegInf, lsum = 0.0f, wsc = kMaxScale;
+#pragma unroll
+  for (int dt = 0; dt < kDT; ++dt) acc[dt] = zero16();
+  const int roff0 = row_off<D>(j, g), coff0 = col_off<D>(lane);
+
+  auto stage = [&](int t) {
+    store(t + 1);
+    load(t + 2);
+    pin_loads();
+  };
+  // (See fattn_pair_kernels.h for the sums' scales.)
+  auto tile = [&](auto fullc, int t) {
+    constexpr bool kFull = decltype(fullc)::value != 0;
+    const int roff = late(roff0), coff = late(coff0), kt0 = t * kRows, cur = t & 1;
+    const Kv& kv = sm.t.kv[cur];
+    stage(t);
+    f16v s = zero16();
+    {
+      h8 kh[kKS];
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) {
+        const Pair k = ld_row<D>(kv.k, roff ^ row_step(ks));
+        kh[ks] = k.h;
+        s = mma_small(k, q[ks], s);
+      }
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) s = mma(kh[ks], q[ks].h, s);
+    }
+    // Live: register r's key, kt0 + 4 g + 8 (r / 4) + r % 4.
+    unsigned live = 0xffffu;
+    if constexpr (!kFull) {
+      const int left = lim - kt0 - 4 * g;
+      live = 0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int at = 8 * (r >> 2) + (r & 3);
+        const bool is = at <= left && (all_ids == nullptr || sm.ids.tile[cur][at + 4 * g] == ids.mine);
+        live |= is ? 1u << r : 0u;
+      }
+      if (ids.mine < 0) live = 0;
+    }
+    if constexpr (kMods) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f4 uk = ld4(&sm.uk[cur][8 * i + 4 * g]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[4 * i + c] *= cq * uk[c];
+      }
+      const float base = fpos - static_cast<float>(kt0);
+      by_cap(a, s, [&](auto capc) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float d;
+          s[r] = score<decltype(capc)::value>(s[r], a.cap2, slope2, base - static_cast<float>(8 * (r >> 2) + (r & 3)), d);
+        }
+      });
+    }
+    f16v e;
+    float psum = 0.0f, wmax = 0.0f;
+    auto exps = [&] {
+      wmax = 0.0f;
+      int r0 = 4 * g;
+      asm("" : "+v"(r0));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f4 uv = ld4(&sm.uv[cur][8 * i + r0]);
+        f4 uk{};
+        if constexpr (!kMods) uk = ld4(&sm.uk[cur][8 * i + r0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int r = 4 * i + c;
+          const float x = exp2_hw(kMods ? s[r] - m : fmaf(s[r], cq * uk[c], -m));
+          const float p = kFull || (live >> r & 1) != 0 ? x : 0.0f;
+          psum = r == 0 ? p : psum + p;
+          e[r] = p * uv[c];
+        }
+        asm("v_max3_f32 %0, %1, %2, %0" : "+v"(wmax) : "v"(e[4 * i]), "v"(e[4 * i + 1]));
+        asm("v_max3_f32 %0, %1, %2, %0" : "+v"(wmax) : "v"(e[4 * i + 2]), "v"(e[4 * i + 3]));
+      }
+    };
+    exps();
+    if (__builtin_amdgcn_ballot_w64(!(psum <= kRowTop && wmax * wsc <= kMaxWeight)) != 0) {
+      float tmax = kNegInf;
+      int r0 = 4 * g;
+      asm("" : "+v"(r0));
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = kMods ? s[r] : s[r] * (cq * sm.uk[cur][8 * (r >> 2) + r0 + (r & 3)]);
+        tmax = fmaxf(tmax, kFull || (live >> r & 1) != 0 ? x : kNegInf);
+      }
+      const float ref = pair_max(tmax) - kRefTop;
+      float to = wsc, alpha = 1.0f;
+      if (!(pair_sum(psum) <= kRowTop) && ref > m) {
+        alpha = m == kNegInf ? 0.0f : exp2_hw(m - ref);
+        to = alpha > 0.0f ? fminf(to * pow2(-exponent(alpha)), kMaxScale) : kMaxScale;
+        m = ref;
+        lsum *= alpha;
+        exps();
+      }
+      wmax = pair_max(fmaxf(wmax, 0.0f));
+      if (wmax * to > kMaxWeight) to = pow2(kWTop - exponent(wmax));
+      const float f = alpha > 0.0f ? alpha * (to / wsc) : 0.0f;
+      wsc = to;
+#pragma unroll
+      for (int dt = 0; dt < kDT; ++dt) acc[dt] *= f;
+    }
+    lsum += psum;
+    const Pair p0 = split_acc<0>(e, wsc), p1 = split_acc<1>(e, wsc);
+#pragma unroll
+    for (int dt = 0; dt < kDT; ++dt) {
+      acc[dt] = mma3(ld_col<D>(kv.v, coff ^ col_step(dt), 0), p0, acc[dt]);
+      acc[dt] = mma3(ld_col<D>(kv.v, coff ^ col_step(dt), 1), p1, acc[dt]);
+    }
+  };
+  __syncthreads();  // tile t0
+#pragma clang loop unroll(disable)
+  for (int t = t0; t < t1; ++t) {
+    int sees = !wave_live || t * kRows > hi ? kNone : t * kRows + kRows - 1 <= lo ? kAll : kSome;
+    if (all_ids != nullptr && sees != kNone) sees = among(sm.ids.tile[t & 1][j], ids, sees);
+    if (sees == kAll) {
+      tile(Const<1>{}, t);
+    } else if (sees == kSome) {
+      tile(Const<0>{}, t);
+    } else {
+      stage(t);
+    }
+    __syncthreads();  // tile t + 1 is staged; every wave is done with tile t
+  }
+  if (!wave_live) return;
+
+  // L = (m + log2 l) ln 2, to one rounding: the backward takes 2^(y - L log2 e).
+  const float l = pair_sum(lsum);
+  float* so = sm.t.o[w];
+  const int lane_e = late(lane);
+  auto put = [&](const f16v (&x)[kDT], float f, float f2) {
+    store_rows<D>(x, f, f2, so, out + ((static_cast<int64_t>(b) * a.SQ + qw0) * a.H + h) * D,
+                  static_cast<int64_t>(a.H) * D, a.SQ - qw0, lane_e);
+  };
+  if (__builtin_amdgcn_ballot_w64(qi < a.SQ && !(probe_finite<kDT>(acc, l * 0.0f) == 0.0f)) != 0) {
+    scored_rows_fp32<D>(a, b, h, qw0, t0, t1, chunk, so, late(lane),
+                        [&](const f16v (&x)[kDT], float inv) { put(x, inv, 1.0f); });
+    return;
+  }
+  // (A row that saw nothing has sums of 0. Two factors: their product may be subnormal.)
+  put(acc, l == 0.0f ? 1.0f : 1.0f / l, pow2(-kTop) / wsc);
+  if (g == 0 && qi < a.SQ) {
+    int le = exponent(l);
+    float f = l * pow2(-le);  // [1, 2), then [0.75, 1.5)
+    if (f > 1.5f) f *= 0.5f, ++le;
+    const double L = l == 0.0f ? kUnseen : fma(static_cast<double>(m), kLn2, fma(le, kLn2, logf(f)));
+    put_l(a, chunk, static_cast<int64_t>(bh) * a.SQ + qi, L);
+  }
+}
+template <int D, bool kMods, int WAVES>
+__global__ void __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES)))
+fwd_scored_kernel(ScoredArgs a) {
+  scored_fwd<D, kMods>(a);
+}
+
+// O and L of the chunks' [nc][b, s, h, d] and [nc][b, h, s]: O = sum_c w_c O_c / sum_c w_c, w_c =
+// exp(L_c - max), L = max + log sum; a chunk in which a row saw nothing (L -infinity) has no O. D / 4 lanes a
+// row.
+template <int D>
+__global__ void __launch_bounds__(256) join_scored_kernel(ScoredArgs a) {
+  constexpr int kLanes = D / 4;
+  const int64_t rows = static_cast<int64_t>(a.B) * a.SQ * a.H;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+  if (row >= rows) return;
+  const int d = threadIdx.x % kLanes * 4;
+  const int h = static_cast<int>(row % a.H), b = static_cast<int>(row / a.H / a.SQ);
+  const int64_t at = (static_cast<int64_t>(b) * a.H + h) * a.SQ + row / a.H % a.SQ;
+  double top = kUnseen;
+  for (int c = 0; c < a.nc; ++c) {
+    const double L = a.l_part[c * rows + at];
+    top = L > top || L != L ? L : top;
+  }
+  float sum = 0.0f;
+  f4 x{};
+  for (int c = 0; c < a.nc; ++c) {
+    const double L = a.l_part[c * rows + at];
+    if (L == kUnseen) continue;
+    const float w = expf(static_cast<float>(L - top));
+    sum += w;
+    x += ld4(a.o_part + (c * rows + row) * D + d) * w;
+  }
+  st4(a.out + row * D + d, top == kUnseen ? f4{} : x * (top == kVanished ? __builtin_nanf("") : 1.0f / sum));
+  if (d == 0) a.lse[at] = top == kUnseen ? kNegInf : static_cast<float>(top + logf(sum));
+}
+
+// --- Backward ----------------------------------------------------------------------------------
+// Key blocks walk the query tiles that see them, of each head of their group in turn, and hold dK and dV;
+// query blocks walk the key tiles that they see and hold dQ.
+template <int D>
+union ScoredTiles {
+  struct {
+    Tile<D> a, b;
+  } t[2];
+  float o[kW][kRows * ((D < 64 ? D : 64) + 4)];
+};
+template <int D>
+struct ScoredSmem {
+  ScoredTiles<D> u;
+  float ua[2][kRows], ub[2][kRows], l[2][kRows], d[2][kRows];
+  IdSmem ids;
+};
+
+template <int D, bool kMods>
+__device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& sm, int item) {
+  constexpr int kKS = D / 16, kDT = D / 32;
+  const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, g = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int HK = a.H / a.G, off = a.SK - a.SQ, SQ = a.SQ;
+  const int bh = item / a.nkb, kb = item % a.nkb, b = bh / HK, hk = bh % HK, h0 = hk * a.G;
+  const int k0 = kb * kBlock, kw0 = k0 + w * kRows, key = kw0 + j, kc = min(key, a.SK - 1);
+  const int prefix = prefix_of(a, b);
+  const int32_t* all_ids = ids_of(a, b);
+  const bool wave_live = kw0 < a.SK;
+  // The queries: all, or from the first at or past the block's first key.
+  int q_first = a.causal && k0 >= prefix ? max(k0 - off, 0) : 0, q_end = SQ;
+  Ids ids{0, 0, 0, true};
+  if (all_ids != nullptr) {
+    ids.take(key < a.SK ? all_ids[kc] : -1);
+    int first, last;
+    find_ids(sm.ids, ids, all_ids, q_first + off, a.SK, w, tid, first, last);
+    q_first = first - off, q_end = last - off;
+  }
+  float* dkv = a.dkv + (static_cast<int64_t>(b) * a.SK + kw0) * 2 * HK * D + static_cast<int64_t>(hk) * D;
+  if (q_first >= q_end) {  // keys that no query sees
+    for (int i = lane; i < min(a.SK - kw0, kRows) * (D / 4); i += 64) {
+      float* row = dkv + static_cast<int64_t>(i / (D / 4)) * 2 * HK * D + i % (D / 4) * 4;
+      st4(row, f4{});
+      st4(row + static_cast<int64_t>(HK) * D, f4{});
+    }
+    return;
+  }
+  const int t0 = q_first / kRows, n = (q_end + kRows - 1) / kRows - t0, steps = n * a.G;
+  const Operand qop{reinterpret_cast<const char*>(a.q.p + b * a.q.sb + h0 * a.q.sh),
+                    static_cast<unsigned>(a.q.ss) * 4u};
+  const Operand gop{reinterpret_cast<const char*>(a.d_o.p + b * a.d_o.sb + h0 * a.d_o.sh),
+                    static_cast<unsigned>(a.d_o.ss) * 4u};
+  const float* op = a.o + (static_cast<int64_t>(b) * SQ * a.H + h0) * D;
+  const float* lp = a.lse + (static_cast<int64_t>(b) * a.H + h0) * SQ;
+
+  const int kp = half_log2(a.SK);
+  Stage<D, kW> st;
+  RowDots<D, kW> ro;
+  float lreg;
+  int id_next = 0;
+  // Step u's head in the group (past the last step: the last) and its tile's first row.
+  auto place = [&](int u, int& hh) {
+    hh = min(u / n, a.G - 1);
+    return (t0 + u - hh * n) * kRows;
+  };
+  auto load = [&](int u) {
+    int hh;
+    const int r0 = place(u, hh);
+    st.load(Operand{qop.p + hh * a.q.sh * 4, qop.ss4}, Operand{gop.p + hh * a.d_o.sh * 4, gop.ss4}, r0, SQ - 1, w,
+            lane);
+    if (all_ids != nullptr && w == 0) id_next = r0 + j < SQ ? all_ids[r0 + j + off] : -1;
+  };
+  auto load_o = [&](int u) {
+    int hh;
+    const int r0 = place(u, hh);
+    ro.load(op + hh * D, static_cast<unsigned>(a.H) * D, r0, SQ - 1, w, lane);
+    lreg = lp[hh * static_cast<int64_t>(SQ) + min(r0 + j, SQ - 1)];
+  };
+  auto store = [&](int u) {
+    const int put = u & 1;
+    st.store(sm.u.t[put].a, sm.u.t[put].b, sm.ua[put], sm.ub[put], w, lane);
+    ro.put(st, sm.d[put], w, lane);
+    if (w == 0 && g == 0) {
+      sm.l[put][j] = shifted_l(lreg, kp);
+      if (all_ids != nullptr) sm.ids.tile[put][j] = id_next;
+    }
+  };
+  Pair kB[kKS], vB[kKS];
+  float uk, uv;  // 1 / the key's scales
+  {
+    OwnRows<D> ok, ov;
+    load(0);
+    load_o(0);
+    ok.load(a.k.p + b * a.k.sb + hk * a.k.sh + kc * a.k.ss, g);
+    ov.load(a.v.p + b * a.v.sb + hk * a.v.sh + kc * a.v.ss, g);
+    uk = ok.split(1.0f, kB);
+    uv = ov.split(1.0f, vB);
+    store(0);
+    load(1);
+    load_o(1);
+  }
+  f16v dk[kDT], dv[kDT];
+#pragma unroll
+  for (int dt = 0; dt < kDT; ++dt) dk[dt] = zero16(), dv[dt] = zero16();
+  const float cs = a.scale * kLog2e * (kMods ? a.unit : 1.0f) * uk, cg = uv;
+  float psc = kMaxScale, dsc = kMaxScale;
+  const int roff0 = row_off<D>(j, g), coff0 = col_off<D>(lane);
+
+  auto tile = [&](auto fullc, int u, int q0, float slope2) {
+    constexpr bool kFull = decltype(fullc)::value != 0;
+    const int roff = late(roff0), coff = late(coff0), cur = u & 1;
+    if (kFull) store(u + 1);
+    const Tile<D>&Q = sm.u.t[cur].a, &G = sm.u.t[cur].b;
+    f16v s = zero16(), dp = zero16();
+    {
+      h8 x[kKS];
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) {
+        const Pair q = ld_row<D>(Q, roff ^ row_step(ks));
+        x[ks] = q.h;
+        // (The forward's order: its A operand is this B.)
+        s = mma(q.l, kB[ks].h, s);
+        s = mma(q.h, kB[ks].l, s);
+      }
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) s = mma(x[ks], kB[ks].h, s);
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) {
+        const Pair y = ld_row<D>(G, roff ^ row_step(ks));
+        x[ks] = y.h;
+        dp = mma_small(y, vB[ks], dp);
+      }
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) dp = mma(x[ks], vB[ks].h, dp);
+    }
+    if (kFull) {
+      load(u + 2);
+      pin_loads();
+    }
+    // Live: register r's query, q0 + 4 g + 8 i + e, below SQ and, causal, not before the key.
+    const int hi = key < a.SK ? SQ - q0 - 4 * g : 0;
+    const int least = a.causal && key >= prefix ? key - off - q0 - 4 * g : 0;
+    auto weights = [&](auto capc) {
+      const float base = static_cast<float>(q0 + 4 * g + off - key);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f4 L = ld4(&sm.l[cur][8 * i + 4 * g]), Dv = ld4(&sm.d[cur][8 * i + 4 * g]);
+        const f4 uq = ld4(&sm.ua[cur][8 * i + 4 * g]), ug = ld4(&sm.ub[cur][8 * i + 4 * g]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * i + e;
+          float slope = 1.0f, x;
+          if constexpr (kMods) {
+            x = score<decltype(capc)::value>(s[r], a.cap2, slope2, base + static_cast<float>(8 * i + e), slope) + L[e];
+          } else {
+            x = fmaf(s[r], cs * uq[e], L[e]);
+          }
+          x = exp2_hw(x) * ug[e];
+          const bool live = kFull || (8 * i + e < hi && 8 * i + e >= least &&
+                                      (all_ids == nullptr || (sm.ids.tile[cur][8 * i + e + 4 * g] == ids.mine && ids.mine >= 0)));
+          const float p = live ? x : 0.0f;
+          float y = p * fmaf(dp[r], cg, -Dv[e]) * uq[e];
+          if constexpr (kMods && decltype(capc)::value != 0) y *= slope;
+          dp[r] = live ? y : 0.0f;
+          s[r] = p;
+        }
+      }
+    };
+    if constexpr (kMods) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f4 uq = ld4(&sm.ua[cur][8 * i + 4 * g]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[4 * i + e] *= cs * uq[e];
+      }
+      by_cap(a, s, weights);
+    } else {
+      weights(Const<0>{});
+    }
+    pin_acc(dv);
+    pin_acc(dk);
+    const float mp = max_weight(s), md = max_weight(dp);
+    if (__builtin_amdgcn_ballot_w64(mp * psc > kMaxWeight || md * dsc > kMaxWeight) != 0) {
+      fit_scale(mp, psc, dv);
+      fit_scale(md, dsc, dk);
+      pin_acc(dv);
+      pin_acc(dk);
+    }
+    {
+      const Pair p0 = split_acc<0>(s, psc), p1 = split_acc<1>(s, psc);
+#pragma unroll
+      for (int dt = 0; dt < kDT; ++dt) {
+        dv[dt] = mma3(ld_col<D>(G, coff ^ col_step(dt), 0), p0, dv[dt]);
+        dv[dt] = mma3(ld_col<D>(G, coff ^ col_step(dt), 1), p1, dv[dt]);
+      }
+    }
+    if (kFull) {
+      load_o(u + 2);
+      pin_loads();
+    }
+    {
+      const Pair p0 = split_acc<0>(dp, dsc), p1 = split_acc<1>(dp, dsc);
+#pragma unroll
+      for (int dt = 0; dt < kDT; ++dt) {
+        dk[dt] = mma3(ld_col<D>(Q, coff ^ col_step(dt), 0), p0, dk[dt]);
+        dk[dt] = mma3(ld_col<D>(Q, coff ^ col_step(dt), 1), p1, dk[dt]);
+      }
+    }
+  };
+  // What the wave's keys are seen by, of a step's tile.
+  auto seen = [&](int u, int q0) {
+    if (!wave_live) return static_cast<int>(kNone);
+    const bool before = a.causal && kw0 >= prefix;  // (else some key of the wave is in the prefix)
+    if (before && q0 + kRows - 1 + off < kw0) return static_cast<int>(kNone);
+    const bool whole = q0 + kRows <= SQ && kw0 + kRows <= a.SK &&
+                       (!a.causal || kw0 + kRows - 1 <= q0 + off || kw0 + kRows <= prefix);
+    const int sees = whole ? kAll : kSome;
+    return all_ids == nullptr ? sees : among(sm.ids.tile[u & 1][j], ids, sees);
+  };
+  // (The staging of steps with a mask is outside their branch: in both its arms the loaded registers and the
+  // sums spill where they join.)
+  __syncthreads();
+  int u = 0;
+  while (u < steps) {
+    int hh, q0 = place(u, hh), sees;
+    while (u < steps && (sees = seen(u, q0 = place(u, hh))) == kAll) {
+      tile(Const<1>{}, u, q0, kMods ? slope_of(a, h0 + hh) : 0.0f);
+      __syncthreads();
+      ++u;
+    }
+    while (u < steps && (sees = seen(u, q0 = place(u, hh))) != kAll) {
+      store(u + 1);
+      load(u + 2);
+      load_o(u + 2);
+      pin_loads();
+      if (sees == kSome) tile(Const<0>{}, u, q0, kMods ? slope_of(a, h0 + hh) : 0.0f);
+      __syncthreads();
+      ++u;
+    }
+  }
+  if (!wave_live) return;
+  // The two factors of dK and of dV: the second is a power of two, exact where it is subnormal.
+  float fk = pow2(-kTop) * a.scale, fk2 = pow2(-kp) / dsc, fv = pow2(-kTop - kp), fv2 = 1.0f / psc;
+  const float z = probe_finite<kDT>(dk, probe_finite<kDT>(dv, fk * 0.0f));
+  if (__builtin_amdgcn_ballot_w64(key < a.SK && !(z == 0.0f)) != 0) {
+    scored_keys_fp32<D>(a, b, hk, kw0, t0, t0 + n, sm.u.o[w], dk, dv, late(lane));
+    fk = a.scale, fk2 = fv = fv2 = 1.0f;
+  }
+  const int lane_e = late(lane);
+  const int64_t stride = static_cast<int64_t>(2) * HK * D;
+  store_rows<D>(dk, fk, fk2, sm.u.o[w], dkv, stride, a.SK - kw0, lane_e);
+  store_rows<D>(dv, fv, fv2, sm.u.o[w], dkv + stride / 2, stride, a.SK - kw0, lane_e);
+}
+
+template <int D, bool kMods>
+__device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D>& sm, int item) {
+  constexpr int kKS = D / 16, kDT = D / 32;
+  const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, g = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int off = a.SK - a.SQ, bh = item / a.nqb, qb = item % a.nqb, b = bh / a.H, h = bh % a.H, hk = h / a.G;
+  const int qw0 = qb * kBlock + w * kRows, qi = qw0 + j, qc = min(qi, a.SQ - 1), pos = qc + off;
+  const int prefix = prefix_of(a, b);
+  const int32_t* all_ids = ids_of(a, b);
+  const int end = last_key(a, min(qb * kBlock + kBlock, a.SQ) - 1 + off, prefix) + 1;
+  const int lim = last_key(a, pos, prefix);
+  const int lo = last_key(a, min(qw0, a.SQ - 1) + off, prefix);
+  const int hi = last_key(a, min(qw0 + kRows, a.SQ) - 1 + off, prefix);
+  const bool wave_live = qw0 < a.SQ;
+  int t0 = 0, t1 = (end + kRows - 1) / kRows;
+  Ids ids{0, 0, 0, true};
+  if (all_ids != nullptr) {
+    ids.take(all_ids[pos]);
+    int first, last;
+    find_ids(sm.ids, ids, all_ids, 0, end, w, tid, first, last);
+    t0 = first / kRows, t1 = first < last ? (last + kRows - 1) / kRows : t0;
+  }
+  float* dq_rows = a.dq + ((static_cast<int64_t>(b) * a.SQ + qw0) * a.H + h) * D;
+  if (t0 >= t1) {  // no key was seen
+    for (int i = lane; i < min(a.SQ - qw0, kRows) * (D / 4); i += 64) {
+      st4(dq_rows + static_cast<int64_t>(i / (D / 4)) * a.H * D + i % (D / 4) * 4, f4{});
+    }
+    return;
+  }
+  const Operand kop{reinterpret_cast<const char*>(a.k.p + b * a.k.sb + hk * a.k.sh),
+                    static_cast<unsigned>(a.k.ss) * 4u};
+  const Operand vop{reinterpret_cast<const char*>(a.v.p + b * a.v.sb + hk * a.v.sh),
+                    static_cast<unsigned>(a.v.ss) * 4u};
+  Stage<D, kW> st;
+  int id_next = 0;
+  auto load = [&](int t) {
+    st.load(kop, vop, t * kRows, a.SK - 1, w, lane);
+    if (all_ids != nullptr && w == 0) id_next = all_ids[min(t * kRows + j, a.SK - 1)];
+  };
+  auto store = [&](int t) {
+    const int put = t & 1;
+    st.store(sm.u.t[put].a, sm.u.t[put].b, sm.ua[put], sm.ub[put], w, lane);
+    if (all_ids != nullptr && w == 0) sm.ids.tile[put][j] = t * kRows + j < a.SK ? id_next : -1;
+  };
+  Pair qB[kKS], gB[kKS];
+  const int kp = half_log2(a.SK);
+  float uq, ug, L, Dq;  // L: kp - L log2 e
+  {
+    OwnRows<D> oq, og, oo;
+    load(t0);
+    oq.load(a.q.p + b * a.q.sb + h * a.q.sh + qc * a.q.ss, g);
+    og.load(a.d_o.p + b * a.d_o.sb + h * a.d_o.sh + qc * a.d_o.ss, g);
+    oo.load(a.o + ((static_cast<int64_t>(b) * a.SQ + qc) * a.H + h) * D, g);
+    L = a.lse[static_cast<int64_t>(bh) * a.SQ + qc];
+    Dq = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < kKS; ++ks) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) Dq = fmaf(og.x[ks][e / 4][e % 4], oo.x[ks][e / 4][e % 4], Dq);
+    }
+    Dq = pair_sum(Dq) * pow2(kTop);  // (dP and D times 2^kTop meet K's unit)
+    L = shifted_l(L, kp);
+    uq = oq.split(1.0f, qB);
+    ug = og.split(1.0f, gB);
+    store(t0);
+    load(t0 + 1);
+  }
+  f16v dq[kDT];
+#pragma unroll
+  for (int dt = 0; dt < kDT; ++dt) dq[dt] = zero16();
+  const float cs = a.scale * kLog2e * (kMods ? a.unit : 1.0f) * uq, cg = ug;
+  const float slope2 = kMods ? slope_of(a, h) : 0.0f, fpos = static_cast<float>(pos - 4 * g);
+  float dsc = kMaxScale;
+  const int roff0 = row_off<D>(j, g), coff0 = col_off<D>(lane);
+
+  auto tile = [&](auto fullc, int t) {
+    constexpr bool kFull = decltype(fullc)::value != 0;
+    const int roff = late(roff0), coff = late(coff0), cur = t & 1, kt0 = t * kRows;
+    store(t + 1);
+    const Tile<D>&K = sm.u.t[cur].a, &V = sm.u.t[cur].b;
+    f16v s = zero16(), dp = zero16();
+    {
+      h8 x[kKS];
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) {
+        const Pair k = ld_row<D>(K, roff ^ row_step(ks));
+        x[ks] = k.h;
+        s = mma_small(k, qB[ks], s);
+      }
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) s = mma(x[ks], qB[ks].h, s);
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) {
+        const Pair v = ld_row<D>(V, roff ^ row_step(ks));
+        x[ks] = v.h;
+        // (The key blocks' order: their A operand is this B.)
+        dp = mma(v.l, gB[ks].h, dp);
+        dp = mma(v.h, gB[ks].l, dp);
+      }
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) dp = mma(x[ks], gB[ks].h, dp);
+    }
+    load(t + 2);
+    pin_loads();
+    auto weights = [&](auto capc) {
+      const float base = fpos - static_cast<float>(kt0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f4 uk = ld4(&sm.ua[cur][8 * i + 4 * g]), uv = ld4(&sm.ub[cur][8 * i + 4 * g]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * i + e, key = kt0 + 8 * i + 4 * g + e;
+          float slope = 1.0f, x;
+          if constexpr (kMods) {
+            x = score<decltype(capc)::value>(s[r], a.cap2, slope2, base - static_cast<float>(8 * i + e), slope) + L;
+          } else {
+            x = fmaf(s[r], cs * uk[e], L);
+          }
+          x = exp2_hw(x) * fmaf(dp[r], cg * uv[e], -Dq) * uk[e];
+          if constexpr (kMods && decltype(capc)::value != 0) x *= slope;
+          const bool live = kFull || (key <= lim && (all_ids == nullptr || (sm.ids.tile[cur][8 * i + 4 * g + e] == ids.mine &&
+                                                                            ids.mine >= 0)));
+          dp[r] = live ? x : 0.0f;
+        }
+      }
+    };
+    if constexpr (kMods) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f4 uk = ld4(&sm.ua[cur][8 * i + 4 * g]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[4 * i + e] *= cs * uk[e];
+      }
+      by_cap(a, s, weights);
+    } else {
+      weights(Const<0>{});
+    }
+    pin_acc(dq);
+    const float md = max_weight(dp);
+    if (__builtin_amdgcn_ballot_w64(md * dsc > kMaxWeight) != 0) {
+      fit_scale(md, dsc, dq);
+      pin_acc(dq);
+    }
+    const Pair p0 = split_acc<0>(dp, dsc), p1 = split_acc<1>(dp, dsc);
+#pragma unroll
+    for (int dt = 0; dt < kDT; ++dt) {
+      dq[dt] = mma3(ld_col<D>(K, coff ^ col_step(dt), 0), p0, dq[dt]);
+      dq[dt] = mma3(ld_col<D>(K, coff ^ col_step(dt), 1), p1, dq[dt]);
+    }
+  };
+  __syncthreads();
+#pragma clang loop unroll(disable)
+  for (int t = t0; t < t1; ++t) {
+    int sees = !wave_live || t * kRows > hi ? kNone : t * kRows + kRows - 1 <= lo ? kAll : kSome;
+    if (all_ids != nullptr && sees != kNone) sees = among(sm.ids.tile[t & 1][j], ids, sees);
+    if (sees == kAll) {
+      tile(Const<1>{}, t);
+    } else if (sees == kSome) {
+      tile(Const<0>{}, t);
+    } else {
+      store(t + 1);
+      load(t + 2);
+      pin_loads();
+    }
+    __syncthreads();
+  }
+  if (!wave_live) return;
+  float f = pow2(-kTop) * a.scale, f2 = pow2(-kp) / dsc;
+  if (__builtin_amdgcn_ballot_w64(qi < a.SQ && !(probe_finite<kDT>(dq, f * 0.0f) == 0.0f)) != 0) {
+    scored_queries_fp32<D>(a, b, h, qw0, t0, t1, sm.u.o[w], dq, late(lane));
+    f = a.scale, f2 = 1.0f;
+  }
+  store_rows<D>(dq, f, f2, sm.u.o[w], dq_rows, static_cast<int64_t>(a.H) * D, a.SQ - qw0, late(lane));
+}
+
+template <int D, bool kMods, int WAVES>
+__global__ void __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES)))
+bwd_scored_kernel(ScoredArgs a) {
+  __shared__ __attribute__((aligned(16))) ScoredSmem<D> sm;
+  const int id = static_cast<int>(blockIdx.x), pairs = a.B * (a.H / a.G), BH = a.B * a.H, keys = a.nkb * pairs;
+  if (id < keys) {
+    // Causal: the low blocks (they are seen by every later query) first.
+    scored_keys<D, kMods>(a, sm, a.causal ? id % pairs * a.nkb + id / pairs : xcd_remap(id, keys));
+  } else {
+    const int i = id - keys;
+    scored_queries<D, kMods>(a, sm, a.causal ? i % BH * a.nqb + a.nqb - 1 - i / BH : xcd_remap(i, a.nqb * BH));
+  }
+}
+
+template <bool kMods>
+const void* fwd_fn(int d) {
+  return d == 32    ? reinterpret_cast<const void*>(fwd_scored_kernel<32, kMods, 4>)
+         : d == 128 ? reinterpret_cast<const void*>(fwd_scored_kernel<128, kMods, 2>)
+                    : reinterpret_cast<const void*>(fwd_scored_kernel<64, kMods, 3>);
+}
+template <bool kMods>
+const void* bwd_fn(int d) {
+  return d == 32    ? reinterpret_cast<const void*>(bwd_scored_kernel<32, kMods, 3>)
+         : d == 128 ? reinterpret_cast<const void*>(bwd_scored_kernel<128, kMods, 1>)
+                    : reinterpret_cast<const void*>(bwd_scored_kernel<64, kMods, 2>);
+}
+bool mods(const ScoredArgs& a) { return a.cap2 != 0.0f || a.slopes != nullptr; }
+int64_t blocks_of(int64_t rows) { return (rows + kBlock - 1) / kBlock; }
+
+}  // namespace
+
+int64_t scored_blocks(int64_t b, int64_t heads, int64_t rows) { return b * heads * blocks_of(rows); }
+
+ScoredPlan scored_plan(int64_t b, int64_t h, int64_t sq, int64_t sk, int64_t d) {
+  ScoredPlan p{1, 0, 0, 0};
+  const int64_t steps = (sk + kRows - 1) / kRows, blocks = scored_blocks(b, h, sq);
+  const int64_t slots = 256 * (d == 32 ? 4 : d == 64 ? 3 : 2);
+  // Chunks of the keys where the blocks do not fill the chip, of 8 tiles or more.
+  const int64_t target = std::max<int64_t>(8, (blocks * steps + slots - 1) / slots);
+  const int64_t want = steps >= 2 * target ? (steps + target - 1) / target : 1;
+  p.chunk = static_cast<int>(std::max<int64_t>(1, (steps + want - 1) / want));
+  p.nc = static_cast<int>(std::max<int64_t>(1, (steps + p.chunk - 1) / p.chunk));
+  if (p.nc > 1) {
+    const size_t parts = static_cast<size_t>(p.nc) * b * h * sq;
+    p.l_part = parts * d * sizeof(float);
+    p.bytes = p.l_part + parts * sizeof(double);
+  }
+  return p;
+}
+
+int launch_scored_forward(ScoredArgs a, int d, const ScoredPlan& plan, void* workspace, void* stream) {
+  a.nqb = static_cast<int>(blocks_of(a.SQ));
+  a.nc = plan.nc, a.chunk = plan.chunk;
+  a.o_part = static_cast<float*>(workspace);
+  a.l_part = reinterpret_cast<double*>(static_cast<char*>(workspace) + plan.l_part);
+  void* args[] = {&a};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const unsigned grid = static_cast<unsigned>(int64_t{a.B} * a.H * a.nqb * a.nc);
+  const hipError_t err = hipLaunchKernel(mods(a) ? fwd_fn<true>(d) : fwd_fn<false>(d), dim3(grid), dim3(64 * kW),
+                                         args, 0, s);
+  if (err != hipSuccess || a.nc == 1) return static_cast<int>(err);
+  const void* join = d == 32    ? reinterpret_cast<const void*>(join_scored_kernel<32>)
+                     : d == 128 ? reinterpret_cast<const void*>(join_scored_kernel<128>)
+                                : reinterpret_cast<const void*>(join_scored_kernel<64>);
+  const int64_t rows = int64_t{a.B} * a.H * a.SQ, per = 1024 / d;
+  return static_cast<int>(hipLaunchKernel(join, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(256), args,
+                                          0, s));
+}
+
+int launch_scored_backward(ScoredArgs a, int d, void* stream) {
+  a.nqb = static_cast<int>(blocks_of(a.SQ)), a.nkb = static_cast<int>(blocks_of(a.SK));
+  a.nc = 1;
+  void* args[] = {&a};
+  const int64_t grid = scored_blocks(a.B, a.H / a.G, a.SK) + scored_blocks(a.B, a.H, a.SQ);
+  return static_cast<int>(hipLaunchKernel(mods(a) ? bwd_fn<true>(d) : bwd_fn<false>(d),
+                                          dim3(static_cast<unsigned>(grid)), dim3(64 * kW), args, 0,
+                                          static_cast<hipStream_t>(stream)));
+}
+
+}  // namespace fattn

@@ -653,6 +653,142 @@ Tensor fused_cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, 
                                   : cross_forward(qa, ka, va, scale, lengths)[0];
 }
 
+// --- Scored attention ------------------------------------------------------------------------------
+
+constexpr const char* kScored = "fused_scored_attention";
+
+// What a call has beside its operands (tensors undefined where absent; cap 0: none).
+struct Scores {
+  double scale;
+  bool causal;
+  float cap;
+  Tensor slopes, documents, prefix;
+};
+void check_scored(const Tensor& q, const Tensor& k, const Tensor& v, const Scores& how) {
+  require(kScored, "q", q, 4, nullptr, {kF32});
+  require(kScored, "k", k, 4, &q, {kF32});
+  require(kScored, "v", v, 4, &q, {kF32});
+  const int64_t b = q.size(0), sk = k.size(2);
+  if (k.sizes() != v.sizes() || k.size(0) != b || k.size(3) != q.size(3) || q.size(2) > sk) {
+    throw OpError(std::string(kScored) + ": q [b, h, sq, d] and k, v [b, kv_heads, sk, d], sq <= sk, expected, "
+                  "got " + shape_of(q.sizes()) + " " + shape_of(k.sizes()) + " " + shape_of(v.sizes()));
+  }
+  check_slopes(kScored, how.slopes, q.size(1), q);
+  if (how.documents.defined()) {
+    const Tensor& t = how.documents;
+    require(kScored, "documents", t, 2, &q, {kI32});
+    if (t.size(0) != b || t.size(1) != sk || (sk > 1 && t.stride(1) != 1)) {
+      throw OpError(std::string(kScored) + ": documents [" + std::to_string(b) + ", " + std::to_string(sk) +
+                    "] with contiguous rows expected, got " + shape_of(t.sizes()));
+    }
+  }
+  if (how.prefix.defined()) {
+    require(kScored, "prefix", how.prefix, 1, &q, {kI32});
+    if (how.prefix.size(0) != b || !how.prefix.is_contiguous()) {
+      throw OpError(std::string(kScored) + ": contiguous prefix lengths [" + std::to_string(b) +
+                    "] expected, got " + shape_of(how.prefix.sizes()));
+    }
+  }
+}
+int64_t rows_apart(const Tensor& t) { return t.defined() ? t.stride(0) : 0; }
+
+// As cross_forward and cross_backward.
+Tensors scored_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Scores& how) {
+  const int64_t b = q.size(0), h = q.size(1), sq = q.size(2), d = q.size(3), hk = k.size(1), sk = k.size(2);
+  Tensor out = at::empty_strided({b, h, sq, d}, {sq * h * d, d, h * d, 1}, q.options());
+  Tensor lse = at::empty({b, h, sq}, q.options());
+  const size_t bytes = fattn_scored_workspace_bytes(b, h, hk, sq, sk, d);
+  const Tensor ws = workspace(q, bytes);
+  launch(q, [&](void* stream) {
+    return fattn_scored_forward(f32(q), q.strides().data(), f32(k), k.strides().data(), f32(v),
+                                v.strides().data(), b, h, hk, sq, sk, d, static_cast<float>(how.scale),
+                                how.causal, how.cap, static_cast<const float*>(address(how.slopes)),
+                                ints(how.documents), rows_apart(how.documents), ints(how.prefix),
+                                static_cast<float*>(out.data_ptr()), static_cast<float*>(lse.data_ptr()),
+                                address(ws), bytes, stream);
+  });
+  return {out, lse};
+}
+Tensors scored_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Scores& how,
+                        const Tensor& out, const Tensor& lse, const Tensor& grad) {
+  const int64_t b = q.size(0), h = q.size(1), sq = q.size(2), d = q.size(3), hk = k.size(1), sk = k.size(2);
+  const Tensor g = aligned_rows(grad);
+  Tensor dq = at::empty_strided({b, h, sq, d}, {sq * h * d, d, h * d, 1}, q.options());
+  Tensor dkv = at::empty({b, sk, 2, hk, d}, q.options());
+  launch(q, [&](void* stream) {
+    return fattn_scored_backward(f32(q), q.strides().data(), f32(k), k.strides().data(), f32(v),
+                                 v.strides().data(), b, h, hk, sq, sk, d, static_cast<float>(how.scale),
+                                 how.causal, how.cap, static_cast<const float*>(address(how.slopes)),
+                                 ints(how.documents), rows_apart(how.documents), ints(how.prefix), f32(out),
+                                 f32(lse), f32(g), g.strides().data(), static_cast<float*>(dq.data_ptr()),
+                                 static_cast<float*>(dkv.data_ptr()), stream);
+  });
+  return {dq, dkv.select(2, 0).transpose(1, 2), dkv.select(2, 1).transpose(1, 2)};
+}
+
+// As NotTwice.
+struct ScoredNotTwice : Function<ScoredNotTwice> {
+  static Tensors forward(AutogradContext*, const Tensor& dq, const Tensor& dk, const Tensor& dv,
+                         const Tensor&, const Tensor&, const Tensor&, const Tensor&) {
+    return {dq.view_as(dq), dk.view_as(dk), dv.view_as(dv)};
+  }
+  static Tensors backward(AutogradContext*, const Tensors&) {
+    return in_backward([]() -> Tensors {
+      throw OpError(std::string(kScored) + ": its gradient is not differentiable");
+    });
+  }
+};
+struct ScoredNode : Function<ScoredNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                        const Scores& how) {
+    const Tensors out = scored_forward(q, k, v, how);
+    ctx->save_for_backward({q, k, v, how.slopes, how.documents, how.prefix, out[0], out[1]});
+    ctx->saved_data["scale"] = how.scale;
+    ctx->saved_data["causal"] = how.causal;
+    ctx->saved_data["cap"] = static_cast<double>(how.cap);
+    return out[0];
+  }
+  static Tensors backward(AutogradContext* ctx, const Tensors& grads) {
+    const Tensors s = ctx->get_saved_variables();
+    return in_backward([&]() -> Tensors {
+      no_tangents(kScored, {&grads[0]});
+      // (Hooks on saved tensors may have replaced them: save_on_cpu brings them back in another layout.)
+      auto whole = [](const Tensor& t) { return t.defined() ? t.contiguous() : t; };
+      const Scores how{ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool(),
+                       static_cast<float>(ctx->saved_data["cap"].toDouble()), whole(s[3]), rows_of_ids(s[4]),
+                       whole(s[5])};
+      check_scored(s[0], s[1], s[2], how);
+      require(kScored, "the saved output", s[6], 4, &s[0], {kF32});
+      require(kScored, "the saved log-sums", s[7], 3, &s[0], {kF32});
+      if (s[6].sizes() != s[0].sizes() || s[7].sizes() != s[0].sizes().slice(0, 3) ||
+          grads[0].sizes() != s[0].sizes()) {
+        throw OpError(std::string(kScored) + ": saved tensors came back in other shapes");
+      }
+      Tensors to;
+      {
+        const c10::AutoGradMode off(false);
+        to = scored_backward(aligned_rows(s[0]), aligned_rows(s[1]), aligned_rows(s[2]), how, merged(s[6]),
+                             s[7].contiguous(), grads[0]);
+      }
+      if (c10::GradMode::is_enabled()) {
+        to = ScoredNotTwice::apply(to[0], to[1], to[2], s[0], s[1], s[2], grads[0]);
+      }
+      to.resize(4);  // (none for `how`)
+      return to;
+    });
+  }
+  static Tensor rows_of_ids(const Tensor& t) {
+    return !t.defined() || t.stride(1) == 1 || t.size(1) <= 1 ? t : t.contiguous();
+  }
+};
+
+Tensor fused_scored_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Scores& how) {
+  no_tangents(kScored, {&q, &k, &v, &how.slopes});
+  check_scored(q, k, v, how);
+  const Tensor qa = aligned_rows(q), ka = aligned_rows(k), va = aligned_rows(v);
+  return records({&qa, &ka, &va}) ? ScoredNode::apply(qa, ka, va, how) : scored_forward(qa, ka, va, how)[0];
+}
+
 // --- Python ----------------------------------------------------------------------------------------
 
 // The positional arguments of a call, read in turn.
@@ -826,6 +962,21 @@ PyObject* py_cross_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+PyObject* py_scored_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return entry("fused_scored_attention", args, n, [](Args& a) {
+    const Tensor &q = a.tensor("q"), &k = a.tensor("k"), &v = a.tensor("v");
+    Scores how;
+    how.scale = a.number(), how.causal = a.truth(), how.cap = check_cap(kScored, a.maybe_cap());
+    how.slopes = a.maybe("slopes"), how.documents = a.maybe("documents"), how.prefix = a.maybe("prefix");
+    Tensor out;
+    {
+      const Unlocked unlocked;
+      out = fused_scored_attention(q, k, v, how);
+    }
+    return one(out);
+  });
+}
+
 PyMethodDef g_methods[] = {
 #define ENTRY(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL, ""}
     ENTRY("rotary", py_rotary),
@@ -834,6 +985,7 @@ PyMethodDef g_methods[] = {
     ENTRY("paged_attention", py_paged_attention),
     ENTRY("paged_read", py_paged_read),
     ENTRY("cross_attention", py_cross_attention),
+    ENTRY("scored_attention", py_scored_attention),
 #undef ENTRY
     {nullptr, nullptr, 0, nullptr}};
 

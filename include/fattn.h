@@ -214,7 +214,8 @@ int fattn_backward(const float* q, int64_t q_offset, const int64_t q_shape[4],
  * Operators around self-attention: rotary positions, a paged key-value cache, cross attention.
  * None has a counterpart in the reference. Element types are FATTN_F32, FATTN_F16, FATTN_BF16;
  * strides are in elements, head_dim contiguous. Messages are prefixed with the operator's name
- * (`fused_rotary:`, `paged_append:`, `paged_attention:`, `fused_cross_attention:`).
+ * (`fused_rotary:`, `paged_append:`, `paged_attention:`, `paged_read:`, `fused_cross_attention:`,
+ * `fused_scored_attention:`).
  * ------------------------------------------------------------------------------------------ */
 #define FATTN_F32 0
 #define FATTN_F16 1
@@ -323,6 +324,34 @@ int fattn_cross_backward(const float* q, const int64_t q_strides[3], const float
                          const int32_t* key_lengths, float scale, const float* out, const float* lse,
                          const float* d_o, const int64_t do_strides[3], float* dq, float* dkv,
                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention of scores of other forms, fp32: q [b, heads, sq, d], the last sq of sk positions, to k, v
+ * [b, kv_heads, sk, d] (strides {batch, head, seq}, rows 16-byte aligned). A score x = scale q.k is taken as
+ * cap tanh(x / cap) (cap 0: as it is; else 1e-30 to 1e30), less slopes[head] times the distance of the
+ * positions (NULL: none; finite floats). A query sees the keys at its position or before it, and the first
+ * prefix[b] of the sample (NULL: none; outside [0, sk]: the nearest), or with causal 0 all; of these, with
+ * documents ([b, sk] ids, rows document_stride apart), those of its own id, a token of a negative id none, and
+ * it is seen by none. out [b, sq, heads, d] contiguous, lse [b, heads, sq]; a query that sees no key has out 0
+ * and lse -infinity. Query head i reads key head i / (heads / kv_heads). The workspace is as
+ * fattn_cross_forward's. Reruns are bit-identical. */
+size_t fattn_scored_workspace_bytes(int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk,
+                                    int64_t d);
+int fattn_scored_forward(const float* q, const int64_t q_strides[3], const float* k,
+                         const int64_t k_strides[3], const float* v, const int64_t v_strides[3],
+                         int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d,
+                         float scale, int causal, float cap, const float* slopes,
+                         const int32_t* documents, int64_t document_stride, const int32_t* prefix,
+                         float* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its gradient, as fattn_cross_backward's: dq [b, sq, heads, d] and dkv [b, sk, 2, kv_heads, d], contiguous,
+ * written whole (0 for what is not seen), in a fixed order. The slopes get none. */
+int fattn_scored_backward(const float* q, const int64_t q_strides[3], const float* k,
+                          const int64_t k_strides[3], const float* v, const int64_t v_strides[3],
+                          int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d,
+                          float scale, int causal, float cap, const float* slopes,
+                          const int32_t* documents, int64_t document_stride, const int32_t* prefix,
+                          const float* out, const float* lse, const float* d_o,
+                          const int64_t do_strides[3], float* dq, float* dkv, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Diagnostics (no counterpart in the reference).

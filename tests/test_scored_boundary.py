@@ -99,3 +99,91 @@ def test_python_refusals():
             call()
     with pytest.raises(TypeError):
         cfa.paged_attention(q, pages, pages, ints[None], ints, 1.0, cap="much")
+
+
+# --- Scored attention -------------------------------------------------------------------------------
+
+
+def forward(b=1, heads=1, hk=1, sq=1, sk=1, d=64, q=BAD, k=BAD, qst=ST, kst=ST, cap=0.0, documents=None, dst=0,
+            out=BAD, ws=BAD, size=1 << 40):
+    return _lib.lib().fattn_scored_forward(q, qst, k, kst, k, kst, b, heads, hk, sq, sk, d, 1.0, 1, cap, None,
+                                           documents, dst, None, out, BAD, ws, size, None)
+
+
+def backward(b=1, heads=1, hk=1, sq=1, sk=1, d=64, q=BAD, k=BAD, qst=ST, kst=ST, cap=0.0, documents=None, dst=0,
+             out=BAD, g=BAD, gst=ST, dq=BAD, dkv=BAD):
+    return _lib.lib().fattn_scored_backward(q, qst, k, kst, k, kst, b, heads, hk, sq, sk, d, 1.0, 1, cap, None,
+                                            documents, dst, None, out, BAD, g, gst, dq, dkv, None)
+
+
+@pytest.mark.parametrize("call", [forward, backward])
+def test_scored_refusals(call):
+    refused(call(b=-1), _lib.FATTN_EINVAL, "fused_scored_attention: negative size")
+    refused(call(sq=-1), _lib.FATTN_EINVAL, "negative size")
+    refused(call(sq=3, sk=2), _lib.FATTN_EINVAL, "3 queries are more than the 2 positions")
+    refused(call(d=48), _lib.FATTN_EHEADDIM, "32, 64 or 128, got 48")
+    refused(call(heads=3, hk=2), _lib.FATTN_EINVAL, "3 query heads are no multiple of 2 key heads")
+    refused(call(heads=0), _lib.FATTN_EINVAL, "0 query heads")
+    for cap in (-1.0, 1e-31, float("inf"), float("nan")):
+        refused(call(cap=cap), _lib.FATTN_EINVAL, "a cap from 1e-30 to 1e30")
+    refused(call(q=None), _lib.FATTN_EINVAL, "null operand")
+    refused(call(k=None), _lib.FATTN_EINVAL, "null operand")
+    refused(call(out=None), _lib.FATTN_EINVAL, "null operand")
+    refused(call(q=ODD), _lib.FATTN_EALIGN, "16-byte aligned")
+    refused(call(k=ODD), _lib.FATTN_EALIGN, "16-byte aligned")
+    refused(call(out=ODD), _lib.FATTN_EALIGN, "16-byte aligned")
+    refused(call(documents=BAD, dst=-1), _lib.FATTN_EINVAL, "negative strides")
+    refused(call(sk=2, kst=_lib.arr([0, 0, 66])), _lib.FATTN_EALIGN, "16-byte aligned")
+    refused(call(sk=2, kst=_lib.arr([0, 0, -4])), _lib.FATTN_EINVAL, "negative strides")
+    refused(call(sk=5, kst=_lib.arr([0, 0, 1 << 28])), _lib.FATTN_ERANGE, "4 GiB")
+    refused(call(b=1 << 16, heads=1 << 10, hk=1 << 10, sk=1 << 10), _lib.FATTN_ERANGE, "32-bit")
+    refused(call(sk=(1 << 31) - 1), _lib.FATTN_ERANGE, "32-bit")
+    assert call(b=0, q=None) == 0 and call(heads=0, hk=0) == 0 and call(sq=0, sk=0, k=None) == 0
+
+
+def test_scored_workspace_and_gradient_refusals():
+    L = _lib.lib()
+    need = L.fattn_scored_workspace_bytes(2, 4, 4, 1, 4096, 64)
+    assert need > 0
+    for ws, size in ((None, need), (ODD, need), (BAD, need - 1)):
+        refused(forward(b=2, heads=4, hk=4, sk=4096, ws=ws, size=size), _lib.FATTN_EWORKSPACE, str(need))
+    assert L.fattn_scored_workspace_bytes(64, 8, 8, 4096, 4096, 64) == 0
+    assert L.fattn_scored_workspace_bytes(2, 4, 3, 1, 4096, 64) == 0
+    assert L.fattn_scored_workspace_bytes(2, 4, 4, 5000, 4096, 64) == 0
+    refused(backward(g=None), _lib.FATTN_EINVAL, "null operand")
+    refused(backward(dq=None), _lib.FATTN_EINVAL, "null operand")
+    refused(backward(dkv=None), _lib.FATTN_EINVAL, "null operand")
+    refused(backward(g=ODD), _lib.FATTN_EALIGN, "16-byte aligned")
+    refused(backward(sq=2, sk=2, gst=_lib.arr([0, 0, 2])), _lib.FATTN_EALIGN, "16-byte aligned")
+    refused(backward(sq=5, sk=5, gst=_lib.arr([0, 0, 1 << 28])), _lib.FATTN_ERANGE, "4 GiB")
+
+
+def test_scored_python_refusals():
+    q, ids = torch.randn(1, 2, 3, 64), torch.zeros(1, 3, dtype=torch.int32)
+    for call, text in [
+        (lambda: cfa.fused_scored_attention(q, q, q, 1.0, True), "not on a HIP device"),
+        (lambda: cfa.fused_scored_attention(q.double(), q, q, 1.0, True), "must be float32"),
+        (lambda: cfa.fused_scored_attention(q[0], q, q, 1.0, True), "4 dimensions"),
+        (lambda: cfa.fused_scored_attention(q, q, [1], 1.0, True), "must be a tensor"),
+        (lambda: cfa.fused_scored_attention(q, q, q, 1.0, True, cap=-1.0), "a cap from"),
+    ]:
+        with pytest.raises(cfa.FusedAttentionError, match=text):
+            call()
+    with pytest.raises(TypeError):
+        cfa.fused_scored_attention(q, q, q, None, True)
+
+
+def test_forward_mode_refused():
+    import torch.autograd.forward_ad as forward_ad
+
+    x, ints, s = torch.randn(1, 2, 3, 64), torch.zeros(1, dtype=torch.int32), torch.zeros(2)
+    with forward_ad.dual_level():
+        dual, slopes = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(s, torch.ones_like(s))
+        for call in (lambda: cfa.fused_scored_attention(dual, x, x, 1.0, True),
+                     lambda: cfa.fused_scored_attention(x, dual, x, 1.0, True),
+                     lambda: cfa.fused_scored_attention(x, x, dual, 1.0, True),
+                     lambda: cfa.fused_scored_attention(x, x, x, 1.0, True, slopes=slopes),
+                     lambda: cfa.paged_attention(x[:, :, :1], x, x, ints[None], ints, 1.0, slopes=slopes),
+                     lambda: cfa.paged_read(dual, x, ints[None], ints, 1)):
+            with pytest.raises(cfa.FusedAttentionError, match="no forward-mode derivative"):
+                call()

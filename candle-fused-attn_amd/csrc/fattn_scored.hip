@@ -25,11 +25,12 @@
 namespace fattn {
 namespace {
 
+typedef int i4 __attribute__((ext_vector_type(4)));
 constexpr int kW = 4;                    // waves of a workgroup
 constexpr int kBlock = kW * kRows;       // its rows
 constexpr double kLn2 = 0.69314718055994530942;
-constexpr double kUnseen = -__builtin_inf();  // L of a row that sees nothing
-constexpr double kVanished = -1e308;          // of one whose every score is minus infinity
+constexpr double kUnseen = -__builtin_inf();  // L of a row that sees nothing (in a chunk)
+constexpr float kFirstRef = -3e38f;           // the softmax's reference before the first score
 enum { kNone, kSome, kAll };                  // what a wave sees of a tile
 
 // --- Who sees whom -----------------------------------------------------------------------------
@@ -45,7 +46,7 @@ __device__ __forceinline__ int wave_most(int x) {
 }
 // LDS of the ids: those of the staged tiles, and what the waves find.
 struct IdSmem {
-  int tile[2][kRows];
+  __attribute__((aligned(16))) int tile[2][kRows];
   int found[2][kW][2];
 };
 // A wave's ids (one per lane j, both halves alike) and its block's.
@@ -104,36 +105,45 @@ __device__ __forceinline__ float slope_of(const ScoredArgs& a, int h) {
 }
 
 // --- Scores ------------------------------------------------------------------------------------
-// One score in units of log2 e from x (in those units; with a cap in units of the cap), `far` the distance:
-// CAP 0: no cap, 1: every |x| of the wave's tile is at most kTanhSmall, 2: any. `slope`: dy / dx.
-template <int CAP>
-__device__ __forceinline__ float score(float x, float cap2, float slope2, float far, float& slope) {
-  float y = x;
-  if constexpr (CAP == 1) {
-    const float t = tanh_small(x);
-    slope = fmaf(-t, t, 1.0f);
-    y = cap2 * t;
-  } else if constexpr (CAP == 2) {
-    y = cap2 * tanh_any(x, slope);
-  } else {
-    slope = 1.0f;
-  }
-  return fmaf(-slope2, fabsf(far), y);
-}
-// One score by its definition, for the rows in fp32.
+// MODS: 0, x as it is; 1, less a slope times the distance; 2, capped, and less that. For 2 the products'
+// factor gives x / cap.
+// One score in units of log2 e by its definition, for the rows in fp32, and dy / dx.
 __device__ __forceinline__ float score_fp32(const ScoredArgs& a, float dot, float slope2, int far, float& slope) {
-  const float x = dot * (a.scale * kLog2e * a.unit);
-  return a.cap2 != 0.0f ? score<2>(x, a.cap2, slope2, static_cast<float>(far), slope)
-                        : score<0>(x, 0.0f, slope2, static_cast<float>(far), slope);
+  float y = dot * (a.scale * kLog2e * a.unit);
+  slope = 1.0f;
+  if (a.cap2 != 0.0f) y = a.cap2 * tanh_any(y, slope);
+  return fmaf(-slope2, fabsf(static_cast<float>(far)), y);
 }
+// Nothing is scheduled across: sixteen polynomials side by side take more registers than there are.
+__device__ __forceinline__ void few_at_once() { __builtin_amdgcn_sched_barrier(0); }
+// x / cap of a wave's tile to y and, times `fn(r, dy / dx)`. (Nearly always every |x| / cap is small, and the
+// polynomial alone is half of the work.)
 template <typename F>
-__device__ __forceinline__ void by_cap(const ScoredArgs& a, const f16v& x, F fn) {
-  if (a.cap2 == 0.0f) {
-    fn(Const<0>{});
-  } else if (__builtin_amdgcn_ballot_w64(max_weight(x) > kTanhSmall) == 0) {
-    fn(Const<1>{});
+__device__ __forceinline__ void capped(f16v& x, float cap2, F fn) {
+  if (__builtin_amdgcn_ballot_w64(max_weight(x) > kTanhSmall) == 0) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float t = tanh_small(x[r]);
+      x[r] = cap2 * t;
+      fn(r, fmaf(-t, t, 1.0f));
+      if (r % 4 == 3) few_at_once();
+    }
   } else {
-    fn(Const<2>{});
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      float slope;
+      x[r] = cap2 * tanh_any(x[r], slope);
+      fn(r, slope);
+      if (r % 2 == 1) few_at_once();
+    }
+  }
+}
+// y less the slope times the distance, of register r |base + sign (8 (r / 4) + r % 4)|.
+template <int SIGN>
+__device__ __forceinline__ void lowered(f16v& y, float slope2, float base) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    y[r] = fmaf(-slope2, fabsf(base + static_cast<float>(SIGN * (8 * (r >> 2) + (r & 3)))), y[r]);
   }
 }
 
@@ -162,7 +172,6 @@ __device__ __forceinline__ void scored_rows_fp32(const ScoredArgs& a, int b, int
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) acc[dt] = zero16();
   float m = kNegInf, l = 0.0f;
-  bool seen = false;
   auto live = [&](int key) {
     return key <= lim && id >= 0 && (ids == nullptr || ids[min(key, a.SK - 1)] == id);
   };
@@ -177,7 +186,6 @@ __device__ __forceinline__ void scored_rows_fp32(const ScoredArgs& a, int b, int
       const bool is = live(key);
       float d;
       s[r] = is ? score_fp32(a, s[r], slope2, p - key, d) : kNegInf;
-      seen = seen || is;
       mn = fmaxf(mn, s[r]);
     }
     mn = pair_max(fmaxf(mn, kNegInf));
@@ -194,11 +202,11 @@ __device__ __forceinline__ void scored_rows_fp32(const ScoredArgs& a, int b, int
     sum_fp32<D, false>(s, vp, a.v.ss, k0, a.SK, live, so, acc, j, g);
   }
   l = pair_sum(l);
-  seen = pair_max(seen ? 1.0f : 0.0f) > 0.0f;
-  // (A row whose every score is minus infinity is NaN, as its formula: 0 / 0; a chunk of such weighs nothing.)
-  store(acc, !seen || (a.nc > 1 && l == 0.0f) ? 1.0f : 1.0f / l);
+  // (Every row with a document sees itself. One whose every score is minus infinity is NaN, as its formula:
+  // 0 / 0; a chunk of such weighs nothing.)
+  store(acc, l == 0.0f && (id < 0 || a.nc > 1) ? 1.0f : 1.0f / l);
   if (g == 0 && qg + j < a.SQ) {
-    const double L = !seen ? kUnseen : l == 0.0f ? kVanished : static_cast<double>(m) * kLn2 + logf(l);
+    const double L = l == 0.0f ? kUnseen : static_cast<double>(m) * kLn2 + logf(l);
     put_l(a, chunk, (static_cast<int64_t>(b) * a.H + h) * a.SQ + qg + j, L);
   }
 }
@@ -302,7 +310,7 @@ __device__ __forceinline__ void scored_queries_fp32(const ScoredArgs& a, int b, 
 // --- Forward -----------------------------------------------------------------------------------
 // A workgroup: 128 queries of one head, over a range of key tiles; where the blocks are too few for the
 // chip the tiles are cut into chunks, whose O and L a second kernel joins in order.
-template <int D, bool kMods>
+template <int D, int MODS>
 __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
   constexpr int kKS = D / 16, kDT = D / 32, kOPitch = (D < 64 ? D : 64) + 4;
   struct Kv {
@@ -380,11 +388,11 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
     own.load(qp + min(qi, a.SQ - 1) * a.q.ss, g);
     store(t0);
     load(t0 + 1);
-    cq = own.split(a.scale < 0.0f ? -1.0f : 1.0f, q) * (fabsf(a.scale) * kLog2e * (kMods ? a.unit : 1.0f));
+    cq = own.split(a.scale < 0.0f ? -1.0f : 1.0f, q) * (fabsf(a.scale) * kLog2e * (MODS == 2 ? a.unit : 1.0f));
   }
-  const float slope2 = kMods ? slope_of(a, h) : 0.0f, fpos = static_cast<float>(pos - 4 * g);
+  const float slope2 = MODS != 0 ? slope_of(a, h) : 0.0f, fpos = static_cast<float>(pos - 4 * g);
   f16v acc[kDT];  // O^T, in units of p / wsc and 2^-kTop
-  float m = kNegInf, lsum = 0.0f, wsc = kMaxScale;
+  float m = kFirstRef, lsum = 0.0f, wsc = kMaxScale;
 #pragma unroll
   for (int dt = 0; dt < kDT; ++dt) acc[dt] = zero16();
   const int roff0 = row_off<D>(j, g), coff0 = col_off<D>(lane);
@@ -395,8 +403,7 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
     pin_loads();
   };
   // (See fattn_pair_kernels.h for the sums' scales.)
-  auto tile = [&](auto fullc, int t) {
-    constexpr bool kFull = decltype(fullc)::value != 0;
+  auto tile = [&](int t, int sees) {
     const int roff = late(roff0), coff = late(coff0), kt0 = t * kRows, cur = t & 1;
     const Kv& kv = sm.t.kv[cur];
     stage(t);
@@ -412,34 +419,29 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
 #pragma unroll
       for (int ks = 0; ks < kKS; ++ks) s = mma(kh[ks], q[ks].h, s);
     }
-    // Live: register r's key, kt0 + 4 g + 8 (r / 4) + r % 4.
-    unsigned live = 0xffffu;
-    if constexpr (!kFull) {
-      const int left = lim - kt0 - 4 * g;
-      live = 0;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int at = 8 * (r >> 2) + (r & 3);
-        const bool is = at <= left && (all_ids == nullptr || sm.ids.tile[cur][at + 4 * g] == ids.mine);
-        live |= is ? 1u << r : 0u;
-      }
-      if (ids.mine < 0) live = 0;
-    }
-    if constexpr (kMods) {
+    if constexpr (MODS != 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const f4 uk = ld4(&sm.uk[cur][8 * i + 4 * g]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[4 * i + c] *= cq * uk[c];
       }
-      const float base = fpos - static_cast<float>(kt0);
-      by_cap(a, s, [&](auto capc) {
+      if constexpr (MODS == 2) capped(s, a.cap2, [](int, float) {});
+      lowered<-1>(s, slope2, fpos - static_cast<float>(kt0));
+    }
+    // What is not seen is minus infinity: register r's key is kt0 + 4 g + 8 (r / 4) + r % 4.
+    if (sees == kSome) {
+      const int left = lim - kt0 - 4 * g;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float d;
-          s[r] = score<decltype(capc)::value>(s[r], a.cap2, slope2, base - static_cast<float>(8 * (r >> 2) + (r & 3)), d);
+      for (int i = 0; i < 4; ++i) {
+        i4 id{};
+        if (all_ids != nullptr) id = *reinterpret_cast<const i4*>(&sm.ids.tile[cur][8 * i + 4 * g]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const bool is = 8 * i + c <= left && id[c] == ids.mine && ids.mine >= 0;
+          s[4 * i + c] = is ? s[4 * i + c] : kNegInf;
         }
-      });
+      }
     }
     f16v e;
     float psum = 0.0f, wmax = 0.0f;
@@ -451,12 +453,11 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
       for (int i = 0; i < 4; ++i) {
         const f4 uv = ld4(&sm.uv[cur][8 * i + r0]);
         f4 uk{};
-        if constexpr (!kMods) uk = ld4(&sm.uk[cur][8 * i + r0]);
+        if constexpr (MODS == 0) uk = ld4(&sm.uk[cur][8 * i + r0]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int r = 4 * i + c;
-          const float x = exp2_hw(kMods ? s[r] - m : fmaf(s[r], cq * uk[c], -m));
-          const float p = kFull || (live >> r & 1) != 0 ? x : 0.0f;
+          const float p = exp2_hw(MODS != 0 ? s[r] - m : fmaf(s[r], cq * uk[c], -m));
           psum = r == 0 ? p : psum + p;
           e[r] = p * uv[c];
         }
@@ -471,13 +472,12 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
       asm("" : "+v"(r0));
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float x = kMods ? s[r] : s[r] * (cq * sm.uk[cur][8 * (r >> 2) + r0 + (r & 3)]);
-        tmax = fmaxf(tmax, kFull || (live >> r & 1) != 0 ? x : kNegInf);
+        tmax = fmaxf(tmax, MODS != 0 ? s[r] : s[r] * (cq * sm.uk[cur][8 * (r >> 2) + r0 + (r & 3)]));
       }
       const float ref = pair_max(tmax) - kRefTop;
       float to = wsc, alpha = 1.0f;
       if (!(pair_sum(psum) <= kRowTop) && ref > m) {
-        alpha = m == kNegInf ? 0.0f : exp2_hw(m - ref);
+        alpha = exp2_hw(m - ref);  // (0 from the first one)
         to = alpha > 0.0f ? fminf(to * pow2(-exponent(alpha)), kMaxScale) : kMaxScale;
         m = ref;
         lsum *= alpha;
@@ -498,19 +498,23 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
       acc[dt] = mma3(ld_col<D>(kv.v, coff ^ col_step(dt), 1), p1, acc[dt]);
     }
   };
+  auto seen = [&](int t) {
+    const int sees = !wave_live || t * kRows > hi ? kNone : t * kRows + kRows - 1 <= lo ? kAll : kSome;
+    return all_ids == nullptr || sees == kNone ? sees : among(sm.ids.tile[t & 1][j], ids, sees);
+  };
   __syncthreads();  // tile t0
-#pragma clang loop unroll(disable)
-  for (int t = t0; t < t1; ++t) {
-    int sees = !wave_live || t * kRows > hi ? kNone : t * kRows + kRows - 1 <= lo ? kAll : kSome;
-    if (all_ids != nullptr && sees != kNone) sees = among(sm.ids.tile[t & 1][j], ids, sees);
-    if (sees == kAll) {
-      tile(Const<1>{}, t);
-    } else if (sees == kSome) {
-      tile(Const<0>{}, t);
-    } else {
-      stage(t);
+  int t = t0, sees;
+  while (t < t1) {
+    while (t < t1 && (sees = seen(t)) != kNone) {
+      tile(t, sees);
+      __syncthreads();  // tile t + 1 is staged; every wave is done with tile t
+      ++t;
     }
-    __syncthreads();  // tile t + 1 is staged; every wave is done with tile t
+    while (t < t1 && seen(t) == kNone) {
+      stage(t);
+      __syncthreads();
+      ++t;
+    }
   }
   if (!wave_live) return;
 
@@ -522,7 +526,8 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
     store_rows<D>(x, f, f2, so, out + ((static_cast<int64_t>(b) * a.SQ + qw0) * a.H + h) * D,
                   static_cast<int64_t>(a.H) * D, a.SQ - qw0, lane_e);
   };
-  if (__builtin_amdgcn_ballot_w64(qi < a.SQ && !(probe_finite<kDT>(acc, l * 0.0f) == 0.0f)) != 0) {
+  const bool lost = l == 0.0f && ids.mine >= 0 && a.nc == 1;  // (every score is minus infinity)
+  if (__builtin_amdgcn_ballot_w64(qi < a.SQ && (lost || !(probe_finite<kDT>(acc, l * 0.0f) == 0.0f))) != 0) {
     scored_rows_fp32<D>(a, b, h, qw0, t0, t1, chunk, so, late(lane),
                         [&](const f16v (&x)[kDT], float inv) { put(x, inv, 1.0f); });
     return;
@@ -537,10 +542,10 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
     put_l(a, chunk, static_cast<int64_t>(bh) * a.SQ + qi, L);
   }
 }
-template <int D, bool kMods, int WAVES>
+template <int D, int MODS, int WAVES>
 __global__ void __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES)))
 fwd_scored_kernel(ScoredArgs a) {
-  scored_fwd<D, kMods>(a);
+  scored_fwd<D, MODS>(a);
 }
 
 // O and L of the chunks' [nc][b, s, h, d] and [nc][b, h, s]: O = sum_c w_c O_c / sum_c w_c, w_c =
@@ -569,7 +574,10 @@ __global__ void __launch_bounds__(256) join_scored_kernel(ScoredArgs a) {
     sum += w;
     x += ld4(a.o_part + (c * rows + row) * D + d) * w;
   }
-  st4(a.out + row * D + d, top == kUnseen ? f4{} : x * (top == kVanished ? __builtin_nanf("") : 1.0f / sum));
+  // (No chunk saw anything: a row without a document, or, NaN, scores that are all minus infinity.)
+  const int32_t* ids = ids_of(a, b);
+  const bool none = top == kUnseen && ids != nullptr && ids[row / a.H % a.SQ + a.SK - a.SQ] < 0;
+  st4(a.out + row * D + d, none ? f4{} : x * (1.0f / sum));
   if (d == 0) a.lse[at] = top == kUnseen ? kNegInf : static_cast<float>(top + logf(sum));
 }
 
@@ -590,7 +598,7 @@ struct ScoredSmem {
   IdSmem ids;
 };
 
-template <int D, bool kMods>
+template <int D, int MODS>
 __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& sm, int item) {
   constexpr int kKS = D / 16, kDT = D / 32;
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, g = lane >> 5;
@@ -655,7 +663,8 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
     st.store(sm.u.t[put].a, sm.u.t[put].b, sm.ua[put], sm.ub[put], w, lane);
     ro.put(st, sm.d[put], w, lane);
     if (w == 0 && g == 0) {
-      sm.l[put][j] = shifted_l(lreg, kp);
+      // (A row that sees nothing has an L of minus infinity, and scores of it too.)
+      sm.l[put][j] = id_next < 0 ? 0.0f : shifted_l(lreg, kp);
       if (all_ids != nullptr) sm.ids.tile[put][j] = id_next;
     }
   };
@@ -676,14 +685,13 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
   f16v dk[kDT], dv[kDT];
 #pragma unroll
   for (int dt = 0; dt < kDT; ++dt) dk[dt] = zero16(), dv[dt] = zero16();
-  const float cs = a.scale * kLog2e * (kMods ? a.unit : 1.0f) * uk, cg = uv;
+  const float cs = a.scale * kLog2e * (MODS == 2 ? a.unit : 1.0f) * uk, cg = uv;
   float psc = kMaxScale, dsc = kMaxScale;
   const int roff0 = row_off<D>(j, g), coff0 = col_off<D>(lane);
 
-  auto tile = [&](auto fullc, int u, int q0, float slope2) {
-    constexpr bool kFull = decltype(fullc)::value != 0;
+  auto tile = [&](int u, int q0, int hh, int sees) {
     const int roff = late(roff0), coff = late(coff0), cur = u & 1;
-    if (kFull) store(u + 1);
+    store(u + 1);
     const Tile<D>&Q = sm.u.t[cur].a, &G = sm.u.t[cur].b;
     f16v s = zero16(), dp = zero16();
     {
@@ -707,49 +715,53 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
 #pragma unroll
       for (int ks = 0; ks < kKS; ++ks) dp = mma(x[ks], vB[ks].h, dp);
     }
-    if (kFull) {
-      load(u + 2);
-      pin_loads();
-    }
-    // Live: register r's query, q0 + 4 g + 8 i + e, below SQ and, causal, not before the key.
-    const int hi = key < a.SK ? SQ - q0 - 4 * g : 0;
-    const int least = a.causal && key >= prefix ? key - off - q0 - 4 * g : 0;
-    auto weights = [&](auto capc) {
-      const float base = static_cast<float>(q0 + 4 * g + off - key);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f4 L = ld4(&sm.l[cur][8 * i + 4 * g]), Dv = ld4(&sm.d[cur][8 * i + 4 * g]);
-        const f4 uq = ld4(&sm.ua[cur][8 * i + 4 * g]), ug = ld4(&sm.ub[cur][8 * i + 4 * g]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * i + e;
-          float slope = 1.0f, x;
-          if constexpr (kMods) {
-            x = score<decltype(capc)::value>(s[r], a.cap2, slope2, base + static_cast<float>(8 * i + e), slope) + L[e];
-          } else {
-            x = fmaf(s[r], cs * uq[e], L[e]);
-          }
-          x = exp2_hw(x) * ug[e];
-          const bool live = kFull || (8 * i + e < hi && 8 * i + e >= least &&
-                                      (all_ids == nullptr || (sm.ids.tile[cur][8 * i + e + 4 * g] == ids.mine && ids.mine >= 0)));
-          const float p = live ? x : 0.0f;
-          float y = p * fmaf(dp[r], cg, -Dv[e]) * uq[e];
-          if constexpr (kMods && decltype(capc)::value != 0) y *= slope;
-          dp[r] = live ? y : 0.0f;
-          s[r] = p;
-        }
-      }
-    };
-    if constexpr (kMods) {
+    // The loads of the step after next from here on (its O later still): held across the products above as
+    // well, they do not fit.
+    load(u + 2);
+    pin_loads();
+    if constexpr (MODS != 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const f4 uq = ld4(&sm.ua[cur][8 * i + 4 * g]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[4 * i + e] *= cs * uq[e];
       }
-      by_cap(a, s, weights);
-    } else {
-      weights(Const<0>{});
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f4 Dv = ld4(&sm.d[cur][8 * i + 4 * g]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dp[4 * i + e] = fmaf(dp[4 * i + e], cg, -Dv[e]);
+    }
+    if constexpr (MODS == 2) capped(s, a.cap2, [&](int r, float slope) { dp[r] *= slope; });
+    if constexpr (MODS != 0) {
+      lowered<1>(s, slope_of(a, h0 + hh), static_cast<float>(q0 + 4 * g + off - key));
+    }
+    // Register r's query is q0 + 4 g + 8 i + e: seen below SQ and, causal, not before the key.
+    if (sees == kSome) {
+      const int end = key < a.SK && ids.mine >= 0 ? SQ - q0 - 4 * g : 0;
+      const int least = a.causal && key >= prefix ? key - off - q0 - 4 * g : 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        i4 id{};
+        if (all_ids != nullptr) id = *reinterpret_cast<const i4*>(&sm.ids.tile[cur][8 * i + 4 * g]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool is = 8 * i + e < end && 8 * i + e >= least && id[e] == ids.mine;
+          s[4 * i + e] = is ? s[4 * i + e] : kNegInf;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f4 L = ld4(&sm.l[cur][8 * i + 4 * g]), uq = ld4(&sm.ua[cur][8 * i + 4 * g]);
+      const f4 ug = ld4(&sm.ub[cur][8 * i + 4 * g]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * i + e;
+        s[r] = exp2_hw(MODS != 0 ? s[r] + L[e] : fmaf(s[r], cs * uq[e], L[e])) * ug[e];
+        dp[r] = s[r] * dp[r] * uq[e];
+      }
     }
     pin_acc(dv);
     pin_acc(dk);
@@ -768,10 +780,8 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
         dv[dt] = mma3(ld_col<D>(G, coff ^ col_step(dt), 1), p1, dv[dt]);
       }
     }
-    if (kFull) {
-      load_o(u + 2);
-      pin_loads();
-    }
+    load_o(u + 2);
+    pin_loads();
     {
       const Pair p0 = split_acc<0>(dp, dsc), p1 = split_acc<1>(dp, dsc);
 #pragma unroll
@@ -791,25 +801,25 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
     const int sees = whole ? kAll : kSome;
     return all_ids == nullptr ? sees : among(sm.ids.tile[u & 1][j], ids, sees);
   };
-  // (The staging of steps with a mask is outside their branch: in both its arms the loaded registers and the
-  // sums spill where they join.)
   __syncthreads();
-  int u = 0;
+  int u = 0, hh = 0, q0 = t0 * kRows, sees;
+  auto next = [&] {
+    ++u, q0 += kRows;
+    if (q0 == (t0 + n) * kRows) q0 = t0 * kRows, ++hh;
+  };
   while (u < steps) {
-    int hh, q0 = place(u, hh), sees;
-    while (u < steps && (sees = seen(u, q0 = place(u, hh))) == kAll) {
-      tile(Const<1>{}, u, q0, kMods ? slope_of(a, h0 + hh) : 0.0f);
+    while (u < steps && (sees = seen(u, q0)) != kNone) {
+      tile(u, q0, hh, sees);
       __syncthreads();
-      ++u;
+      next();
     }
-    while (u < steps && (sees = seen(u, q0 = place(u, hh))) != kAll) {
+    while (u < steps && seen(u, q0) == kNone) {
       store(u + 1);
       load(u + 2);
       load_o(u + 2);
       pin_loads();
-      if (sees == kSome) tile(Const<0>{}, u, q0, kMods ? slope_of(a, h0 + hh) : 0.0f);
       __syncthreads();
-      ++u;
+      next();
     }
   }
   if (!wave_live) return;
@@ -826,7 +836,7 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
   store_rows<D>(dv, fv, fv2, sm.u.o[w], dkv + stride / 2, stride, a.SK - kw0, lane_e);
 }
 
-template <int D, bool kMods>
+template <int D, int MODS>
 __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D>& sm, int item) {
   constexpr int kKS = D / 16, kDT = D / 32;
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, g = lane >> 5;
@@ -887,7 +897,7 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
       for (int e = 0; e < 8; ++e) Dq = fmaf(og.x[ks][e / 4][e % 4], oo.x[ks][e / 4][e % 4], Dq);
     }
     Dq = pair_sum(Dq) * pow2(kTop);  // (dP and D times 2^kTop meet K's unit)
-    L = shifted_l(L, kp);
+    L = ids.mine < 0 ? 0.0f : shifted_l(L, kp);  // (as for the key blocks)
     uq = oq.split(1.0f, qB);
     ug = og.split(1.0f, gB);
     store(t0);
@@ -896,13 +906,12 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
   f16v dq[kDT];
 #pragma unroll
   for (int dt = 0; dt < kDT; ++dt) dq[dt] = zero16();
-  const float cs = a.scale * kLog2e * (kMods ? a.unit : 1.0f) * uq, cg = ug;
-  const float slope2 = kMods ? slope_of(a, h) : 0.0f, fpos = static_cast<float>(pos - 4 * g);
+  const float cs = a.scale * kLog2e * (MODS == 2 ? a.unit : 1.0f) * uq, cg = ug;
+  const float slope2 = MODS != 0 ? slope_of(a, h) : 0.0f, fpos = static_cast<float>(pos - 4 * g);
   float dsc = kMaxScale;
   const int roff0 = row_off<D>(j, g), coff0 = col_off<D>(lane);
 
-  auto tile = [&](auto fullc, int t) {
-    constexpr bool kFull = decltype(fullc)::value != 0;
+  auto tile = [&](int t, int sees) {
     const int roff = late(roff0), coff = late(coff0), cur = t & 1, kt0 = t * kRows;
     store(t + 1);
     const Tile<D>&K = sm.u.t[cur].a, &V = sm.u.t[cur].b;
@@ -930,38 +939,43 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
     }
     load(t + 2);
     pin_loads();
-    auto weights = [&](auto capc) {
-      const float base = fpos - static_cast<float>(kt0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f4 uk = ld4(&sm.ua[cur][8 * i + 4 * g]), uv = ld4(&sm.ub[cur][8 * i + 4 * g]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * i + e, key = kt0 + 8 * i + 4 * g + e;
-          float slope = 1.0f, x;
-          if constexpr (kMods) {
-            x = score<decltype(capc)::value>(s[r], a.cap2, slope2, base - static_cast<float>(8 * i + e), slope) + L;
-          } else {
-            x = fmaf(s[r], cs * uk[e], L);
-          }
-          x = exp2_hw(x) * fmaf(dp[r], cg * uv[e], -Dq) * uk[e];
-          if constexpr (kMods && decltype(capc)::value != 0) x *= slope;
-          const bool live = kFull || (key <= lim && (all_ids == nullptr || (sm.ids.tile[cur][8 * i + 4 * g + e] == ids.mine &&
-                                                                            ids.mine >= 0)));
-          dp[r] = live ? x : 0.0f;
-        }
-      }
-    };
-    if constexpr (kMods) {
+    if constexpr (MODS != 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const f4 uk = ld4(&sm.ua[cur][8 * i + 4 * g]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[4 * i + e] *= cs * uk[e];
       }
-      by_cap(a, s, weights);
-    } else {
-      weights(Const<0>{});
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f4 uv = ld4(&sm.ub[cur][8 * i + 4 * g]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dp[4 * i + e] = fmaf(dp[4 * i + e], cg * uv[e], -Dq);
+    }
+    if constexpr (MODS == 2) capped(s, a.cap2, [&](int r, float slope) { dp[r] *= slope; });
+    if constexpr (MODS != 0) lowered<-1>(s, slope2, fpos - static_cast<float>(kt0));
+    if (sees == kSome) {
+      const int left = lim - kt0 - 4 * g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        i4 id{};
+        if (all_ids != nullptr) id = *reinterpret_cast<const i4*>(&sm.ids.tile[cur][8 * i + 4 * g]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool is = 8 * i + e <= left && id[e] == ids.mine && ids.mine >= 0;
+          s[4 * i + e] = is ? s[4 * i + e] : kNegInf;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f4 uk = ld4(&sm.ua[cur][8 * i + 4 * g]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * i + e;
+        dp[r] = exp2_hw(MODS != 0 ? s[r] + L : fmaf(s[r], cs * uk[e], L)) * dp[r] * uk[e];
+      }
     }
     pin_acc(dq);
     const float md = max_weight(dp);
@@ -976,21 +990,25 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
       dq[dt] = mma3(ld_col<D>(K, coff ^ col_step(dt), 1), p1, dq[dt]);
     }
   };
+  auto seen = [&](int t) {
+    const int sees = !wave_live || t * kRows > hi ? kNone : t * kRows + kRows - 1 <= lo ? kAll : kSome;
+    return all_ids == nullptr || sees == kNone ? sees : among(sm.ids.tile[t & 1][j], ids, sees);
+  };
   __syncthreads();
-#pragma clang loop unroll(disable)
-  for (int t = t0; t < t1; ++t) {
-    int sees = !wave_live || t * kRows > hi ? kNone : t * kRows + kRows - 1 <= lo ? kAll : kSome;
-    if (all_ids != nullptr && sees != kNone) sees = among(sm.ids.tile[t & 1][j], ids, sees);
-    if (sees == kAll) {
-      tile(Const<1>{}, t);
-    } else if (sees == kSome) {
-      tile(Const<0>{}, t);
-    } else {
+  int t = t0, sees;
+  while (t < t1) {
+    while (t < t1 && (sees = seen(t)) != kNone) {
+      tile(t, sees);
+      __syncthreads();
+      ++t;
+    }
+    while (t < t1 && seen(t) == kNone) {
       store(t + 1);
       load(t + 2);
       pin_loads();
+      __syncthreads();
+      ++t;
     }
-    __syncthreads();
   }
   if (!wave_live) return;
   float f = pow2(-kTop) * a.scale, f2 = pow2(-kp) / dsc;
@@ -1001,33 +1019,34 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
   store_rows<D>(dq, f, f2, sm.u.o[w], dq_rows, static_cast<int64_t>(a.H) * D, a.SQ - qw0, late(lane));
 }
 
-template <int D, bool kMods, int WAVES>
+template <int D, int MODS, int WAVES>
 __global__ void __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES)))
 bwd_scored_kernel(ScoredArgs a) {
   __shared__ __attribute__((aligned(16))) ScoredSmem<D> sm;
   const int id = static_cast<int>(blockIdx.x), pairs = a.B * (a.H / a.G), BH = a.B * a.H, keys = a.nkb * pairs;
   if (id < keys) {
     // Causal: the low blocks (they are seen by every later query) first.
-    scored_keys<D, kMods>(a, sm, a.causal ? id % pairs * a.nkb + id / pairs : xcd_remap(id, keys));
+    scored_keys<D, MODS>(a, sm, a.causal ? id % pairs * a.nkb + id / pairs : xcd_remap(id, keys));
   } else {
     const int i = id - keys;
-    scored_queries<D, kMods>(a, sm, a.causal ? i % BH * a.nqb + a.nqb - 1 - i / BH : xcd_remap(i, a.nqb * BH));
+    scored_queries<D, MODS>(a, sm, a.causal ? i % BH * a.nqb + a.nqb - 1 - i / BH : xcd_remap(i, a.nqb * BH));
   }
 }
 
-template <bool kMods>
+template <int MODS>
 const void* fwd_fn(int d) {
-  return d == 32    ? reinterpret_cast<const void*>(fwd_scored_kernel<32, kMods, 4>)
-         : d == 128 ? reinterpret_cast<const void*>(fwd_scored_kernel<128, kMods, 2>)
-                    : reinterpret_cast<const void*>(fwd_scored_kernel<64, kMods, 3>);
+  return d == 32    ? reinterpret_cast<const void*>(fwd_scored_kernel<32, MODS, 4>)
+         : d == 128 ? reinterpret_cast<const void*>(fwd_scored_kernel<128, MODS, 2>)
+                    : reinterpret_cast<const void*>(fwd_scored_kernel<64, MODS, 3>);
 }
-template <bool kMods>
+template <int MODS>
 const void* bwd_fn(int d) {
-  return d == 32    ? reinterpret_cast<const void*>(bwd_scored_kernel<32, kMods, 3>)
-         : d == 128 ? reinterpret_cast<const void*>(bwd_scored_kernel<128, kMods, 1>)
-                    : reinterpret_cast<const void*>(bwd_scored_kernel<64, kMods, 2>);
+  return d == 32    ? reinterpret_cast<const void*>(bwd_scored_kernel<32, MODS, 3>)
+         : d == 128 ? reinterpret_cast<const void*>(bwd_scored_kernel<128, MODS, 1>)
+                    : reinterpret_cast<const void*>(bwd_scored_kernel<64, MODS, 2>);
 }
-bool mods(const ScoredArgs& a) { return a.cap2 != 0.0f || a.slopes != nullptr; }
+// (Scale 0: the products are multiplied by it before what is not seen becomes minus infinity.)
+int mods(const ScoredArgs& a) { return a.cap2 != 0.0f ? 2 : a.slopes != nullptr || a.scale == 0.0f ? 1 : 0; }
 int64_t blocks_of(int64_t rows) { return (rows + kBlock - 1) / kBlock; }
 
 }  // namespace
@@ -1059,7 +1078,7 @@ int launch_scored_forward(ScoredArgs a, int d, const ScoredPlan& plan, void* wor
   void* args[] = {&a};
   hipStream_t s = static_cast<hipStream_t>(stream);
   const unsigned grid = static_cast<unsigned>(int64_t{a.B} * a.H * a.nqb * a.nc);
-  const hipError_t err = hipLaunchKernel(mods(a) ? fwd_fn<true>(d) : fwd_fn<false>(d), dim3(grid), dim3(64 * kW),
+  const hipError_t err = hipLaunchKernel(mods(a) == 2 ? fwd_fn<2>(d) : mods(a) == 1 ? fwd_fn<1>(d) : fwd_fn<0>(d), dim3(grid), dim3(64 * kW),
                                          args, 0, s);
   if (err != hipSuccess || a.nc == 1) return static_cast<int>(err);
   const void* join = d == 32    ? reinterpret_cast<const void*>(join_scored_kernel<32>)
@@ -1075,7 +1094,7 @@ int launch_scored_backward(ScoredArgs a, int d, void* stream) {
   a.nc = 1;
   void* args[] = {&a};
   const int64_t grid = scored_blocks(a.B, a.H / a.G, a.SK) + scored_blocks(a.B, a.H, a.SQ);
-  return static_cast<int>(hipLaunchKernel(mods(a) ? bwd_fn<true>(d) : bwd_fn<false>(d),
+  return static_cast<int>(hipLaunchKernel(mods(a) == 2 ? bwd_fn<2>(d) : mods(a) == 1 ? bwd_fn<1>(d) : bwd_fn<0>(d),
                                           dim3(static_cast<unsigned>(grid)), dim3(64 * kW), args, 0,
                                           static_cast<hipStream_t>(stream)));
 }

@@ -58,6 +58,7 @@ EXPORTS = (
     "fattn_cross_backward",
     "fattn_scored_workspace_bytes",
     "fattn_scored_forward",
+    "fattn_scored_backward_workspace_bytes",
     "fattn_scored_backward",
     "fattn_last_error",
     "fattn_version",
@@ -129,6 +130,8 @@ def _declare(L: ctypes.CDLL) -> None:
                                                P, I64, I64, P, C_FLOAT, C_FLOAT, P, P, SIZE, P]
     L.fattn_paged_read.argtypes = [C_INT, C_INT, I64, I64, I64, I64, P, P, P, P, I64, I64, P, I64, I64, P,
                                    P, P, P, P]
+    L.fattn_scored_backward_workspace_bytes.argtypes = [I64, I64, I64, I64, I64, I64, C_INT]
+    L.fattn_scored_backward_workspace_bytes.restype = SIZE
     for name in ("fattn_cross_workspace_bytes", "fattn_cross_backward_workspace_bytes",
                  "fattn_scored_workspace_bytes"):
         getattr(L, name).argtypes = [I64, I64, I64, I64, I64, I64]
@@ -139,7 +142,7 @@ def _declare(L: ctypes.CDLL) -> None:
                                        P, P, P, P, P, SIZE, P]
     scored = [P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, C_FLOAT, C_INT, C_FLOAT, P, P, I64, P]
     L.fattn_scored_forward.argtypes = [*scored, P, P, P, SIZE, P]
-    L.fattn_scored_backward.argtypes = [*scored, P, P, P, P, P, P, P]
+    L.fattn_scored_backward.argtypes = [*scored, P, P, P, P, P, P, P, SIZE, P]
     L.fattn_bwd_status.argtypes = [P, SIZE, I64, I64, I64, P, ctypes.POINTER(C_INT)]
     for name in EXPORTS:
         if name not in ("fattn_last_error", "fattn_version") and "workspace" not in name:

@@ -311,9 +311,9 @@ struct ScoredArgs {
   const float* slopes;
   const int32_t *documents, *prefix;
   int64_t document_stride;
-  // The launchers': blocks of 128 queries and keys, chunks of the forward's walks and their tiles, and where
-  // the chunks' O and L go.
-  int nqb, nkb, nc, chunk;
+  // The launchers': blocks of 128 queries and keys; chunks of the forward's walks and their tiles, and where
+  // their O and L go; those of the backward's key and query blocks (dq, dkv of chunk c at c times their size).
+  int nqb, nkb, nc, chunk, nck, chk, ncq, chq;
   float* o_part;
   double* l_part;
 };
@@ -321,10 +321,16 @@ struct ScoredPlan {
   int nc, chunk;
   size_t l_part, bytes;
 };
+struct ScoredBackwardPlan {
+  int nck, chk, ncq, chq;
+  size_t k_part, bytes;
+};
 ScoredPlan scored_plan(int64_t b, int64_t h, int64_t sq, int64_t sk, int64_t d);
+ScoredBackwardPlan scored_backward_plan(int64_t b, int64_t h, int64_t hk, int64_t sq, int64_t sk, int64_t d,
+                                        int causal);
 int64_t scored_blocks(int64_t b, int64_t heads, int64_t rows);
 int launch_scored_forward(ScoredArgs a, int d, const ScoredPlan& plan, void* workspace, void* stream);
-int launch_scored_backward(ScoredArgs a, int d, void* stream);
+int launch_scored_backward(ScoredArgs a, int d, const ScoredBackwardPlan& plan, void* workspace, void* stream);
 
 // Sets this thread's message (fattn_last_error) and returns `code`; done() clears it and returns 0.
 int set_error(int code, const char* format, ...) __attribute__((format(printf, 2, 3)));

@@ -550,6 +550,12 @@ size_t fattn_scored_workspace_bytes(int64_t b, int64_t heads, int64_t kv_heads, 
   return fattn::scored_plan(b, heads, sq, sk, d).bytes;
 }
 
+size_t fattn_scored_backward_workspace_bytes(int64_t b, int64_t heads, int64_t kv_heads, int64_t sq,
+                                             int64_t sk, int64_t d, int causal) {
+  if (!split_shape(b, heads, kv_heads, d) || sq < 0 || sk < sq) return 0;
+  return fattn::scored_backward_plan(b, heads, kv_heads, sq, sk, d, causal).bytes;
+}
+
 int fattn_scored_forward(const float* q, const int64_t q_strides[3], const float* k,
                          const int64_t k_strides[3], const float* v, const int64_t v_strides[3],
                          int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d,
@@ -582,7 +588,8 @@ int fattn_scored_backward(const float* q, const int64_t q_strides[3], const floa
                           float scale, int causal, float cap, const float* slopes,
                           const int32_t* documents, int64_t document_stride, const int32_t* prefix,
                           const float* out, const float* lse, const float* d_o,
-                          const int64_t do_strides[3], float* dq, float* dkv, void* stream) {
+                          const int64_t do_strides[3], float* dq, float* dkv, void* workspace,
+                          size_t workspace_bytes, void* stream) {
   fattn::ScoredArgs a{};
   bool none = false;
   if (int rc = scored_operands(a, q, q_strides, k, k_strides, v, v_strides, b, heads, kv_heads, sq, sk, d, scale,
@@ -600,8 +607,13 @@ int fattn_scored_backward(const float* q, const int64_t q_strides[3], const floa
   if (!slice_fits(a.q, sq, d) || !slice_fits(a.d_o, sq, d) || sq * heads * d > int64_t{UINT32_MAX}) {
     return set_error(FATTN_ERANGE, "%s: the queries of one sample span more than 4 GiB", kScored);
   }
+  const fattn::ScoredBackwardPlan plan = fattn::scored_backward_plan(b, heads, kv_heads, sq, sk, d, causal);
+  if (fattn::scored_blocks(b, heads, sq) * plan.ncq + fattn::scored_blocks(b, kv_heads, sk) * plan.nck > kMaxGrid) {
+    return set_error(FATTN_ERANGE, "%s: the grid exceeds the launch limit", kScored);
+  }
+  if (int rc = check_workspace(kScored, workspace, workspace_bytes, plan.bytes)) return rc;
   a.o = out, a.lse = const_cast<float*>(lse), a.dq = dq, a.dkv = dkv;
-  const int err = fattn::launch_scored_backward(a, static_cast<int>(d), stream);
+  const int err = fattn::launch_scored_backward(a, static_cast<int>(d), plan, workspace, stream);
   if (err) return fattn::hip_error(err, kScored, "backward launch");
   return fattn::done();
 }

@@ -105,8 +105,8 @@ __device__ __forceinline__ float slope_of(const ScoredArgs& a, int h) {
 }
 
 // --- Scores ------------------------------------------------------------------------------------
-// MODS: 0, x as it is; 1, less a slope times the distance; 2, capped, and less that. For 2 the products'
-// factor gives x / cap.
+// MODS, bits: 1, less a slope times the distance; 2, capped. With a cap the products' factor gives x / cap, a
+// walk holds tanh of it, and cap2 of that (cap log2 e) enters with what the exponent adds anyway.
 // One score in units of log2 e by its definition, for the rows in fp32, and dy / dx.
 __device__ __forceinline__ float score_fp32(const ScoredArgs& a, float dot, float slope2, int far, float& slope) {
   float y = dot * (a.scale * kLog2e * a.unit);
@@ -116,34 +116,59 @@ __device__ __forceinline__ float score_fp32(const ScoredArgs& a, float dot, floa
 }
 // Nothing is scheduled across: sixteen polynomials side by side take more registers than there are.
 __device__ __forceinline__ void few_at_once() { __builtin_amdgcn_sched_barrier(0); }
-// x / cap of a wave's tile to y and, times `fn(r, dy / dx)`. (Nearly always every |x| / cap is small, and the
-// polynomial alone is half of the work.)
+// x / cap of a wave's tile to its tanh t and `fn(r, dt / dx)`. (Nearly always every |x| / cap is small, where a
+// polynomial does it: of degree 7 or 11 in x, against those and an exponential and a quotient besides.)
 template <typename F>
-__device__ __forceinline__ void capped(f16v& x, float cap2, F fn) {
-  if (__builtin_amdgcn_ballot_w64(max_weight(x) > kTanhSmall) == 0) {
+__device__ __forceinline__ void capped(f16v& x, F fn) {
+  const float most = max_weight(x);
+  if (__builtin_amdgcn_ballot_w64(most > kTanhTiny) == 0) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const float t = tanh_small(x[r]);
-      x[r] = cap2 * t;
-      fn(r, fmaf(-t, t, 1.0f));
+      x[r] = tanh_tiny(x[r]);
+      fn(r, fmaf(-x[r], x[r], 1.0f));
+      if (r % 4 == 3) few_at_once();
+    }
+  } else if (__builtin_amdgcn_ballot_w64(most > kTanhSmall) == 0) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      x[r] = tanh_small(x[r]);
+      fn(r, fmaf(-x[r], x[r], 1.0f));
       if (r % 4 == 3) few_at_once();
     }
   } else {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       float slope;
-      x[r] = cap2 * tanh_any(x[r], slope);
+      x[r] = tanh_any(x[r], slope);
       fn(r, slope);
       if (r % 2 == 1) few_at_once();
     }
   }
 }
-// y less the slope times the distance, of register r |base + sign (8 (r / 4) + r % 4)|.
+// The slope's part. Register r is 8 (r / 4) + r % 4 places from the lane's base; where no seen pair of the
+// tile has its key after its query, the distance is a sum of both, and slope x place (one value for the wave)
+// is added to the score while the lane's part goes with what the exponent adds: no instruction of its own.
+__device__ __forceinline__ int place_of(int r) { return 8 * (r >> 2) + (r & 3); }
+struct Places {
+  float by[16];  // slope2 times the place of register r, in scalar registers
+  __device__ __forceinline__ void set(float slope2) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      by[r] = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(slope2 * static_cast<float>(place_of(r)))));
+    }
+  }
+};
+// s, in units of 1 / f log2 e, to scores: plus its places' part (a key's place brings it nearer to the query).
+__device__ __forceinline__ void nearer(f16v& s, float f, const Places& places) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], f, places.by[r]);
+}
+// Otherwise: less slope2 |base + SIGN place|.
 template <int SIGN>
-__device__ __forceinline__ void lowered(f16v& y, float slope2, float base) {
+__device__ __forceinline__ void lowered(f16v& s, float f, float slope2, float base) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    y[r] = fmaf(-slope2, fabsf(base + static_cast<float>(SIGN * (8 * (r >> 2) + (r & 3)))), y[r]);
+    s[r] = fmaf(s[r], f, -slope2 * fabsf(base + static_cast<float>(SIGN * place_of(r))));
   }
 }
 
@@ -211,10 +236,11 @@ __device__ __forceinline__ void scored_rows_fp32(const ScoredArgs& a, int b, int
   }
 }
 
-// dK and dV of 32 keys from kw0 (walking the tiles t0 .. t1 of the G query heads' queries), in fp32.
+// dK and dV of 32 keys from kw0, over steps u0 .. u1 of the walk of n tiles from t0 of each head of the group,
+// in fp32.
 template <int D>
-__device__ __forceinline__ void scored_keys_fp32(const ScoredArgs& a, int b, int hk, int kw0, int t0, int t1,
-                                                 float* so, f16v (&dk)[D / 32], f16v (&dv)[D / 32], int lane) {
+__device__ __forceinline__ void scored_keys_fp32(const ScoredArgs& a, int b, int hk, int kw0, int t0, int n,
+                                                 int u0, int u1, float* so, f16v (&dk)[D / 32], f16v (&dv)[D / 32], int lane) {
   const int j = lane & 31, g = lane >> 5, key = kw0 + j, kc = min(key, a.SK - 1), off = a.SK - a.SQ;
   const float* kr = a.k.p + b * a.k.sb + hk * a.k.sh + kc * a.k.ss;
   const float* vr = a.v.p + b * a.v.sb + hk * a.v.sh + kc * a.v.ss;
@@ -228,8 +254,8 @@ __device__ __forceinline__ void scored_keys_fp32(const ScoredArgs& a, int b, int
            (ids == nullptr || ids[min(qi, a.SQ - 1) + off] == id);
   };
 #pragma clang loop unroll(disable)
-  for (int u = 0; u < a.G * (t1 - t0); ++u) {
-    const int h = hk * a.G + u / (t1 - t0), q0 = (t0 + u % (t1 - t0)) * kRows;
+  for (int u = u0; u < u1; ++u) {
+    const int h = hk * a.G + u / n, q0 = (t0 + u % n) * kRows;
     const float* qp = a.q.p + b * a.q.sb + h * a.q.sh;
     const float* gp = a.d_o.p + b * a.d_o.sb + h * a.d_o.sh;
     const float* op = a.o + (static_cast<int64_t>(b) * a.SQ * a.H + h) * D;
@@ -342,6 +368,9 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
   const int lim = last_key(a, pos, prefix);
   const int lo = last_key(a, min(qw0, a.SQ - 1) + off, prefix);
   const int hi = last_key(a, min(qw0 + kRows, a.SQ) - 1 + off, prefix);
+  // No key that is seen after its query; the wave's first position (past the last query: the last).
+  const bool ordered = a.causal && prefix == 0;
+  const int lo_pos = min(qw0, a.SQ - 1) + off;
   const bool wave_live = qw0 < a.SQ;
   int t0 = 0, t1 = (end + kRows - 1) / kRows;
   Ids ids{0, 0, 0, true};
@@ -388,9 +417,12 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
     own.load(qp + min(qi, a.SQ - 1) * a.q.ss, g);
     store(t0);
     load(t0 + 1);
-    cq = own.split(a.scale < 0.0f ? -1.0f : 1.0f, q) * (fabsf(a.scale) * kLog2e * (MODS == 2 ? a.unit : 1.0f));
+    cq = own.split(a.scale < 0.0f ? -1.0f : 1.0f, q) * (fabsf(a.scale) * kLog2e * ((MODS & 2) != 0 ? a.unit : 1.0f));
   }
-  const float slope2 = MODS != 0 ? slope_of(a, h) : 0.0f, fpos = static_cast<float>(pos - 4 * g);
+  const float slope2 = (MODS & 1) != 0 ? slope_of(a, h) : 0.0f, fpos = static_cast<float>(pos - 4 * g);
+  const float f2 = (MODS & 2) != 0 ? a.cap2 : 1.0f;
+  Places places;
+  if constexpr ((MODS & 1) != 0) places.set(slope2);
   f16v acc[kDT];  // O^T, in units of p / wsc and 2^-kTop
   float m = kFirstRef, lsum = 0.0f, wsc = kMaxScale;
 #pragma unroll
@@ -419,6 +451,7 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
 #pragma unroll
       for (int ks = 0; ks < kKS; ++ks) s = mma(kh[ks], q[ks].h, s);
     }
+    float shift = 0.0f;  // of what is held less the score
     if constexpr (MODS != 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -426,8 +459,16 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[4 * i + c] *= cq * uk[c];
       }
-      if constexpr (MODS == 2) capped(s, a.cap2, [](int, float) {});
-      lowered<-1>(s, slope2, fpos - static_cast<float>(kt0));
+      if constexpr ((MODS & 2) != 0) capped(s, [](int, float) {});
+      if constexpr ((MODS & 1) != 0) {
+        const float base = fpos - static_cast<float>(kt0);
+        if (ordered || kt0 + kRows - 1 <= lo_pos) {
+          shift = slope2 * base;
+          nearer(s, f2, places);
+        } else {
+          lowered<-1>(s, f2, slope2, base);
+        }
+      }
     }
     // What is not seen is minus infinity: register r's key is kt0 + 4 g + 8 (r / 4) + r % 4.
     if (sees == kSome) {
@@ -449,6 +490,7 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
       wmax = 0.0f;
       int r0 = 4 * g;
       asm("" : "+v"(r0));
+      const float ref = m + shift;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const f4 uv = ld4(&sm.uv[cur][8 * i + r0]);
@@ -457,7 +499,9 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int r = 4 * i + c;
-          const float p = exp2_hw(MODS != 0 ? s[r] - m : fmaf(s[r], cq * uk[c], -m));
+          const float p = exp2_hw(MODS == 0   ? fmaf(s[r], cq * uk[c], -m)
+                                  : MODS == 2 ? fmaf(s[r], f2, -m)
+                                              : s[r] - ref);
           psum = r == 0 ? p : psum + p;
           e[r] = p * uv[c];
         }
@@ -474,7 +518,8 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
       for (int r = 0; r < 16; ++r) {
         tmax = fmaxf(tmax, MODS != 0 ? s[r] : s[r] * (cq * sm.uk[cur][8 * (r >> 2) + r0 + (r & 3)]));
       }
-      const float ref = pair_max(tmax) - kRefTop;
+      if constexpr (MODS == 2) tmax *= f2;
+      const float ref = pair_max(tmax - shift) - kRefTop;
       float to = wsc, alpha = 1.0f;
       if (!(pair_sum(psum) <= kRowTop) && ref > m) {
         alpha = exp2_hw(m - ref);  // (0 from the first one)
@@ -595,11 +640,12 @@ template <int D>
 struct ScoredSmem {
   ScoredTiles<D> u;
   float ua[2][kRows], ub[2][kRows], l[2][kRows], d[2][kRows];
+  float ls[2][kRows];  // (key blocks) l less the slope times the row's place after the block's first key
   IdSmem ids;
 };
 
 template <int D, int MODS>
-__device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& sm, int item) {
+__device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& sm, int item, int chunk) {
   constexpr int kKS = D / 16, kDT = D / 32;
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -618,8 +664,12 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
     find_ids(sm.ids, ids, all_ids, q_first + off, a.SK, w, tid, first, last);
     q_first = first - off, q_end = last - off;
   }
-  float* dkv = a.dkv + (static_cast<int64_t>(b) * a.SK + kw0) * 2 * HK * D + static_cast<int64_t>(hk) * D;
-  if (q_first >= q_end) {  // keys that no query sees
+  // The walk: n tiles from t0 of each head of the group, or a chunk of these steps, from u0 on.
+  const int t0 = q_first / kRows, n = (q_end + kRows - 1) / kRows - t0, u0 = chunk * a.chk;
+  const int steps = q_first < q_end ? min(n * a.G - u0, a.chk) : 0;
+  float* dkv = a.dkv + ((static_cast<int64_t>(chunk) * a.B + b) * a.SK + kw0) * 2 * HK * D +
+               static_cast<int64_t>(hk) * D;
+  if (steps <= 0) {  // keys that no query sees
     for (int i = lane; i < min(a.SK - kw0, kRows) * (D / 4); i += 64) {
       float* row = dkv + static_cast<int64_t>(i / (D / 4)) * 2 * HK * D + i % (D / 4) * 4;
       st4(row, f4{});
@@ -627,7 +677,6 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
     }
     return;
   }
-  const int t0 = q_first / kRows, n = (q_end + kRows - 1) / kRows - t0, steps = n * a.G;
   const Operand qop{reinterpret_cast<const char*>(a.q.p + b * a.q.sb + h0 * a.q.sh),
                     static_cast<unsigned>(a.q.ss) * 4u};
   const Operand gop{reinterpret_cast<const char*>(a.d_o.p + b * a.d_o.sb + h0 * a.d_o.sh),
@@ -638,12 +687,12 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
   const int kp = half_log2(a.SK);
   Stage<D, kW> st;
   RowDots<D, kW> ro;
-  float lreg;
-  int id_next = 0;
+  float lreg, slope_next = 0.0f;
+  int id_next = 0, row_next = 0;
   // Step u's head in the group (past the last step: the last) and its tile's first row.
   auto place = [&](int u, int& hh) {
-    hh = min(u / n, a.G - 1);
-    return (t0 + u - hh * n) * kRows;
+    hh = min((u + u0) / n, a.G - 1);
+    return (t0 + u + u0 - hh * n) * kRows;
   };
   auto load = [&](int u) {
     int hh;
@@ -657,6 +706,9 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
     const int r0 = place(u, hh);
     ro.load(op + hh * D, static_cast<unsigned>(a.H) * D, r0, SQ - 1, w, lane);
     lreg = lp[hh * static_cast<int64_t>(SQ) + min(r0 + j, SQ - 1)];
+    if constexpr ((MODS & 1) != 0) {
+      if (w == 0) slope_next = slope_of(a, h0 + hh), row_next = r0 + j + off - k0;
+    }
   };
   auto store = [&](int u) {
     const int put = u & 1;
@@ -664,7 +716,9 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
     ro.put(st, sm.d[put], w, lane);
     if (w == 0 && g == 0) {
       // (A row that sees nothing has an L of minus infinity, and scores of it too.)
-      sm.l[put][j] = id_next < 0 ? 0.0f : shifted_l(lreg, kp);
+      const float l = id_next < 0 ? 0.0f : shifted_l(lreg, kp);
+      sm.l[put][j] = l;
+      if constexpr ((MODS & 1) != 0) sm.ls[put][j] = fmaf(-slope_next, static_cast<float>(row_next), l);
       if (all_ids != nullptr) sm.ids.tile[put][j] = id_next;
     }
   };
@@ -685,7 +739,9 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
   f16v dk[kDT], dv[kDT];
 #pragma unroll
   for (int dt = 0; dt < kDT; ++dt) dk[dt] = zero16(), dv[dt] = zero16();
-  const float cs = a.scale * kLog2e * (MODS == 2 ? a.unit : 1.0f) * uk, cg = uv;
+  const float cs = a.scale * kLog2e * ((MODS & 2) != 0 ? a.unit : 1.0f) * uk, cg = uv;
+  const float f2 = (MODS & 2) != 0 ? a.cap2 : 1.0f;
+  const bool ordered = a.causal && prefix == 0;
   float psc = kMaxScale, dsc = kMaxScale;
   const int roff0 = row_off<D>(j, g), coff0 = col_off<D>(lane);
 
@@ -733,9 +789,21 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
 #pragma unroll
       for (int e = 0; e < 4; ++e) dp[4 * i + e] = fmaf(dp[4 * i + e], cg, -Dv[e]);
     }
-    if constexpr (MODS == 2) capped(s, a.cap2, [&](int r, float slope) { dp[r] *= slope; });
-    if constexpr (MODS != 0) {
-      lowered<1>(s, slope_of(a, h0 + hh), static_cast<float>(q0 + 4 * g + off - key));
+    if constexpr ((MODS & 2) != 0) capped(s, [&](int r, float slope) { dp[r] *= slope; });
+    // The slope's part: a row's (staged with its L) and the lane's, or, where a key may be after a query that
+    // sees it, of the distance.
+    const float* l_of = sm.l[cur];
+    float shift = 0.0f;
+    float f = f2;
+    if constexpr ((MODS & 1) != 0) {
+      const float slope2 = slope_of(a, h0 + hh);
+      if (ordered || kw0 + kRows - 1 <= q0 + off) {
+        l_of = sm.ls[cur];
+        shift = slope2 * static_cast<float>(key - k0);
+      } else {
+        lowered<1>(s, f2, slope2, static_cast<float>(q0 + 4 * g + off - key));
+        f = 1.0f;
+      }
     }
     // Register r's query is q0 + 4 g + 8 i + e: seen below SQ and, causal, not before the key.
     if (sees == kSome) {
@@ -754,12 +822,13 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const f4 L = ld4(&sm.l[cur][8 * i + 4 * g]), uq = ld4(&sm.ua[cur][8 * i + 4 * g]);
-      const f4 ug = ld4(&sm.ub[cur][8 * i + 4 * g]);
+      f4 L = ld4(l_of + 8 * i + 4 * g);
+      const f4 uq = ld4(&sm.ua[cur][8 * i + 4 * g]), ug = ld4(&sm.ub[cur][8 * i + 4 * g]);
+      if constexpr ((MODS & 1) != 0) L += shift;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r = 4 * i + e;
-        s[r] = exp2_hw(MODS != 0 ? s[r] + L[e] : fmaf(s[r], cs * uq[e], L[e])) * ug[e];
+        s[r] = exp2_hw(MODS != 0 ? fmaf(s[r], f, L[e]) : fmaf(s[r], cs * uq[e], L[e])) * ug[e];
         dp[r] = s[r] * dp[r] * uq[e];
       }
     }
@@ -802,7 +871,7 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
     return all_ids == nullptr ? sees : among(sm.ids.tile[u & 1][j], ids, sees);
   };
   __syncthreads();
-  int u = 0, hh = 0, q0 = t0 * kRows, sees;
+  int u = 0, hh, q0 = place(0, hh), sees;
   auto next = [&] {
     ++u, q0 += kRows;
     if (q0 == (t0 + n) * kRows) q0 = t0 * kRows, ++hh;
@@ -827,7 +896,7 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
   float fk = pow2(-kTop) * a.scale, fk2 = pow2(-kp) / dsc, fv = pow2(-kTop - kp), fv2 = 1.0f / psc;
   const float z = probe_finite<kDT>(dk, probe_finite<kDT>(dv, fk * 0.0f));
   if (__builtin_amdgcn_ballot_w64(key < a.SK && !(z == 0.0f)) != 0) {
-    scored_keys_fp32<D>(a, b, hk, kw0, t0, t0 + n, sm.u.o[w], dk, dv, late(lane));
+    scored_keys_fp32<D>(a, b, hk, kw0, t0, n, u0, u0 + steps, sm.u.o[w], dk, dv, late(lane));
     fk = a.scale, fk2 = fv = fv2 = 1.0f;
   }
   const int lane_e = late(lane);
@@ -837,7 +906,7 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
 }
 
 template <int D, int MODS>
-__device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D>& sm, int item) {
+__device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D>& sm, int item, int chunk) {
   constexpr int kKS = D / 16, kDT = D / 32;
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -849,6 +918,9 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
   const int lim = last_key(a, pos, prefix);
   const int lo = last_key(a, min(qw0, a.SQ - 1) + off, prefix);
   const int hi = last_key(a, min(qw0 + kRows, a.SQ) - 1 + off, prefix);
+  // No key that is seen after its query; the wave's first position (past the last query: the last).
+  const bool ordered = a.causal && prefix == 0;
+  const int lo_pos = min(qw0, a.SQ - 1) + off;
   const bool wave_live = qw0 < a.SQ;
   int t0 = 0, t1 = (end + kRows - 1) / kRows;
   Ids ids{0, 0, 0, true};
@@ -858,7 +930,8 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
     find_ids(sm.ids, ids, all_ids, 0, end, w, tid, first, last);
     t0 = first / kRows, t1 = first < last ? (last + kRows - 1) / kRows : t0;
   }
-  float* dq_rows = a.dq + ((static_cast<int64_t>(b) * a.SQ + qw0) * a.H + h) * D;
+  t0 += chunk * a.chq, t1 = min(t1, t0 + a.chq);
+  float* dq_rows = a.dq + (((static_cast<int64_t>(chunk) * a.B + b) * a.SQ + qw0) * a.H + h) * D;
   if (t0 >= t1) {  // no key was seen
     for (int i = lane; i < min(a.SQ - qw0, kRows) * (D / 4); i += 64) {
       st4(dq_rows + static_cast<int64_t>(i / (D / 4)) * a.H * D + i % (D / 4) * 4, f4{});
@@ -906,8 +979,11 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
   f16v dq[kDT];
 #pragma unroll
   for (int dt = 0; dt < kDT; ++dt) dq[dt] = zero16();
-  const float cs = a.scale * kLog2e * (MODS == 2 ? a.unit : 1.0f) * uq, cg = ug;
-  const float slope2 = MODS != 0 ? slope_of(a, h) : 0.0f, fpos = static_cast<float>(pos - 4 * g);
+  const float cs = a.scale * kLog2e * ((MODS & 2) != 0 ? a.unit : 1.0f) * uq, cg = ug;
+  const float slope2 = (MODS & 1) != 0 ? slope_of(a, h) : 0.0f, fpos = static_cast<float>(pos - 4 * g);
+  const float f2 = (MODS & 2) != 0 ? a.cap2 : 1.0f;
+  Places places;
+  if constexpr ((MODS & 1) != 0) places.set(slope2);
   float dsc = kMaxScale;
   const int roff0 = row_off<D>(j, g), coff0 = col_off<D>(lane);
 
@@ -953,8 +1029,17 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
 #pragma unroll
       for (int e = 0; e < 4; ++e) dp[4 * i + e] = fmaf(dp[4 * i + e], cg * uv[e], -Dq);
     }
-    if constexpr (MODS == 2) capped(s, a.cap2, [&](int r, float slope) { dp[r] *= slope; });
-    if constexpr (MODS != 0) lowered<-1>(s, slope2, fpos - static_cast<float>(kt0));
+    if constexpr ((MODS & 2) != 0) capped(s, [&](int r, float slope) { dp[r] *= slope; });
+    float l = L;
+    if constexpr ((MODS & 1) != 0) {
+      const float base = fpos - static_cast<float>(kt0);
+      if (ordered || kt0 + kRows - 1 <= lo_pos) {
+        l = fmaf(-slope2, base, L);
+        nearer(s, f2, places);
+      } else {
+        lowered<-1>(s, f2, slope2, base);
+      }
+    }
     if (sees == kSome) {
       const int left = lim - kt0 - 4 * g;
 #pragma unroll
@@ -974,7 +1059,9 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r = 4 * i + e;
-        dp[r] = exp2_hw(MODS != 0 ? s[r] + L : fmaf(s[r], cs * uk[e], L)) * dp[r] * uk[e];
+        dp[r] = exp2_hw(MODS == 0   ? fmaf(s[r], cs * uk[e], L)
+                        : MODS == 2 ? fmaf(s[r], f2, L)
+                                    : s[r] + l) * dp[r] * uk[e];
       }
     }
     pin_acc(dq);
@@ -1011,26 +1098,39 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
     }
   }
   if (!wave_live) return;
-  float f = pow2(-kTop) * a.scale, f2 = pow2(-kp) / dsc;
+  float f = pow2(-kTop) * a.scale, fq = pow2(-kp) / dsc;
   if (__builtin_amdgcn_ballot_w64(qi < a.SQ && !(probe_finite<kDT>(dq, f * 0.0f) == 0.0f)) != 0) {
     scored_queries_fp32<D>(a, b, h, qw0, t0, t1, sm.u.o[w], dq, late(lane));
-    f = a.scale, f2 = 1.0f;
+    f = a.scale, fq = 1.0f;
   }
-  store_rows<D>(dq, f, f2, sm.u.o[w], dq_rows, static_cast<int64_t>(a.H) * D, a.SQ - qw0, late(lane));
+  store_rows<D>(dq, f, fq, sm.u.o[w], dq_rows, static_cast<int64_t>(a.H) * D, a.SQ - qw0, late(lane));
 }
 
 template <int D, int MODS, int WAVES>
 __global__ void __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES)))
 bwd_scored_kernel(ScoredArgs a) {
   __shared__ __attribute__((aligned(16))) ScoredSmem<D> sm;
-  const int id = static_cast<int>(blockIdx.x), pairs = a.B * (a.H / a.G), BH = a.B * a.H, keys = a.nkb * pairs;
+  const int id = static_cast<int>(blockIdx.x), pairs = a.B * (a.H / a.G), BH = a.B * a.H;
+  const int per_k = a.nkb * a.nck, per_q = a.nqb * a.ncq, keys = per_k * pairs;
   if (id < keys) {
     // Causal: the low blocks (they are seen by every later query) first.
-    scored_keys<D, MODS>(a, sm, a.causal ? id % pairs * a.nkb + id / pairs : xcd_remap(id, keys));
+    const int item = a.causal ? id % pairs * per_k + id / pairs : xcd_remap(id, keys);
+    const int pair = item / per_k, in = item - pair * per_k, kb = in / a.nck;
+    scored_keys<D, MODS>(a, sm, pair * a.nkb + kb, in - kb * a.nck);
   } else {
-    const int i = id - keys;
-    scored_queries<D, MODS>(a, sm, a.causal ? i % BH * a.nqb + a.nqb - 1 - i / BH : xcd_remap(i, a.nqb * BH));
+    const int i = id - keys, item = a.causal ? i % BH * per_q + per_q - 1 - i / BH : xcd_remap(i, per_q * BH);
+    const int bh = item / per_q, in = item - bh * per_q, qb = in / a.ncq;
+    scored_queries<D, MODS>(a, sm, bh * a.nqb + qb, in - qb * a.ncq);
   }
+}
+// out = sum_c part[c], of `n` vectors of four, chunks in order.
+__global__ void __launch_bounds__(256) sum_scored_kernel(const float* part, float* out, int64_t n, int nc) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= n) return;
+  f4 x{};
+#pragma unroll 4
+  for (int c = 0; c < nc; ++c) x += ld4(part + (c * n + i) * 4);
+  st4(out + i * 4, x);
 }
 
 template <int MODS>
@@ -1046,27 +1146,59 @@ const void* bwd_fn(int d) {
                     : reinterpret_cast<const void*>(bwd_scored_kernel<64, MODS, 2>);
 }
 // (Scale 0: the products are multiplied by it before what is not seen becomes minus infinity.)
-int mods(const ScoredArgs& a) { return a.cap2 != 0.0f ? 2 : a.slopes != nullptr || a.scale == 0.0f ? 1 : 0; }
+int mods(const ScoredArgs& a) {
+  const int m = (a.slopes != nullptr ? 1 : 0) + (a.cap2 != 0.0f ? 2 : 0);
+  return m == 0 && a.scale == 0.0f ? 1 : m;
+}
 int64_t blocks_of(int64_t rows) { return (rows + kBlock - 1) / kBlock; }
 
 }  // namespace
 
 int64_t scored_blocks(int64_t b, int64_t heads, int64_t rows) { return b * heads * blocks_of(rows); }
 
+// Chunks of a walk of `steps`, and their length: none until the walk is half as long again as `target`.
+static void cut(int64_t steps, int64_t target, int* n, int* length) {
+  const int64_t want = 2 * steps > 3 * target ? (steps + target - 1) / target : 1;
+  *length = static_cast<int>(std::max<int64_t>(1, (steps + want - 1) / want));
+  *n = static_cast<int>(std::max<int64_t>(1, (steps + *length - 1) / *length));
+}
+// The part of sq x sk pairs that a causal mask leaves (documents and prefixes are on the device).
+static double seen_part(int64_t sq, int64_t sk, int causal) {
+  return causal ? 1.0 - 0.5 * static_cast<double>(sq) / static_cast<double>(sk) : 1.0;
+}
+
 ScoredPlan scored_plan(int64_t b, int64_t h, int64_t sq, int64_t sk, int64_t d) {
-  ScoredPlan p{1, 0, 0, 0};
+  ScoredPlan p{};
+  p.nc = 1;
+  if (sq == 0 || sk == 0) return p;
   const int64_t steps = (sk + kRows - 1) / kRows, blocks = scored_blocks(b, h, sq);
   const int64_t slots = 256 * (d == 32 ? 4 : d == 64 ? 3 : 2);
-  // Chunks of the keys where the blocks do not fill the chip, of 8 tiles or more.
-  const int64_t target = std::max<int64_t>(8, (blocks * steps + slots - 1) / slots);
-  const int64_t want = steps >= 2 * target ? (steps + target - 1) / target : 1;
-  p.chunk = static_cast<int>(std::max<int64_t>(1, (steps + want - 1) / want));
-  p.nc = static_cast<int>(std::max<int64_t>(1, (steps + p.chunk - 1) / p.chunk));
+  // Chunks of the keys where the blocks do not fill the chip, of 3 tiles or more.
+  if (4 * blocks <= 3 * slots) cut(steps, std::max<int64_t>(3, blocks * steps / slots), &p.nc, &p.chunk);
   if (p.nc > 1) {
     const size_t parts = static_cast<size_t>(p.nc) * b * h * sq;
     p.l_part = parts * d * sizeof(float);
     p.bytes = p.l_part + parts * sizeof(double);
   }
+  return p;
+}
+
+ScoredBackwardPlan scored_backward_plan(int64_t b, int64_t h, int64_t hk, int64_t sq, int64_t sk, int64_t d,
+                                        int causal) {
+  ScoredBackwardPlan p{1, 1, 1, 1, 0, 0};
+  if (sq == 0 || sk == 0) return p;
+  const int64_t slots = 256 * (d == 32 ? 3 : d == 64 ? 2 : 1), g = h / hk;
+  const int64_t tq = (sq + kRows - 1) / kRows, tk = (sk + kRows - 1) / kRows;
+  // A step of a key block takes four products, of a query block three. Chunks of 24 products or more.
+  const double all = (static_cast<double>(scored_blocks(b, hk, sk)) * g * tq * 4 +
+                      static_cast<double>(scored_blocks(b, h, sq)) * tk * 3) * seen_part(sq, sk, causal);
+  const int64_t target = std::max<int64_t>(24, static_cast<int64_t>(all / slots) + 1);
+  cut(g * tq, (target + 3) / 4, &p.nck, &p.chk);
+  cut(tk, (target + 2) / 3, &p.ncq, &p.chq);
+  const size_t q = static_cast<size_t>(b) * h * sq * d * sizeof(float);
+  const size_t k = static_cast<size_t>(b) * hk * sk * d * 2 * sizeof(float);
+  p.k_part = p.ncq > 1 ? p.ncq * q : 0;
+  p.bytes = p.k_part + (p.nck > 1 ? p.nck * k : 0);
   return p;
 }
 
@@ -1078,8 +1210,9 @@ int launch_scored_forward(ScoredArgs a, int d, const ScoredPlan& plan, void* wor
   void* args[] = {&a};
   hipStream_t s = static_cast<hipStream_t>(stream);
   const unsigned grid = static_cast<unsigned>(int64_t{a.B} * a.H * a.nqb * a.nc);
-  const hipError_t err = hipLaunchKernel(mods(a) == 2 ? fwd_fn<2>(d) : mods(a) == 1 ? fwd_fn<1>(d) : fwd_fn<0>(d), dim3(grid), dim3(64 * kW),
-                                         args, 0, s);
+  const int m = mods(a);
+  const void* fn = m == 3 ? fwd_fn<3>(d) : m == 2 ? fwd_fn<2>(d) : m == 1 ? fwd_fn<1>(d) : fwd_fn<0>(d);
+  const hipError_t err = hipLaunchKernel(fn, dim3(grid), dim3(64 * kW), args, 0, s);
   if (err != hipSuccess || a.nc == 1) return static_cast<int>(err);
   const void* join = d == 32    ? reinterpret_cast<const void*>(join_scored_kernel<32>)
                      : d == 128 ? reinterpret_cast<const void*>(join_scored_kernel<128>)
@@ -1089,14 +1222,30 @@ int launch_scored_forward(ScoredArgs a, int d, const ScoredPlan& plan, void* wor
                                           0, s));
 }
 
-int launch_scored_backward(ScoredArgs a, int d, void* stream) {
+int launch_scored_backward(ScoredArgs a, int d, const ScoredBackwardPlan& plan, void* workspace, void* stream) {
   a.nqb = static_cast<int>(blocks_of(a.SQ)), a.nkb = static_cast<int>(blocks_of(a.SK));
   a.nc = 1;
+  a.nck = plan.nck, a.chk = plan.chk, a.ncq = plan.ncq, a.chq = plan.chq;
+  if (a.SQ == 0) a.nck = a.ncq = 1;
+  float *q_part = static_cast<float*>(workspace), *dq = a.dq, *dkv = a.dkv;
+  float* k_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.k_part);
+  if (a.ncq > 1) a.dq = q_part;
+  if (a.nck > 1) a.dkv = k_part;
   void* args[] = {&a};
-  const int64_t grid = scored_blocks(a.B, a.H / a.G, a.SK) + scored_blocks(a.B, a.H, a.SQ);
-  return static_cast<int>(hipLaunchKernel(mods(a) == 2 ? bwd_fn<2>(d) : mods(a) == 1 ? bwd_fn<1>(d) : bwd_fn<0>(d),
-                                          dim3(static_cast<unsigned>(grid)), dim3(64 * kW), args, 0,
-                                          static_cast<hipStream_t>(stream)));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int HK = a.H / a.G;
+  const int64_t grid = scored_blocks(a.B, HK, a.SK) * a.nck + scored_blocks(a.B, a.H, a.SQ) * a.ncq;
+  const int m = mods(a);
+  const void* fn = m == 3 ? bwd_fn<3>(d) : m == 2 ? bwd_fn<2>(d) : m == 1 ? bwd_fn<1>(d) : bwd_fn<0>(d);
+  hipError_t err = hipLaunchKernel(fn, dim3(static_cast<unsigned>(grid)), dim3(64 * kW), args, 0, s);
+  auto sum = [&](const float* part, float* out, int64_t n, int nc) {
+    void* sargs[] = {&part, &out, &n, &nc};
+    return hipLaunchKernel(reinterpret_cast<const void*>(sum_scored_kernel),
+                           dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), sargs, 0, s);
+  };
+  if (err == hipSuccess && a.ncq > 1) err = sum(q_part, dq, int64_t{a.B} * a.SQ * a.H * d / 4, a.ncq);
+  if (err == hipSuccess && a.nck > 1) err = sum(k_part, dkv, int64_t{a.B} * a.SK * HK * d / 2, a.nck);
+  return static_cast<int>(err);
 }
 
 }  // namespace fattn

@@ -715,13 +715,15 @@ Tensors scored_backward(const Tensor& q, const Tensor& k, const Tensor& v, const
   const Tensor g = aligned_rows(grad);
   Tensor dq = at::empty_strided({b, h, sq, d}, {sq * h * d, d, h * d, 1}, q.options());
   Tensor dkv = at::empty({b, sk, 2, hk, d}, q.options());
+  const size_t bytes = fattn_scored_backward_workspace_bytes(b, h, hk, sq, sk, d, how.causal);
+  const Tensor ws = workspace(q, bytes);
   launch(q, [&](void* stream) {
     return fattn_scored_backward(f32(q), q.strides().data(), f32(k), k.strides().data(), f32(v),
                                  v.strides().data(), b, h, hk, sq, sk, d, static_cast<float>(how.scale),
                                  how.causal, how.cap, static_cast<const float*>(address(how.slopes)),
                                  ints(how.documents), rows_apart(how.documents), ints(how.prefix), f32(out),
                                  f32(lse), f32(g), g.strides().data(), static_cast<float*>(dq.data_ptr()),
-                                 static_cast<float*>(dkv.data_ptr()), stream);
+                                 static_cast<float*>(dkv.data_ptr()), address(ws), bytes, stream);
   });
   return {dq, dkv.select(2, 0).transpose(1, 2), dkv.select(2, 1).transpose(1, 2)};
 }

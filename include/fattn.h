@@ -332,8 +332,8 @@ int fattn_cross_backward(const float* q, const int64_t q_strides[3], const float
  * prefix[b] of the sample (NULL: none; outside [0, sk]: the nearest), or with causal 0 all; of these, with
  * documents ([b, sk] ids, rows document_stride apart), those of its own id, a token of a negative id none, and
  * it is seen by none. out [b, sq, heads, d] contiguous, lse [b, heads, sq]; a query that sees no key has out 0
- * and lse -infinity. Query head i reads key head i / (heads / kv_heads). The workspace is as
- * fattn_cross_forward's. Reruns are bit-identical. */
+ * and lse -infinity. Query head i reads key head i / (heads / kv_heads). The workspaces are
+ * as fattn_cross_forward's (the backward's sized by causal too). Reruns are bit-identical. */
 size_t fattn_scored_workspace_bytes(int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk,
                                     int64_t d);
 int fattn_scored_forward(const float* q, const int64_t q_strides[3], const float* k,
@@ -345,13 +345,16 @@ int fattn_scored_forward(const float* q, const int64_t q_strides[3], const float
 
 /* Its gradient, as fattn_cross_backward's: dq [b, sq, heads, d] and dkv [b, sk, 2, kv_heads, d], contiguous,
  * written whole (0 for what is not seen), in a fixed order. The slopes get none. */
+size_t fattn_scored_backward_workspace_bytes(int64_t b, int64_t heads, int64_t kv_heads, int64_t sq,
+                                             int64_t sk, int64_t d, int causal);
 int fattn_scored_backward(const float* q, const int64_t q_strides[3], const float* k,
                           const int64_t k_strides[3], const float* v, const int64_t v_strides[3],
                           int64_t b, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d,
                           float scale, int causal, float cap, const float* slopes,
                           const int32_t* documents, int64_t document_stride, const int32_t* prefix,
                           const float* out, const float* lse, const float* d_o,
-                          const int64_t do_strides[3], float* dq, float* dkv, void* stream);
+                          const int64_t do_strides[3], float* dq, float* dkv, void* workspace,
+                          size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Diagnostics (no counterpart in the reference).

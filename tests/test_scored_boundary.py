@@ -111,9 +111,9 @@ def forward(b=1, heads=1, hk=1, sq=1, sk=1, d=64, q=BAD, k=BAD, qst=ST, kst=ST, 
 
 
 def backward(b=1, heads=1, hk=1, sq=1, sk=1, d=64, q=BAD, k=BAD, qst=ST, kst=ST, cap=0.0, documents=None, dst=0,
-             out=BAD, g=BAD, gst=ST, dq=BAD, dkv=BAD):
+             out=BAD, g=BAD, gst=ST, dq=BAD, dkv=BAD, ws=BAD, size=1 << 40):
     return _lib.lib().fattn_scored_backward(q, qst, k, kst, k, kst, b, heads, hk, sq, sk, d, 1.0, 1, cap, None,
-                                            documents, dst, None, out, BAD, g, gst, dq, dkv, None)
+                                            documents, dst, None, out, BAD, g, gst, dq, dkv, ws, size, None)
 
 
 @pytest.mark.parametrize("call", [forward, backward])
@@ -143,13 +143,15 @@ def test_scored_refusals(call):
 
 def test_scored_workspace_and_gradient_refusals():
     L = _lib.lib()
-    need = L.fattn_scored_workspace_bytes(2, 4, 4, 1, 4096, 64)
-    assert need > 0
-    for ws, size in ((None, need), (ODD, need), (BAD, need - 1)):
-        refused(forward(b=2, heads=4, hk=4, sk=4096, ws=ws, size=size), _lib.FATTN_EWORKSPACE, str(need))
-    assert L.fattn_scored_workspace_bytes(64, 8, 8, 4096, 4096, 64) == 0
-    assert L.fattn_scored_workspace_bytes(2, 4, 3, 1, 4096, 64) == 0
-    assert L.fattn_scored_workspace_bytes(2, 4, 4, 5000, 4096, 64) == 0
+    for size_of, call, more in ((L.fattn_scored_workspace_bytes, forward, ()),
+                                (L.fattn_scored_backward_workspace_bytes, backward, (1,))):
+        need = size_of(2, 4, 4, 1, 4096, 64, *more)
+        assert need > 0
+        for ws, size in ((None, need), (ODD, need), (BAD, need - 1)):
+            refused(call(b=2, heads=4, hk=4, sk=4096, ws=ws, size=size), _lib.FATTN_EWORKSPACE, str(need))
+        assert size_of(64, 8, 8, 4096, 4096, 64, *more) == 0
+        assert size_of(2, 4, 3, 1, 4096, 64, *more) == 0
+        assert size_of(2, 4, 4, 5000, 4096, 64, *more) == 0
     refused(backward(g=None), _lib.FATTN_EINVAL, "null operand")
     refused(backward(dq=None), _lib.FATTN_EINVAL, "null operand")
     refused(backward(dkv=None), _lib.FATTN_EINVAL, "null operand")

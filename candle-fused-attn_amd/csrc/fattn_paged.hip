@@ -585,14 +585,18 @@ split_kernel(SplitArgs a) {
       const C *k, *v;
       int live;
     };
-    auto half = [&](int t, int h) {
+    // Its page is read a tile ahead of its keys, or every tile would wait for two loads, one after the other.
+    auto page_of = [&](int t, int h) {
+      const int at = min(2 * t + h, (len - 1) / 16);
+      return a.table[b * a.table_stride + divide(at, a.by_page)];
+    };
+    auto half = [&](int t, int h, int listed) {
       const int at = min(2 * t + h, (len - 1) / 16);
       Half x;
       x.live = min(len - 16 * at, 16);
       if constexpr (kPaged) {
         const int pi = divide(at, a.by_page), slot = 16 * (at - pi * (a.page_size / 16));
-        const bool had = a.wgs == 0 && at == 2 * w + h;
-        int page = __builtin_amdgcn_readfirstlane(had ? early[h] : a.table[b * a.table_stride + pi]);
+        int page = __builtin_amdgcn_readfirstlane(listed);
         if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pages)) page = 0, wrong = 1;
         x.k = kp + page * a.ks[0] + slot * a.ks[2];
         x.v = vp + page * a.vs[0] + slot * a.vs[2];
@@ -608,12 +612,22 @@ split_kernel(SplitArgs a) {
     const unsigned vss = static_cast<unsigned>(a.vs[2] * sizeof(C));
     int t = t0 + w;
     Half at[2];
+    int listed[2] = {};
+    auto list = [&](int t) {
+      if constexpr (kPaged) listed[0] = page_of(t, 0), listed[1] = page_of(t, 1);
+    };
     if (t < t1) {
+      if (a.wgs == 0) {
+        listed[0] = early[0], listed[1] = early[2 * w + 1 <= (len - 1) / 16 ? 1 : 0];
+      } else {
+        list(t);
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        at[h] = half(t, h);
+        at[h] = half(t, h, listed[h]);
         x.load_k(h, at[h].k, kss, at[h].live, j, g);
       }
+      list(t + kSplitWaves);
 #pragma unroll
       for (int h = 0; h < 2; ++h) x.load_v(h, at[h].v, vss, at[h].live, j, g);
     }
@@ -625,9 +639,10 @@ split_kernel(SplitArgs a) {
       if (more) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          at[h] = half(t + kSplitWaves, h);
+          at[h] = half(t + kSplitWaves, h, listed[h]);
           x.load_k(h, at[h].k, kss, at[h].live, j, g);
         }
+        list(t + 2 * kSplitWaves);
       }
       x.weights(s, live, g, a.cap2, a.cap_inv);
       x.sums(s, live, g);

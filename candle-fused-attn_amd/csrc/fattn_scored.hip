@@ -149,6 +149,19 @@ __device__ __forceinline__ void capped(f16v& x, F fn) {
 // tile has its key after its query, the distance is a sum of both, and slope x place (one value for the wave)
 // is added to the score while the lane's part goes with what the exponent adds: no instruction of its own.
 __device__ __forceinline__ int place_of(int r) { return 8 * (r >> 2) + (r & 3); }
+// Minus infinity to the registers of places outside [least, most]; to those of other ids than the lane's.
+__device__ __forceinline__ void hide(f16v& s, int least, int most) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = place_of(r) >= least && place_of(r) <= most ? s[r] : kNegInf;
+}
+__device__ __forceinline__ void hide_others(f16v& s, const int* tile, int mine, int g) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const i4 id = *reinterpret_cast<const i4*>(&tile[8 * i + 4 * g]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[4 * i + e] = id[e] == mine ? s[4 * i + e] : kNegInf;
+  }
+}
 struct Places {
   float by[16];  // slope2 times the place of register r, in scalar registers
   __device__ __forceinline__ void set(float slope2) {
@@ -158,17 +171,19 @@ struct Places {
     }
   }
 };
-// s, in units of 1 / f log2 e, to scores: plus its places' part (a key's place brings it nearer to the query).
-__device__ __forceinline__ void nearer(f16v& s, float f, const Places& places) {
-#pragma unroll
-  for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], f, places.by[r]);
-}
 // Otherwise: less slope2 |base + SIGN place|.
 template <int SIGN>
-__device__ __forceinline__ void lowered(f16v& s, float f, float slope2, float base) {
+__device__ __forceinline__ float far_by(int r, float slope2, float base) {
+  return -slope2 * fabsf(base + static_cast<float>(SIGN * place_of(r)));
+}
+// s[r] = s[r] f + by(r), f as fn(i)[c] of register 4 i + c.
+template <typename F, typename B>
+__device__ __forceinline__ void scale_add(f16v& s, F fn, B by) {
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    s[r] = fmaf(s[r], f, -slope2 * fabsf(base + static_cast<float>(SIGN * place_of(r))));
+  for (int i = 0; i < 4; ++i) {
+    const f4 f = fn(i);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s[4 * i + c] = fmaf(s[4 * i + c], f[c], by(4 * i + c));
   }
 }
 
@@ -452,37 +467,32 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
       for (int ks = 0; ks < kKS; ++ks) s = mma(kh[ks], q[ks].h, s);
     }
     float shift = 0.0f;  // of what is held less the score
-    if constexpr (MODS != 0) {
+    if constexpr ((MODS & 2) != 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const f4 uk = ld4(&sm.uk[cur][8 * i + 4 * g]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[4 * i + c] *= cq * uk[c];
       }
-      if constexpr ((MODS & 2) != 0) capped(s, [](int, float) {});
-      if constexpr ((MODS & 1) != 0) {
-        const float base = fpos - static_cast<float>(kt0);
-        if (ordered || kt0 + kRows - 1 <= lo_pos) {
-          shift = slope2 * base;
-          nearer(s, f2, places);
-        } else {
-          lowered<-1>(s, f2, slope2, base);
-        }
+      capped(s, [](int, float) {});
+    }
+    if constexpr ((MODS & 1) != 0) {
+      auto f = [&](int i) {
+        if constexpr ((MODS & 2) != 0) return f4{f2, f2, f2, f2};
+        return ld4(&sm.uk[cur][8 * i + 4 * g]) * cq;
+      };
+      const float base = fpos - static_cast<float>(kt0);
+      if (ordered || kt0 + kRows - 1 <= lo_pos) {
+        shift = slope2 * base;
+        scale_add(s, f, [&](int r) { return places.by[r]; });
+      } else {
+        scale_add(s, f, [&](int r) { return far_by<-1>(r, slope2, base); });
       }
     }
     // What is not seen is minus infinity: register r's key is kt0 + 4 g + 8 (r / 4) + r % 4.
     if (sees == kSome) {
-      const int left = lim - kt0 - 4 * g;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        i4 id{};
-        if (all_ids != nullptr) id = *reinterpret_cast<const i4*>(&sm.ids.tile[cur][8 * i + 4 * g]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const bool is = 8 * i + c <= left && id[c] == ids.mine && ids.mine >= 0;
-          s[4 * i + c] = is ? s[4 * i + c] : kNegInf;
-        }
-      }
+      hide(s, 0, ids.mine >= 0 ? lim - kt0 - 4 * g : -1);
+      if (all_ids != nullptr) hide_others(s, sm.ids.tile[cur], ids.mine, g);
     }
     f16v e;
     float psum = 0.0f, wmax = 0.0f;
@@ -775,7 +785,7 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
     // well, they do not fit.
     load(u + 2);
     pin_loads();
-    if constexpr (MODS != 0) {
+    if constexpr ((MODS & 2) != 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const f4 uq = ld4(&sm.ua[cur][8 * i + 4 * g]);
@@ -792,43 +802,36 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
     if constexpr ((MODS & 2) != 0) capped(s, [&](int r, float slope) { dp[r] *= slope; });
     // The slope's part: a row's (staged with its L) and the lane's, or, where a key may be after a query that
     // sees it, of the distance.
-    const float* l_of = sm.l[cur];
-    float shift = 0.0f;
-    float f = f2;
+    // (With a slope s becomes the whole exponent.)
     if constexpr ((MODS & 1) != 0) {
       const float slope2 = slope_of(a, h0 + hh);
+      auto f = [&](int i) {
+        if constexpr ((MODS & 2) != 0) return f4{f2, f2, f2, f2};
+        return ld4(&sm.ua[cur][8 * i + 4 * g]) * cs;
+      };
       if (ordered || kw0 + kRows - 1 <= q0 + off) {
-        l_of = sm.ls[cur];
-        shift = slope2 * static_cast<float>(key - k0);
+        const float shift = slope2 * static_cast<float>(key - k0);
+        scale_add(s, f, [&](int r) { return sm.ls[cur][place_of(r) + 4 * g] + shift; });
       } else {
-        lowered<1>(s, f2, slope2, static_cast<float>(q0 + 4 * g + off - key));
-        f = 1.0f;
+        const float base = static_cast<float>(q0 + 4 * g + off - key);
+        scale_add(s, f, [&](int r) { return sm.l[cur][place_of(r) + 4 * g] + far_by<1>(r, slope2, base); });
       }
     }
     // Register r's query is q0 + 4 g + 8 i + e: seen below SQ and, causal, not before the key.
     if (sees == kSome) {
-      const int end = key < a.SK && ids.mine >= 0 ? SQ - q0 - 4 * g : 0;
-      const int least = a.causal && key >= prefix ? key - off - q0 - 4 * g : 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        i4 id{};
-        if (all_ids != nullptr) id = *reinterpret_cast<const i4*>(&sm.ids.tile[cur][8 * i + 4 * g]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool is = 8 * i + e < end && 8 * i + e >= least && id[e] == ids.mine;
-          s[4 * i + e] = is ? s[4 * i + e] : kNegInf;
-        }
-      }
+      hide(s, a.causal && key >= prefix ? key - off - q0 - 4 * g : 0,
+           key < a.SK && ids.mine >= 0 ? SQ - 1 - q0 - 4 * g : -1);
+      if (all_ids != nullptr) hide_others(s, sm.ids.tile[cur], ids.mine, g);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      f4 L = ld4(l_of + 8 * i + 4 * g);
       const f4 uq = ld4(&sm.ua[cur][8 * i + 4 * g]), ug = ld4(&sm.ub[cur][8 * i + 4 * g]);
-      if constexpr ((MODS & 1) != 0) L += shift;
+      f4 L{};
+      if constexpr ((MODS & 1) == 0) L = ld4(&sm.l[cur][8 * i + 4 * g]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r = 4 * i + e;
-        s[r] = exp2_hw(MODS != 0 ? fmaf(s[r], f, L[e]) : fmaf(s[r], cs * uq[e], L[e])) * ug[e];
+        s[r] = exp2_hw((MODS & 1) != 0 ? s[r] : fmaf(s[r], MODS == 0 ? cs * uq[e] : f2, L[e])) * ug[e];
         dp[r] = s[r] * dp[r] * uq[e];
       }
     }
@@ -1015,7 +1018,7 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
     }
     load(t + 2);
     pin_loads();
-    if constexpr (MODS != 0) {
+    if constexpr ((MODS & 2) != 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const f4 uk = ld4(&sm.ua[cur][8 * i + 4 * g]);
@@ -1032,26 +1035,21 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
     if constexpr ((MODS & 2) != 0) capped(s, [&](int r, float slope) { dp[r] *= slope; });
     float l = L;
     if constexpr ((MODS & 1) != 0) {
+      auto f = [&](int i) {
+        if constexpr ((MODS & 2) != 0) return f4{f2, f2, f2, f2};
+        return ld4(&sm.ua[cur][8 * i + 4 * g]) * cs;
+      };
       const float base = fpos - static_cast<float>(kt0);
       if (ordered || kt0 + kRows - 1 <= lo_pos) {
         l = fmaf(-slope2, base, L);
-        nearer(s, f2, places);
+        scale_add(s, f, [&](int r) { return places.by[r]; });
       } else {
-        lowered<-1>(s, f2, slope2, base);
+        scale_add(s, f, [&](int r) { return far_by<-1>(r, slope2, base); });
       }
     }
     if (sees == kSome) {
-      const int left = lim - kt0 - 4 * g;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        i4 id{};
-        if (all_ids != nullptr) id = *reinterpret_cast<const i4*>(&sm.ids.tile[cur][8 * i + 4 * g]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool is = 8 * i + e <= left && id[e] == ids.mine && ids.mine >= 0;
-          s[4 * i + e] = is ? s[4 * i + e] : kNegInf;
-        }
-      }
+      hide(s, 0, ids.mine >= 0 ? lim - kt0 - 4 * g : -1);
+      if (all_ids != nullptr) hide_others(s, sm.ids.tile[cur], ids.mine, g);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -1156,9 +1154,9 @@ int64_t blocks_of(int64_t rows) { return (rows + kBlock - 1) / kBlock; }
 
 int64_t scored_blocks(int64_t b, int64_t heads, int64_t rows) { return b * heads * blocks_of(rows); }
 
-// Chunks of a walk of `steps`, and their length: none until the walk is half as long again as `target`.
-static void cut(int64_t steps, int64_t target, int* n, int* length) {
-  const int64_t want = 2 * steps > 3 * target ? (steps + target - 1) / target : 1;
+// Chunks of a walk of `steps`, and their length: none until the walk is `most` times as long as `target`.
+static void cut(int64_t steps, int64_t target, double most, int* n, int* length) {
+  const int64_t want = steps > most * target ? (steps + target - 1) / target : 1;
   *length = static_cast<int>(std::max<int64_t>(1, (steps + want - 1) / want));
   *n = static_cast<int>(std::max<int64_t>(1, (steps + *length - 1) / *length));
 }
@@ -1174,7 +1172,7 @@ ScoredPlan scored_plan(int64_t b, int64_t h, int64_t sq, int64_t sk, int64_t d) 
   const int64_t steps = (sk + kRows - 1) / kRows, blocks = scored_blocks(b, h, sq);
   const int64_t slots = 256 * (d == 32 ? 4 : d == 64 ? 3 : 2);
   // Chunks of the keys where the blocks do not fill the chip, of 3 tiles or more.
-  if (4 * blocks <= 3 * slots) cut(steps, std::max<int64_t>(3, blocks * steps / slots), &p.nc, &p.chunk);
+  if (4 * blocks <= 3 * slots) cut(steps, std::max<int64_t>(3, blocks * steps / slots), 1.5, &p.nc, &p.chunk);
   if (p.nc > 1) {
     const size_t parts = static_cast<size_t>(p.nc) * b * h * sq;
     p.l_part = parts * d * sizeof(float);
@@ -1193,8 +1191,9 @@ ScoredBackwardPlan scored_backward_plan(int64_t b, int64_t h, int64_t hk, int64_
   const double all = (static_cast<double>(scored_blocks(b, hk, sk)) * g * tq * 4 +
                       static_cast<double>(scored_blocks(b, h, sq)) * tk * 3) * seen_part(sq, sk, causal);
   const int64_t target = std::max<int64_t>(24, static_cast<int64_t>(all / slots) + 1);
-  cut(g * tq, (target + 3) / 4, &p.nck, &p.chk);
-  cut(tk, (target + 2) / 3, &p.ncq, &p.chq);
+  // (Whole walks of up to 2.5 targets end beside the others': 2 x 16 heads s 1024 d 64 causal 91, cut at 1.5 98.)
+  cut(g * tq, (target + 3) / 4, 2.5, &p.nck, &p.chk);
+  cut(tk, (target + 2) / 3, 2.5, &p.ncq, &p.chq);
   const size_t q = static_cast<size_t>(b) * h * sq * d * sizeof(float);
   const size_t k = static_cast<size_t>(b) * hk * sk * d * 2 * sizeof(float);
   p.k_part = p.ncq > 1 ? p.ncq * q : 0;

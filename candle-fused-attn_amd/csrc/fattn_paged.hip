@@ -91,7 +91,8 @@ __device__ __forceinline__ float row_sum(float x) {
 // cut off towards 0 and none is 0 where x is not (a rest of nothing counts as 2^-30 of x): all have x's
 // sign, and an infinity that they multiply stays one.
 __device__ __forceinline__ float rest(float x, float least) { return fabsf(x) > fabsf(least) ? x : least; }
-template <int N>
+// (kRest false: the rest as it is, where nothing that is multiplied is infinite.)
+template <int N, bool kRest = true>
 __device__ __forceinline__ void terms2(float x, float y, unsigned (&w)[N], __bf16) {
   typedef __bf16 b2 __attribute__((ext_vector_type(2)));
   const float lx = x * 0x1p-30f, ly = y * 0x1p-30f;
@@ -99,7 +100,8 @@ __device__ __forceinline__ void terms2(float x, float y, unsigned (&w)[N], __bf1
   for (int i = 0; i < N - 1; ++i) {
     const unsigned hx = __float_as_uint(x) & 0xffff0000u, hy = __float_as_uint(y) & 0xffff0000u;
     w[i] = __builtin_amdgcn_perm(hy, hx, 0x07060302u);
-    x = rest(x - __uint_as_float(hx), lx), y = rest(y - __uint_as_float(hy), ly);
+    x = x - __uint_as_float(hx), y = y - __uint_as_float(hy);
+    if constexpr (kRest) x = rest(x, lx), y = rest(y, ly);
   }
   w[N - 1] = __builtin_bit_cast(unsigned, b2{static_cast<__bf16>(x), static_cast<__bf16>(y)});
 }
@@ -265,10 +267,11 @@ struct Wave {
     for (int i = 0; i < kAcc; ++i) o[i] = f4{};
   }
   // Half h of a tile, from the row of its first key (uniform, so a load is a scalar base and a 32-bit
-  // offset of the lane); `live` of its 16 keys are there (the others repeat the last).
+  // offset of the lane); `live` of its 16 keys are there (the others repeat the last; 4-bit rows, which are
+  // a page's, are there whatever they hold, and no offset changes from tile to tile).
   __device__ __forceinline__ void load_k(int h, const C* p, unsigned ss, int live, int j, int g) {
     const char* base = reinterpret_cast<const char*>(p);
-    const unsigned row = static_cast<unsigned>(min(j, live - 1)) * ss;
+    const unsigned row = static_cast<unsigned>(kFour ? j : min(j, live - 1)) * ss;
     if constexpr (kFour) {
       struct alignas(4) Words {
         unsigned w[kKLoads];
@@ -287,16 +290,17 @@ struct Wave {
     const char* base = reinterpret_cast<const char*>(p);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const unsigned first = static_cast<unsigned>(min(4 * g + r, live - 1)) * ss;
       if constexpr (kFour) {
+        const char* row = base + r * ss;
+        const unsigned first = 4u * g * ss;
         typedef std::conditional_t<kC == 8, unsigned, std::conditional_t<kC == 4, unsigned short, unsigned char>>
             Codes;
-        raw.v[h][r] = *reinterpret_cast<const Codes*>(base + (first + static_cast<unsigned>(kC / 2) * j));
+        raw.v[h][r] = *reinterpret_cast<const Codes*>(row + (first + static_cast<unsigned>(kC / 2) * j));
         raw.v_scale[h][r] =
-            *reinterpret_cast<const unsigned char*>(base + (first + D / 2 + static_cast<unsigned>(kC) * j / 32));
-        continue;
+            *reinterpret_cast<const unsigned char*>(row + (first + D / 2 + static_cast<unsigned>(kC) * j / 32));
       } else {
-        const unsigned at = first + static_cast<unsigned>(kC * sizeof(C)) * j;
+        const unsigned at =
+            static_cast<unsigned>(min(4 * g + r, live - 1)) * ss + static_cast<unsigned>(kC * sizeof(C)) * j;
 #pragma unroll
         for (int t = 0; t < kBlocks; ++t) {
           const char* row = base + (at + static_cast<unsigned>(16 * kC * sizeof(C)) * t);
@@ -360,19 +364,29 @@ struct Wave {
   __device__ __forceinline__ void weights(f4 (&s)[2], int live, int g, float cap2, float cap_inv) {
     float top = kNegInf;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < 2; ++h) s[h] *= c2;
+    if constexpr (kMods) {
+      if (cap2 != 0.0f) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float x = s[h][r] * c2;
-        if constexpr (kMods) {
+        for (int i = 0; i < 8; ++i) {
           float d;
-          if (cap2 != 0.0f) x = cap2 * tanh_any(x * cap_inv, d);
-          x = fmaf(-slope2, static_cast<float>(live - 1 - 16 * h - 4 * g - r), x);
+          s[i / 4][i % 4] = cap2 * tanh_any(s[i / 4][i % 4] * cap_inv, d);
         }
-        s[h][r] = 16 * h + 4 * g + r < live ? x : kNegInf;
-        top = fmaxf(top, s[h][r]);
+      }
+      const float last = static_cast<float>(live - 1 - 4 * g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        s[i / 4][i % 4] = fmaf(-slope2, last - static_cast<float>(16 * (i / 4) + i % 4), s[i / 4][i % 4]);
       }
     }
+    if (!kFour || live < kTile) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        s[i / 4][i % 4] = 16 * (i / 4) + 4 * g + i % 4 < live ? s[i / 4][i % 4] : kNegInf;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, s[i / 4][i % 4]);
     // The reference moves only when a weight passes it by 2^kRoom (or there is none yet).
     if (__builtin_amdgcn_ballot_w64(top > m + kRoom) != 0) {
       const float to = fmaxf(m, row_max(top));
@@ -391,6 +405,9 @@ struct Wave {
         l += s[h][r];
       }
     }
+  }
+  static __device__ __forceinline__ void bf16_terms2(float x, float y, unsigned (&w)[kPT]) {
+    terms2<kPT, !kFour>(x, y, w, __bf16{});
   }
   // o += V^T P^T. Values of absent keys count as 0, whatever memory holds there.
   __device__ __forceinline__ void sums(const f4 (&p)[2], int live, int g) {
@@ -444,7 +461,7 @@ struct Wave {
       u4 b[kPT];
       unsigned w[4][kPT];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) terms2(p[e / 2][2 * (e % 2)], p[e / 2][2 * (e % 2) + 1], w[e], M{});
+      for (int e = 0; e < 4; ++e) bf16_terms2(p[e / 2][2 * (e % 2)], p[e / 2][2 * (e % 2) + 1], w[e]);
 #pragma unroll
       for (int t = 0; t < kPT; ++t) b[t] = u4{w[0][t], w[1][t], w[2][t], w[3][t]};
 #pragma unroll
@@ -470,7 +487,7 @@ struct Wave {
 // Waves per SIMD (so workgroups per CU) that the registers allow.
 template <typename Q, typename C, int D>
 constexpr int kOccupancy = D == 32    ? 4
-                           : std::is_same<C, four>::value ? (std::is_same<Q, float>::value ? (D == 64 ? 3 : 2) : D == 64 ? 4 : 3)
+                           : std::is_same<C, four>::value ? (std::is_same<Q, __bf16>::value ? 4 : 3) - (D == 128 ? 1 : 0)
                            : D == 128 ? 2
                            : std::is_same<C, _Float16>::value || (std::is_same<C, __bf16>::value &&
                                                                   std::is_same<Q, C>::value)

@@ -223,7 +223,8 @@ struct RotaryArgs {
   Divider by_per[3], by_items[3], by_seq, by_pairs;
 };
 // vec: values per access, 8, 4 or 1 (2 interleaved): every pointer, stride and part of a head is a
-// multiple of it, where it is 4 or more. (To a 4-bit cache: 8, of accesses of 16 bytes, or less.)
+// multiple of it, where it is 4 or more. (To a 4-bit cache: 16, two halves of a
+// part of a head in accesses of 16 bytes, or 8, one by one.)
 int launch_rotary(RotaryArgs a, int dtype, int cache_dtype, int vec, void* stream);
 
 // Tokens starts[b] + i (starts null: i), i < S, of a paged cache, to k and v, [B, HK, S, d] contiguous: 0

@@ -124,15 +124,15 @@ int run_rotary(const char* who, fattn::RotaryArgs& a, int dtype, int cache_dtype
   a.pairs = static_cast<int>(dim / 2);
   int64_t vec = 16 / size;
   if (cache_dtype == FATTN_FP4) {
-    // Eight values at a time, in accesses of 16 bytes, or one by one.
-    bool wide = a.interleaved || dim / 2 % 8 == 0;
+    // Sixteen values at a time, in two halves of which each is whole scales, or eight.
+    bool pairs = d >= 64 && (a.interleaved ? dim % 8 == 0 : dim % 64 == 0 && (d - dim) % 64 == 0);
     for (int i = 0; i < 3; ++i) {
       const fattn::RotaryPart& p = a.part[i];
       if (p.heads == 0) continue;
-      wide = wide && fits(vec, p.x, size, p.xs, b, p.heads, s);
-      if (i == 0) wide = wide && fits(vec, p.y, size, p.ys, b, p.heads, s);
+      pairs = pairs && fits(vec, p.x, size, p.xs, b, p.heads, s);
+      if (i == 0) pairs = pairs && fits(vec, p.y, size, p.ys, b, p.heads, s);
     }
-    const int err = fattn::launch_rotary(a, dtype, cache_dtype, wide ? 8 : 1, stream);
+    const int err = fattn::launch_rotary(a, dtype, cache_dtype, pairs ? 16 : 8, stream);
     if (err) return fattn::hip_error(err, who, "launch");
     return fattn::done();
   }

@@ -238,102 +238,86 @@ __device__ __forceinline__ float to_odd(double x) {
   const unsigned u = __float_as_uint(r) - (fabs(back) > fabs(x) ? 1u : 0u);
   return __uint_as_float(u | 1u);
 }
-// Eight values, of a group of 32 that four neighbouring lanes have: their codes, and the group's scale byte.
-__device__ __forceinline__ unsigned codes_of(const float (&x)[8], unsigned& scale) {
-  unsigned top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+// Of a group of 32 values that four neighbouring lanes have eight each of, the bits of whose largest magnitude
+// are `top`: over all four.
+__device__ __forceinline__ unsigned group_top(unsigned top) {
   top = max(top, static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0xB1, 0xF, 0xF, true)));
-  top = max(top, static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0x4E, 0xF, 0xF, true)));
-  // (1.m 2^E <= 7 2^(E - 2) up to 1.75.)
+  return max(top, static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0x4E, 0xF, 0xF, true)));
+}
+__device__ __forceinline__ unsigned bits_of(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// Its scale byte (1.m 2^E <= 7 2^(E - 2) up to 1.75), 255 where a value is not finite.
+__device__ __forceinline__ unsigned scale_byte(unsigned top) {
   const int e = static_cast<int>(top >> 23) - 2 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-  const bool finite = top < 0x7f800000u;
-  scale = finite ? static_cast<unsigned>(max(e, 0)) : 255u;
+  return top < 0x7f800000u ? static_cast<unsigned>(max(e, 0)) : 255u;
+}
+// The eight's codes under it, no negative zeros among them (a token has one code for 0).
+__device__ __forceinline__ unsigned codes_of(const float (&x)[8], unsigned scale) {
   const float s = __uint_as_float(scale << 23);
   unsigned w = 0;
   w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
   w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
   w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
   w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
-  // No negative zeros: a token has one code for 0.
   const unsigned some = (w | w >> 1 | w >> 2) & 0x11111111u;
   w &= 0x77777777u | some << 3;
-  return finite ? w : 0u;
+  return scale != 255u ? w : 0u;
+}
+// The same, and the scale they take.
+__device__ __forceinline__ unsigned scaled_codes(const float (&x)[8], unsigned& scale) {
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, bits_of(x[i]));
+  scale = scale_byte(group_top(top));
+  return codes_of(x, scale);
+}
+// Codes of values that are within `off` of x, and whether these decide them: the same scale and codes at both
+// ends (and no overflow, nor values among the least, where `off` does not hold).
+__device__ __forceinline__ unsigned codes_within(const float (&x)[8], const float (&off)[8], unsigned& scale,
+                                                 bool& sure) {
+  float lo[8], hi[8];
+  unsigned most = 0, least = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    lo[i] = x[i] - off[i], hi[i] = x[i] + off[i];
+    most = max(most, bits_of(fabsf(x[i]) + off[i]));
+    least = max(least, __float_as_uint(fmaxf(fabsf(x[i]) - off[i], 0.0f)));
+  }
+  most = group_top(most), least = group_top(least);
+  scale = scale_byte(most);
+  const unsigned w = codes_of(lo, scale);
+  sure = scale == scale_byte(least) && w == codes_of(hi, scale) && most < 0x7f800000u && most > 0x0d800000u;
+  return w;
 }
 
-constexpr int kMaxAngles64 = 1024;
-
-// As rotary_kernel, an item 8 values of a head: of part 0 (q) written turned, of parts 1 and 2 as codes.
-// kWide: an operand's values are moved 8 at a time.
-template <typename T, bool kWide, bool kInterleaved>
-__global__ void __launch_bounds__(kRotThreads) append_four_kernel(RotaryArgs a) {
-  __shared__ double2 cs[kMaxAngles64];
-  __shared__ int64_t at_of[kMaxTokens];
-  __shared__ int pos_of[kMaxTokens];
-  const int tid = threadIdx.x, n = a.pairs, D = a.D;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens, all = static_cast<int64_t>(a.B) * a.S;
-  const int nt = static_cast<int>(all - t0 < a.tokens ? all - t0 : a.tokens);
-  const int y = static_cast<int>(blockIdx.y);
-  const int pi = y < a.first_share[1] ? 0 : y < a.first_share[2] ? 1 : 2;
-  const RotaryPart& part = a.part[pi];
-  const bool turns = part.rotate != 0 && n > 0;
-  const int of = a.items[pi], per = of * part.heads, items = nt * per;
-  const int shares = a.first_share[pi + 1] - a.first_share[pi];
-  const int share = (items / of + shares - 1) / shares * of;  // (whole heads)
-  const int first = (y - a.first_share[pi]) * share;
-  const int last = first + share < items ? first + share : items;
-  constexpr int kInFlight = 2;
-
-  struct Item {
-    T x[8], z[8];  // the values, and those that they turn with
-    int64_t to;
-    int t, e, head, low;  // token, first value (-1: no item), head; low: (half layout) the first of the pairs
-  };
-  Item it[kInFlight];
-  auto load = [&](int base) {
-#pragma unroll
-    for (int u = 0; u < kInFlight; ++u) {
-      const int item = base + u * kRotThreads;
-      it[u].e = -1;
-      if (item >= last) continue;
-      const int t = divide(item, a.by_per[pi]);
-      const int r = item - t * per, head = divide(r, a.by_items[pi]), e = 8 * (r - head * of);
-      const int tok = static_cast<int>(t0) + t, b = divide(tok, a.by_seq), i = tok - b * a.S;
-      it[u].t = t, it[u].e = e, it[u].head = head;
-      it[u].to = pi == 0 ? b * part.ys[0] + head * part.ys[1] + i * part.ys[2] : 0;
-      const T* row = static_cast<const T*>(part.x) + b * part.xs[0] + head * part.xs[1] + i * part.xs[2];
-      if constexpr (kWide) {
-        typedef Vec<T, 16 / sizeof(T)> In;
-        constexpr int kIn = 16 / sizeof(T);
-#pragma unroll
-        for (int k = 0; k < 8; k += kIn) {
-          const In x = *reinterpret_cast<const In*>(row + e + k);
-#pragma unroll
-          for (int c = 0; c < kIn; ++c) it[u].x[k + c] = x.v[c];
-        }
-        if (!kInterleaved && turns && e < 2 * n) {
-          const T* other = row + (e < n ? e + n : e - n);
-#pragma unroll
-          for (int k = 0; k < 8; k += kIn) {
-            const In x = *reinterpret_cast<const In*>(other + k);
-#pragma unroll
-            for (int c = 0; c < kIn; ++c) it[u].z[k + c] = x.v[c];
-          }
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int c = e + k;
-          it[u].x[k] = row[c];
-          if (!kInterleaved && turns && c < 2 * n) it[u].z[k] = row[c < n ? c + n : c - n];
-        }
-      }
-    }
-  };
-  load(first + tid);
-
-  if (tid < nt) {
-    const int tok = static_cast<int>(t0) + tid, b = divide(tok, a.by_seq), i = tok - b * a.S;
+// What a workgroup of an append has: `nt` tokens from t0 of operand pi (as rotary_kernel's), items first ..
+// last (whole heads), where its tokens go and their angles.
+struct AppendBlock {
+  int64_t t0;
+  int nt, pi, of, per, first, last;
+  bool turns;
+  __device__ __forceinline__ explicit AppendBlock(const RotaryArgs& a) {
+    const int64_t all = static_cast<int64_t>(a.B) * a.S;
+    t0 = static_cast<int64_t>(blockIdx.x) * a.tokens;
+    nt = static_cast<int>(all - t0 < a.tokens ? all - t0 : a.tokens);
+    const int y = static_cast<int>(blockIdx.y);
+    pi = y < a.first_share[1] ? 0 : y < a.first_share[2] ? 1 : 2;
+    turns = a.part[pi].rotate != 0 && a.pairs > 0;
+    of = a.items[pi], per = of * a.part[pi].heads;
+    const int items = nt * per, shares = a.first_share[pi + 1] - a.first_share[pi];
+    const int share = (items / of + shares - 1) / shares * of;
+    first = (y - a.first_share[pi]) * share;
+    last = first + share < items ? first + share : items;
+  }
+};
+struct AppendSmem {
+  float2 cs[kMaxAngles];
+  int64_t at_of[kMaxTokens];  // the token's slot, -1: none
+  int pos_of[kMaxTokens];     // what its sequence holds before
+};
+__device__ __forceinline__ void append_tokens(const RotaryArgs& a, const AppendBlock& k, AppendSmem& sm) {
+  const int tid = threadIdx.x, n = a.pairs;
+  if (tid < k.nt) {
+    const int tok = static_cast<int>(k.t0) + tid, b = divide(tok, a.by_seq), i = tok - b * a.S;
     const int held = a.lengths[b];
     const int64_t p = static_cast<int64_t>(held) + i;
     // (As in rotary_kernel.)
@@ -342,97 +326,324 @@ __global__ void __launch_bounds__(kRotThreads) append_four_kernel(RotaryArgs a) 
     if (counted && held >= 0 && p / a.page_size < a.table_width) {
       page = a.table[b * a.table_stride + p / a.page_size];
     }
-    const int64_t* st = a.page_strides + (pi == 2 ? 3 : 0);
-    at_of[tid] = page >= 0 && page < a.pages ? page * st[0] + p % a.page_size * st[2] : -1;
-    pos_of[tid] = held;
+    const int64_t* st = a.page_strides + (k.pi == 2 ? 3 : 0);
+    sm.at_of[tid] = page >= 0 && page < a.pages ? page * st[0] + p % a.page_size * st[2] : -1;
+    sm.pos_of[tid] = held;
   }
   __syncthreads();
-  // Angles: q's in 32 bits, as fused_rotary's.
-  float2* cs32 = reinterpret_cast<float2*>(cs);
-  if (turns) {
-    for (int i = tid; i < nt * n; i += kRotThreads) {
-      const int t = divide(i, a.by_pairs);
-      const int tok = static_cast<int>(t0) + t, b = divide(tok, a.by_seq);
-      const double p = static_cast<double>(static_cast<int64_t>(pos_of[t]) + (tok - b * a.S));
-      const double f = a.frequencies[i - t * n];
-      if (pi == 0) {
-        cs32[i] = turn(p, f, a.magnitude);
-      } else {
-        cs[i] = turn64(p, f, a.magnitude);
-      }
+  if (!k.turns) return;
+  for (int i = tid; i < k.nt * n; i += kRotThreads) {
+    const int t = divide(i, a.by_pairs);
+    const int tok = static_cast<int>(k.t0) + t, b = divide(tok, a.by_seq);
+    const double p = static_cast<double>(static_cast<int64_t>(sm.pos_of[t]) + (tok - b * a.S));
+    const double f = a.frequencies[i - t * n];
+    if (k.pi == 0) {  // (q's as fused_rotary's)
+      sm.cs[i] = turn(p, f, a.magnitude);
+    } else {
+      const double2 w = turn64(p, f, a.magnitude);
+      sm.cs[i] = float2{static_cast<float>(w.x), static_cast<float>(w.y)};
     }
-    __syncthreads();
   }
-
-  // fn(k, value, its partner, whether it is the first of the pair, its pair) of an item's turned values.
-  auto each = [&](const Item& x, auto turned_value, auto plain_value) {
+  __syncthreads();
+}
+// The position of the block's token t.
+__device__ __forceinline__ double position_of(const RotaryArgs& a, const AppendBlock& k, const AppendSmem& sm, int t) {
+  const int tok = static_cast<int>(k.t0) + t, b = divide(tok, a.by_seq);
+  return static_cast<double>(static_cast<int64_t>(sm.pos_of[t]) + (tok - b * a.S));
+}
+// Eight values to 16-byte aligned memory.
+template <typename T>
+__device__ __forceinline__ void put8(T* to, const T (&x)[8]) {
+  constexpr int kOut = 16 / sizeof(T);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int c = x.e + k;
-      if (!turns || c >= 2 * n) {
-        plain_value(k);
-      } else if (kInterleaved) {
-        turned_value(k, x.x[k], x.x[k ^ 1], (k & 1) == 0, x.t * n + c / 2);
-      } else {
-        turned_value(k, x.x[k], x.z[k], c < n, x.t * n + (c < n ? c : c - n));
-      }
+  for (int k = 0; k < 8; k += kOut) {
+    Vec<T, kOut> v;
+#pragma unroll
+    for (int c = 0; c < kOut; ++c) v.v[c] = x[k + c];
+    *reinterpret_cast<Vec<T, kOut>*>(to + k) = v;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void get8(T (&x)[8], const T* from) {
+  constexpr int kIn = 16 / sizeof(T);
+#pragma unroll
+  for (int k = 0; k < 8; k += kIn) {
+    const Vec<T, kIn> v = *reinterpret_cast<const Vec<T, kIn>*>(from + k);
+#pragma unroll
+    for (int c = 0; c < kIn; ++c) x[k + c] = v.v[c];
+  }
+}
+// Eight values of a key, y = x c + z s (w(k): c, and s with z's sign), as codes, formed in 32 bits: off by 3 x
+// 2^-24 of |x| + |z| at most. `sure`: that leaves no code in doubt.
+template <typename T, typename W>
+__device__ __forceinline__ unsigned turned_codes(const T (&x)[8], const T (&z)[8], float magnitude, W w,
+                                                 unsigned& scale, bool& sure) {
+  float v[8], off[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float2 c = w(k);
+    const float fx = static_cast<float>(x[k]), fz = static_cast<float>(z[k]);
+    v[k] = fmaf(fx, c.x, fz * c.y);
+    off[k] = (fabsf(fx) + fabsf(fz)) * (magnitude * 0x1p-21f);
+  }
+  bool here;
+  const unsigned codes = codes_within(v, off, scale, here);
+  sure = sure && here;
+  return codes;
+}
+// Value c of a turned head: its pair (-1: not turned), whether it is the pair's first, the other's place.
+template <bool kInterleaved>
+struct Pairing {
+  int pair, other;
+  bool low;
+  __device__ __forceinline__ Pairing(int c, int n, bool turns) {
+    pair = !turns || c >= 2 * n ? -1 : kInterleaved ? c / 2 : c < n ? c : c - n;
+    low = kInterleaved ? c % 2 == 0 : c < n;
+    other = pair < 0 ? c : kInterleaved ? (low ? c + 1 : c - 1) : low ? c + n : c - n;
+  }
+};
+// The codes of values e .. e + 7 of the block's token t, formed in 64 bits.
+template <typename T, bool kInterleaved>
+__device__ __forceinline__ unsigned exact_codes(const RotaryArgs& a, const AppendBlock& blk, const AppendSmem& sm,
+                                                int t, const T* row, int e, unsigned& scale) {
+  const double p = position_of(a, blk, sm, t);
+  float v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const Pairing<kInterleaved> at(e + k, a.pairs, blk.turns);
+    const float x = static_cast<float>(row[e + k]);
+    v[k] = x;
+    if (at.pair >= 0) {
+      const double2 c = turn64(p, a.frequencies[at.pair], a.magnitude);
+      const double z = static_cast<double>(static_cast<float>(row[at.other])) * c.y;
+      v[k] = to_odd(fma(static_cast<double>(x), c.x, at.low ? -z : z));
+    }
+    __builtin_amdgcn_sched_barrier(0);  // (one after the other: registers)
+  }
+  return scaled_codes(v, scale);
+}
+template <typename T>
+__device__ __forceinline__ unsigned plain_codes(const T (&x)[8], unsigned& scale) {
+  float v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = static_cast<float>(x[k]);
+  return scaled_codes(v, scale);
+}
+
+// An item: 8 values from e and 8 from e + gap on of one head: of the turned part, in the half layout, those that
+// turn together (gap n); of the rest, or of a head that is not turned or turned in neighbours, its halves.
+// Every part's half is a multiple of 32, so that four neighbours have a scale's values, and all is moved 16
+// bytes at a time.
+template <typename T, bool kInterleaved>
+__global__ void __launch_bounds__(kRotThreads)
+append_four_kernel(RotaryArgs a) {
+  __shared__ AppendSmem sm;
+  const AppendBlock blk(a);
+  const RotaryPart& part = a.part[blk.pi];
+  const int n = a.pairs, D = a.D, pi = blk.pi;
+  const bool halves = !kInterleaved && blk.turns;  // the turned part's halves turn together
+  constexpr int kInFlight = 2;
+  struct Item {
+    T x[8], z[8];
+    int64_t to;
+    int t, e, head, gap;  // e -1: no item
+  };
+  Item it[kInFlight];
+  // An item's token, head, first value and gap; its row.
+  auto place = [&](int item, int& t, int& head, int& e, int& gap) {
+    t = divide(item, a.by_per[pi]);
+    const int r = item - t * blk.per;
+    head = divide(r, a.by_items[pi]);
+    e = 8 * (r - head * blk.of), gap = D / 2;
+    if (halves) {
+      const bool rest = e >= n;
+      gap = rest ? D / 2 - n : n;
+      e += rest ? n : 0;
     }
   };
-  for (int base = first + tid; base < last; base += kRotThreads * kInFlight) {
-    if (base != first + tid) load(base);
+  auto row_of = [&](int t, int head, int64_t& to) {
+    const int tok = static_cast<int>(blk.t0) + t, b = divide(tok, a.by_seq), i = tok - b * a.S;
+    to = pi == 0 ? b * part.ys[0] + head * part.ys[1] + i * part.ys[2] : 0;
+    return static_cast<const T*>(part.x) + b * part.xs[0] + head * part.xs[1] + i * part.xs[2];
+  };
+  auto load = [&](int base) {
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
-      const Item& x = it[u];
-      if (x.e < 0) continue;
+      const int item = base + u * kRotThreads;
+      it[u].e = -1;
+      if (item >= blk.last) continue;
+      place(item, it[u].t, it[u].head, it[u].e, it[u].gap);
+      const T* row = row_of(it[u].t, it[u].head, it[u].to) + it[u].e;
+      get8(it[u].x, row);
+      get8(it[u].z, row + it[u].gap);
+    }
+  };
+  load(blk.first + static_cast<int>(threadIdx.x));
+  append_tokens(a, blk, sm);
+  const float magnitude = fabsf(static_cast<float>(a.magnitude));
+
+  // Sixteen values, turned where they are turned, of q.
+  auto put_q = [&](const Item& x) {
+    T* to = static_cast<T*>(part.y) + x.to + x.e;
+    T y[8], w[8];
+    const float2* cs = sm.cs + x.t * n + x.e;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y[k] = x.x[k], w[k] = x.z[k];
+    if (halves && x.e < n) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float p = static_cast<float>(x.x[k]), q = static_cast<float>(x.z[k]);
+        y[k] = static_cast<T>(turned(p, cs[k].x, -(q * cs[k].y)));
+        w[k] = static_cast<T>(turned(q, cs[k].x, p * cs[k].y));
+      }
+    } else if (kInterleaved && blk.turns) {
+      auto pairs = [&](T (&y)[8], int e) {
+        if (e >= 2 * n) return;
+        const float2* cs = sm.cs + x.t * n + e / 2;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float p = static_cast<float>(y[2 * k]), q = static_cast<float>(y[2 * k + 1]);
+          y[2 * k] = static_cast<T>(turned(p, cs[k].x, -(q * cs[k].y)));
+          y[2 * k + 1] = static_cast<T>(turned(q, cs[k].x, p * cs[k].y));
+        }
+      };
+      pairs(y, x.e);
+      pairs(w, x.e + x.gap);
+    }
+    put8(to, y);
+    put8(to + x.gap, w);
+  };
+  // Codes and scales of a key's or value's item.
+  auto put = [&](int t, int head, int e, int gap, unsigned cx, unsigned cz, unsigned sx, unsigned sz) {
+    unsigned word = sx << (e / 32 * 8) | sz << ((e + gap) / 32 * 8);
+    // (The head's scale bytes, in order, from its groups' lanes.)
+    if (D == 128) word |= static_cast<unsigned>(__shfl_xor(static_cast<int>(word), 4));
+    unsigned char* row =
+        static_cast<unsigned char*>(part.y) + sm.at_of[t] + head * a.page_strides[pi == 2 ? 4 : 1];
+    *reinterpret_cast<unsigned*>(row + e / 2) = cx;
+    *reinterpret_cast<unsigned*>(row + (e + gap) / 2) = cz;
+    if (e == 0) *reinterpret_cast<unsigned*>(row + D / 2) = word;
+  };
+  auto put_codes = [&](const Item& x) {
+    unsigned cx, cz, sx, sz;
+    bool sure = true;
+    const float2* cs = sm.cs + x.t * n;
+    if (halves && x.e < n) {
+      cs += x.e;
+      cx = turned_codes(x.x, x.z, magnitude, [&](int k) { return float2{cs[k].x, -cs[k].y}; }, sx, sure);
+      cz = turned_codes(x.z, x.x, magnitude, [&](int k) { return cs[k]; }, sz, sure);
+    } else if (kInterleaved && blk.turns) {
+      auto pairs = [&](const T (&y)[8], int e, unsigned& scale) {
+        if (e >= 2 * n) return plain_codes(y, scale);
+        T other[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) other[k] = y[k ^ 1];
+        return turned_codes(
+            y, other, magnitude,
+            [&](int k) {
+              const float2 w = cs[(e + k) / 2];
+              return k % 2 == 0 ? float2{w.x, -w.y} : w;
+            },
+            scale, sure);
+      };
+      cx = pairs(x.x, x.e, sx);
+      cz = pairs(x.z, x.e + x.gap, sz);
+    } else {
+      cx = plain_codes(x.x, sx);
+      cz = plain_codes(x.z, sz);
+    }
+    const bool done = __builtin_amdgcn_ballot_w64(!sure) == 0;
+    if (done) put(x.t, x.head, x.e, x.gap, cx, cz, sx, sz);
+    return done;
+  };
+  for (int base = blk.first + static_cast<int>(threadIdx.x); base < blk.last; base += kRotThreads * kInFlight) {
+    if (base != blk.first + static_cast<int>(threadIdx.x)) load(base);
+    unsigned doubt = 0;
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      if (it[u].e < 0) continue;
       if (pi == 0) {
-        T out[8];
-        each(
-            x,
-            [&](int k, T v, T o, bool low, int at) {
-              const float2 w = cs32[at];
-              const float fv = static_cast<float>(v), fo = static_cast<float>(o);
-              out[k] = static_cast<T>(turned(fv, w.x, low ? -(fo * w.y) : fo * w.y));
-            },
-            [&](int k) { out[k] = x.x[k]; });
-        T* to = static_cast<T*>(part.y) + x.to + x.e;
-        if constexpr (kWide) {
-          constexpr int kOut = 16 / sizeof(T);
-#pragma unroll
-          for (int k = 0; k < 8; k += kOut) {
-            Vec<T, kOut> v;
-#pragma unroll
-            for (int c = 0; c < kOut; ++c) v.v[c] = out[k + c];
-            *reinterpret_cast<Vec<T, kOut>*>(to + k) = v;
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) to[k] = out[k];
-        }
-      } else {
-        float v[8];
-        each(
-            x,
-            [&](int k, T p, T o, bool low, int at) {
-              const double2 w = cs[at];
-              const double dp = static_cast<double>(static_cast<float>(p));
-              const double dq = static_cast<double>(static_cast<float>(o)) * w.y;
-              v[k] = to_odd(fma(dp, w.x, low ? -dq : dq));
-            },
-            [&](int k) { v[k] = static_cast<float>(x.x[k]); });
-        unsigned scale;
-        const unsigned codes = codes_of(v, scale);
-        // The head's scale bytes, in order, from its groups' lanes.
-        unsigned word = scale << (x.e / 32 * 8);
-        if (D >= 64) word |= static_cast<unsigned>(__shfl_xor(static_cast<int>(word), 4));
-        if (D == 128) word |= static_cast<unsigned>(__shfl_xor(static_cast<int>(word), 8));
-        const int64_t at = at_of[x.t];
-        if (at >= 0) {
-          unsigned char* row = static_cast<unsigned char*>(part.y) + at + x.head * a.page_strides[pi == 2 ? 4 : 1];
-          *reinterpret_cast<unsigned*>(row + x.e / 2) = codes;
-          if (x.e == 0) *reinterpret_cast<unsigned*>(row + D / 2) = word;
-        }
+        put_q(it[u]);
+      } else if (sm.at_of[it[u].t] >= 0) {  // (a token's lanes alike)
+        if (!put_codes(it[u])) doubt |= 1u << u;
       }
     }
+    // What is in doubt (an item of a wave in some hundreds) once more, in 64 bits.
+#pragma clang loop unroll(disable)
+    for (int u = 0; doubt != 0; ++u, doubt >>= 1) {
+      if ((doubt & 1u) == 0) continue;
+      int t, head, e, gap;
+      int64_t to;
+      place(base + u * kRotThreads, t, head, e, gap);
+      const T* row = row_of(t, head, to);
+      unsigned codes[2], scale[2];
+#pragma clang loop unroll(disable)
+      for (int i = 0; i < 2; ++i) {
+        unsigned s;
+        const unsigned c = exact_codes<T, kInterleaved>(a, blk, sm, t, row, e + i * gap, s);
+        (i == 0 ? codes[0] : codes[1]) = c, (i == 0 ? scale[0] : scale[1]) = s;
+      }
+      put(t, head, e, gap, codes[0], codes[1], scale[0], scale[1]);
+    }
+  }
+}
+
+// The same for every other head, rotation and alignment: an item 8 values, moved one by one.
+template <typename T, bool kInterleaved>
+__global__ void __launch_bounds__(kRotThreads)
+append_four_any_kernel(RotaryArgs a) {
+  __shared__ AppendSmem sm;
+  const AppendBlock blk(a);
+  const RotaryPart& part = a.part[blk.pi];
+  const int n = a.pairs, D = a.D, pi = blk.pi;
+  append_tokens(a, blk, sm);
+  const float magnitude = fabsf(static_cast<float>(a.magnitude));
+  for (int item = blk.first + static_cast<int>(threadIdx.x); item < blk.last; item += kRotThreads) {
+    const int t = divide(item, a.by_per[pi]);
+    const int r = item - t * blk.per, head = divide(r, a.by_items[pi]), e = 8 * (r - head * blk.of);
+    if (pi != 0 && sm.at_of[t] < 0) continue;
+    const int tok = static_cast<int>(blk.t0) + t, b = divide(tok, a.by_seq), i = tok - b * a.S;
+    const T* row = static_cast<const T*>(part.x) + b * part.xs[0] + head * part.xs[1] + i * part.xs[2];
+    T x[8], z[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const Pairing<kInterleaved> p(e + k, n, blk.turns);
+      x[k] = row[e + k];
+      z[k] = p.pair < 0 ? static_cast<T>(0.0f) : row[p.other];
+    }
+    auto w = [&](int k) {
+      const Pairing<kInterleaved> p(e + k, n, blk.turns);
+      if (p.pair < 0) return float2{1.0f, 0.0f};
+      const float2 c = sm.cs[t * n + p.pair];
+      return float2{c.x, p.low ? -c.y : c.y};
+    };
+    if (pi == 0) {
+      T* to = static_cast<T*>(part.y) + b * part.ys[0] + head * part.ys[1] + i * part.ys[2] + e;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float2 c = w(k);
+        to[k] = !blk.turns || e + k >= 2 * n
+                    ? x[k]
+                    : static_cast<T>(turned(static_cast<float>(x[k]), c.x, static_cast<float>(z[k]) * c.y));
+      }
+      continue;
+    }
+    unsigned scale, codes;
+    bool sure = true;
+    if (blk.turns) {
+      codes = turned_codes(x, z, fmaxf(magnitude, 1.0f), w, scale, sure);
+      if (__builtin_amdgcn_ballot_w64(!sure) != 0) {
+        codes = exact_codes<T, kInterleaved>(a, blk, sm, t, row, e, scale);
+      }
+    } else {
+      codes = plain_codes(x, scale);
+    }
+    unsigned word = scale << (e / 32 * 8);
+    if (D >= 64) word |= static_cast<unsigned>(__shfl_xor(static_cast<int>(word), 4));
+    if (D == 128) word |= static_cast<unsigned>(__shfl_xor(static_cast<int>(word), 8));
+    unsigned char* to = static_cast<unsigned char*>(part.y) + sm.at_of[t] + head * a.page_strides[pi == 2 ? 4 : 1];
+    *reinterpret_cast<unsigned*>(to + e / 2) = codes;
+    if (e == 0) *reinterpret_cast<unsigned*>(to + D / 2) = word;
   }
 }
 
@@ -510,7 +721,14 @@ __global__ void __launch_bounds__(256) read_kernel(PagedReadArgs a) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) y.v[k] = convert<O, C>(x[u].v[k]);
     }
-    *reinterpret_cast<Out*>(out + static_cast<int64_t>(item) * 8) = y;
+    O* to = out + static_cast<int64_t>(item) * 8;
+    typedef unsigned w4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(O)) / 2; ++i) {
+      w4 v;
+      __builtin_memcpy(&v, reinterpret_cast<const char*>(&y) + 16 * i, 16);
+      __builtin_nontemporal_store(v, reinterpret_cast<w4*>(to) + i);
+    }
   }
 }
 
@@ -526,11 +744,11 @@ const void* read_fn(int dtype, int d) {
 }
 
 template <typename T>
-const void* append_four_fn(bool wide, bool interleaved) {
-  return wide ? (interleaved ? reinterpret_cast<const void*>(append_four_kernel<T, true, true>)
-                             : reinterpret_cast<const void*>(append_four_kernel<T, true, false>))
-              : (interleaved ? reinterpret_cast<const void*>(append_four_kernel<T, false, true>)
-                             : reinterpret_cast<const void*>(append_four_kernel<T, false, false>));
+const void* append_four_fn(bool pairs, bool interleaved) {
+  return pairs ? (interleaved ? reinterpret_cast<const void*>(append_four_kernel<T, true>)
+                              : reinterpret_cast<const void*>(append_four_kernel<T, false>))
+               : (interleaved ? reinterpret_cast<const void*>(append_four_any_kernel<T, true>)
+                              : reinterpret_cast<const void*>(append_four_any_kernel<T, false>));
 }
 
 template <typename T, typename C, bool kPaged>
@@ -556,11 +774,10 @@ int launch_rotary(RotaryArgs a, int dtype, int cache_dtype, int vec, void* strea
   const void* fn = nullptr;
   const bool il = a.interleaved != 0;
   if (to_four) {
-    const bool wide = vec == 8;
-    fn = dtype == kF32   ? append_four_fn<float>(wide, il)
-         : dtype == kF16 ? append_four_fn<_Float16>(wide, il)
-                         : append_four_fn<__bf16>(wide, il);
-    vec = 8;
+    const bool pairs = vec == 16;
+    fn = dtype == kF32   ? append_four_fn<float>(pairs, il)
+         : dtype == kF16 ? append_four_fn<_Float16>(pairs, il)
+                         : append_four_fn<__bf16>(pairs, il);
   } else if (!paged) {
     fn = dtype == kF32   ? rotary_fn<float, float, false>(vec, il)
          : dtype == kF16 ? rotary_fn<_Float16, _Float16, false>(vec, il)
@@ -585,7 +802,7 @@ int launch_rotary(RotaryArgs a, int dtype, int cache_dtype, int vec, void* strea
   }
   const int64_t fill = (kRotThreads + most - 1) / most;
   int64_t tokens = std::min(std::max(fill, all / 1024), std::max(fill, 2 * kUnroll * kRotThreads / most));
-  if (a.pairs > 0) tokens = std::min<int64_t>(tokens, (to_four ? kMaxAngles64 : kMaxAngles) / a.pairs);
+  if (a.pairs > 0) tokens = std::min<int64_t>(tokens, kMaxAngles / a.pairs);
   tokens = std::min<int64_t>(tokens, kMaxTokens);
   a.tokens = static_cast<int>(tokens);
   const int64_t blocks = (all + tokens - 1) / tokens;

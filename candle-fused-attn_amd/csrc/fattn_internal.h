@@ -270,7 +270,8 @@ struct SplitPlan {
   int row_blocks, part_rows, wgs, min_run, begin;
   size_t before, bytes;  // where `before` lies in the workspace, its size
 };
-SplitPlan split_plan(int64_t b, int64_t hk, int64_t rows, int64_t d, int64_t capacity);
+SplitPlan split_plan(int64_t b, int64_t hk, int64_t rows, int64_t d, int64_t capacity,
+                     bool four_bits = false);  // (needs no more workspace with them than without)
 int launch_split(const SplitArgs& a, int dtype, int cache_dtype, int d, void* stream);
 
 // Cross attention by blocks of 128 queries and 128 keys (fattn_cross.hip). dq [b, sq, h, d], dkv

@@ -165,7 +165,7 @@ int check_workspace(const char* who, const void* workspace, size_t bytes, size_t
 int run_split(const char* who, fattn::SplitArgs& a, int dtype, int cache_dtype, int64_t d,
               int64_t capacity, void* workspace, size_t workspace_bytes, void* stream) {
   const int64_t rows = static_cast<int64_t>(a.G) * a.SQ;
-  const fattn::SplitPlan plan = fattn::split_plan(a.B, a.HK, rows, d, capacity);
+  const fattn::SplitPlan plan = fattn::split_plan(a.B, a.HK, rows, d, capacity, cache_dtype == fattn::kFP4);
   if (static_cast<int64_t>(a.B) * a.HK * plan.row_blocks > kMaxGrid ||
       static_cast<int64_t>(a.B) * a.H * a.SQ > kMaxGrid) {
     return set_error(FATTN_ERANGE, "%s: the grid exceeds the launch limit", who);

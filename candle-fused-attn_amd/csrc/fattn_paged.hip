@@ -845,7 +845,8 @@ int by_type(const SplitArgs& a, int dtype, int cache_dtype, int d, hipStream_t s
 
 }  // namespace
 
-SplitPlan split_plan(int64_t b, int64_t hk, int64_t rows, int64_t d, int64_t capacity) {
+SplitPlan split_plan(int64_t b, int64_t hk, int64_t rows, int64_t d, int64_t capacity,
+                     bool four_bits) {
   SplitPlan p{};
   p.row_blocks = static_cast<int>((rows + kRowsMax - 1) / kRowsMax);
   p.part_rows = static_cast<int>(rows < kRowsMax ? rows : kRowsMax);
@@ -858,7 +859,14 @@ SplitPlan split_plan(int64_t b, int64_t hk, int64_t rows, int64_t d, int64_t cap
   // 384 heads of 1024 tokens 45.9 / 52.6, of 1 to 700 25.6 / 29.9; bf16 d 128, 256 of 1000 28.8 / 35.5,
   // 192 26.0 / 29.7; past it 384 of 1 to 2048 64.9 / 54.7, 48 of 1000 28.2 / 20.8, of 1500 37.8 / 23.0. (A
   // wave alone takes 2 us a tile, the memory's latency twice; eight waves a workgroup change little.)
-  const int64_t direct = b * hk * p.row_blocks >= 192 ? 8 * kSplitWaves : 4 * kSplitWaves;
+  // A 4-bit tile is a quarter of the bytes, and beginning a run and joining it weigh more: twelve tiles a wave
+  // then, sixteen with two workgroups a CU. d 128, lengths up to the capacity: 192 heads, capacity 1100
+  // 13.5 / 16.0, 1536 18.9 / 17.6 (all full 20.1 / 20.0), 2048 24.0 / 18.6; 256 of 1536 19.1 / 19.3 (20.4 /
+  // 23.9), of 2048 24.4 / 21.9; 512 of 2048 30.4 / 32.9 (32.9 / 40.1), of 3000 42.2 / 38.1; d 64, 384 of 1536
+  // 19.5 / 19.3 (21.1 / 23.8), 768 of 2048 29.4 / 31.4 (32.3 / 40.6).
+  const int64_t blocks = b * hk * p.row_blocks;
+  const int64_t most = !four_bits ? 8 : blocks >= 512 ? 16 : 12;
+  const int64_t direct = (blocks >= 192 ? most : 4) * kSplitWaves;
   p.wgs = tiles <= direct ? 0 : kMostRuns;
   p.before = static_cast<size_t>(p.wgs) * 2 * p.part_rows * static_cast<size_t>(d + 4) * sizeof(float);
   p.bytes = p.wgs == 0 ? 0 : p.before + static_cast<size_t>(b + 1) * sizeof(int64_t);

@@ -293,6 +293,18 @@ def test_attention_grouped_heads(cuda, h, hk):
     assert rel(out, ref) <= bar(torch.bfloat16, top)
 
 
+@pytest.mark.parametrize("b,hk,most", [(32, 6, 1536), (32, 6, 1568), (64, 8, 2048), (64, 8, 2080)])
+def test_attention_batches(cuda, b, hk, most):
+    """Batches that a workgroup per key head takes, and the next capacity, that it does not."""
+    gen = torch.Generator().manual_seed(most)
+    lengths = [most, 0, 1, most - 1] + torch.randint(1, most, (b - 4,), generator=gen).tolist()
+    c = Four(cuda, hk, 32, 32, lengths, seed=10)
+    q = q_of(cuda, torch.float32, b, hk, 32)
+    out = cfa.paged_attention(q, c.k, c.v, c.table, c.lengths, 0.2)
+    ref, top = attended(q, c, lengths, 0.2)
+    assert rel(out, ref) <= bar(torch.float32, max(top, 10.0))
+
+
 def test_attention_bad_sequences_and_groups(cuda):
     """A length or a page that the cache does not have: NaN there, the neighbours as they are. A group of
     NaN: seen as a value in its own 32 head_dims, as a key everywhere; behind the last token not at all."""

@@ -58,8 +58,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ([h] f32, one per query head) it is lowered by the slope times the distance lengths[b] - 1 - j to
     token j: what fused_scored_attention does of a sequence's last token.
 
-    q: [b, h, 1, d], of the cache's type or f32 (any over a 4-bit cache), h a multiple of the cache's key heads (query head i
-    reads key head i // (h // kv_heads)). Returns [b, h, 1, d] of q's type. A sequence of length 0
+    q: [b, h, 1, d], of the cache's type or f32 (any over a 4-bit cache), h a multiple of the cache's key
+    heads (query head i reads key head i // (h // kv_heads)). Returns [b, h, 1, d] of q's type. A sequence of length 0
     gives 0; one whose length the table cannot hold, or that names a page outside the cache, NaN.
     Infinities and NaN that a token sees give what the formula gives of them. Not differentiable.
     """
@@ -79,5 +79,5 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
     """
     if dtype is not None and dtype not in DTYPES:
         raise FusedAttentionError(f"paged_read: dtype must be float32, float16 or bfloat16, got {dtype}")
-    return operators().paged_read(k_pages, v_pages, page_table, lengths, int(s), starts,
+    return operators().paged_read(k_pages, v_pages, page_table, lengths, s, starts,
                                   -1 if dtype is None else DTYPES[dtype])

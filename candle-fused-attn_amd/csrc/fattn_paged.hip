@@ -852,20 +852,22 @@ SplitPlan split_plan(int64_t b, int64_t hk, int64_t rows, int64_t d, int64_t cap
   p.part_rows = static_cast<int>(rows < kRowsMax ? rows : kRowsMax);
   const int64_t tiles = (capacity + kTile - 1) / kTile;
   p.min_run = kSplitWaves;
-  p.begin = kSplitWaves;
+  // (What beginning a head costs, in tiles. 4-bit ones are the shorter: 64 x 6 heads of 1 to 2048, fp32 d 64,
+  // 26.2 us at 4 of them, 22.7 at 8, 22.7 at 12; 256 d 128 heads of 1 to 3000 25.6, 23.5, 24.0.)
+  p.begin = four_bits ? 2 * kSplitWaves : kSplitWaves;
   // One workgroup per key head, and no join, where no sequence can have more than four tiles a wave, or
   // eight with a workgroup for most CUs: by what the tables have room for, since the lengths are on the
   // device. Direct / in runs, us (with 6 us of a graph's launch): fp32 d 64,
   // 384 heads of 1024 tokens 45.9 / 52.6, of 1 to 700 25.6 / 29.9; bf16 d 128, 256 of 1000 28.8 / 35.5,
   // 192 26.0 / 29.7; past it 384 of 1 to 2048 64.9 / 54.7, 48 of 1000 28.2 / 20.8, of 1500 37.8 / 23.0. (A
   // wave alone takes 2 us a tile, the memory's latency twice; eight waves a workgroup change little.)
-  // A 4-bit tile is a quarter of the bytes, and beginning a run and joining it weigh more: twelve tiles a wave
-  // then, sixteen with two workgroups a CU. d 128, lengths up to the capacity: 192 heads, capacity 1100
-  // 13.5 / 16.0, 1536 18.9 / 17.6 (all full 20.1 / 20.0), 2048 24.0 / 18.6; 256 of 1536 19.1 / 19.3 (20.4 /
-  // 23.9), of 2048 24.4 / 21.9; 512 of 2048 30.4 / 32.9 (32.9 / 40.1), of 3000 42.2 / 38.1; d 64, 384 of 1536
-  // 19.5 / 19.3 (21.1 / 23.8), 768 of 2048 29.4 / 31.4 (32.3 / 40.6).
+  // Beginning a run and joining it weigh more against 4-bit tiles: ten a wave then, sixteen with two
+  // workgroups a CU. Lengths up to the capacity (all of it in brackets): d 128, 192 heads of 1100 13.5 / 15.0
+  // (15.7 / 17.9), of 1536 17.0 / 15.4 (20.0 / 19.7); 256 of 1100 14.6 / 17.3, of 1536 18.8 / 17.5 (20.3 /
+  // 22.9); 512 of 2048 31.8 / 29.4 (32.7 / 38.4), of 3000 39.8 / 35.5 (45.8 / 50.2); d 64, 384 of 1100 15.1 /
+  // 17.1, 768 of 2048 29.7 / 29.1 (32.2 / 40.1).
   const int64_t blocks = b * hk * p.row_blocks;
-  const int64_t most = !four_bits ? 8 : blocks >= 512 ? 16 : 12;
+  const int64_t most = !four_bits ? 8 : blocks >= 512 ? 16 : 10;
   const int64_t direct = (blocks >= 192 ? most : 4) * kSplitWaves;
   p.wgs = tiles <= direct ? 0 : kMostRuns;
   p.before = static_cast<size_t>(p.wgs) * 2 * p.part_rows * static_cast<size_t>(d + 4) * sizeof(float);

@@ -383,9 +383,13 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int BH = a.B * a.H, off = a.SK - a.SQ;
-  // (Causal: the blocks that see most first.)
-  const int id = static_cast<int>(blockIdx.x), per = a.nqb * a.nc;
-  const int item = a.causal ? id % BH * per + per - 1 - id / BH : xcd_remap(id, per * BH);
+  // (Causal: the blocks that see most first, and the heads of a group, which read the same keys, in one XCD's L2
+  // where the key heads are a multiple of the XCDs. 2 x 32 heads in 8 groups 512 x 4097 d 128 so 97 MB from
+  // memory and 286 us, group heads side by side 780 and 289; the backward's query blocks, 4 x 16 heads in 4
+  // groups of 777, take 2 % longer so.)
+  const int id = static_cast<int>(blockIdx.x), per = a.nqb * a.nc, pairs = a.B * (a.H / a.G), in_pair = id / pairs;
+  const int item = a.causal ? (id % pairs * a.G + in_pair % a.G) * per + per - 1 - in_pair / a.G
+                            : xcd_remap(id, per * BH);
   const int bh = item / per, in = item - bh * per, qb = in / a.nc, chunk = in - qb * a.nc;
   const int b = bh / a.H, h = bh % a.H, hk = h / a.G;
   const int qw0 = qb * kBlock + w * kRows, qi = qw0 + j, pos = min(qi, a.SQ - 1) + off;
@@ -621,31 +625,49 @@ fwd_scored_kernel(ScoredArgs a) {
 // row.
 template <int D>
 __global__ void __launch_bounds__(256) join_scored_kernel(ScoredArgs a) {
-  constexpr int kLanes = D / 4;
-  const int64_t rows = static_cast<int64_t>(a.B) * a.SQ * a.H;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+  constexpr int kLanes = D / 4, kAtOnce = 4;  // (chunks in flight)
+  const int rows = a.B * a.SQ * a.H, row = static_cast<int>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
   if (row >= rows) return;
   const int d = threadIdx.x % kLanes * 4;
-  const int h = static_cast<int>(row % a.H), b = static_cast<int>(row / a.H / a.SQ);
-  const int64_t at = (static_cast<int64_t>(b) * a.H + h) * a.SQ + row / a.H % a.SQ;
+  const int r = row / a.H, h = row - r * a.H, b = r / a.SQ, i = r - b * a.SQ;
+  const int64_t at = (static_cast<int64_t>(b) * a.H + h) * a.SQ + i;
+  f4 o[kAtOnce];
+  auto load = [&](int c0) {
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      o[u] = ld4(a.o_part + (static_cast<int64_t>(min(c0 + u, a.nc - 1)) * rows + row) * D + d);
+    }
+  };
+  auto l_of = [&](int c) { return a.l_part[static_cast<int64_t>(min(c, a.nc - 1)) * rows + at]; };
+  load(0);
   double top = kUnseen;
-  for (int c = 0; c < a.nc; ++c) {
-    const double L = a.l_part[c * rows + at];
-    top = L > top || L != L ? L : top;
+  for (int c0 = 0; c0 < a.nc; c0 += 2 * kAtOnce) {
+    double L[2 * kAtOnce];
+#pragma unroll
+    for (int u = 0; u < 2 * kAtOnce; ++u) L[u] = l_of(c0 + u);
+#pragma unroll
+    for (int u = 0; u < 2 * kAtOnce; ++u) top = L[u] > top || L[u] != L[u] ? L[u] : top;
   }
   float sum = 0.0f;
   f4 x{};
-  for (int c = 0; c < a.nc; ++c) {
-    const double L = a.l_part[c * rows + at];
-    if (L == kUnseen) continue;
-    const float w = expf(static_cast<float>(L - top));
-    sum += w;
-    x += ld4(a.o_part + (c * rows + row) * D + d) * w;
+  for (int c0 = 0; c0 < a.nc; c0 += kAtOnce) {
+    if (c0 > 0) load(c0);
+    double L[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) L[u] = l_of(c0 + u);
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      // (What lies in the O of a chunk that saw nothing is not looked at.)
+      if (c0 + u >= a.nc || L[u] == kUnseen) continue;
+      const float w = expf(static_cast<float>(L[u] - top));
+      sum += w;
+      x += o[u] * w;
+    }
   }
   // (No chunk saw anything: a row without a document, or, NaN, scores that are all minus infinity.)
   const int32_t* ids = ids_of(a, b);
-  const bool none = top == kUnseen && ids != nullptr && ids[row / a.H % a.SQ + a.SK - a.SQ] < 0;
-  st4(a.out + row * D + d, none ? f4{} : x * (1.0f / sum));
+  const bool none = top == kUnseen && ids != nullptr && ids[i + a.SK - a.SQ] < 0;
+  st4(a.out + static_cast<int64_t>(row) * D + d, none ? f4{} : x * (1.0f / sum));
   if (d == 0) a.lse[at] = top == kUnseen ? kNegInf : static_cast<float>(top + logf(sum));
 }
 
@@ -1121,7 +1143,7 @@ template <int D, int MODS, int WAVES>
 __global__ void __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES)))
 bwd_scored_kernel(ScoredArgs a) {
   __shared__ __attribute__((aligned(16))) ScoredSmem<D> sm;
-  const int id = static_cast<int>(blockIdx.x), pairs = a.B * (a.H / a.G), BH = a.B * a.H;
+  const int id = static_cast<int>(blockIdx.x), pairs = a.B * (a.H / a.G);
   const int per_k = a.nkb * a.nck, per_q = a.nqb * a.ncq, keys = per_k * pairs;
   if (id < keys) {
     // Causal: the low blocks (they are seen by every later query) first.
@@ -1129,7 +1151,8 @@ bwd_scored_kernel(ScoredArgs a) {
     const int pair = item / per_k, in = item - pair * per_k, kb = in / a.nck;
     scored_keys<D, MODS>(a, sm, pair * a.nkb + kb, in - kb * a.nck);
   } else {
-    const int i = id - keys, item = a.causal ? i % BH * per_q + per_q - 1 - i / BH : xcd_remap(i, per_q * BH);
+    const int BH = a.B * a.H, i = id - keys;
+    const int item = a.causal ? i % BH * per_q + per_q - 1 - i / BH : xcd_remap(i, per_q * BH);
     const int bh = item / per_q, in = item - bh * per_q, qb = in / a.ncq;
     scored_queries<D, MODS>(a, sm, bh * a.nqb + qb, in - qb * a.ncq);
   }
@@ -1181,11 +1204,21 @@ static double seen_part(int64_t sq, int64_t sk, int causal) {
 ScoredPlan scored_plan(int64_t b, int64_t h, int64_t sq, int64_t sk, int64_t d) {
   ScoredPlan p{};
   p.nc = 1;
-  if (sq == 0 || sk == 0) return p;
+  if (b == 0 || sq == 0 || sk == 0) return p;
   const int64_t steps = (sk + kRows - 1) / kRows, blocks = scored_blocks(b, h, sq);
   const int64_t slots = 256 * (d == 32 ? 4 : d == 64 ? 3 : 2);
-  // Chunks of the keys where the blocks do not fill the chip, of 3 tiles or more.
-  if (4 * blocks <= 3 * slots) cut(steps, std::max<int64_t>(3, blocks * steps / slots), 1.5, &p.nc, &p.chunk);
+  // Chunks of the keys, as many as run at once (one more is a second round: 2 x 32 heads 512 x 4097 d 128 two
+  // chunks 297 us, three 320; 1 x 32 heads four 158, five 193; 5 x 12 heads of 1000 d 64 whole 79, two 92), of 2
+  // tiles or more, where that saves the 3 tiles that a join takes as long as (6 heads 240 x 240 d 64: whole 17.4,
+  // in four 12.5). The join reads them four at a time: more than sqrt(8 steps) take longer there than they save (a tile is some
+  // eight chunks of a join: one query to 131072 keys, 683 chunks 230 us, 179 96).
+  const int64_t most = std::max<int64_t>(1, static_cast<int64_t>(sqrt(8.0 * static_cast<double>(steps))));
+  const int64_t fit = std::min(most, blocks <= slots ? slots / blocks : 1);
+  const int64_t longest = std::max<int64_t>(2, (steps + fit - 1) / fit);
+  if (fit > 1 && steps - longest >= 3) {
+    p.chunk = static_cast<int>(longest);
+    p.nc = static_cast<int>((steps + longest - 1) / longest);
+  }
   if (p.nc > 1) {
     const size_t parts = static_cast<size_t>(p.nc) * b * h * sq;
     p.l_part = parts * d * sizeof(float);

@@ -152,6 +152,8 @@ def test_scored_workspace_and_gradient_refusals():
         assert size_of(64, 8, 8, 4096, 4096, 64, *more) == 0
         assert size_of(2, 4, 3, 1, 4096, 64, *more) == 0
         assert size_of(2, 4, 4, 5000, 4096, 64, *more) == 0
+        assert size_of(0, 4, 4, 1, 4096, 64, *more) == 0 and size_of(0, 4, 4, 0, 0, 64, *more) == 0
+        assert size_of(2, 4, 4, 0, 0, 64, *more) == 0
     refused(backward(g=None), _lib.FATTN_EINVAL, "null operand")
     refused(backward(dq=None), _lib.FATTN_EINVAL, "null operand")
     refused(backward(dkv=None), _lib.FATTN_EINVAL, "null operand")

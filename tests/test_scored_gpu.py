@@ -354,6 +354,18 @@ def test_captured(cuda, sq):
         assert all(torch.equal(a, e) for a, e in zip(out, want)), i
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_many_chunks(cuda, d):
+    """Few rows over many keys: walks in a hundred chunks, many of which a row does not see at all."""
+    sk = 40000 if d == 64 else 20000
+    q, k, v, g = operands(1, 2, 1, 5, sk, d, seed=21)
+    ids = ids_of([[sk // 7] * 6 + [sk - 6 * (sk // 7) - 2]], sk)
+    for how in ({}, {"documents": ids}, {"documents": ids, "prefix": torch.tensor([sk - 9], dtype=torch.int32)}):
+        got = run(cuda, q, k, v, g, d ** -0.5, True, cap=9.0, **how)
+        ref, top = formula(q, k, v, g, d ** -0.5, True, cap=9.0, **how)
+        check(got, ref, top)
+
+
 def test_side_streams(cuda):
     """Two calls in flight, each with its own workspace (chunks of a long walk)."""
     cases = [[t.to(cuda) for t in operands(1, 2, 2, 5, 4000, 64, seed=15 + i)] for i in range(2)]

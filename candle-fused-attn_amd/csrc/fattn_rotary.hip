@@ -209,8 +209,13 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotaryArgs a) {
 // terms of pi / 2), brought to 32 bits by rounding to odd, so that no second rounding moves a value across
 // the border between two codes, and a token has the same codes on whatever path it came.
 //
-// Bound: memory, and for few tokens the launch. A thread has 8 values, so that four neighbours share a scale
-// and a head's scales are one word; the values that a rotation pairs with them are read by the neighbours too.
+// 32 bits decide nearly every code: with the bound on what they are off by, both ends of a value's interval have
+// the same one. Only where that leaves a doubt (an item of a wave in some hundreds) is it formed in 64.
+//
+// Bound: memory, and for few tokens the launch. A thread has 16 values, in two halves that turn together, so that
+// four neighbours share a scale, a head's scales are one word and each value is read once. 16 x 2048 tokens, 32
+// + 8 heads d 128 bf16, into pages: 145 us (4.7 TB/s; all codes in 64 bits 8 values at a time 200; four items in
+// flight for two 179; queries in a launch of their own 198); 64 single tokens of 6 + 6 heads fp32 d 64 5.6 us.
 
 // cos and sin of the angle p f (rounded once), times the magnitude, in 64 bits: less q quarter turns, |y| <=
 // pi / 4, where the Taylor series to y^17 and y^16 are exact to 1e-17.
@@ -650,7 +655,9 @@ append_four_any_kernel(RotaryArgs a) {
 // --- Tokens back out of a paged cache ------------------------------------------------------------------
 // Bound: memory, each row read and each result written once. A thread has 8 values of a token's head; the
 // results of one (sample, head) are contiguous, and those of neighbouring tokens lie in one page, so a wave
-// reads and writes whole rows one after the other.
+// reads and writes whole rows one after the other. Results are stored past the caches, which they would sweep. 4
+// x 8 heads 20000 to 32767 tokens of 4 bits to bf16, d 128: 157 us a call, 4.2 TB/s (the kernel itself 88: what
+// it wrote drains behind it); 5 x 12 heads 333 tokens f16 d 32 4.4 us.
 template <typename C, typename O, int D>
 __global__ void __launch_bounds__(256) read_kernel(PagedReadArgs a) {
   constexpr int kOf = D / 8, kInFlight = 4;

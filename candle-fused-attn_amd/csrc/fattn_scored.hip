@@ -12,6 +12,17 @@
 // documents have them, leave only their own tiles; other orders are walked over and masked). A tile's ids
 // are staged beside it: a wave passes over a tile in which it sees nothing, and takes one in which it sees
 // everything without a mask.
+//
+// Bound: the vector units. A step of 32 x 32 pairs has 24 (forward), 36 and 48 (backward) matrix instructions at
+// d 64, 32 cycles each, and 300 to 600 others of 4 and more: the staged tiles' split into f16, the scores'
+// tanh and exponent, the weights' split; at d 64 two waves of the backward share a SIMD, at d 128 one has it alone
+// and waits for its LDS reads besides. One body per walk, whose masked scores are minus infinity, and a kernel
+// per kind of score (slopes, cap): bodies with and without a mask side by side took registers for both.
+// Measured: 8 x 12 heads of 2048, d 64, causal: one document, plain scores, forward 217 us, backward 643 (79 and
+// 67 TFLOP/s of 4 d and 10 d operations a pair, 237 and 200 of f16 products; fused_attention 230 and 717), capped
+// 220 and 702; packed documents with a mean of 600, capped, 143 and 407; 4 x 16 heads in 4 groups of 777, d 128,
+// slopes and prefixes, 88 and 264 + 10 (the sum of the chunks); 2 x 32 heads in 8 groups 512 x 4097, d 128,
+// slopes, forward 286 with its join (225 TFLOP/s, 675 of f16 products).
 #include <hip/hip_runtime.h>
 #include <limits.h>
 #include <math.h>
@@ -1210,8 +1221,8 @@ ScoredPlan scored_plan(int64_t b, int64_t h, int64_t sq, int64_t sk, int64_t d) 
   // Chunks of the keys, as many as run at once (one more is a second round: 2 x 32 heads 512 x 4097 d 128 two
   // chunks 297 us, three 320; 1 x 32 heads four 158, five 193; 5 x 12 heads of 1000 d 64 whole 79, two 92), of 2
   // tiles or more, where that saves the 3 tiles that a join takes as long as (6 heads 240 x 240 d 64: whole 17.4,
-  // in four 12.5). The join reads them four at a time: more than sqrt(8 steps) take longer there than they save (a tile is some
-  // eight chunks of a join: one query to 131072 keys, 683 chunks 230 us, 179 96).
+  // in four 12.5). The join reads them four at a time: more than sqrt(8 steps) take longer there than they save (a
+  // tile is some eight chunks of a join: one query to 131072 keys, 683 chunks 230 us, 179 96).
   const int64_t most = std::max<int64_t>(1, static_cast<int64_t>(sqrt(8.0 * static_cast<double>(steps))));
   const int64_t fit = std::min(most, blocks <= slots ? slots / blocks : 1);
   const int64_t longest = std::max<int64_t>(2, (steps + fit - 1) / fit);

@@ -245,7 +245,7 @@ int fattn_rotary(int dtype, int64_t b, int64_t s, int64_t d, const int64_t heads
  * is token lengths[b] + i of sequence b, and goes to slot t % page_size of page
  * table[b][t / page_size] of k_pages and v_pages ([pages, kv_heads, page_size, d], page_strides
  * {page, head, slot}), rounded to cache_dtype (the activations' type or FATTN_FP4, or any for fp32
- * ones; with FATTN_FP4 q_out is not q, and the codes are those of the keys turned in 64 bits). Keys are
+ * ones; with FATTN_FP4 q_out does not overlap q, and the codes are those of the keys turned in 64 bits). Keys are
  * turned as by fattn_rotary at position t (frequencies NULL: not), and so is q ([b, heads, s, d],
  * heads 0: absent) into q_out, in all s rows. A token whose page the table ([b, table_width], row
  * stride table_stride) or the cache does not have is not written; nor is anything else. page_size is

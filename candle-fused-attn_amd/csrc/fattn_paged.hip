@@ -33,17 +33,18 @@
 // workgroups, whatever the lengths; a workgroup's run crosses heads and sequences. Where a run ends
 // inside a head the workgroup leaves its unnormalised sums in the workspace (at most two: its first
 // and its last head), and a second kernel joins them in order. Reruns are bit-identical. A head counts
-// kSplitWaves tiles more than it has (over 4 bits twice as many), which is what beginning one costs: without, the workgroup that the
-// shortest sequences fall to ends last (64 sequences of 1 to 2048, 6 heads, fp32 d 64: 79 us, 46 so).
+// kSplitWaves tiles more than it has (over 4 bits twice as many), which is what beginning one costs: without,
+// the workgroup that the shortest sequences fall to ends last (64 sequences of 1 to 2048, 6 heads, fp32 d 64: 79
+// us, 46 so).
 //
 // Measured (kernel and join): 4 contexts of 60000 to 131071, 32 heads in 8 groups, d 128 bf16, 263 to 273 + 5
 // us (5.7 to 5.9 TB/s, by card); that ragged batch 45 + 5 us (4.5 TB/s); 8 x 6 heads 1 x 1536 fp32 12.4 + 3.9
 // us (3.0 TB/s); the ragged batch in bf16 27 us in all, 29 with a cap and slopes (3.4 TB/s). Over 4 bits those
 // contexts 102 + 5 us (4.1 TB/s: 331 vector instructions a tile of 32 keys, which take 70 % of that time), the
-// ragged batch with fp32 queries 19 + 4 (1.4 TB/s: what each head and run begins and ends with; two tiles in hand,
-// for fewer workgroups a CU: 106 us -> 118 and no gain). One sequence of 240, 6 heads, 7.8 us, the latency of one workgroup, where the table has room
-// for little more (split_plan); under one for 4096 or 131072 tokens the same sequence takes runs and a join,
-// 10.5 us for 7.3 from a graph, 64 such sequences 20.1 for 12.6.
+// ragged batch with fp32 queries 23 in all (1.2 TB/s: what each head and run begins and ends with). (Two tiles in
+// hand, for fewer workgroups a CU: 106 us -> 118, and no gain.) One sequence of 240, 6 heads, 7.8 us, the latency
+// of one workgroup, where the table has room for little more (split_plan); under one for 4096 or 131072 tokens the
+// same sequence takes runs and a join, 10.5 us for 7.3 from a graph, 64 such sequences 20.1 for 12.6.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -490,7 +491,8 @@ struct Wave {
 // Waves per SIMD (so workgroups per CU) that the registers allow.
 template <typename Q, typename C, int D>
 constexpr int kOccupancy = D == 32    ? 4
-                           : std::is_same<C, four>::value ? (std::is_same<Q, __bf16>::value ? 4 : 3) - (D == 128 ? 1 : 0)
+                           : std::is_same<C, four>::value
+                               ? (std::is_same<Q, __bf16>::value ? 4 : 3) - (D == 128 ? 1 : 0)
                            : D == 128 ? 2
                            : std::is_same<C, _Float16>::value || (std::is_same<C, __bf16>::value &&
                                                                   std::is_same<Q, C>::value)

@@ -171,7 +171,10 @@ __device__ __forceinline__ void capped(f16v& x, F fn) {
 }
 // The slope's part. Register r is 8 (r / 4) + r % 4 places from the lane's base; where no seen pair of the
 // tile has its key after its query, the distance is a sum of both, and slope x place (one value for the wave)
-// is added to the score while the lane's part goes with what the exponent adds: no instruction of its own.
+// is added to the score while the lane's part goes with what the exponent adds: no instruction of its own. Both
+// parts are of the tile's places, up to 32 slopes, and their roundings stay where they cancel; so a steep slope
+// (past 1 in the exponent: 2^-19 then) takes the distance itself, whose rounding is one of the score.
+constexpr float kSteep = 1.0f;
 __device__ __forceinline__ int place_of(int r) { return 8 * (r >> 2) + (r & 3); }
 // Minus infinity to the registers of places outside [least, most]; to those of other ids than the lane's.
 __device__ __forceinline__ void hide(f16v& s, int least, int most) {
@@ -510,7 +513,7 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
         return ld4(&sm.uk[cur][8 * i + 4 * g]) * cq;
       };
       const float base = fpos - static_cast<float>(kt0);
-      if (ordered || kt0 + kRows - 1 <= lo_pos) {
+      if (fabsf(slope2) <= kSteep && (ordered || kt0 + kRows - 1 <= lo_pos)) {
         shift = slope2 * base;
         scale_add(s, f, [&](int r) { return places.by[r]; });
       } else {
@@ -696,7 +699,7 @@ template <int D>
 struct ScoredSmem {
   ScoredTiles<D> u;
   float ua[2][kRows], ub[2][kRows], l[2][kRows], d[2][kRows];
-  float ls[2][kRows];  // (key blocks) l less the slope times the row's place after the block's first key
+  float ls[2][kRows];  // (key blocks) l less the slope times the row's place in the tile
   IdSmem ids;
 };
 
@@ -744,7 +747,7 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
   Stage<D, kW> st;
   RowDots<D, kW> ro;
   float lreg, slope_next = 0.0f;
-  int id_next = 0, row_next = 0;
+  int id_next = 0;
   // Step u's head in the group (past the last step: the last) and its tile's first row.
   auto place = [&](int u, int& hh) {
     hh = min((u + u0) / n, a.G - 1);
@@ -763,7 +766,7 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
     ro.load(op + hh * D, static_cast<unsigned>(a.H) * D, r0, SQ - 1, w, lane);
     lreg = lp[hh * static_cast<int64_t>(SQ) + min(r0 + j, SQ - 1)];
     if constexpr ((MODS & 1) != 0) {
-      if (w == 0) slope_next = slope_of(a, h0 + hh), row_next = r0 + j + off - k0;
+      if (w == 0) slope_next = slope_of(a, h0 + hh);
     }
   };
   auto store = [&](int u) {
@@ -774,7 +777,7 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
       // (A row that sees nothing has an L of minus infinity, and scores of it too.)
       const float l = id_next < 0 ? 0.0f : shifted_l(lreg, kp);
       sm.l[put][j] = l;
-      if constexpr ((MODS & 1) != 0) sm.ls[put][j] = fmaf(-slope_next, static_cast<float>(row_next), l);
+      if constexpr ((MODS & 1) != 0) sm.ls[put][j] = fmaf(-slope_next, static_cast<float>(j), l);
       if (all_ids != nullptr) sm.ids.tile[put][j] = id_next;
     }
   };
@@ -855,8 +858,8 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
         if constexpr ((MODS & 2) != 0) return f4{f2, f2, f2, f2};
         return ld4(&sm.ua[cur][8 * i + 4 * g]) * cs;
       };
-      if (ordered || kw0 + kRows - 1 <= q0 + off) {
-        const float shift = slope2 * static_cast<float>(key - k0);
+      if (fabsf(slope2) <= kSteep && (ordered || kw0 + kRows - 1 <= q0 + off)) {
+        const float shift = slope2 * static_cast<float>(key - q0 - off);
         scale_add(s, f, [&](int r) { return sm.ls[cur][place_of(r) + 4 * g] + shift; });
       } else {
         const float base = static_cast<float>(q0 + 4 * g + off - key);
@@ -1086,7 +1089,7 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
         return ld4(&sm.ua[cur][8 * i + 4 * g]) * cs;
       };
       const float base = fpos - static_cast<float>(kt0);
-      if (ordered || kt0 + kRows - 1 <= lo_pos) {
+      if (fabsf(slope2) <= kSteep && (ordered || kt0 + kRows - 1 <= lo_pos)) {
         l = fmaf(-slope2, base, L);
         scale_add(s, f, [&](int r) { return places.by[r]; });
       } else {

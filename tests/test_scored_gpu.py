@@ -184,6 +184,29 @@ def test_caps(cuda, cap, spread):
     check(got, ref, top, 2 * 2.0 ** -23 * spread / cap)
 
 
+@pytest.mark.parametrize("causal,prefix", [(True, None), (True, [90, 400]), (False, None)], ids=["causal", "prefix", "all"])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_steep_slopes(cuda, d, causal, prefix):
+    """Slopes under which only a key's next neighbours weigh: as exact as gentle ones, whose distances are sums."""
+    slopes = torch.tensor([0.6, 0.8, 3.0, 17.0, 300.0, -0.9, 1e6, 0.7])
+    q, k, v, g = operands(2, 8, 4, 400, 400, d, seed=22)
+    how = dict(slopes=slopes, prefix=None if prefix is None else torch.tensor(prefix, dtype=torch.int32))
+    got = run(cuda, q, k, v, g, d ** -0.5, causal, **how)
+    ref, _ = formula(q, k, v, g, d ** -0.5, causal, **how)
+    # O and dV, head by head: |y| of a key that weighs 1e-3 is that of the scores and 7 more, but for the head of
+    # slope -0.9, where it is 0.9 x 400 (the third of the four key heads has it too).
+    for i, keep in ((0, [0, 1, 2, 3, 4, 6, 7]), (3, [0, 1, 3])):
+        check([got[i][:, keep].contiguous()], [ref[i][:, keep]], 12.0)
+    check([got[0]], [ref[0]], 0.9 * 400)
+    check([got[3]], [ref[3]], 0.9 * 400)
+    # dQ and dK beside the largest head's: where one key has all the weight, dS = P (dP - D) is the difference of
+    # two sums that are as large as where it has not, and carries their errors, 2e-6 of these, alone.
+    for x, y in zip(got[1:3], ref[1:3]):
+        n = y.flatten(2).norm(dim=-1).max()
+        err = (x.double().cpu() - y).flatten(2).norm(dim=-1) / n
+        assert float(err.max()) <= 2e-6 + 5 * 2.0 ** -24 * 0.9 * 400, float(err.max())
+
+
 def test_equals_plain_attention(cuda):
     """Without any of the forms: fused_attention's and fused_cross_attention's results, to rounding."""
     q, k, v, g = operands(2, 4, 4, 300, 300, 64, seed=6)

@@ -465,7 +465,7 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
     load(t0 + 1);
     cq = own.split(a.scale < 0.0f ? -1.0f : 1.0f, q) * (fabsf(a.scale) * kLog2e * ((MODS & 2) != 0 ? a.unit : 1.0f));
   }
-  const float slope2 = (MODS & 1) != 0 ? slope_of(a, h) : 0.0f, fpos = static_cast<float>(pos - 4 * g);
+  const float slope2 = (MODS & 1) != 0 ? slope_of(a, h) : 0.0f;
   const float f2 = (MODS & 2) != 0 ? a.cap2 : 1.0f;
   Places places;
   if constexpr ((MODS & 1) != 0) places.set(slope2);
@@ -512,7 +512,7 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
         if constexpr ((MODS & 2) != 0) return f4{f2, f2, f2, f2};
         return ld4(&sm.uk[cur][8 * i + 4 * g]) * cq;
       };
-      const float base = fpos - static_cast<float>(kt0);
+      const float base = static_cast<float>(pos - 4 * g - kt0);
       if (fabsf(slope2) <= kSteep && (ordered || kt0 + kRows - 1 <= lo_pos)) {
         shift = slope2 * base;
         scale_add(s, f, [&](int r) { return places.by[r]; });
@@ -1032,7 +1032,7 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
 #pragma unroll
   for (int dt = 0; dt < kDT; ++dt) dq[dt] = zero16();
   const float cs = a.scale * kLog2e * ((MODS & 2) != 0 ? a.unit : 1.0f) * uq, cg = ug;
-  const float slope2 = (MODS & 1) != 0 ? slope_of(a, h) : 0.0f, fpos = static_cast<float>(pos - 4 * g);
+  const float slope2 = (MODS & 1) != 0 ? slope_of(a, h) : 0.0f;
   const float f2 = (MODS & 2) != 0 ? a.cap2 : 1.0f;
   Places places;
   if constexpr ((MODS & 1) != 0) places.set(slope2);
@@ -1088,7 +1088,7 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
         if constexpr ((MODS & 2) != 0) return f4{f2, f2, f2, f2};
         return ld4(&sm.ua[cur][8 * i + 4 * g]) * cs;
       };
-      const float base = fpos - static_cast<float>(kt0);
+      const float base = static_cast<float>(pos - 4 * g - kt0);
       if (fabsf(slope2) <= kSteep && (ordered || kt0 + kRows - 1 <= lo_pos)) {
         l = fmaf(-slope2, base, L);
         scale_add(s, f, [&](int r) { return places.by[r]; });

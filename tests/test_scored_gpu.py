@@ -426,6 +426,22 @@ def test_far_rows(cuda):
     assert torch.equal(out, cfa.fused_scored_attention(*(t.to(cuda) for t in (q, k, v)), 0.125, True))
 
 
+def test_far_positions(cuda):
+    """Positions past 2^24, which are no floats: their distances are those of near ones."""
+    sk, near = 2 ** 24 + 77, 3000
+    q, k, v, g = operands(1, 2, 1, 40, near, 32, seed=23)
+    far = [torch.zeros(1, 1, sk, 32, device=cuda) for _ in range(2)]
+    for x, y in zip(far, (k, v)):
+        x[:, :, -near:] = y.to(cuda)
+    slopes = torch.tensor([0.05, 0.3])  # (a key 3000 away weighs e^-150)
+    leaves = [t.requires_grad_(True) for t in (q.to(cuda), *far)]
+    out = cfa.fused_scored_attention(*leaves, 0.2, True, slopes=slopes.to(cuda))
+    dq, dk, dv = torch.autograd.grad(out, leaves, g.to(cuda))
+    ref, top = formula(q, k, v, g, 0.2, True, slopes=slopes)
+    check([out.detach(), dq, dk[:, :, -near:], dv[:, :, -near:]], ref, top)
+    assert float(dk[:, :, :-near].abs().max()) == 0.0 and float(dv[:, :, :-near].abs().max()) < 1e-30
+
+
 def test_saved_tensors_elsewhere(cuda):
     """Activations kept on the host between the forward and the backward, which come back contiguous."""
     q, k, v, g = operands(2, 4, 2, 100, 100, 64, seed=17)

@@ -59,8 +59,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     token j: what fused_scored_attention does of a sequence's last token.
 
     q: [b, h, 1, d], of the cache's type or f32 (any over a 4-bit cache), h a multiple of the cache's key
-    heads (query head i reads key head i // (h // kv_heads)). Returns [b, h, 1, d] of q's type. A sequence of length 0
-    gives 0; one whose length the table cannot hold, or that names a page outside the cache, NaN.
+    heads (query head i reads key head i // (h // kv_heads)). Returns [b, h, 1, d] of q's type. A sequence of
+    length 0 gives 0; one whose length the table cannot hold, or that names a page outside the cache, NaN.
     Infinities and NaN that a token sees give what the formula gives of them. Not differentiable.
     """
     return operators().paged_attention(q, k_pages, v_pages, page_table, lengths, scale, cap, slopes)

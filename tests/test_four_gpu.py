@@ -480,6 +480,31 @@ def test_decoding_step_captured(cuda):
     assert torch.equal(kp, ek) and torch.equal(vp, ev) and torch.equal(lengths, el)
 
 
+def test_two_calls_in_flight(cuda):
+    """Two batches on two streams, each call with a workspace of its own, an append before each on its stream."""
+    caches = [Four(cuda, 2, 16, 64, [3000, 40, 1700], room=8, seed=30 + i) for i in range(2)]
+    q = [q_of(cuda, torch.bfloat16, 3, 8, 64, seed=40 + i) for i in range(2)]
+    k = [torch.randn(3, 2, 8, 64, generator=torch.Generator().manual_seed(50 + i)).bfloat16().to(cuda) for i in range(2)]
+    start = [(c.k.clone(), c.v.clone()) for c in caches]
+
+    def step(i, kp, vp):
+        c = caches[i]
+        cfa.paged_append(k[i], k[i], kp, vp, c.table, c.lengths)
+        return [cfa.paged_attention(q[i], kp, vp, c.table, c.lengths + 8, 0.125, cap=20.0),
+                *cfa.paged_read(kp, vp, c.table, c.lengths + 8, 64, starts=c.lengths - 30)]
+
+    want = [step(i, caches[i].k, caches[i].v) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(i, *start[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for i in range(2) for out in got[i] for x, y in zip(out, want[i]))
+
+
 def test_saved_pages_refuse_their_backward(cuda):
     """An append of codes counts as a write of the pages, as the others do."""
     c = Four(cuda, 1, 16, 32, [3], room=2, seed=16)

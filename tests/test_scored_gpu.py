@@ -426,6 +426,25 @@ def test_far_rows(cuda):
     assert torch.equal(out, cfa.fused_scored_attention(*(t.to(cuda) for t in (q, k, v)), 0.125, True))
 
 
+def test_some_gradients_alone(cuda):
+    """Gradients of q alone, and with frozen keys and values: those of the full call."""
+    q, k, v, g = (t.to(cuda) for t in operands(2, 4, 2, 130, 200, 64, seed=24))
+    how = dict(cap=4.0, slopes=torch.tensor([0.1, 0.2, 0.3, 0.4], device=cuda))
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    full = torch.autograd.grad(cfa.fused_scored_attention(*leaves, 0.125, True, **how), leaves, g)
+    x = q.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(cfa.fused_scored_attention(x, k, v, 0.125, True, **how), x, g)[0], full[0])
+    x = v.clone().requires_grad_(True)
+    cfa.fused_scored_attention(q, k, x, 0.125, True, **how).backward(g)
+    assert torch.equal(x.grad, full[2])
+    # One tensor as keys and values: the sum of both gradients.
+    x = k.clone().requires_grad_(True)
+    y = [k.clone().requires_grad_(True) for _ in range(2)]
+    one = torch.autograd.grad(cfa.fused_scored_attention(q, x, x, 0.125, True, **how), x, g)[0]
+    two = torch.autograd.grad(cfa.fused_scored_attention(q, *y, 0.125, True, **how), y, g)
+    assert torch.equal(one, two[0] + two[1])
+
+
 def test_far_positions(cuda):
     """Positions past 2^24, which are no floats: their distances are those of near ones."""
     sk, near = 2 ** 24 + 77, 3000

@@ -379,17 +379,19 @@ __device__ __forceinline__ void get8(T (&x)[8], const T* from) {
   }
 }
 // Eight values of a key, y = x c + z s (w(k): c, and s with z's sign), as codes, formed in 32 bits: off by 3 x
-// 2^-24 of |x| + |z| at most. `sure`: that leaves no code in doubt.
+// 2^-24 of |x| + |z| at most, times the magnitude; `bound`: 2^-21 of that, or 0 of values that are not turned (c 1
+// and z 0: y is x). `sure`: that leaves no code in doubt. A scale's four lanes come here together, since
+// they exchange its largest magnitude: a branch that some of them take would hide the others' values.
 template <typename T, typename W>
-__device__ __forceinline__ unsigned turned_codes(const T (&x)[8], const T (&z)[8], float magnitude, W w,
-                                                 unsigned& scale, bool& sure) {
+__device__ __forceinline__ unsigned turned_codes(const T (&x)[8], const T (&z)[8], float bound, W w, unsigned& scale,
+                                                 bool& sure) {
   float v[8], off[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const float2 c = w(k);
     const float fx = static_cast<float>(x[k]), fz = static_cast<float>(z[k]);
     v[k] = fmaf(fx, c.x, fz * c.y);
-    off[k] = (fabsf(fx) + fabsf(fz)) * (magnitude * 0x1p-21f);
+    off[k] = (fabsf(fx) + fabsf(fz)) * bound;
   }
   bool here;
   const unsigned codes = codes_within(v, off, scale, here);
@@ -437,8 +439,9 @@ __device__ __forceinline__ unsigned plain_codes(const T (&x)[8], unsigned& scale
 
 // An item: 8 values from e and 8 from e + gap on of one head: of the turned part, in the half layout, those that
 // turn together (gap n); of the rest, or of a head that is not turned or turned in neighbours, its halves.
-// Every part's half is a multiple of 32, so that four neighbours have a scale's values, and all is moved 16
-// bytes at a time.
+// Four neighbours have a scale's values: in the half layout every part's half is a multiple of 32; in
+// neighbours the turned part may end within a scale, and its lanes, whose eight values are turned or not, go one
+// way. All is moved 16 bytes at a time.
 template <typename T, bool kInterleaved>
 __global__ void __launch_bounds__(kRotThreads)
 append_four_kernel(RotaryArgs a) {
@@ -485,7 +488,7 @@ append_four_kernel(RotaryArgs a) {
   };
   load(blk.first + static_cast<int>(threadIdx.x));
   append_tokens(a, blk, sm);
-  const float magnitude = fabsf(static_cast<float>(a.magnitude));
+  const float bound = fabsf(static_cast<float>(a.magnitude)) * 0x1p-21f;
 
   // Sixteen values, turned where they are turned, of q.
   auto put_q = [&](const Item& x) {
@@ -535,18 +538,19 @@ append_four_kernel(RotaryArgs a) {
     const float2* cs = sm.cs + x.t * n;
     if (halves && x.e < n) {
       cs += x.e;
-      cx = turned_codes(x.x, x.z, magnitude, [&](int k) { return float2{cs[k].x, -cs[k].y}; }, sx, sure);
-      cz = turned_codes(x.z, x.x, magnitude, [&](int k) { return cs[k]; }, sz, sure);
+      cx = turned_codes(x.x, x.z, bound, [&](int k) { return float2{cs[k].x, -cs[k].y}; }, sx, sure);
+      cz = turned_codes(x.z, x.x, bound, [&](int k) { return cs[k]; }, sz, sure);
     } else if (kInterleaved && blk.turns) {
       auto pairs = [&](const T (&y)[8], int e, unsigned& scale) {
-        if (e >= 2 * n) return plain_codes(y, scale);
+        const bool in = e < 2 * n;
+        if (n % 16 == 0 && !in) return plain_codes(y, scale);  // (no scale has both: four lanes alike)
         T other[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) other[k] = y[k ^ 1];
+        for (int k = 0; k < 8; ++k) other[k] = in ? y[k ^ 1] : static_cast<T>(0.0f);
         return turned_codes(
-            y, other, magnitude,
+            y, other, in ? bound : 0.0f,
             [&](int k) {
-              const float2 w = cs[(e + k) / 2];
+              const float2 w = in ? cs[(e + k) / 2] : float2{1.0f, 0.0f};
               return k % 2 == 0 ? float2{w.x, -w.y} : w;
             },
             scale, sure);
@@ -636,7 +640,7 @@ append_four_any_kernel(RotaryArgs a) {
     unsigned scale, codes;
     bool sure = true;
     if (blk.turns) {
-      codes = turned_codes(x, z, fmaxf(magnitude, 1.0f), w, scale, sure);
+      codes = turned_codes(x, z, fmaxf(magnitude, 1.0f) * 0x1p-21f, w, scale, sure);
       if (__builtin_amdgcn_ballot_w64(!sure) != 0) {
         codes = exact_codes<T, kInterleaved>(a, blk, sm, t, row, e, scale);
       }

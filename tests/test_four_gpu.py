@@ -539,3 +539,37 @@ def test_refusals_on_the_device(cuda):
     off = buf[2:].view(c.k.shape)
     with pytest.raises(cfa.FusedAttentionError, match="4-byte aligned"):
         cfa.paged_attention(q, off, c.v, c.table, c.lengths, 1.0)
+
+
+@pytest.mark.parametrize("interleaved", [False, True], ids=["half", "interleaved"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,dim", [(64, 8), (64, 16), (64, 40), (64, 48), (64, 56), (128, 8), (128, 16), (128, 72),
+                                   (128, 80), (128, 96), (128, 120)])
+def test_append_partly_turned_groups(cuda, d, dim, dtype, interleaved):
+    """Turned and other values under one scale: alike, one part 50 times the other, one of zeros, a NaN or an
+    infinity in one part; the same bytes for a token alone, whose neighbours leave nothing in doubt."""
+    dt, n = TYPES[dtype], 24
+    gen = torch.Generator().manual_seed(d + dim)
+    k = torch.randn(7, 2, n, d, generator=gen)
+    k[1, ..., :dim] *= 50.0
+    k[2, ..., dim:] *= 50.0
+    k[3, ..., :dim] = 0.0
+    k[4, ..., dim:] = 0.0
+    k[5, :, ::2, dim], k[5, :, 1::2, dim - 1] = float("nan"), float("nan")
+    k[6, :, ::2, dim], k[6, :, 1::2, dim - 1] = float("inf"), -float("inf")
+    k = k.to(dt)
+    v = torch.randn(7, 2, n, d, generator=gen).to(dt)
+    f = cfa.rotary_frequencies(dim, device=cuda)
+    table = torch.arange(14, dtype=torch.int32, device=cuda).view(7, 2)
+    held = ints([0, 1, 2, 3, 4, 5, 6], cuda)
+    kp, vp, k1, v1 = (torch.zeros(14, 2, 16, cfa.fp4_row_bytes(d), dtype=torch.uint8, device=cuda) for _ in range(4))
+    cfa.paged_append(k.to(cuda), v.to(cuda), kp, vp, table, held, frequencies=f, interleaved=interleaved)
+    got_k, got_v = (x.view(7, 2, 2, 16, -1).transpose(1, 2).flatten(2, 3).cpu() for x in (kp, vp))
+    for i in range(7):
+        want = encode(turned(k[i], torch.arange(i, i + n), f, interleaved))
+        assert torch.equal(got_k[i, :, i:i + n], want), i
+        assert torch.equal(got_v[i, :, i:i + n], encode(v[i])), i
+    for t in range(n):
+        cfa.paged_append(k[:, :, t:t + 1].to(cuda), v[:, :, t:t + 1].to(cuda), k1, v1, table, held + t, frequencies=f,
+                         interleaved=interleaved)
+    assert torch.equal(kp, k1) and torch.equal(vp, v1)

@@ -12,7 +12,9 @@ cache.
 A 4-bit cache holds a sign and a magnitude of 0, .5, 1, 1.5, 2, 3, 4 or 6 per value, times a power of two per
 32 values of a row: the least under which none of them passes 7. An append takes the nearest (the even code
 of two), so a value is off by half a step at most: a quarter of the power of two near 0, one of it at 6. A
-group of 32 that has a value that is not finite becomes NaN. d 128 takes 68 bytes, of 256 in 16 bits.
+group of 32 that has a value that is not finite becomes NaN. Values of 3.5 x 2^126 (2.98e38) and more, with which
+a group has the power 2^126, become 4 x 2^126, which no float holds: an infinity where the cache is read or attended
+over; keys turned past the largest float count as that. d 128 takes 68 bytes, of 256 in 16 bits.
 """
 from __future__ import annotations
 

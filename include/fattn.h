@@ -225,7 +225,8 @@ int fattn_backward(const float* q, int64_t q_offset, const int64_t q_shape[4],
  * values, then zeros. A code is a sign and the index of a magnitude among 0, .5, 1, 1.5, 2, 3, 4, 6 (no
  * negative 0); a scale byte e means times 2^(e - 127), 255 NaN. An append takes the least scale (byte 0 at
  * least) under which none of the 32 values passes 7, and the nearest code, the even one of two; a group
- * with a value that is not finite is NaN. The values are bf16 values. */
+ * with a value that is not finite is NaN. The values are bf16 values, but for 4 and 6 times 2^126 and 2 and more
+ * times 2^127, which are infinities where they are read: a value of 3.5 x 2^126 and more becomes 4 x 2^126. */
 #define FATTN_FP4 3
 #define FATTN_FP4_ROW(d) ((d) / 2 + ((d) < 128 ? 4 : (d) / 32))
 

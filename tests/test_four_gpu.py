@@ -573,3 +573,88 @@ def test_append_partly_turned_groups(cuda, d, dim, dtype, interleaved):
         cfa.paged_append(k[:, :, t:t + 1].to(cuda), v[:, :, t:t + 1].to(cuda), k1, v1, table, held + t, frequencies=f,
                          interleaved=interleaved)
     assert torch.equal(kp, k1) and torch.equal(vp, v1)
+
+
+def codes_under(byte):
+    """A row of 32: every code twice, in order and back, under one scale byte."""
+    row = torch.zeros(20, dtype=torch.uint8)
+    codes = list(range(16)) + list(range(15, -1, -1))
+    row[:16] = torch.tensor([x | y << 4 for x, y in zip(codes[0::2], codes[1::2])], dtype=torch.uint8)
+    row[16] = byte
+    return row
+
+
+BYTES = [0, 1, 2, 64, 126, 127, 128, 252, 253, 254, 255]
+
+
+def same(x, y):
+    """Equal, infinities by their sign, NaN where the other is."""
+    x, y = x.cpu(), y.cpu()
+    return torch.equal(x.isnan(), y.isnan()) and torch.equal(x[~x.isnan()], y[~y.isnan()])
+
+
+@pytest.mark.parametrize("to", TYPES)
+def test_read_every_code_at_the_ends(cuda, to):
+    """Scales from 2^-127 on (subnormal values) to 2^127, past which codes are infinities, and NaN."""
+    kp = torch.zeros(1, 1, 16, 20, dtype=torch.uint8)
+    kp[0, 0, :len(BYTES)] = torch.stack([codes_under(x) for x in BYTES])
+    vp = kp.flip(2)
+    n = len(BYTES)
+    k, v = cfa.paged_read(kp.to(cuda), vp.to(cuda), ints([[0]], cuda), ints([16], cuda), 16, dtype=TYPES[to])
+    ref = decode(kp[0, 0], 32).float().to(TYPES[to])
+    assert bool(ref[BYTES.index(253)].isinf().any()) and bool(ref[n - 1].isnan().all())
+    assert same(k[0, 0], ref) and same(v[0, 0], ref.flip(0))
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_values_at_the_ends(cuda, dtype, d):
+    """One token's weight is 1, whose lower terms are 0: its values come back, infinities among them. (Of type f16
+    or bf16 rounded once.) In a longer sequence they leave the other 32 head_dims as they are."""
+    n = len(BYTES)
+    rows = torch.zeros(n, 1, 16, cfa.fp4_row_bytes(d), dtype=torch.uint8)
+    for i, byte in enumerate(BYTES):
+        row = codes_under(byte)
+        for g in range(d // 32):
+            rows[i, 0, 0, 16 * g:16 * (g + 1)] = row[:16]
+            rows[i, 0, 0, d // 2 + g] = byte if g == 0 else 127
+    kp = torch.zeros_like(rows)
+    kp[..., d // 2:d // 2 + d // 32] = 127
+    table = torch.arange(n, dtype=torch.int32, device=cuda)[:, None]
+    q = q_of(cuda, TYPES[dtype], n, 1, d)
+    out = cfa.paged_attention(q, kp.to(cuda), rows.to(cuda), table, ints([1] * n, cuda), 1.0)
+    ref = decode(rows[:, 0, 0], d).float().to(TYPES[dtype])
+    for i, byte in enumerate(BYTES):
+        if byte > 2:
+            assert same(out[i, 0, 0], ref[i]), (byte, out[i, 0, 0], ref[i])
+        else:  # (values below the least normal float: products may flush them)
+            assert float((out[i, 0, 0].double().cpu() - ref[i].double()).abs().max()) <= 2.0 ** -126
+    c = Four(cuda, 2, 16, d, [300, 700], seed=18)
+    q = q_of(cuda, TYPES[dtype], 2, 4, d)
+    clean = cfa.paged_attention(q, c.k, c.v, c.table, c.lengths, d ** -0.5)
+    for byte, code in ((253, 6), (253, 15), (254, 4), (254, 13)):
+        v = c.v.clone()
+        row = v[int(c.table[1, 20]), 1, 3]
+        row[:16], row[d // 2] = code | code << 4, byte
+        out = cfa.paged_attention(q, c.k, v, c.table, c.lengths, d ** -0.5)
+        assert torch.equal(out[0], clean[0]) and torch.equal(out[1, :2], clean[1, :2])
+        assert torch.equal(out[1, 2:, :, 32:], clean[1, 2:, :, 32:])
+        want = -float("inf") if code & 8 else float("inf")
+        assert bool((out[1, 2:, :, :32] == want).all())
+
+
+@pytest.mark.parametrize("interleaved", [False, True], ids=["half", "interleaved"])
+def test_append_keys_past_the_largest_float(cuda, interleaved):
+    """Turned past the largest float, a key counts as it; a value from 3.5 x 2^126 on is stored as 4 x 2^126."""
+    big = torch.finfo(torch.float32).max
+    k = torch.full((1, 1, 3, 64), 3e38)
+    k[..., 1::2] = -2.9e38
+    k[0, 0, 2] = torch.linspace(-1.0, 1.0, 64) * big
+    f = torch.full((32,), 0.7, dtype=torch.float64, device=cuda)
+    kp, vp = (torch.zeros(1, 1, 16, 36, dtype=torch.uint8, device=cuda) for _ in range(2))
+    cfa.paged_append(k.to(cuda), k.to(cuda), kp, vp, ints([[0]], cuda), ints([1], cuda), frequencies=f,
+                     interleaved=interleaved)
+    y = turned(k[0], torch.arange(1, 4), f, interleaved)
+    assert float(y.abs().max()) > big
+    assert torch.equal(kp[0, :, 1:4].cpu(), encode(y.clamp(-big, big)))
+    assert torch.equal(vp[0, :, 1:4].cpu(), encode(k[0]))

@@ -44,6 +44,11 @@ __device__ __forceinline__ float vmax(float a, float b) {
   return r;
 }
 
+// A slope of scores in units of log2 e, a float where the slope is one (past it, at distance 0, 0 x infinity).
+__device__ __forceinline__ float slope_log2(float slope) {
+  const float s = slope * kLog2e;
+  return fabsf(s) == __builtin_inff() ? copysignf(3.402823466e38f, s) : s;
+}
 // tanh z, |z| <= kTanhSmall: z + z^3 P(z^2), P of degree 4 the minimax fit on that range (relative error of
 // the result 2^-27.7; with the roundings 1.3 x 2^-24 at most, 0.43 in the mean square).
 constexpr float kTanhSmall = 0.625f;

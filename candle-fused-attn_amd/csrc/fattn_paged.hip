@@ -615,7 +615,7 @@ split_kernel(SplitArgs a) {
       int head, i;
       row_of(a, kvh, r0 + min(j, rows - 1), head, i);
       x.load_q(static_cast<const Q*>(a.q) + b * a.qs[0] + head * a.qs[1] + i * a.qs[2], a.scale, g);
-      if constexpr (kMods) x.slope2 = a.slopes != nullptr ? a.slopes[head] * kLog2e : 0.0f;
+      if constexpr (kMods) x.slope2 = a.slopes != nullptr ? slope_log2(a.slopes[head]) : 0.0f;
     }
     const C* kp = static_cast<const C*>(a.k) + kvh * a.ks[1];
     const C* vp = static_cast<const C*>(a.v) + kvh * a.vs[1];

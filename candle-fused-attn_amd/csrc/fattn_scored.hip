@@ -125,7 +125,7 @@ __device__ __forceinline__ const int32_t* ids_of(const ScoredArgs& a, int b) {
   return a.documents != nullptr ? a.documents + b * a.document_stride : nullptr;
 }
 __device__ __forceinline__ float slope_of(const ScoredArgs& a, int h) {
-  return a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.0f;
+  return a.slopes != nullptr ? slope_log2(a.slopes[h]) : 0.0f;
 }
 
 // --- Scores ------------------------------------------------------------------------------------

@@ -280,7 +280,7 @@ int fattn_paged_attention(int dtype, int cache_dtype, int64_t b, int64_t heads, 
 
 /* The same, of scores x = scale q.k taken as cap tanh(x / cap) (cap 0: as they are; else 1e-30 to 1e30),
  * less slopes[head] times the distance lengths[b] - 1 - j to cached token j (slopes NULL: none; [heads]
- * finite floats on the device). The workspace is fattn_paged_attention's. */
+ * finite floats on the device, a negative one a float times every distance too). The workspace is fattn_paged_attention's. */
 int fattn_paged_scored_attention(int dtype, int cache_dtype, int64_t b, int64_t heads, int64_t kv_heads,
                                  int64_t d, const void* q, const int64_t q_strides[2], void* out,
                                  const void* k_pages, const int64_t k_page_strides[3],
@@ -329,7 +329,7 @@ int fattn_cross_backward(const float* q, const int64_t q_strides[3], const float
 /* Attention of scores of other forms, fp32: q [b, heads, sq, d], the last sq of sk positions, to k, v
  * [b, kv_heads, sk, d] (strides {batch, head, seq}, rows 16-byte aligned). A score x = scale q.k is taken as
  * cap tanh(x / cap) (cap 0: as it is; else 1e-30 to 1e30), less slopes[head] times the distance of the
- * positions (NULL: none; finite floats). A query sees the keys at its position or before it, and the first
+ * positions (NULL: none; floats as there). A query sees the keys at its position or before it, and the first
  * prefix[b] of the sample (NULL: none; outside [0, sk]: the nearest), or with causal 0 all; of these, with
  * documents ([b, sk] ids, rows document_stride apart), those of its own id, a token of a negative id none, and
  * it is seen by none. out [b, sq, heads, d] contiguous, lse [b, heads, sq]; a query that sees no key has out 0

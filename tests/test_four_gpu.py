@@ -658,3 +658,15 @@ def test_append_keys_past_the_largest_float(cuda, interleaved):
     assert float(y.abs().max()) > big
     assert torch.equal(kp[0, :, 1:4].cpu(), encode(y.clamp(-big, big)))
     assert torch.equal(vp[0, :, 1:4].cpu(), encode(k[0]))
+
+
+@pytest.mark.parametrize("cap", [None, 3.0], ids=["plain", "capped"])
+def test_attention_slopes_to_the_largest_float(cuda, cap):
+    """Slopes that are floats but not in units of log2 e, or not times a distance: the last token alone."""
+    lengths = [1, 2, 33, 700, 3000]
+    c = Four(cuda, 2, 16, 64, lengths, seed=19)
+    q = q_of(cuda, torch.float32, len(lengths), 4, 64)
+    slopes = torch.tensor([torch.finfo(torch.float32).max, 2.4e38, 1e38, 1e37], device=cuda)
+    out = cfa.paged_attention(q, c.k, c.v, c.table, c.lengths, 0.125, cap=cap, slopes=slopes)
+    ref, _ = attended(q, c, lengths, 0.125, cap, slopes)
+    assert rel(out, ref) <= bar(torch.float32)

@@ -545,3 +545,18 @@ def test_trained_and_served_alike(cuda, cache):
         at = torch.full((b,), t + 1, dtype=torch.int32, device=cuda)
         out = cfa.paged_attention(qt[:, :, t:t + 1], kp, vp, table, at, 0.125, **how)
         assert rel(out[:, :, 0], whole[:, :, t]) <= bar, t
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("causal", [False, True], ids=["all", "causal"])
+@pytest.mark.parametrize("cap", [None, 3.0], ids=["plain", "capped"])
+def test_slopes_to_the_largest_float(cuda, d, causal, cap):
+    """Slopes that are floats but not in units of log2 e, or not times a distance: a query's own key alone."""
+    big = torch.finfo(torch.float32).max
+    slopes = torch.tensor([big, 2.4e38, 1e38, 1e37])
+    q, k, v, g = operands(2, 4, 2, 150, 300, d, seed=24)
+    got = run(cuda, q, k, v, g, d ** -0.5, causal, cap=cap, slopes=slopes)
+    ref, _ = formula(q, k, v, g, d ** -0.5, causal, cap=cap, slopes=slopes)
+    check([got[0], got[3]], [ref[0], ref[3]])
+    # (No gradient of the scores: P (dP - D) of a weight of 1, where dP and D are the same sum but for roundings.)
+    assert all(float(x.abs().max()) <= 1e-5 for x in got[1:3])

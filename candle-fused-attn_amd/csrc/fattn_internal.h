@@ -309,7 +309,9 @@ struct ScoredArgs {
   int B, H, G, SQ, SK;  // G: query heads per key head; queries are the last SQ of SK positions
   float scale;
   int causal;
-  float cap2, unit;  // cap log2 e (0: none), and its inverse (1: none)
+  // cap log2 e (0: none), and its inverse as a product: `unit` (1: none) goes with the operands' units, and what
+  // that would take out of a float's range, past 2^+-40, is `unit_rest` (nearly always 1).
+  float cap2, unit, unit_rest;
   const float* slopes;
   const int32_t *documents, *prefix;
   int64_t document_stride;

@@ -263,7 +263,9 @@ int scored_operands(fattn::ScoredArgs& a, const float* q, const int64_t q_stride
   a.B = static_cast<int>(b), a.H = static_cast<int>(heads), a.G = static_cast<int>(heads / kv_heads);
   a.SQ = static_cast<int>(sq), a.SK = static_cast<int>(sk);
   a.scale = scale, a.causal = causal ? 1 : 0;
-  a.cap2 = cap * kLog2e, a.unit = cap == 0.0f ? 1.0f : 1.0f / a.cap2;
+  const float inverse = cap == 0.0f ? 1.0f : 1.0f / (cap * kLog2e);
+  a.cap2 = cap * kLog2e, a.unit_rest = inverse > 0x1p40f ? 0x1p60f : inverse < 0x1p-40f ? 0x1p-60f : 1.0f;
+  a.unit = inverse / a.unit_rest;
   a.slopes = slopes, a.documents = documents, a.document_stride = document_stride, a.prefix = prefix;
   return 0;
 }

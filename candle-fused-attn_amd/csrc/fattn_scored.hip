@@ -133,17 +133,19 @@ __device__ __forceinline__ float slope_of(const ScoredArgs& a, int h) {
 // walk holds tanh of it, and cap2 of that (cap log2 e) enters with what the exponent adds anyway.
 // One score in units of log2 e by its definition, for the rows in fp32, and dy / dx.
 __device__ __forceinline__ float score_fp32(const ScoredArgs& a, float dot, float slope2, int far, float& slope) {
-  float y = dot * (a.scale * kLog2e * a.unit);
+  float y = dot * (a.scale * kLog2e * a.unit) * a.unit_rest;
   slope = 1.0f;
   if (a.cap2 != 0.0f) y = a.cap2 * tanh_any(y, slope);
   return fmaf(-slope2, fabsf(static_cast<float>(far)), y);
 }
 // Nothing is scheduled across: sixteen polynomials side by side take more registers than there are.
 __device__ __forceinline__ void few_at_once() { __builtin_amdgcn_sched_barrier(0); }
-// x / cap of a wave's tile to its tanh t and `fn(r, dt / dx)`. (Nearly always every |x| / cap is small, where a
-// polynomial does it: of degree 7 or 11 in x, against those and an exponential and a quotient besides.)
+// x / cap of a wave's tile (less the factor `rest`) to its tanh t and `fn(r, dt / dx)`. (Nearly always every |x| /
+// cap is small, where a polynomial does it: of degree 7 or 11 in x, against those and an exponential and a quotient
+// besides.)
 template <typename F>
-__device__ __forceinline__ void capped(f16v& x, F fn) {
+__device__ __forceinline__ void capped(f16v& x, float rest, F fn) {
+  if (rest != 1.0f) x *= rest;
   const float most = max_weight(x);
   if (__builtin_amdgcn_ballot_w64(most > kTanhTiny) == 0) {
 #pragma unroll
@@ -505,7 +507,7 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[4 * i + c] *= cq * uk[c];
       }
-      capped(s, [](int, float) {});
+      capped(s, a.unit_rest, [](int, float) {});
     }
     if constexpr ((MODS & 1) != 0) {
       auto f = [&](int i) {
@@ -848,7 +850,7 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
 #pragma unroll
       for (int e = 0; e < 4; ++e) dp[4 * i + e] = fmaf(dp[4 * i + e], cg, -Dv[e]);
     }
-    if constexpr ((MODS & 2) != 0) capped(s, [&](int r, float slope) { dp[r] *= slope; });
+    if constexpr ((MODS & 2) != 0) capped(s, a.unit_rest, [&](int r, float slope) { dp[r] *= slope; });
     // The slope's part: a row's (staged with its L) and the lane's, or, where a key may be after a query that
     // sees it, of the distance.
     // (With a slope s becomes the whole exponent.)
@@ -1081,7 +1083,7 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
 #pragma unroll
       for (int e = 0; e < 4; ++e) dp[4 * i + e] = fmaf(dp[4 * i + e], cg * uv[e], -Dq);
     }
-    if constexpr ((MODS & 2) != 0) capped(s, [&](int r, float slope) { dp[r] *= slope; });
+    if constexpr ((MODS & 2) != 0) capped(s, a.unit_rest, [&](int r, float slope) { dp[r] *= slope; });
     float l = L;
     if constexpr ((MODS & 1) != 0) {
       auto f = [&](int i) {

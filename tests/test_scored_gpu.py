@@ -560,3 +560,19 @@ def test_slopes_to_the_largest_float(cuda, d, causal, cap):
     check([got[0], got[3]], [ref[0], ref[3]])
     # (No gradient of the scores: P (dP - D) of a weight of 1, where dP and D are the same sum but for roundings.)
     assert all(float(x.abs().max()) <= 1e-5 for x in got[1:3])
+
+
+@pytest.mark.parametrize("cap,scale,spread", [(1e30, 1e-9, 1e9), (1e30, 0.125, 1.0), (1e25, 1e-12, 1e12), (1e13, 1e-3, 1e3),
+                                              (1e-13, 0.125, 1.0), (1e-30, 1e9, 1.0), (1e-30, 1e-9, 1.0)])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_caps_to_the_ends(cuda, cap, scale, spread, d):
+    """Caps whose quotient with the scale, and with the operands' units, leaves the range of floats; scores of 0
+    among them. (x / cap is off by as much as x, so the scores' derivative by nothing that counts.)"""
+    q, k, v, g = operands(1, 4, 2, 150, 180, d, seed=25, spread=spread)
+    q[:, :, ::3] = 0.0
+    for causal in (True, False):
+        ref, top = formula(q, k, v, g, scale, causal, cap=cap)
+        check(run(cuda, q, k, v, g, scale, causal, cap=cap), ref, top)
+    slopes = torch.tensor([0.1, 0.0, 0.01, 1.5])
+    ref, top = formula(q, k, v, g, scale, True, cap=cap, slopes=slopes)
+    check(run(cuda, q, k, v, g, scale, True, cap=cap, slopes=slopes), ref, top)

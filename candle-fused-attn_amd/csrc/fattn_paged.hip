@@ -185,9 +185,9 @@ __device__ __forceinline__ float four_scale(unsigned byte) { return __uint_as_fl
 // A sum of weights times 4-bit values that is not finite. Under the scales 2^126 (4 and 6) and 2^127 (2 to 6) a
 // code is an infinity, and makes a NaN of a weight's rest of 0; what the sum is then lies in the values alone: NaN
 // with a NaN among them or with infinities of both signs, else the infinity. `row(t)`: token t's value row; value d
-// of D, tokens t0 .. t1. (64 sequences of 1 to 2048, 6 heads, d 64, f32 23.2 -> 23.6 us, bf16 with a cap 25.6 -> 26.8,
-// long contexts as before. With a look at every tile's scales, and their infinities in a pass of their own, 24.4 and
-// 28.1, 4 contexts d 128 bf16 98 -> 107.)
+// of D, tokens t0 .. t1. (64 sequences of 1 to 2048, 6 heads, d 64: f32 23.6 -> 23.9 us, bf16 with a cap 25.3 -> 25.9,
+// where the compiler is told that it is rare, 26.8 else; long contexts as before. With a look at every tile's scales,
+// and their infinities in a pass of their own, 24.4 and 28.1, 4 contexts d 128 bf16 98 -> 107.)
 template <int D, typename Row>
 __device__ __forceinline__ float infinite_sum(float sum, int d, int t0, int t1, Row row) {
   bool up = false, down = false;
@@ -734,7 +734,7 @@ split_kernel(SplitArgs a) {
       }
       if constexpr (W::kFour) {
         // (A token without a page, or a weight that is not finite: l is NaN.)
-        if (l > 0.0f && !((o[0] + o[1]) * 0.0f + (o[2] + o[3]) * 0.0f == 0.0f)) {
+        if (__builtin_expect(l > 0.0f && !((o[0] + o[1]) * 0.0f + (o[2] + o[3]) * 0.0f == 0.0f), 0)) {
           // (Formed here again, in vector registers: what is held for this place takes registers of every head's
           // beginning.)
           int at_b = b, at_head = kvh, from = t0, to = t1;

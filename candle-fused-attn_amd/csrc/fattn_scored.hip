@@ -129,8 +129,10 @@ __device__ __forceinline__ float slope_of(const ScoredArgs& a, int h) {
 }
 
 // --- Scores ------------------------------------------------------------------------------------
-// MODS, bits: 1, less a slope times the distance; 2, capped. With a cap the products' factor gives x / cap, a
-// walk holds tanh of it, and cap2 of that (cap log2 e) enters with what the exponent adds anyway.
+// MODS, bits: 1, less a slope times the distance; 2, capped; 4 (with both), by a cap of which a part is multiplied
+// last, ScoredArgs::unit_rest. With a cap the products' factor gives x / cap, a walk holds tanh of it, and cap2 of that
+// (cap log2 e) enters with what the exponent adds anyway. (A kernel of its own: as a branch of the others that part
+// takes 473 -> 486 us forward and backward, 8 x 12 heads of 2048 in documents.)
 // One score in units of log2 e by its definition, for the rows in fp32, and dy / dx.
 __device__ __forceinline__ float score_fp32(const ScoredArgs& a, float dot, float slope2, int far, float& slope) {
   float y = dot * (a.scale * kLog2e * a.unit) * a.unit_rest;
@@ -140,12 +142,10 @@ __device__ __forceinline__ float score_fp32(const ScoredArgs& a, float dot, floa
 }
 // Nothing is scheduled across: sixteen polynomials side by side take more registers than there are.
 __device__ __forceinline__ void few_at_once() { __builtin_amdgcn_sched_barrier(0); }
-// x / cap of a wave's tile (less the factor `rest`) to its tanh t and `fn(r, dt / dx)`. (Nearly always every |x| /
-// cap is small, where a polynomial does it: of degree 7 or 11 in x, against those and an exponential and a quotient
-// besides.)
+// x / cap of a wave's tile to its tanh t and `fn(r, dt / dx)`. (Nearly always every |x| / cap is small, where a
+// polynomial does it: of degree 7 or 11 in x, against those and an exponential and a quotient besides.)
 template <typename F>
-__device__ __forceinline__ void capped(f16v& x, float rest, F fn) {
-  if (rest != 1.0f) x *= rest;
+__device__ __forceinline__ void capped(f16v& x, F fn) {
   const float most = max_weight(x);
   if (__builtin_amdgcn_ballot_w64(most > kTanhTiny) == 0) {
 #pragma unroll
@@ -507,7 +507,8 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[4 * i + c] *= cq * uk[c];
       }
-      capped(s, a.unit_rest, [](int, float) {});
+      if constexpr ((MODS & 4) != 0) s *= a.unit_rest;
+      capped(s, [](int, float) {});
     }
     if constexpr ((MODS & 1) != 0) {
       auto f = [&](int i) {
@@ -843,6 +844,7 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[4 * i + e] *= cs * uq[e];
       }
+      if constexpr ((MODS & 4) != 0) s *= a.unit_rest;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -850,7 +852,7 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
 #pragma unroll
       for (int e = 0; e < 4; ++e) dp[4 * i + e] = fmaf(dp[4 * i + e], cg, -Dv[e]);
     }
-    if constexpr ((MODS & 2) != 0) capped(s, a.unit_rest, [&](int r, float slope) { dp[r] *= slope; });
+    if constexpr ((MODS & 2) != 0) capped(s, [&](int r, float slope) { dp[r] *= slope; });
     // The slope's part: a row's (staged with its L) and the lane's, or, where a key may be after a query that
     // sees it, of the distance.
     // (With a slope s becomes the whole exponent.)
@@ -1076,6 +1078,7 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[4 * i + e] *= cs * uk[e];
       }
+      if constexpr ((MODS & 4) != 0) s *= a.unit_rest;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -1083,7 +1086,7 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
 #pragma unroll
       for (int e = 0; e < 4; ++e) dp[4 * i + e] = fmaf(dp[4 * i + e], cg * uv[e], -Dq);
     }
-    if constexpr ((MODS & 2) != 0) capped(s, a.unit_rest, [&](int r, float slope) { dp[r] *= slope; });
+    if constexpr ((MODS & 2) != 0) capped(s, [&](int r, float slope) { dp[r] *= slope; });
     float l = L;
     if constexpr ((MODS & 1) != 0) {
       auto f = [&](int i) {
@@ -1197,6 +1200,7 @@ const void* bwd_fn(int d) {
 }
 // (Scale 0: the products are multiplied by it before what is not seen becomes minus infinity.)
 int mods(const ScoredArgs& a) {
+  if (a.unit_rest != 1.0f) return 7;
   const int m = (a.slopes != nullptr ? 1 : 0) + (a.cap2 != 0.0f ? 2 : 0);
   return m == 0 && a.scale == 0.0f ? 1 : m;
 }
@@ -1272,7 +1276,7 @@ int launch_scored_forward(ScoredArgs a, int d, const ScoredPlan& plan, void* wor
   hipStream_t s = static_cast<hipStream_t>(stream);
   const unsigned grid = static_cast<unsigned>(int64_t{a.B} * a.H * a.nqb * a.nc);
   const int m = mods(a);
-  const void* fn = m == 3 ? fwd_fn<3>(d) : m == 2 ? fwd_fn<2>(d) : m == 1 ? fwd_fn<1>(d) : fwd_fn<0>(d);
+  const void* fn = m == 7 ? fwd_fn<7>(d) : m == 3 ? fwd_fn<3>(d) : m == 2 ? fwd_fn<2>(d) : m == 1 ? fwd_fn<1>(d) : fwd_fn<0>(d);
   const hipError_t err = hipLaunchKernel(fn, dim3(grid), dim3(64 * kW), args, 0, s);
   if (err != hipSuccess || a.nc == 1) return static_cast<int>(err);
   const void* join = d == 32    ? reinterpret_cast<const void*>(join_scored_kernel<32>)
@@ -1297,7 +1301,7 @@ int launch_scored_backward(ScoredArgs a, int d, const ScoredBackwardPlan& plan, 
   const int HK = a.H / a.G;
   const int64_t grid = scored_blocks(a.B, HK, a.SK) * a.nck + scored_blocks(a.B, a.H, a.SQ) * a.ncq;
   const int m = mods(a);
-  const void* fn = m == 3 ? bwd_fn<3>(d) : m == 2 ? bwd_fn<2>(d) : m == 1 ? bwd_fn<1>(d) : bwd_fn<0>(d);
+  const void* fn = m == 7 ? bwd_fn<7>(d) : m == 3 ? bwd_fn<3>(d) : m == 2 ? bwd_fn<2>(d) : m == 1 ? bwd_fn<1>(d) : bwd_fn<0>(d);
   hipError_t err = hipLaunchKernel(fn, dim3(static_cast<unsigned>(grid)), dim3(64 * kW), args, 0, s);
   auto sum = [&](const float* part, float* out, int64_t n, int nc) {
     void* sargs[] = {&part, &out, &n, &nc};

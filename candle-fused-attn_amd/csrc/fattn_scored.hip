@@ -140,6 +140,8 @@ __device__ __forceinline__ float score_fp32(const ScoredArgs& a, float dot, floa
   if (a.cap2 != 0.0f) y = a.cap2 * tanh_any(y, slope);
   return fmaf(-slope2, fabsf(static_cast<float>(far)), y);
 }
+// The sign of the scale goes with a wave's own rows: what is hidden, minus infinity, meets a factor above 0.
+__device__ __forceinline__ float sign_of(float scale) { return scale < 0.0f ? -1.0f : 1.0f; }
 // Nothing is scheduled across: sixteen polynomials side by side take more registers than there are.
 __device__ __forceinline__ void few_at_once() { __builtin_amdgcn_sched_barrier(0); }
 // x / cap of a wave's tile to its tanh t and `fn(r, dt / dx)`. (Nearly always every |x| / cap is small, where a
@@ -465,7 +467,7 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
     own.load(qp + min(qi, a.SQ - 1) * a.q.ss, g);
     store(t0);
     load(t0 + 1);
-    cq = own.split(a.scale < 0.0f ? -1.0f : 1.0f, q) * (fabsf(a.scale) * kLog2e * ((MODS & 2) != 0 ? a.unit : 1.0f));
+    cq = own.split(sign_of(a.scale), q) * (fabsf(a.scale) * kLog2e * ((MODS & 2) != 0 ? a.unit : 1.0f));
   }
   const float slope2 = (MODS & 1) != 0 ? slope_of(a, h) : 0.0f;
   const float f2 = (MODS & 2) != 0 ? a.cap2 : 1.0f;
@@ -792,7 +794,7 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
     load_o(0);
     ok.load(a.k.p + b * a.k.sb + hk * a.k.sh + kc * a.k.ss, g);
     ov.load(a.v.p + b * a.v.sb + hk * a.v.sh + kc * a.v.ss, g);
-    uk = ok.split(1.0f, kB);
+    uk = ok.split(sign_of(a.scale), kB);
     uv = ov.split(1.0f, vB);
     store(0);
     load(1);
@@ -801,7 +803,7 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
   f16v dk[kDT], dv[kDT];
 #pragma unroll
   for (int dt = 0; dt < kDT; ++dt) dk[dt] = zero16(), dv[dt] = zero16();
-  const float cs = a.scale * kLog2e * ((MODS & 2) != 0 ? a.unit : 1.0f) * uk, cg = uv;
+  const float cs = fabsf(a.scale) * kLog2e * ((MODS & 2) != 0 ? a.unit : 1.0f) * uk, cg = uv;
   const float f2 = (MODS & 2) != 0 ? a.cap2 : 1.0f;
   const bool ordered = a.causal && prefix == 0;
   float psc = kMaxScale, dsc = kMaxScale;
@@ -1027,7 +1029,7 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
     }
     Dq = pair_sum(Dq) * pow2(kTop);  // (dP and D times 2^kTop meet K's unit)
     L = ids.mine < 0 ? 0.0f : shifted_l(L, kp);  // (as for the key blocks)
-    uq = oq.split(1.0f, qB);
+    uq = oq.split(sign_of(a.scale), qB);
     ug = og.split(1.0f, gB);
     store(t0);
     load(t0 + 1);
@@ -1035,7 +1037,7 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
   f16v dq[kDT];
 #pragma unroll
   for (int dt = 0; dt < kDT; ++dt) dq[dt] = zero16();
-  const float cs = a.scale * kLog2e * ((MODS & 2) != 0 ? a.unit : 1.0f) * uq, cg = ug;
+  const float cs = fabsf(a.scale) * kLog2e * ((MODS & 2) != 0 ? a.unit : 1.0f) * uq, cg = ug;
   const float slope2 = (MODS & 1) != 0 ? slope_of(a, h) : 0.0f;
   const float f2 = (MODS & 2) != 0 ? a.cap2 : 1.0f;
   Places places;

@@ -576,3 +576,19 @@ def test_caps_to_the_ends(cuda, cap, scale, spread, d):
     slopes = torch.tensor([0.1, 0.0, 0.01, 1.5])
     ref, top = formula(q, k, v, g, scale, True, cap=cap, slopes=slopes)
     check(run(cuda, q, k, v, g, scale, True, cap=cap, slopes=slopes), ref, top)
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("causal", [False, True], ids=["all", "causal"])
+def test_a_negative_scale_is_a_sign_of_the_queries(cuda, d, causal):
+    """The same bits as of negated queries (by another path, in fp32, they would differ): scores that are hidden
+    stay hidden whatever the scale's sign. (dK sums the queries themselves, whose signs a matrix instruction need not
+    round alike.)"""
+    ids = ids_of([[100, 130, 60], [300]], 300)
+    q, k, v, g = operands(2, 4, 2, 200, 300, d, seed=26)
+    for how in (dict(), dict(documents=ids), dict(cap=3.0), dict(slopes=torch.tensor([0.1, 0.0, 2.0, -0.01]))):
+        got = run(cuda, q, k, v, g, -0.2, causal, **how)
+        want = run(cuda, -q, k, v, g, 0.2, causal, **how)
+        want[1] = -want[1]
+        assert [torch.equal(got[i], want[i]) for i in (0, 1, 3)] == [True] * 3
+        check(got, formula(q, k, v, g, -0.2, causal, **how)[0], 10.0)

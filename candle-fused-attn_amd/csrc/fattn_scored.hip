@@ -142,6 +142,11 @@ __device__ __forceinline__ float score_fp32(const ScoredArgs& a, float dot, floa
 }
 // The sign of the scale goes with a wave's own rows: what is hidden, minus infinity, meets a factor above 0.
 __device__ __forceinline__ float sign_of(float scale) { return scale < 0.0f ? -1.0f : 1.0f; }
+// That factor, without a cap or slopes: of two rows' units, of which the product may be below the least float (two rows
+// of zeros, as padding has them: 2^-252) or the scale 0. The least float more changes none that counts, and costs
+// nothing beside a product. (8 x 12 heads of 2048, the second half zeros: 1566 and 5770 us without, every wave of zeros
+// once more in fp32; 175 and 575 so.)
+__device__ __forceinline__ float factor(float own, float staged) { return fmaf(own, staged, 0x1p-149f); }
 // Nothing is scheduled across: sixteen polynomials side by side take more registers than there are.
 __device__ __forceinline__ void few_at_once() { __builtin_amdgcn_sched_barrier(0); }
 // x / cap of a wave's tile to its tanh t and `fn(r, dt / dx)`. (Nearly always every |x| / cap is small, where a
@@ -545,7 +550,7 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int r = 4 * i + c;
-          const float p = exp2_hw(MODS == 0   ? fmaf(s[r], cq * uk[c], -m)
+          const float p = exp2_hw(MODS == 0   ? fmaf(s[r], factor(cq, uk[c]), -m)
                                   : MODS == 2 ? fmaf(s[r], f2, -m)
                                               : s[r] - ref);
           psum = r == 0 ? p : psum + p;
@@ -562,7 +567,7 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
       asm("" : "+v"(r0));
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        tmax = fmaxf(tmax, MODS != 0 ? s[r] : s[r] * (cq * sm.uk[cur][8 * (r >> 2) + r0 + (r & 3)]));
+        tmax = fmaxf(tmax, MODS != 0 ? s[r] : s[r] * factor(cq, sm.uk[cur][8 * (r >> 2) + r0 + (r & 3)]));
       }
       if constexpr (MODS == 2) tmax *= f2;
       const float ref = pair_max(tmax - shift) - kRefTop;
@@ -886,7 +891,7 @@ __device__ __forceinline__ void scored_keys(const ScoredArgs& a, ScoredSmem<D>& 
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r = 4 * i + e;
-        s[r] = exp2_hw((MODS & 1) != 0 ? s[r] : fmaf(s[r], MODS == 0 ? cs * uq[e] : f2, L[e])) * ug[e];
+        s[r] = exp2_hw((MODS & 1) != 0 ? s[r] : fmaf(s[r], MODS == 0 ? factor(cs, uq[e]) : f2, L[e])) * ug[e];
         dp[r] = s[r] * dp[r] * uq[e];
       }
     }
@@ -1113,7 +1118,7 @@ __device__ __forceinline__ void scored_queries(const ScoredArgs& a, ScoredSmem<D
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r = 4 * i + e;
-        dp[r] = exp2_hw(MODS == 0   ? fmaf(s[r], cs * uk[e], L)
+        dp[r] = exp2_hw(MODS == 0   ? fmaf(s[r], factor(cs, uk[e]), L)
                         : MODS == 2 ? fmaf(s[r], f2, L)
                                     : s[r] + l) * dp[r] * uk[e];
       }
@@ -1200,11 +1205,9 @@ const void* bwd_fn(int d) {
          : d == 128 ? reinterpret_cast<const void*>(bwd_scored_kernel<128, MODS, 1>)
                     : reinterpret_cast<const void*>(bwd_scored_kernel<64, MODS, 2>);
 }
-// (Scale 0: the products are multiplied by it before what is not seen becomes minus infinity.)
 int mods(const ScoredArgs& a) {
   if (a.unit_rest != 1.0f) return 7;
-  const int m = (a.slopes != nullptr ? 1 : 0) + (a.cap2 != 0.0f ? 2 : 0);
-  return m == 0 && a.scale == 0.0f ? 1 : m;
+  return (a.slopes != nullptr ? 1 : 0) + (a.cap2 != 0.0f ? 2 : 0);
 }
 int64_t blocks_of(int64_t rows) { return (rows + kBlock - 1) / kBlock; }
 

@@ -592,3 +592,25 @@ def test_a_negative_scale_is_a_sign_of_the_queries(cuda, d, causal):
         want[1] = -want[1]
         assert [torch.equal(got[i], want[i]) for i in (0, 1, 3)] == [True] * 3
         check(got, formula(q, k, v, g, -0.2, causal, **how)[0], 10.0)
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("spread", [0.0, 1e-4, 1.0])
+def test_rows_of_zeros(cuda, d, spread):
+    """Padding of zeros behind a sample, and zero keys under small queries: where every score is 0 a score formed
+    another way (less a slope of 0) has the same bits, those of fp32 would differ. Scale 0 likewise."""
+    q, k, v, g = operands(2, 4, 2, 290, 300, d, seed=27)
+    q[:, :, 150:] *= spread
+    k[:, :, 160:] = 0.0
+    for scale in (0.125, -0.125, 0.0):
+        for causal in (True, False):
+            got = run(cuda, q, k, v, g, scale, causal)
+            check(got, formula(q, k, v, g, scale, causal)[0] if scale else
+                  [torch.zeros_like(x, dtype=torch.float64) if i in (1, 2) else x
+                   for i, x in enumerate(formula(q, k, v, g, 0.0, causal)[0])])
+            if spread == 0.0 or scale == 0.0:
+                other = run(cuda, q, k, v, g, scale, causal, slopes=torch.zeros(4))
+                assert torch.equal(got[0][:, :, 192:], other[0][:, :, 192:])
+                assert torch.equal(got[1][:, :, 192:], other[1][:, :, 192:])
+                if causal:
+                    assert torch.equal(got[3][:, :, 256:], other[3][:, :, 256:])

@@ -379,11 +379,12 @@ __device__ __forceinline__ void get8(T (&x)[8], const T* from) {
   }
 }
 // Eight values of a key, y = x c + z s (w(k): c, and s with z's sign), as codes, formed in 32 bits: off by 3 x
-// 2^-24 of |x| + |z| at most, times the magnitude; `bound`: 2^-21 of that, or 0 of values that are not turned (c 1
-// and z 0: y is x). `sure`: that leaves no code in doubt. A scale's four lanes come here together, since
-// they exchange its largest magnitude: a branch that some of them take would hide the others' values.
-template <typename T, typename W>
-__device__ __forceinline__ unsigned turned_codes(const T (&x)[8], const T (&z)[8], float bound, W w, unsigned& scale,
+// 2^-24 of |x| + |z| at most, times the magnitude; `bound(k)`: 2^-21 of that, or 0 of values that are not turned (c
+// 1, s 0 and z of the same scale: y is x, and in doubt it would be at every border, where 1 of 90 bf16 values lies).
+// `sure`: that leaves no code in doubt. A scale's four lanes come here together, since they exchange its largest
+// magnitude: a branch that some of them take would hide the others' values.
+template <typename T, typename B, typename W>
+__device__ __forceinline__ unsigned turned_codes(const T (&x)[8], const T (&z)[8], B bound, W w, unsigned& scale,
                                                  bool& sure) {
   float v[8], off[8];
 #pragma unroll
@@ -391,7 +392,7 @@ __device__ __forceinline__ unsigned turned_codes(const T (&x)[8], const T (&z)[8
     const float2 c = w(k);
     const float fx = static_cast<float>(x[k]), fz = static_cast<float>(z[k]);
     v[k] = fmaf(fx, c.x, fz * c.y);
-    off[k] = (fabsf(fx) + fabsf(fz)) * bound;
+    off[k] = (fabsf(fx) + fabsf(fz)) * bound(k);
   }
   bool here;
   const unsigned codes = codes_within(v, off, scale, here);
@@ -538,17 +539,18 @@ append_four_kernel(RotaryArgs a) {
     const float2* cs = sm.cs + x.t * n;
     if (halves && x.e < n) {
       cs += x.e;
-      cx = turned_codes(x.x, x.z, bound, [&](int k) { return float2{cs[k].x, -cs[k].y}; }, sx, sure);
-      cz = turned_codes(x.z, x.x, bound, [&](int k) { return cs[k]; }, sz, sure);
+      auto off = [&](int) { return bound; };
+      cx = turned_codes(x.x, x.z, off, [&](int k) { return float2{cs[k].x, -cs[k].y}; }, sx, sure);
+      cz = turned_codes(x.z, x.x, off, [&](int k) { return cs[k]; }, sz, sure);
     } else if (kInterleaved && blk.turns) {
       auto pairs = [&](const T (&y)[8], int e, unsigned& scale) {
         const bool in = e < 2 * n;
         if (n % 16 == 0 && !in) return plain_codes(y, scale);  // (no scale has both: four lanes alike)
         T other[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) other[k] = in ? y[k ^ 1] : static_cast<T>(0.0f);
+        for (int k = 0; k < 8; ++k) other[k] = y[k ^ 1];
         return turned_codes(
-            y, other, in ? bound : 0.0f,
+            y, other, [&](int) { return in ? bound : 0.0f; },
             [&](int k) {
               const float2 w = in ? cs[(e + k) / 2] : float2{1.0f, 0.0f};
               return k % 2 == 0 ? float2{w.x, -w.y} : w;
@@ -606,7 +608,7 @@ append_four_any_kernel(RotaryArgs a) {
   const RotaryPart& part = a.part[blk.pi];
   const int n = a.pairs, D = a.D, pi = blk.pi;
   append_tokens(a, blk, sm);
-  const float magnitude = fabsf(static_cast<float>(a.magnitude));
+  const float bound = fabsf(static_cast<float>(a.magnitude)) * 0x1p-21f;
   for (int item = blk.first + static_cast<int>(threadIdx.x); item < blk.last; item += kRotThreads) {
     const int t = divide(item, a.by_per[pi]);
     const int r = item - t * blk.per, head = divide(r, a.by_items[pi]), e = 8 * (r - head * blk.of);
@@ -640,7 +642,8 @@ append_four_any_kernel(RotaryArgs a) {
     unsigned scale, codes;
     bool sure = true;
     if (blk.turns) {
-      codes = turned_codes(x, z, fmaxf(magnitude, 1.0f) * 0x1p-21f, w, scale, sure);
+      auto off = [&](int k) { return Pairing<kInterleaved>(e + k, n, true).pair < 0 ? 0.0f : bound; };
+      codes = turned_codes(x, z, off, w, scale, sure);
       if (__builtin_amdgcn_ballot_w64(!sure) != 0) {
         codes = exact_codes<T, kInterleaved>(a, blk, sm, t, row, e, scale);
       }

@@ -383,6 +383,8 @@ __device__ __forceinline__ void get8(T (&x)[8], const T* from) {
 // 1, s 0 and z of the same scale: y is x, and in doubt it would be at every border, where 1 of 90 bf16 values lies).
 // `sure`: that leaves no code in doubt. A scale's four lanes come here together, since they exchange its largest
 // magnitude: a branch that some of them take would hide the others' values.
+// (Of a magnitude below 2^-100 the bound and the factors lose their bits: nothing is sure.)
+constexpr float kLeastBound = 0x1p-121f;
 template <typename T, typename B, typename W>
 __device__ __forceinline__ unsigned turned_codes(const T (&x)[8], const T (&z)[8], B bound, W w, unsigned& scale,
                                                  bool& sure) {
@@ -535,7 +537,7 @@ append_four_kernel(RotaryArgs a) {
   };
   auto put_codes = [&](const Item& x) {
     unsigned cx, cz, sx, sz;
-    bool sure = true;
+    bool sure = !blk.turns || bound >= kLeastBound;
     const float2* cs = sm.cs + x.t * n;
     if (halves && x.e < n) {
       cs += x.e;
@@ -640,7 +642,7 @@ append_four_any_kernel(RotaryArgs a) {
       continue;
     }
     unsigned scale, codes;
-    bool sure = true;
+    bool sure = bound >= kLeastBound;
     if (blk.turns) {
       auto off = [&](int k) { return Pairing<kInterleaved>(e + k, n, true).pair < 0 ? 0.0f : bound; };
       codes = turned_codes(x, z, off, w, scale, sure);

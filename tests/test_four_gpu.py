@@ -670,3 +670,21 @@ def test_attention_slopes_to_the_largest_float(cuda, cap):
     out = cfa.paged_attention(q, c.k, c.v, c.table, c.lengths, 0.125, cap=cap, slopes=slopes)
     ref, _ = attended(q, c, lengths, 0.125, cap, slopes)
     assert rel(out, ref) <= bar(torch.float32)
+
+
+@pytest.mark.parametrize("interleaved", [False, True], ids=["half", "interleaved"])
+@pytest.mark.parametrize("d,dim", [(32, 32), (64, 64), (64, 40), (128, 128)])
+@pytest.mark.parametrize("magnitude,spread", [(1e-42, 1e30), (1e-45, 1e37), (1e-38, 1e30), (1e-31, 1e30), (0.0, 1.0),
+                                              (-1.0, 1.0), (1e30, 1e-30)])
+def test_append_magnitudes(cuda, d, dim, magnitude, spread, interleaved):
+    """Magnitudes that 32 bits hold with few bits or as 0, of keys that make up for them; 0, and a negative one."""
+    k = torch.randn(1, 2, 60, d, generator=torch.Generator().manual_seed(d)) * spread
+    k[..., dim:] /= spread
+    f = cfa.rotary_frequencies(dim, device=cuda)
+    kp, vp = (torch.zeros(4, 2, 16, cfa.fp4_row_bytes(d), dtype=torch.uint8, device=cuda) for _ in range(2))
+    table = torch.arange(4, dtype=torch.int32, device=cuda)[None]
+    cfa.paged_append(k.to(cuda), k.to(cuda), kp, vp, table, ints([1], cuda), frequencies=f, interleaved=interleaved,
+                     magnitude=magnitude)
+    got_k, got_v = (x.transpose(0, 1).flatten(1, 2)[:, 1:61].cpu() for x in (kp, vp))
+    assert torch.equal(got_k, encode(turned(k[0], torch.arange(1, 61), f, interleaved, magnitude)))
+    assert torch.equal(got_v, encode(k[0]))

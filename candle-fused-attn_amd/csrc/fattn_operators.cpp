@@ -124,7 +124,8 @@ int run_rotary(const char* who, fattn::RotaryArgs& a, int dtype, int cache_dtype
   a.pairs = static_cast<int>(dim / 2);
   int64_t vec = 16 / size;
   if (cache_dtype == FATTN_FP4) {
-    // Sixteen values at a time, in two halves of which each is whole scales, or eight.
+    // Sixteen values at a time, in two halves (of whole scales each in the half layout; of neighbours, eight values are
+    // turned or not), or eight.
     bool pairs = d >= 64 && (a.interleaved ? dim % 8 == 0 : dim % 64 == 0 && (d - dim) % 64 == 0);
     for (int i = 0; i < 3; ++i) {
       const fattn::RotaryPart& p = a.part[i];

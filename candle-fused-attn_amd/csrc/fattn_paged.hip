@@ -39,10 +39,12 @@
 //
 // Measured (kernel and join): 4 contexts of 60000 to 131071, 32 heads in 8 groups, d 128 bf16, 263 to 273 + 5
 // us (5.7 to 5.9 TB/s, by card); that ragged batch 45 + 5 us (4.5 TB/s); 8 x 6 heads 1 x 1536 fp32 12.4 + 3.9
-// us (3.0 TB/s); the ragged batch in bf16 27 us in all, 29 with a cap and slopes (3.4 TB/s). Over 4 bits those
-// contexts 102 + 5 us (4.1 TB/s: 331 vector instructions a tile of 32 keys, which take 70 % of that time), the
-// ragged batch with fp32 queries 23 in all (1.2 TB/s: what each head and run begins and ends with). (Two tiles in
-// hand, for fewer workgroups a CU: 106 us -> 118, and no gain.) One sequence of 240, 6 heads, 7.8 us, the latency
+// us (3.0 TB/s); the ragged batch in bf16 27 us in all, 29 with a cap and slopes (3.4 TB/s), in f16 28 and 32,
+// f32 over f16 30 and 33, over bf16 28 and 31, over f32 43 and 45 (4.4 TB/s). Over 4 bits those contexts 104 + 5
+// us with slopes (4.0 TB/s: 331 vector instructions a tile of 32 keys, which take 70 % of that time); without, in
+// all, bf16 98, f16 queries 119, f32 124; the ragged batch with f32 queries 24 in all (1.1 TB/s: what each head and
+// run begins and ends with), f16 23, bf16 21. (Two tiles in hand, for fewer workgroups a CU: 106 us -> 118, and no
+// gain.) One sequence of 240, 6 heads, 7.8 us, the latency
 // of one workgroup, where the table has room for little more (split_plan); under one for 4096 or 131072 tokens the
 // same sequence takes runs and a join, 10.5 us for 7.3 from a graph, 64 such sequences 20.1 for 12.6.
 #include <hip/hip_runtime.h>

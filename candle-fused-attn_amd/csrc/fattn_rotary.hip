@@ -210,11 +210,12 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotaryArgs a) {
 // the border between two codes, and a token has the same codes on whatever path it came.
 //
 // 32 bits decide nearly every code: with the bound on what they are off by, both ends of a value's interval have
-// the same one. Only where that leaves a doubt (an item of a wave in some hundreds) is it formed in 64.
+// the same one. Only where that leaves a doubt (an item of a wave in some hundreds; a group of values below 2^-100, all
+// zeros among them; any turned by a magnitude below 2^-100) is it formed in 64.
 //
 // Bound: memory, and for few tokens the launch. A thread has 16 values, in two halves that turn together, so that
 // four neighbours share a scale, a head's scales are one word and each value is read once. 16 x 2048 tokens, 32
-// + 8 heads d 128 bf16, into pages: 145 us (4.7 TB/s; all codes in 64 bits 8 values at a time 200; four items in
+// + 8 heads d 128 bf16, into pages: 139 to 147 us (4.7 TB/s; all codes in 64 bits 8 values at a time 200; four items in
 // flight for two 179; queries in a launch of their own 198); 64 single tokens of 6 + 6 heads fp32 d 64 5.6 us.
 
 // cos and sin of the angle p f (rounded once), times the magnitude, in 64 bits: less q quarter turns, |y| <=
@@ -601,7 +602,9 @@ append_four_kernel(RotaryArgs a) {
   }
 }
 
-// The same for every other head, rotation and alignment: an item 8 values, moved one by one.
+// The same for every other head, rotation and alignment (d 32, half layouts whose parts are no whole scales twice): an
+// item 8 values, moved one by one, which is what bounds it. 16 x 2048 tokens, 32 + 8 heads, bf16, half layout: d 32 130
+// us (1.4 TB/s), d 64 with 32 turned 290 (1.2 TB/s), d 128 with 96 571; f32 224, 385 and 814.
 template <typename T, bool kInterleaved>
 __global__ void __launch_bounds__(kRotThreads)
 append_four_any_kernel(RotaryArgs a) {

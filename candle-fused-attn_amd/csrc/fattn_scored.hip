@@ -18,11 +18,12 @@
 // tanh and exponent, the weights' split; at d 64 two waves of the backward share a SIMD, at d 128 one has it alone
 // and waits for its LDS reads besides. One body per walk, whose masked scores are minus infinity, and a kernel
 // per kind of score (slopes, cap): bodies with and without a mask side by side took registers for both.
-// Measured: 8 x 12 heads of 2048, d 64, causal: one document, plain scores, forward 217 us, backward 643 (79 and
-// 67 TFLOP/s of 4 d and 10 d operations a pair, 237 and 200 of f16 products; fused_attention 230 and 717), capped
-// 220 and 702; packed documents with a mean of 600, capped, 143 and 407; 4 x 16 heads in 4 groups of 777, d 128,
-// slopes and prefixes, 88 and 264 + 10 (the sum of the chunks); 2 x 32 heads in 8 groups 512 x 4097, d 128,
-// slopes, forward 286 with its join (225 TFLOP/s, 675 of f16 products).
+// Measured (kernels in a queue; the first twenty or so run at a lower clock, up to 20 % slower): 8 x 12 heads of 2048,
+// d 64, causal, plain scores, forward 204 us, backward 646 (252 and 200 TFLOP/s of 4 d and 10 d operations a pair,
+// each as three products of f16; fused_attention 198 and 635), capped 231 and 723; in documents of 600, capped, 124
+// and 347; 4 x 16 heads in 4 groups of 777, d 128, slopes and prefixes, 81 and 235 + 10 (the sum of the chunks); 2 x
+// 32 heads in 8 groups 512 x 4097, d 128, slopes, forward 280 and 16 its join (218 TFLOP/s). Cards differ by some
+// percent; figures side by side are of one card.
 #include <hip/hip_runtime.h>
 #include <limits.h>
 #include <math.h>
@@ -408,8 +409,8 @@ __device__ __forceinline__ void scored_fwd(const ScoredArgs& a) {
   const int BH = a.B * a.H, off = a.SK - a.SQ;
   // (Causal: the blocks that see most first, and the heads of a group, which read the same keys, in one XCD's L2
   // where the key heads are a multiple of the XCDs. 2 x 32 heads in 8 groups 512 x 4097 d 128 so 97 MB from
-  // memory and 286 us, group heads side by side 780 and 289; the backward's query blocks, 4 x 16 heads in 4
-  // groups of 777, take 2 % longer so.)
+  // memory and, on one card, 286 us with the join, group heads side by side 780 and 289; the backward's query
+  // blocks, 4 x 16 heads in 4 groups of 777, take 2 % longer so.)
   const int id = static_cast<int>(blockIdx.x), per = a.nqb * a.nc, pairs = a.B * (a.H / a.G), in_pair = id / pairs;
   const int item = a.causal ? (id % pairs * a.G + in_pair % a.G) * per + per - 1 - in_pair / a.G
                             : xcd_remap(id, per * BH);
@@ -1281,7 +1282,11 @@ int launch_scored_forward(ScoredArgs a, int d, const ScoredPlan& plan, void* wor
   hipStream_t s = static_cast<hipStream_t>(stream);
   const unsigned grid = static_cast<unsigned>(int64_t{a.B} * a.H * a.nqb * a.nc);
   const int m = mods(a);
-  const void* fn = m == 7 ? fwd_fn<7>(d) : m == 3 ? fwd_fn<3>(d) : m == 2 ? fwd_fn<2>(d) : m == 1 ? fwd_fn<1>(d) : fwd_fn<0>(d);
+  const void* fn = m == 7   ? fwd_fn<7>(d)
+                   : m == 3 ? fwd_fn<3>(d)
+                   : m == 2 ? fwd_fn<2>(d)
+                   : m == 1 ? fwd_fn<1>(d)
+                            : fwd_fn<0>(d);
   const hipError_t err = hipLaunchKernel(fn, dim3(grid), dim3(64 * kW), args, 0, s);
   if (err != hipSuccess || a.nc == 1) return static_cast<int>(err);
   const void* join = d == 32    ? reinterpret_cast<const void*>(join_scored_kernel<32>)
@@ -1306,7 +1311,11 @@ int launch_scored_backward(ScoredArgs a, int d, const ScoredBackwardPlan& plan, 
   const int HK = a.H / a.G;
   const int64_t grid = scored_blocks(a.B, HK, a.SK) * a.nck + scored_blocks(a.B, a.H, a.SQ) * a.ncq;
   const int m = mods(a);
-  const void* fn = m == 7 ? bwd_fn<7>(d) : m == 3 ? bwd_fn<3>(d) : m == 2 ? bwd_fn<2>(d) : m == 1 ? bwd_fn<1>(d) : bwd_fn<0>(d);
+  const void* fn = m == 7   ? bwd_fn<7>(d)
+                   : m == 3 ? bwd_fn<3>(d)
+                   : m == 2 ? bwd_fn<2>(d)
+                   : m == 1 ? bwd_fn<1>(d)
+                            : bwd_fn<0>(d);
   hipError_t err = hipLaunchKernel(fn, dim3(static_cast<unsigned>(grid)), dim3(64 * kW), args, 0, s);
   auto sum = [&](const float* part, float* out, int64_t n, int nc) {
     void* sargs[] = {&part, &out, &n, &nc};

@@ -16,7 +16,7 @@ def fused_scored_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sc
                            prefix: torch.Tensor | None = None) -> torch.Tensor:
     """softmax(y) v over the keys that a query sees, y the score x = scale q.k, with `cap` (1e-30 to 1e30)
     taken as cap tanh(x / cap), and with `slopes` ([h] f32, finite, one per query head) lowered by the slope times the
-    distance |i - j| of the positions (of a negative slope a float at every distance).
+    distance |i - j| of the positions (a negative slope times the largest distance has to be finite too).
 
     q: [b, h, sq, d], the last sq of sk positions, k, v: [b, kv_heads, sk, d] f32 on one HIP device, any
     strides (copied first when the kernels cannot read them in place), d 32, 64 or 128, h a multiple of

@@ -280,7 +280,8 @@ int fattn_paged_attention(int dtype, int cache_dtype, int64_t b, int64_t heads, 
 
 /* The same, of scores x = scale q.k taken as cap tanh(x / cap) (cap 0: as they are; else 1e-30 to 1e30),
  * less slopes[head] times the distance lengths[b] - 1 - j to cached token j (slopes NULL: none; [heads]
- * finite floats on the device, a negative one a float times every distance too). The workspace is fattn_paged_attention's. */
+ * finite floats on the device; a negative one times the largest distance is a float too). The workspace is
+ * fattn_paged_attention's. */
 int fattn_paged_scored_attention(int dtype, int cache_dtype, int64_t b, int64_t heads, int64_t kv_heads,
                                  int64_t d, const void* q, const int64_t q_strides[2], void* out,
                                  const void* k_pages, const int64_t k_page_strides[3],
